@@ -42,6 +42,11 @@ def _cuda():
     return cuda
 
 
+from . import kv8 as _kv8, logprobs as _logprobs  # noqa: E402  (they read COUNTS)
+from .kv8 import KV8  # noqa: E402
+from .logprobs import TokenLogprobs  # noqa: E402,F401
+
+
 # --------------------------------------------------------------------------------------------------------------
 def embedding(idx, weight, dtype):
     if native(weight):
@@ -194,6 +199,63 @@ def lmhead_loss(x, w, targets, vocab, cap, reduction="mean", row_weights=None, l
         for tk, wk in aux:
             out = out + RF.softcap_cross_entropy(x, w.to(x.dtype), tk, vocab, cap, wk, "mean")
     return out
+
+
+def token_logprobs(logits, tokens, topk=0, vocab=None):
+    """What each row of ``logits [.., C]`` (its first ``vocab`` columns; default all) says: ``TokenLogprobs`` with the log-probability
+    of the row's token in ``tokens [..]`` (0 where that is outside the vocabulary, as -1), the entropy in nats and the ``topk`` (32 at
+    most) most probable tokens, equal logits in the order of their index, with their log-probabilities.  All but the ids have gradients.
+    A row that holds a NaN or +inf, or nothing but -inf, has NaN for results.  Logits in bf16 or fp32, sums in fp32."""
+    vocab = logits.shape[-1] if vocab is None and logits.dim() else vocab
+    _logprobs.check(logits, tokens, topk, vocab)
+    if native(logits):
+        return _logprobs.native(logits, tokens, topk, vocab)
+    return _logprobs.statement(logits, tokens, topk, vocab)
+
+
+# -- key/value cache in 8 bits -----------------------------------------------------------------------------------
+def kv8_cache(batch, max_len, n_head, head_dim, device=None) -> KV8:
+    """An empty cache of one layer (``ops.kv8.KV8``) for ``batch`` sequences of up to ``max_len`` tokens (rounded up to 64): int8 codes with
+    one scale for each block of 64 tokens and head; the tokens of a block that is not full yet are held in bf16."""
+    return _kv8.cache(batch, max_len, n_head, head_dim, device)
+
+
+def kv8_append(cache, k, v, pos, lens=None):
+    """Tokens ``k, v [B, t, H, D]`` (keys behind RoPE and norm) into the cache, in place: sequence b's first ``lens[b]`` (default all)
+    at position ``pos[b]``, which is where its last ones ended; ``pos`` and ``lens`` are ints or int32 on the device (one value or B).
+    What the cache holds does not depend on the pieces it came in.  A sequence at a negative position, without tokens or with more
+    than fit is left as it was."""
+    _kv8.check_append(cache, k, v, pos, lens)
+    _kv8.no_gradient(k, v)
+    if native(k):
+        return _kv8.append(cache, k, v, pos, lens)
+    b = k.shape[0]
+    RF.kv8_append(cache, k, v, _kv8.numbers(pos, b), _kv8.numbers(k.shape[1] if lens is None else lens, b))
+
+
+def kv8_read(cache, held, length):
+    """``(k, v) [B, length, H, D]`` in bf16: what the cache holds of each sequence's first ``length`` positions, zeros from ``held[b]`` on
+    (the number of its tokens; an int or int32 on the device)."""
+    _kv8.check_cache(cache)
+    _kv8.check_per_sequence(held, cache.k.shape[0], "held", cache.k.device)
+    if length < 0 or (isinstance(held, int) and not 0 <= held <= cache.capacity):
+        raise ValueError(f"8-bit cache: {length} positions of {held} tokens, capacity {cache.capacity}")
+    if native(cache.k):
+        return _kv8.read(cache, held, length)
+    return RF.kv8_read(cache, _kv8.numbers(held, cache.k.shape[0]), length)
+
+
+def kv8_attention(qkv, cos, sin, cache, pos, scale, doc_start=None, window=0):
+    """One token a sequence: ``qkv [B, 3*H*D]`` -> RoPE and norm of the query and the key, key and value appended at ``pos[b]`` (in place),
+    soft-max attention over the positions from ``doc_start[b]`` (and the band of ``window`` tokens, as in ``attention``) to ``pos[b]``
+    -> ``[B, H*D]``.  A sequence at a negative position, or one past the cache or the rotary tables, is left as it was and gets
+    zeros; so does a query that sees no key.  No gradient."""
+    _kv8.check_attention(qkv, cos, sin, cache, pos, doc_start, window)
+    _kv8.no_gradient(qkv)
+    if native(qkv):
+        return _kv8.attention(qkv, cos, sin, cache, pos, scale, doc_start, window)
+    b = qkv.shape[0]
+    return RF.kv8_attention(qkv, cos, sin, cache, _kv8.numbers(pos, b), scale, None if doc_start is None else doc_start.tolist(), window)
 
 
 # -- output-side hashed table ------------------------------------------------------------------------------------

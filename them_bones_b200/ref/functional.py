@@ -570,3 +570,134 @@ def stochastic_round_bf16(x: torch.Tensor, generator=None) -> torch.Tensor:
     r = torch.randint(0, 1 << 16, bits.shape, dtype=torch.int32, device=x.device, generator=generator)
     out = ((bits + r) & -65536).view(torch.float32)
     return torch.where(torch.isfinite(x), out, x).to(torch.bfloat16)
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# Keys and values in 8 bits: int8 codes, one scale for each block of 64 tokens and head, the block that is not full yet in bf16
+# ----------------------------------------------------------------------------------------------------------------
+
+KV8_BLOCK = 64
+KV8_TINY = 2.0 ** -100        # a block whose largest value is below this is stored as zeros (127 / most would leave fp32)
+
+
+def kv8_quantise(x: torch.Tensor):
+    """Whole blocks ``x [.., 64, D]`` -> int8 codes and fp32 scales ``[..]``: ``most = max |x|``, ``scale = most / 127``,
+    ``code = round(x * (127 / most))``, ties to even.  A value that is not finite gets the code -128, which reads back as NaN;
+    it does not count for ``most``, and the scale of its block carries a minus sign."""
+    xf = x.float()
+    fine = torch.isfinite(xf)
+    xf = torch.where(fine, xf, torch.zeros_like(xf))
+    most = xf.abs().amax((-1, -2))
+    used = torch.where(most >= KV8_TINY, most, torch.zeros_like(most))
+    top = torch.full_like(used, 127.0)                 # a tensor: by a number, PyTorch on a GPU multiplies by the reciprocal instead of dividing
+    inv = torch.where(used > 0, top / used.clamp_min(KV8_TINY), torch.zeros_like(used))
+    codes = torch.round(xf * inv[..., None, None]).clamp(-127, 127)
+    codes = torch.where(fine, codes, torch.full_like(codes, -128)).to(torch.int8)
+    scale = used / top
+    return codes, torch.where(fine.flatten(-2).all(-1), scale, -scale)
+
+
+def kv8_values(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """What the codes ``[.., 64, D]`` stand for, fp32."""
+    x = codes.float() * scale.abs()[..., None, None]
+    return torch.where(codes == -128, torch.full_like(x, float("nan")), x)
+
+
+def _kv8_line(cache, b: int, blocks: int):
+    """Keys and values ``[H, blocks * 64, D]`` (fp32) of sequence ``b`` from its full blocks."""
+    k8, v8, ks, vs = cache[:4]
+    _, h, _, d = k8.shape
+    k = kv8_values(k8[b, :, :blocks * KV8_BLOCK].reshape(h, blocks, KV8_BLOCK, d), ks[b, :, :blocks])
+    v = kv8_values(v8[b, :, :blocks].transpose(-1, -2), vs[b, :, :blocks])
+    return k.reshape(h, -1, d), v.reshape(h, -1, d)
+
+
+@torch.no_grad()
+def kv8_append(cache, k, v, pos, lens):
+    """Tokens ``k, v [B, t, H, D]`` into the cache (in place), sequence b's first ``lens[b]`` at ``pos[b]`` (lists of ints).  A
+    sequence without tokens, or whose tokens do not all fit, is left as it was."""
+    k8, v8, ks, vs, kt, vt = cache
+    cap = k8.shape[2]
+    for b, (p, n) in enumerate(zip(pos, lens)):
+        n = min(n, k.shape[1])
+        if p < 0 or n <= 0 or p + n > cap:
+            continue
+        first, end = p // KV8_BLOCK, (p + n) // KV8_BLOCK
+        for new, tail, codes, scales in ((k, kt, k8, ks), (v, vt, v8, vs)):
+            line = torch.cat([tail[b, :, :p - first * KV8_BLOCK], new[b, :n].transpose(0, 1).to(tail.dtype)], 1)
+            full, rest = line[:, :(end - first) * KV8_BLOCK], line[:, (end - first) * KV8_BLOCK:]
+            if end > first:
+                q, s = kv8_quantise(full.reshape(full.shape[0], end - first, KV8_BLOCK, -1))
+                if codes is k8:
+                    k8[b, :, first * KV8_BLOCK:end * KV8_BLOCK] = q.flatten(1, 2)
+                else:
+                    v8[b, :, first:end] = q.transpose(-1, -2)
+                scales[b, :, first:end] = s
+                tail[b, :, :rest.shape[1]] = rest
+            else:
+                tail[b, :, p - first * KV8_BLOCK:rest.shape[1]] = rest[:, p - first * KV8_BLOCK:]
+
+
+@torch.no_grad()
+def kv8_read(cache, held, length: int):
+    """Keys and values ``[B, length, H, D]`` (bf16) of the first ``held[b]`` tokens, zeros behind them."""
+    k8, kt, vt = cache[0], cache[4], cache[5]
+    b, h, _, d = k8.shape
+    out = [torch.zeros(b, length, h, d, dtype=kt.dtype, device=k8.device) for _ in range(2)]
+    for i, n in enumerate(held):
+        n = min(n, length, k8.shape[2])
+        if n <= 0:
+            continue
+        blk = held[i] // KV8_BLOCK
+        for dst, line, tail in zip(out, _kv8_line(cache, i, min(blk, -(-n // KV8_BLOCK))), (kt, vt)):
+            line = torch.cat([line.to(kt.dtype), tail[i]], 1)[:, :n]
+            dst[i, :n] = line.transpose(0, 1)
+    return tuple(out)
+
+
+@torch.no_grad()
+def kv8_attention(qkv, cos, sin, cache, pos, scale: float, doc_start=None, window: int = 0):
+    """One token a sequence: RoPE and norm of ``q`` and ``k`` from the packed ``qkv [B, 3*H*D]`` in fp32, ``k`` and ``v``
+    appended at ``pos[b]``, ``q`` against the keys from ``max(doc_start[b], band)`` on -> ``[B, H*D]``.  Sequences at a
+    position outside the cache or the rotary tables get zeros and their cache is left as it was; a query that sees no key gets zeros."""
+    k8 = cache[0]
+    b, h, cap, d = k8.shape
+    y = torch.zeros(b, h * d, dtype=qkv.dtype, device=qkv.device)
+    for i, p in enumerate(pos):
+        if p < 0 or p >= min(cap, cos.shape[0]):
+            continue
+        q, k, v = qkv[i].float().view(3, h, d).unbind(0)
+        c, s = cos[p].float(), sin[p].float()
+        q, k = (torch.cat([x[:, :d // 2] * c + x[:, d // 2:] * s, -x[:, :d // 2] * s + x[:, d // 2:] * c], -1) for x in (q, k))
+        q, k = (x * torch.rsqrt(x.square().mean(-1, keepdim=True) + RMS_EPS) for x in (q, k))
+        lo = max(doc_start[i] if doc_start is not None else 0, (p // 128 - (window // 128 - 1)) * 128 if window else 0, 0)
+        first = p // KV8_BLOCK * KV8_BLOCK
+        keys, vals = (torch.cat([line, tail[i, :, :p - first].float(), new.to(tail.dtype).float()[:, None]], 1)
+                      for line, tail, new in zip(_kv8_line(cache, i, first // KV8_BLOCK), cache[4:6], (k, v)))
+        if lo <= p:
+            w = torch.softmax(torch.einsum("hd,hnd->hn", q, keys[:, lo:]) * scale, -1)
+            y[i] = torch.einsum("hn,hnd->hd", w, vals[:, lo:]).reshape(-1).to(y.dtype)
+        one = [x.to(kt.dtype)[None, None] for x, kt in zip((k, v), cache[4:6])]
+        kv8_append([t[i:i + 1] for t in cache], one[0], one[1], [p], [1])
+        for tail, x in zip(cache[4:6], one):                # the open block keeps its last token when it becomes codes
+            tail[i, :, p - first] = x[0, 0]
+    return y
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# Log-probabilities of given tokens, entropy, alternatives
+# ----------------------------------------------------------------------------------------------------------------
+
+def token_logprobs(logits, tokens, topk: int, vocab: int):
+    """``(logprob, entropy, top_logprob, top_id)`` of the soft-max over the first ``vocab`` columns of ``logits [n, C]``; fp32.
+    Differentiable.  A token outside the vocabulary has log-probability 0; alternatives descend, equal logits in the order of
+    their index, a NaN before everything; a row with a NaN, with +inf or with nothing but -inf has NaN for results."""
+    z = logits[:, :vocab].float()
+    logp = torch.log_softmax(z, -1)
+    gone = logp == float("-inf")                       # probability 0: no part in the entropy or its gradient
+    entropy = -(logp.exp() * logp.masked_fill(gone, 0.0)).masked_fill(gone, 0.0).sum(-1)
+    some = (tokens >= 0) & (tokens < vocab)
+    given = logp.gather(1, torch.where(some, tokens, torch.zeros_like(tokens))[:, None])[:, 0]
+    given = torch.where(some, given, torch.zeros_like(given))
+    ids = torch.sort(z.detach(), dim=-1, descending=True, stable=True).indices[:, :topk]
+    return given, entropy, logp.gather(1, ids), ids
