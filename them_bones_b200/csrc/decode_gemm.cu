@@ -313,20 +313,6 @@ static int launch_dec_gemm_epi(int epi, const CUtensorMap& tw, const CUtensorMap
 // 207 / 250 / 400; batch 64 (U = 2) 225 / 295 / 525 -> 222 / 277 / 466, with U = 4 231 / 277 / 465.
 // The fixed soft-max shift of the training kernels applies (q and k are RMS-normalised).
 // ---------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void unpack8(const uint4& u, float* f) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-}
-__device__ __forceinline__ int ld_relaxed(const int* p) {      // from L2: an earlier look may have left the line in L1
-  int v;
-  asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ void st_relaxed(int* p, int v) { asm volatile("st.relaxed.gpu.global.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory"); }
 __device__ __forceinline__ void prefetch_l2(const void* a) { asm volatile("prefetch.global.L2 [%0];" ::"l"(a)); }
 constexpr int kDaWarps = 8;
 template <int U, int CTAS>

@@ -5,7 +5,9 @@
 //
 // A value that is not finite gets the code -128, which stands for NaN, and its block a scale with a minus sign, so that blocks
 // without one need not look for it.  A block is quantised once, from its 64 bf16 tokens, when it is full.
-#include "common.cuh"
+#include "decode_common.cuh"
+
+#include <cuda_fp16.h>
 
 namespace bones {
 
@@ -33,26 +35,15 @@ __device__ __forceinline__ int kv8_code(float x, float inv) {
 }
 __device__ __forceinline__ float kv8_value(int code, float scale) { return code == -128 ? __int_as_float(0x7fc00000) : (float)code * fabsf(scale); }
 
-__device__ __forceinline__ void unpack8(const uint4& u, float* f) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 t = unpack_bf16(w[i]);
-    f[2 * i] = t.x;
-    f[2 * i + 1] = t.y;
-  }
-}
-
-constexpr int QT = 256;                         // threads that quantise a block
 struct __align__(16) QuantShared {
-  float most[QT / 32];
-  int bad[QT / 32];
+  float most[8];
+  int bad[8];
   int8_t turn[128][KB + 16];                    // value codes on their way to [D][64]; rows stay 16-byte aligned
 };
 
-// A whole block by a CTA of QT threads: 16-byte piece i of the block is token i / (D / 8), dimensions 8 (i % (D / 8)) ..; `piece(token, dim)`
+// A whole block by a CTA of QT threads (256 at most): 16-byte piece i of the block is token i / (D / 8), dimensions 8 (i % (D / 8)) ..; `piece(token, dim)`
 // is its address.  Key codes go out as they lie, value codes through shared memory to be transposed.
-template <int D, bool VALUES, class Piece>
+template <int QT, int D, bool VALUES, class Piece>
 __device__ __forceinline__ void kv8_quantise_block(Piece piece, int8_t* __restrict__ out, float* __restrict__ scale, QuantShared& sm) {
   constexpr int PER = KB * D / 8 / QT, ROW = D / 8;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -106,6 +97,7 @@ __device__ __forceinline__ void kv8_quantise_block(Piece piece, int8_t* __restri
   }
 }
 
+constexpr int kAppendThreads = 256;
 // Tokens pos .. pos + len of a sequence.  A CTA takes one block that the run touches, of the keys or of the values of one head; the first
 // one also stores what is left over for the open block, after it has read the tokens that were in it before.
 template <int D, bool VALUES>
@@ -113,7 +105,7 @@ __device__ __forceinline__ void kv8_append_block(const __nv_bfloat16* __restrict
                                                  __nv_bfloat16* __restrict__ tail, int pos, int len, int i, QuantShared& sm) {
   const int first = pos / KB, end = pos + len, blk = first + i;
   if ((long long)(blk + 1) * KB <= end)
-    kv8_quantise_block<D, VALUES>(
+    kv8_quantise_block<kAppendThreads, D, VALUES>(
         [&](int t, int d) -> const __nv_bfloat16* {
           const int j = blk * KB + t;
           return j < pos ? tail + t * D + d : src + (long long)(j - pos) * st + d;
@@ -121,7 +113,7 @@ __device__ __forceinline__ void kv8_append_block(const __nv_bfloat16* __restrict
         codes + (long long)blk * KB * D, scales + blk, sm);
   if (i == 0) {
     const int open = end / KB * KB, from = max(pos, open);
-    for (int p = threadIdx.x; p < (end - from) * (D / 8); p += QT) {
+    for (int p = threadIdx.x; p < (end - from) * (D / 8); p += kAppendThreads) {
       const int j = from + p / (D / 8), d = p % (D / 8) * 8;
       *reinterpret_cast<uint4*>(tail + (j - open) * D + d) = *reinterpret_cast<const uint4*>(src + (long long)(j - pos) * st + d);
     }
@@ -129,7 +121,7 @@ __device__ __forceinline__ void kv8_append_block(const __nv_bfloat16* __restrict
 }
 
 template <int D>
-__global__ void __launch_bounds__(QT) kv8_append_kernel(Kv8 c, const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ v, long long kb,
+__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(Kv8 c, const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ v, long long kb,
                                                         long long kt, long long kh, long long vb, long long vt, long long vh, PerSeq pos_, PerSeq len_, int t,
                                                         int H, int cap) {
   __shared__ QuantShared sm;
@@ -184,129 +176,492 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, __nv_bfloat16* __r
   }
 }
 
-// One CTA per (head, sequence): a block at a time, four threads a key for the scores, two threads a dimension for the output, a running
-// maximum.
+// ---------------------------------------------------------------------------------------------------------------
+// Attention.  Per (head, sequence) a cluster of up to 16 CTAs; a warp takes 4 KB of keys and of values, half a block of 128
+// dimensions or a block of 64, at a time,
+//
+//   s_t = scale ks sum_d q_d k_td,   m' = max(m, s),   p_t = 2^(s_t - m'),   o = o 2^(m - m') + vs sum_t p_t v_td,
+//
+// and keeps its own maximum, sum and output; the warps', then the CTAs' (through distributed shared memory, no workspace) are
+// joined at the end.  Both sums are matrix products (mma.sync m16n8k16: codes as fp16, which holds them exactly, times one column;
+// tcgen05 would want its operands in shared memory and 64 rows of queries, and there is one): the codes' rows are the MMA's rows,
+// and a lane's consecutive bytes of a row are its columns of several MMAs, so that codes go from memory to the operands with
+// two byte permutations and two subtractions for four of them.  The query is two fp16 numbers, hi and lo, in alternate columns of
+// B: the scores lose nothing to it.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int AW = 4;                           // warps of a CTA
+constexpr int kMaxSplit = 16;                   // CTAs of a cluster
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// four codes as two pairs of fp16: with the sign bit turned, byte u below 0x64 is 1024 + u, and u = code + 128
+__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  w ^= 0x80808080u;
+  const __half2 off = __half2half2(__ushort_as_half((unsigned short)0x6480));          // 1152
+  uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+  __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), off), y = __hsub2(*reinterpret_cast<__half2*>(&b), off);
+  lo = *reinterpret_cast<uint32_t*>(&x);
+  hi = *reinterpret_cast<uint32_t*>(&y);
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The other half of a line is the neighbouring warp's: the whole line comes to L2.
+__device__ __forceinline__ void ld_stream(uint32_t (&w)[4], const void* p) {
+  asm volatile("ld.global.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
+}
+__device__ __forceinline__ void ld_stream(uint32_t (&w)[2], const void* p) {
+  asm volatile("ld.global.L1::no_allocate.L2::128B.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+}
+// bytes of `w` that are -128, as the top bits of theirs
+__device__ __forceinline__ uint32_t bad_codes(uint32_t w) { return __vcmpeq4(w, 0x80808080u) & 0x80808080u; }
+
+// RoPE of a row by a warp, and what norm multiplies it by: dimensions lane + 32 i of the first half in `a`, their partners in `e`.
+template <int D, class T>
+__device__ __forceinline__ T turn_and_norm(const __nv_bfloat16* __restrict__ x, const float* __restrict__ cs, const float* __restrict__ sn, T (&a)[D / 64],
+                                           T (&e)[D / 64]) {
+  const int lane = threadIdx.x & 31;
+  T ss = 0;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) {
+    const int d = lane + 32 * i;
+    const T x0 = (T)__bfloat162float(x[d]), x1 = (T)__bfloat162float(x[d + D / 2]), c = (T)cs[d], s = (T)sn[d];
+    a[i] = x0 * c + x1 * s;
+    e[i] = x1 * c - x0 * s;
+    ss += a[i] * a[i] + e[i] * e[i];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  ss = ss * (T)(1.0 / D) + (T)1.1920928955078125e-07;
+  const T r = (T)rsqrtf((float)ss);
+  return r * ((T)1.5 - (T)0.5 * ss * r * r);                       // a step of Newton's: to the rounding of T
+}
+
 template <int D>
-__global__ void __launch_bounds__(256) kv8_attn_kernel(const __nv_bfloat16* __restrict__ qkv, long long ldq, const float* __restrict__ cosT,
-                                                       const float* __restrict__ sinT, int rope_rows, Kv8 c, PerSeq pos_, const int* __restrict__ doc_start,
-                                                       __nv_bfloat16* __restrict__ y, int H, int cap, float scale, int window_tiles) {
-  __shared__ QuantShared sm;
-  __shared__ __align__(16) float s_q[D];
-  __shared__ __align__(16) __nv_bfloat16 s_new[2][D];
-  __shared__ float s_p[KB], s_red[8], s_out[2][D];
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+struct __align__(16) AttnShared {
+  float acc[2 * AW][D];                         // full blocks of each warp, then the open block's part of each
+  float part[kMaxSplit][D + 4];                 // every CTA's output, sum and maximum, in the first CTA
+  float q[D];
+  __nv_bfloat16 fresh[2][D];                    // the new token's key and value
+  float m[2 * AW], l[2 * AW];
+};
+
+template <int D>
+__global__ void __launch_bounds__(32 * AW, D == 128 ? 3 : 4) kv8_attn_kernel(const __nv_bfloat16* __restrict__ qkv, long long ldq, const float* __restrict__ cosT,
+                                                              const float* __restrict__ sinT, int rope_rows, Kv8 c, PerSeq pos_, const int* doc_start,
+                                                              __nv_bfloat16* __restrict__ y, int H, int cap, float scale2, int window_tiles) {
+  constexpr int TT = 4096 / D, PER = TT / 8, VW = TT / 16;                // tokens of a turn, of a lane; words of a lane's piece of V
+  constexpr int KL = D / 64, NT = D / 16, LPT = D / 8, TPI = 32 / LPT, RP = 4, PASS = KB / (AW * TPI * RP);
+  __shared__ union {
+    AttnShared<D> at;
+    QuantShared quant;
+  } sm_;
+  AttnShared<D>& sm = sm_.at;
+  pdl_launch();
+  const int S = (int)cluster_size(), rank = (int)cluster_rank();
+  const int h = blockIdx.x / S, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, c4 = lane & 3;
+  // the first kernel of a decode step may be storing a new document start: looked at again behind the wait
+  int lo = doc_start ? ld_relaxed(doc_start + b) : 0;
   const int pos = pos_[b];
   __nv_bfloat16* out = y + ((long long)b * H + h) * D;
   if (pos < 0 || pos >= min(cap, rope_rows)) {
-    if (tid < D) out[tid] = __float2bfloat16(0.f);
+    pdl_wait();
+    if (rank == 0 && tid < D / 2) reinterpret_cast<uint32_t*>(out)[tid] = 0u;
     return;
   }
+  if (S > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // waited for before the first store to another CTA
   const long long bh = (long long)b * H + h, nb = cap / KB;
-  const int slot = pos % KB, blk_new = pos / KB;
-  if (warp < 3) {
-    constexpr int HALF = D / 2, N = HALF / 32;
+  const int slot = pos % KB, last = pos / KB;
+  const bool tail_cta = rank == S - 1;          // its warps come last in the walk over the full blocks
+  const int band = window_tiles > 0 ? max((pos / 128 - (window_tiles - 1)) * 128, 0) : 0;
+  lo = max(lo, band);
+  const int8_t *kp = c.k + bh * cap * D + PER * g * D + 16 * c4, *vp = c.v + bh * cap * D + g * KB + 4 * VW * c4;
+  uint32_t kr[VW][2][KL][4], vr[NT][2][VW];
+  auto load_k = [&](int u) {
+    const int8_t* p = kp + (long long)u * (TT * D);
+#pragma unroll
+    for (int i = 0; i < VW; ++i)
+#pragma unroll
+      for (int f = 0; f < 2; ++f)
+#pragma unroll
+        for (int l = 0; l < KL; ++l) ld_stream(kr[i][f][l], p + (2 * i + f) * D + 64 * l);
+  };
+  auto load_v = [&](int u) {
+    const int8_t* p = vp + (long long)(u * TT / KB) * (KB * D) + u * TT % KB;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int f = 0; f < 2; ++f) ld_stream(vr[t][f], p + (16 * t + 8 * f) * KB);
+  };
+  // the open block over the lanes in 16-byte pieces: a warp's pass is RP * TPI of its tokens
+  const int sub = lane / LPT, piece = lane % LPT * 8;
+  uint4 tk[RP], tv[RP];
+  auto tail_slot = [&](int pass, int r) { return ((pass * RP + r) * AW + warp) * TPI + sub; };
+  auto load_tail = [&](int pass) {
+    const __nv_bfloat16 *kt = c.kt + bh * KB * D + piece, *vt = c.vt + bh * KB * D + piece;
+#pragma unroll
+    for (int r = 0; r < RP; ++r) {
+      const int t = tail_slot(pass, r);
+      tk[r] = tv[r] = make_uint4(0u, 0u, 0u, 0u);
+      if (t < slot) {
+        tk[r] = *reinterpret_cast<const uint4*>(kt + t * D);
+        tv[r] = *reinterpret_cast<const uint4*>(vt + t * D);
+      }
+    }
+  };
+  const int step = S * AW, end = last * (KB / TT);
+  int u = lo / TT + rank * AW + warp;
+  if (u < end) load_k(u);
+  if (tail_cta) load_tail(0);
+  pdl_wait();
+  if (doc_start) {
+    const int now = max(ld_relaxed(doc_start + b), band);
+    if (now != lo) {
+      lo = now;
+      u = lo / TT + rank * AW + warp;
+      if (u < end) load_k(u);
+    }
+  }
+  if (warp < (tail_cta ? 3 : 1)) {
     const __nv_bfloat16* x = qkv + b * ldq + ((long long)warp * H + h) * D;
-    float a[N], e[N], ss = 0.f;
+    const float *cs = cosT + (long long)pos * (D / 2), *sn = sinT + (long long)pos * (D / 2);
+    if (warp == 0) {
+      float a[D / 64], e[D / 64];
+      const float r = turn_and_norm<D, float>(x, cs, sn, a, e);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int d = lane + 32 * i;
-      a[i] = __bfloat162float(x[d]);
-      e[i] = __bfloat162float(x[d + HALF]);
-      if (warp < 2) {
-        const float cs = cosT[(long long)pos * HALF + d], sn = sinT[(long long)pos * HALF + d], a0 = a[i], e0 = e[i];
-        a[i] = a0 * cs + e0 * sn;
-        e[i] = e0 * cs - a0 * sn;
-        ss += a[i] * a[i] + e[i] * e[i];
+      for (int i = 0; i < D / 64; ++i) {
+        sm.q[lane + 32 * i] = a[i] * r;
+        sm.q[lane + 32 * i + D / 2] = e[i] * r;
       }
-    }
-    const float r = warp < 2 ? rsqrtf(warp_sum(ss) / D + 1.1920928955078125e-07f) : 1.f;
-    __nv_bfloat16* tail = (warp == 1 ? c.kt : c.vt) + (bh * KB + slot) * D;
+    } else {
+      __nv_bfloat16 *tail = (warp == 1 ? c.kt : c.vt) + (bh * KB + slot) * D, v0[D / 64], v1[D / 64];
+      if (warp == 1) {                          // in 64 bits: the key's rounding to bf16 is the only one, and it stays
+        double a[D / 64], e[D / 64];
+        const double r = turn_and_norm<D, double>(x, cs, sn, a, e);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int d = lane + 32 * i;
-      if (warp == 0) {
-        s_q[d] = a[i] * r;
-        s_q[d + HALF] = e[i] * r;
+        for (int i = 0; i < D / 64; ++i) {
+          v0[i] = __float2bfloat16((float)(a[i] * r));
+          v1[i] = __float2bfloat16((float)(e[i] * r));
+        }
       } else {
-        const __nv_bfloat16 u = __float2bfloat16(a[i] * r), w = __float2bfloat16(e[i] * r);
-        s_new[warp - 1][d] = u;
-        s_new[warp - 1][d + HALF] = w;
-        tail[d] = u;
-        tail[d + HALF] = w;
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+          v0[i] = x[lane + 32 * i];
+          v1[i] = x[lane + 32 * i + D / 2];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) {
+        const int d = lane + 32 * i;
+        sm.fresh[warp - 1][d] = v0[i];
+        sm.fresh[warp - 1][d + D / 2] = v1[i];
+        tail[d] = v0[i];
+        tail[d + D / 2] = v1[i];
       }
     }
+  }
+  if (u < end) load_v(u);
+  __syncthreads();
+
+  // The open block, in plain fp32.
+  if (tail_cta) {
+    const int from = lo - last * KB;                                // slots from .. slot are seen
+    float q[8], m = -INFINITY, l = 0.f, acc[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { q[i] = sm.q[piece + i]; acc[i] = 0.f; }
+#pragma unroll 1
+    for (int pass = 0; pass < PASS && pass * RP * AW * TPI <= slot; ++pass) {
+      if (pass) load_tail(pass);
+      float s[RP], mn = m;
+#pragma unroll
+      for (int r = 0; r < RP; ++r) {
+        const int t = tail_slot(pass, r);
+        if (t == slot) {
+          tk[r] = *reinterpret_cast<const uint4*>(&sm.fresh[0][piece]);
+          tv[r] = *reinterpret_cast<const uint4*>(&sm.fresh[1][piece]);
+        }
+        float f[8], s0 = 0.f, s1 = 0.f;
+        unpack8(tk[r], f);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) { s0 += q[i] * f[i]; s1 += q[i + 1] * f[i + 1]; }
+        s[r] = s0 + s1;
+      }
+#pragma unroll
+      for (int r = 0; r < RP; ++r) {
+#pragma unroll
+        for (int o = LPT / 2; o > 0; o >>= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], o);
+        s[r] *= scale2;
+        const int t = tail_slot(pass, r);
+        if (t >= from && t <= slot) mn = fmaxf(mn, s[r]);
+      }
+#pragma unroll
+      for (int o = LPT; o < 32; o <<= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      const float base = mn == -INFINITY ? 0.f : mn, corr = exp2_fast(m - base);
+      m = mn;
+      l *= corr;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] *= corr;
+#pragma unroll
+      for (int r = 0; r < RP; ++r) {
+        const int t = tail_slot(pass, r);
+        if (t >= from && t <= slot) {
+          const float p = exp2_fast(s[r] - base);
+          float f[8];
+          unpack8(tv[r], f);
+          l += p;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[i] += p * f[i];
+        }
+      }
+    }
+#pragma unroll
+    for (int o = LPT; o < 32; o <<= 1) {
+      l += __shfl_xor_sync(0xffffffffu, l, o);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
+    }
+    if (sub == 0) {
+      float4* to = reinterpret_cast<float4*>(&sm.acc[AW + warp][piece]);
+      to[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      to[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+    }
+    if (lane == 0) { sm.m[AW + warp] = m; sm.l[AW + warp] = l; }
+  }
+
+  // The full blocks.  Token PER g + 2 i + f of a turn is row g + 8 f of MMA i, so a lane ends up with the scores of the PER tokens from
+  // PER g on.
+  {
+    float m = -INFINITY, l = 0.f, acc[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = 0.f;
+    if (u < end) {
+      uint32_t qf[4 * KL][2];
+#pragma unroll
+      for (int l2 = 0; l2 < KL; ++l2)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float4 f = *reinterpret_cast<const float4*>(&sm.q[64 * l2 + 16 * c4 + 4 * w]);
+          uint32_t u0 = pack_f16(f.x, f.y), u1 = pack_f16(f.z, f.w);
+          if (g & 1) {
+            const float2 h0 = __half22float2(*reinterpret_cast<__half2*>(&u0)), h1 = __half22float2(*reinterpret_cast<__half2*>(&u1));
+            u0 = pack_f16(f.x - h0.x, f.y - h0.y);
+            u1 = pack_f16(f.z - h1.x, f.w - h1.y);
+          }
+          qf[4 * l2 + w][0] = u0;
+          qf[4 * l2 + w][1] = u1;
+        }
+      const float *ksp = c.ks + bh * nb, *vsp = c.vs + bh * nb;
+      float ks_n = ksp[u * TT / KB], vs_n = vsp[u * TT / KB];
+#pragma unroll 1
+      while (true) {
+        const int next = u + step, j = u * TT + PER * g;
+        const float ks = ks_n, vs = vs_n;
+        if (next < end) { ks_n = ksp[next * TT / KB]; vs_n = vsp[next * TT / KB]; }
+        float s[PER];
+        {
+          float d[VW][KL][4];                   // chains of four MMAs
+#pragma unroll
+          for (int i = 0; i < VW; ++i)
+#pragma unroll
+            for (int l2 = 0; l2 < KL; ++l2) d[i][l2][0] = d[i][l2][1] = d[i][l2][2] = d[i][l2][3] = 0.f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int l2 = 0; l2 < KL; ++l2)
+#pragma unroll
+              for (int i = 0; i < VW; ++i) {
+                uint32_t a0, a1, a2, a3;
+                codes_f16(kr[i][0][l2][w], a0, a2);
+                codes_f16(kr[i][1][l2][w], a1, a3);
+                mma_f16(d[i][l2], a0, a1, a2, a3, qf[4 * l2 + w][0], qf[4 * l2 + w][1]);
+              }
+#pragma unroll
+          for (int i = 0; i < VW; ++i) {
+            s[2 * i] = d[i][0][0] + d[i][0][1];
+            s[2 * i + 1] = d[i][0][2] + d[i][0][3];
+            if (KL == 2) {
+              s[2 * i] += d[i][KL - 1][0] + d[i][KL - 1][1];
+              s[2 * i + 1] += d[i][KL - 1][2] + d[i][KL - 1][3];
+            }
+          }
+        }
+        if (signbit(ks)) {                      // a key with a value that is not finite
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            uint32_t bad = 0;
+#pragma unroll
+            for (int l2 = 0; l2 < KL; ++l2)
+#pragma unroll
+              for (int w = 0; w < 4; ++w) bad |= bad_codes(kr[i >> 1][i & 1][l2][w]);
+            bad |= __shfl_xor_sync(0xffffffffu, bad, 1);
+            bad |= __shfl_xor_sync(0xffffffffu, bad, 2);
+            if (bad) s[i] = __int_as_float(0x7fc00000);
+          }
+        }
+        if (next < end) load_k(next);
+        const float f = fabsf(ks) * scale2;
+        float mn = m;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          s[i] = j + i >= lo ? s[i] * f : -INFINITY;
+          mn = fmaxf(mn, s[i]);
+        }
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+        const float base = mn == -INFINITY ? 0.f : mn, corr = exp2_fast(m - base);
+        m = mn;
+        l *= corr;
+        uint32_t pr[VW], pf[VW][2];
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+          const float p0 = exp2_fast(s[2 * i] - base), p1 = exp2_fast(s[2 * i + 1] - base);
+          l += p0 + p1;
+          pr[i] = pack_f16(p0, p1);
+        }
+        // B's rows of MMA w are tokens 4 VW c + 4 w ..: with the lanes of g = 2 c, and 2 c + 1 from the middle on
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int i = 0; i < VW; ++i) pf[(k * VW + i) >> 1][(k * VW + i) & 1] = __shfl_sync(0xffffffffu, pr[i], 4 * (2 * c4 + k));
+        const float fv = fabsf(vs);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            uint32_t a0, a1, a2, a3;
+            codes_f16(vr[t][0][w], a0, a2);
+            codes_f16(vr[t][1][w], a1, a3);
+            mma_f16(d, a0, a1, a2, a3, pf[w][0], pf[w][1]);
+          }
+          acc[t][0] = acc[t][0] * corr + fv * d[0];
+          acc[t][1] = acc[t][1] * corr + fv * d[2];
+        }
+        if (signbit(vs)) {                      // values that are not finite, of tokens that are seen
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              bool bad = false;
+#pragma unroll
+              for (int w = 0; w < VW; ++w)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) bad |= ((bad_codes(vr[t][e][w]) >> (8 * i)) & 0x80u) && u * TT + 4 * (VW * c4 + w) + i >= lo;
+              bad |= __shfl_xor_sync(0xffffffffu, (int)bad, 1) != 0;
+              bad |= __shfl_xor_sync(0xffffffffu, (int)bad, 2) != 0;
+              if (bad) acc[t][e] = __int_as_float(0x7fc00000);
+            }
+        }
+        u = next;
+        if (u >= end) break;
+        load_v(u);
+      }
+    }
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (c4 == 0) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        sm.acc[warp][16 * t + g] = acc[t][0];
+        sm.acc[warp][16 * t + 8 + g] = acc[t][1];
+      }
+    }
+    if (lane == 0) { sm.m[warp] = m; sm.l[warp] = l; }
   }
   __syncthreads();
-  int lo = doc_start ? doc_start[b] : 0;
-  if (window_tiles > 0) lo = max(lo, (pos / 128 - (window_tiles - 1)) * 128);
-  lo = max(lo, 0);
-  float m = -INFINITY, l = 0.f, acc = 0.f;
-  const int od = tid % D, oh = tid / D;                  // thread's dimension and half of the block's tokens (D = 64: a quarter)
-  constexpr int PARTS = 256 / D, PT = KB / PARTS;
-  for (int blk = lo / KB; blk <= blk_new; ++blk) {
-    const bool open = blk == blk_new;
-    const int t = tid >> 2, j = blk * KB + t, d0 = (tid & 3) * (D / 4);
-    float s = 0.f;
-    const bool seen = j >= lo && j <= pos;
-    if (seen) {
-      if (open) {
-        const __nv_bfloat16* kr = t == slot ? s_new[0] : c.kt + (bh * KB + t) * D;
-#pragma unroll 8
-        for (int i = 0; i < D / 4; ++i) s += s_q[d0 + i] * __bfloat162float(kr[d0 + i]);
-      } else {
-        const float sc = c.ks[bh * nb + blk];
-        const int8_t* kr = c.k + (bh * cap + j) * D;
-#pragma unroll 8
-        for (int i = 0; i < D / 4; ++i) s += s_q[d0 + i] * kv8_value(kr[d0 + i], sc);
+
+  // The CTA's own parts, then the cluster's.  A part without a token has -inf and 0.
+  const int parts = tail_cta ? 2 * AW : AW;
+  float M = -INFINITY, L = 0.f, o = 0.f;
+  if (tid < D) {
+    for (int e = 0; e < parts; ++e) M = fmaxf(M, sm.m[e]);
+    const float base = M == -INFINITY ? 0.f : M;
+    for (int e = 0; e < parts; ++e) {
+      const float w = exp2_fast(sm.m[e] - base);
+      L += w * sm.l[e];
+      o += w * sm.acc[e][tid];
+    }
+  }
+  if (S > 1) {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (tid < D) {
+      const uint32_t to = map_to_rank(smem_u32(&sm.part[rank][0]), 0);
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4u * (uint32_t)tid), "f"(o) : "memory");
+      if (tid == 0) {
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4u * D), "f"(L) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4u * D + 4u), "f"(M) : "memory");
       }
     }
-    s += __shfl_xor_sync(0xffffffffu, s, 1);
-    s += __shfl_xor_sync(0xffffffffu, s, 2);
-    s = seen ? s * scale : -INFINITY;
-    const float wm = warp_max(s);
-    if (lane == 0) s_red[warp] = wm;
-    __syncthreads();
-    float mn = m;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) mn = fmaxf(mn, s_red[w]);
-    // a score that is not a number has no part in the maximum but makes its probability, and with it the row, not a number
-    const float base = mn == -INFINITY ? 0.f : mn;
-    if ((tid & 3) == 0) s_p[t] = seen ? expf(s - base) : 0.f;
-    __syncthreads();
-    const float corr = m == -INFINITY ? 0.f : expf(m - base);
-    m = mn;
-    l *= corr;
-    acc *= corr;
-    const float vsc = open ? 0.f : c.vs[bh * nb + blk];
-#pragma unroll 4
-    for (int i = 0; i < KB; ++i) l += s_p[i];
-    for (int i = 0; i < PT; ++i) {
-      const int tt = oh * PT + i, jj = blk * KB + tt;
-      if (jj < lo || jj > pos) continue;
-      float vv;
-      if (open) vv = __bfloat162float(tt == slot ? s_new[1][od] : c.vt[(bh * KB + tt) * D + od]);
-      else vv = kv8_value(c.v[(bh * nb + blk) * KB * D + od * KB + tt], vsc);
-      acc += s_p[tt] * vv;
+    cluster_barrier();
+    if (rank == 0 && tid < D) {
+      M = -INFINITY;
+      for (int r = 0; r < S; ++r) M = fmaxf(M, sm.part[r][D + 1]);
+      const float base = M == -INFINITY ? 0.f : M;
+      L = o = 0.f;
+      for (int r = 0; r < S; ++r) {
+        const float w = exp2_fast(sm.part[r][D + 1] - base);
+        L += w * sm.part[r][D];
+        o += w * sm.part[r][tid];
+      }
     }
-    __syncthreads();
   }
-  if (PARTS == 2) {
-    s_out[oh][od] = acc;
+  if (rank == 0 && tid < D) out[tid] = __float2bfloat16(L != 0.f ? o / L : 0.f);
+  if (tail_cta && slot == KB - 1) {
+    // the block is full: its last token is in memory since the first barrier of the CTA
     __syncthreads();
-    if (tid < D) out[tid] = __float2bfloat16(l != 0.f ? (s_out[0][tid] + s_out[1][tid]) / l : 0.f);
-  } else {
-    float* four = reinterpret_cast<float*>(sm.turn);
-    four[tid] = acc;
-    __syncthreads();
-    if (tid < D) out[tid] = __float2bfloat16(l != 0.f ? ((four[tid] + four[tid + D]) + (four[tid + 2 * D] + four[tid + 3 * D])) / l : 0.f);
+    auto tail_of = [&](const __nv_bfloat16* t0) { return [=](int t, int d) { return t0 + t * D + d; }; };
+    kv8_quantise_block<32 * AW, D, false>(tail_of(c.kt + bh * KB * D), c.k + (bh * cap + (long long)last * KB) * D, c.ks + bh * nb + last, sm_.quant);
+    kv8_quantise_block<32 * AW, D, true>(tail_of(c.vt + bh * KB * D), c.v + (bh * cap + (long long)last * KB) * D, c.vs + bh * nb + last, sm_.quant);
   }
-  if (slot == KB - 1) {
-    __syncthreads();
-    kv8_quantise_block<D, false>([&](int t, int d) -> const __nv_bfloat16* { return t == slot ? s_new[0] + d : c.kt + (bh * KB + t) * D + d; },
-                                 c.k + (bh * cap + (long long)blk_new * KB) * D, c.ks + bh * nb + blk_new, sm);
-    kv8_quantise_block<D, true>([&](int t, int d) -> const __nv_bfloat16* { return t == slot ? s_new[1] + d : c.vt + (bh * KB + t) * D + d; },
-                                c.v + (bh * cap + (long long)blk_new * KB) * D, c.vs + bh * nb + blk_new, sm);
-  }
+}
+
+// CTAs of a cluster: doubled until there are one and a half for each SM, as long as the cache's length (the band's, if there is one) can give
+// every warp a turn.  us by 1 / 2 / 4 / 8 / 16 CTAs, heads of 128: 10 heads, 300 tokens 5.8 / 5.9 / 4.5 / 4.7 / 5.2, 2040 tokens 21 / 14 / 9.9 / 7.9 / 6.9;
+// 40 heads, 2040 tokens 22 / 15 / 11 / 9.4 / 14, 131000 tokens 1116 / 571 / 351 / 240 / 253; 160 heads, 2040 tokens 27 / 21 / 25 / 32 / 50; 320 heads,
+// 16000 tokens 233 / 245 / 242 / 245 / 272; 640 heads, 64 tokens 11 / 16 / 31 / 59 / 133, 2040 tokens 68 / 63 / 82 / 109 / 185.
+inline int kv8_splits(int B, int H, int D, int cap, int window_tiles, int sms) {
+  const long long tokens = window_tiles > 0 && window_tiles < cap / 128 ? window_tiles * 128ll : cap;
+  int s = 1;
+  while (s < kMaxSplit && 2ll * B * H * s < 3ll * sms && tokens >= (long long)s * AW * (4096 / D)) s *= 2;
+  return s;
+}
+
+struct AttnArgs {
+  const __nv_bfloat16* qkv;
+  long long ldq;
+  const float *cosT, *sinT;
+  int rope_rows;
+  Kv8 c;
+  PerSeq pos;
+  const int* doc_start;
+  __nv_bfloat16* y;
+  int H, cap;
+  float scale2;
+  int window_tiles;
+};
+template <int D>
+int launch_kv8_attn(const AttnArgs& p, int B, int split, int pdl, cudaStream_t s) {
+  static OncePerDevice once;
+  BONES_ONCE(once, BONES_CHECK(cudaFuncSetAttribute(kv8_attn_kernel<D>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)););
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[2];
+  cfg.gridDim = dim3((unsigned)(p.H * split), (unsigned)B);
+  cfg.blockDim = dim3(32 * AW);
+  cfg.stream = s;
+  cfg.attrs = at;
+  cfg.numAttrs = (unsigned)dec_launch_attrs(at, split, pdl);
+  return (int)cudaLaunchKernelEx(&cfg, kv8_attn_kernel<D>, p.qkv, p.ldq, p.cosT, p.sinT, p.rope_rows, p.c, p.pos, p.doc_start, p.y, p.H, p.cap, p.scale2,
+                                 p.window_tiles);
 }
 
 inline bool kv8_refused(const Kv8& c, int B, int H, int D, int cap) {
@@ -330,7 +685,7 @@ int bones_kv8_append(void* k8, void* v8, float* ks, float* vs, void* kt, void* v
   // t tokens touch this many blocks at most; none lies past the capacity
   const long long blocks = min(((long long)t + KB - 2) / KB + 1, (long long)cap / KB);
   const dim3 grid((unsigned)(2 * blocks), (unsigned)H, (unsigned)B);
-  (D == 128 ? kv8_append_kernel<128> : kv8_append_kernel<64>)<<<grid, QT, 0, (cudaStream_t)stream>>>(
+  (D == 128 ? kv8_append_kernel<128> : kv8_append_kernel<64>)<<<grid, kAppendThreads, 0, (cudaStream_t)stream>>>(
       c, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, kb, kst, kh, vb, vst, vh, PerSeq{pos, pos_step, pos0}, PerSeq{len, len_step, len0}, t, H, cap);
   return (int)cudaGetLastError();
 }
@@ -353,10 +708,13 @@ int bones_kv8_attention(const void* qkv, long long ldq, const float* cosT, const
                         int window_tiles, int pdl, void* stream) {
   const Kv8 c{(int8_t*)k8, (int8_t*)v8, ks, vs, (__nv_bfloat16*)kt, (__nv_bfloat16*)vt};
   if (kv8_refused(c, B, H, D, cap) || !qkv || !cosT || !sinT || !y || misaligned16(qkv, y) || (B > 1 && ldq % 8) || window_tiles < 0) return -2;
-  (void)pdl;
-  const dim3 grid((unsigned)H, (unsigned)B);
-  (D == 128 ? kv8_attn_kernel<128> : kv8_attn_kernel<64>)<<<grid, 256, 0, (cudaStream_t)stream>>>(
-      (const __nv_bfloat16*)qkv, ldq, cosT, sinT, rope_rows, c, PerSeq{pos, pos_step, pos0}, doc_start, (__nv_bfloat16*)y, H, cap, scale, window_tiles);
-  return (int)cudaGetLastError();
+  const AttnArgs p{(const __nv_bfloat16*)qkv, ldq, cosT, sinT, rope_rows, c, PerSeq{pos, pos_step, pos0}, doc_start, (__nv_bfloat16*)y, H, cap,
+                   scale * 1.4426950408889634f, window_tiles};
+  int dev = 0, sms = 0;
+  BONES_CHECK(cudaGetDevice(&dev));
+  BONES_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  const int split = kv8_splits(B, H, D, cap, window_tiles, sms);
+  cudaStream_t s = (cudaStream_t)stream;
+  return D == 128 ? launch_kv8_attn<128>(p, B, split, pdl, s) : launch_kv8_attn<64>(p, B, split, pdl, s);
 }
 }  // extern "C"
