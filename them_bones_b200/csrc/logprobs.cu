@@ -5,17 +5,48 @@
 //   d z_v = -p_v (G + g_H (log p_v + entropy)) + [v = t] g + sum_j [v = id_j] g_j,   G = g + sum_j g_j
 //
 // Alternatives are ordered by their logits, equal ones by their index, a NaN before everything.
-#include "common.cuh"
+//
+// Forward: one pass over the row.  A thread keeps a running maximum with its S and T, and where its maximum was; the alternatives come
+// out of that: among the maxima of groups of threads the k-th largest bounds the row's k-th largest from below, so only threads whose
+// maximum reaches it hold an alternative, and only their columns (a few percent of the row, still in L2) are looked at again.
+// Gradient: one element-wise pass; the few columns with a gradient of their own are written once more.
+#include "decode_common.cuh"
 
 namespace bones {
 
-constexpr int LP_T = 512;
+constexpr int LP_T = 256;
+constexpr int LP_U = 4;                         // 16-byte vectors of a thread in flight
 constexpr int LP_TOP = 32;                      // alternatives at most
+constexpr int LP_GROUPS = LP_T / 4;             // of threads, whose maxima give the bound: two for each alternative at most
+constexpr int LP_CAND = 1024;                   // columns kept for the final choice; a row that needs more is gone over once for each alternative
+constexpr int LP_SPLIT = 16;                    // CTAs of a cluster, one row
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float lp_load(const float* p) { return *p; }
 __device__ __forceinline__ float lp_load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ void lp_store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void lp_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
+// a 16-byte vector: four fp32 or eight bf16
+__device__ __forceinline__ void lp_unpack(const uint4& u, float (&f)[4]) {
+  f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+}
+__device__ __forceinline__ void lp_unpack(const uint4& u, float (&f)[8]) { unpack8(u, f); }
+__device__ __forceinline__ uint4 lp_pack(const float (&f)[4]) {
+  return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+__device__ __forceinline__ uint4 lp_pack(const float (&f)[8]) {
+  return make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+}
+__device__ __forceinline__ float lp_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint4 lp_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
 
 // Order-preserving code of a logit: larger logits have larger codes, -0 and +0 the same, NaN the largest.  0 is below every logit's.
 __device__ __forceinline__ uint32_t lp_code(float v) {
@@ -23,104 +54,313 @@ __device__ __forceinline__ uint32_t lp_code(float v) {
   const uint32_t u = __float_as_uint(v == 0.f ? 0.f : v);
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
-// (logit, column) as one number: the larger comes first among alternatives
-__device__ __forceinline__ unsigned long long lp_key(float v, int c) { return (unsigned long long)lp_code(v) << 32 | (uint32_t)~c; }
-
-template <class F>
-__device__ __forceinline__ F lp_block(F v, F* red, F (*op)(F, F)) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if (lane == 0) red[warp] = v;
-  __syncthreads();
-  v = red[0];
-  for (int w = 1; w < LP_T / 32; ++w) v = op(v, red[w]);
-  return v;
+__device__ __forceinline__ float lp_value(uint32_t code) {
+  return code == 0xfffffffeu ? __int_as_float(0x7fc00000) : __uint_as_float((code & 0x80000000u) ? code & 0x7fffffffu : ~code);
 }
-__device__ __forceinline__ float lp_add(float a, float b) { return a + b; }
-__device__ __forceinline__ float lp_max(float a, float b) { return fmaxf(a, b); }
-__device__ __forceinline__ unsigned long long lp_first(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
+// (logit, column) as one number: the larger comes first among alternatives; no two are equal
+typedef unsigned long long LpKey;
+__device__ __forceinline__ LpKey lp_key(float v, int c) { return (LpKey)lp_code(v) << 32 | (uint32_t)~c; }
+__device__ __forceinline__ LpKey lp_first(LpKey a, LpKey b) { return a > b ? a : b; }
 
-// One CTA a row.  stats [rows][4]: m, log S, entropy, 0.
-template <class Z>
-__global__ void __launch_bounds__(LP_T) logprobs_fwd_kernel(const Z* __restrict__ logits, long long ldl, int V, const long long* __restrict__ tokens, int k,
-                                                            float* __restrict__ given, float* __restrict__ entropy, float* __restrict__ top,
-                                                            long long* __restrict__ ids, float4* __restrict__ stats) {
-  __shared__ float fred[LP_T / 32];
-  __shared__ unsigned long long kred[LP_T / 32];
-  const long long row = blockIdx.x;
-  const Z* z = logits + row * ldl;
-  float m = -INFINITY;
-  for (int c = threadIdx.x; c < V; c += LP_T) m = fmaxf(m, lp_load(z + c));
-  m = lp_block<float>(m, fred, lp_max);
-  float s = 0.f, t = 0.f;
-  for (int c = threadIdx.x; c < V; c += LP_T) {
-    const float w = lp_load(z + c) - m, e = expf(w);
+// running maximum, sum and weighted sum
+struct LpSum {
+  float m, s, t;
+  // a larger maximum `n`; 1000 is further than any probability reaches, and keeps infinities out of the products
+  __device__ __forceinline__ void raise(float n) {
+    const float d = fmaxf(m - n, -1000.f), f = lp_exp2(d * kLog2e);
+    t = f * fmaf(d, s, t);
+    s *= f;
+    m = n;
+  }
+  __device__ __forceinline__ void add(float z) {
+    const float w = z - m, e = lp_exp2(w * kLog2e);
     s += e;
-    t += e * fmaxf(w, -1000.f);                // e is 0 there; -inf has no part
+    t = fmaf(e, fmaxf(w, -1000.f), t);         // -inf has probability 0 and no part
   }
-  s = lp_block<float>(s, fred, lp_add);
-  t = lp_block<float>(t, fred, lp_add);
-  const float ls = logf(s), h = ls - t / s;
-  unsigned long long last = ~0ull;
-  for (int j = 0; j < k; ++j) {
-    unsigned long long best = 0;
-    for (int c = threadIdx.x; c < V; c += LP_T) {
-      const unsigned long long q = lp_key(lp_load(z + c), c);
-      if (q < last && q > best) best = q;
-    }
-    best = lp_block<unsigned long long>(best, kred, lp_first);
-    last = best;
-    if (threadIdx.x == 0) {
-      const int c = (int)~(uint32_t)best;
-      ids[row * k + j] = c;
-      top[row * k + j] = lp_load(z + c) - m - ls;
-    }
+  __device__ __forceinline__ void join(LpSum o) {
+    const float n = fmaxf(m, o.m);
+    raise(n);
+    o.raise(n);
+    s += o.s;
+    t += o.t;
   }
-  if (threadIdx.x == 0) {
-    const long long tk = tokens[row];
-    given[row] = tk >= 0 && tk < V ? lp_load(z + tk) - m - ls : 0.f;
-    entropy[row] = h;
-    if (stats) stats[row] = make_float4(m, ls, h, 0.f);
+};
+
+struct LpShared {
+  LpKey group[LP_GROUPS], cand[LP_CAND], top[LP_TOP], bound, all[LP_SPLIT][LP_TOP];
+  LpSum warp[LP_T / 32], part[LP_SPLIT];
+  int n_cand, n_hold;
+  unsigned short hold[LP_T];
+};
+
+// Places among n keys: key i with fewer than k larger ones goes to out[that number].
+__device__ __forceinline__ void lp_rank(const LpKey* keys, int n, int k, LpKey* out) {
+  for (int i = threadIdx.x; i < n; i += LP_T) {
+    const LpKey mine = keys[i];
+    int r = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) r += keys[j] > mine;
+    if (mine && r < k) out[r] = mine;
   }
 }
 
-// One CTA a row; the given token's and the alternatives' columns are done once more, with what they get besides.
+// Row r of a cluster: the columns of this CTA are `vecs` 16-byte vectors from `body` on (column `col0`), and in the first CTA up to
+// 2 * (VE - 1) single columns before and behind the row's vectors.
+template <class Z>
+__global__ void __launch_bounds__(LP_T, 4) logprobs_fwd_kernel(const Z* __restrict__ logits, long long ldl, int V, const long long* __restrict__ tokens, int k,
+                                                               float* __restrict__ given, float* __restrict__ entropy, float* __restrict__ top,
+                                                               long long* __restrict__ ids, float4* __restrict__ stats) {
+  constexpr int VE = 16 / sizeof(Z);
+  __shared__ LpShared sm;
+  const int S = (int)cluster_size(), rank = (int)cluster_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (S > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // waited for before the first store to another CTA
+  const long long row = blockIdx.x / S;
+  const Z* z = logits + row * ldl;
+  const long long tk = rank == 0 && tid == 0 ? tokens[row] : -1;
+  const float zt = tk >= 0 && tk < V ? lp_load(z + tk) : 0.f;
+  if (tid == 0) sm.n_cand = sm.n_hold = 0;
+  const int head = min(V, (int)((16 - ((uintptr_t)z & 15)) & 15) / (int)sizeof(Z)), nv = (V - head) / VE, rest = V - head - nv * VE;
+  const int v0 = (int)((long long)nv * rank / S), vecs = (int)((long long)nv * (rank + 1) / S) - v0, col0 = head + v0 * VE;
+  const uint4* body = reinterpret_cast<const uint4*>(z + col0);
+  auto single = [&](int i) { return i < head ? i : V - rest + (i - head); };             // column of single i
+  const int singles = rank == 0 ? head + rest : 0;
+
+  LpSum a{-3.402823466e38f, 0.f, 0.f};
+  float best = -INFINITY;                       // of the vectors, and the round of them in which it came
+  int at = 0;
+  bool held = tid < vecs;
+  for (int i = tid, it = 0; i < vecs; i += LP_U * LP_T, ++it) {
+    uint4 u[LP_U];
+#pragma unroll
+    for (int j = 0; j < LP_U; ++j)
+      if (i + j * LP_T < vecs) u[j] = lp_stream(body + i + j * LP_T);
+    float f[LP_U][VE], n = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < LP_U; ++j) {
+      lp_unpack(u[j], f[j]);
+      if (i + j * LP_T >= vecs) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) f[j][e] = -INFINITY;
+      }
+#pragma unroll
+      for (int e = 0; e < VE; ++e) n = fmaxf(n, f[j][e]);
+    }
+    if (n > best) {
+      best = n;
+      at = it;
+      if (n > a.m) a.raise(n);                  // (not for the lowest number)
+    }
+#pragma unroll
+    for (int j = 0; j < LP_U; ++j)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) a.add(f[j][e]);
+  }
+  // a thread's own first column of its largest logit
+  LpKey mine = 0;
+  if (k > 0 && held) {
+    for (int j = 0; j < LP_U; ++j) {
+      const int i = tid + (at * LP_U + j) * LP_T;
+      if (i >= vecs) break;
+      float f[VE];
+      lp_unpack(lp_stream(body + i), f);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) mine = lp_first(mine, lp_key(f[e], col0 + i * VE + e));
+    }
+  }
+  if (tid < singles) {
+    const int c = single(tid);
+    const float v = lp_load(z + c);
+    if (v > a.m) a.raise(v);
+    a.add(v);
+    mine = lp_first(mine, lp_key(v, c));
+  }
+  // the CTA's sums
+  {
+    LpSum w = a;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) w.join(LpSum{__shfl_xor_sync(0xffffffffu, w.m, o), __shfl_xor_sync(0xffffffffu, w.s, o), __shfl_xor_sync(0xffffffffu, w.t, o)});
+    if (lane == 0) sm.warp[warp] = w;
+  }
+  if (k > 0) {
+    LpKey gr = mine;
+    gr = lp_first(gr, __shfl_xor_sync(0xffffffffu, gr, 1));
+    gr = lp_first(gr, __shfl_xor_sync(0xffffffffu, gr, 2));
+    if ((lane & 3) == 0) sm.group[tid >> 2] = gr;
+  }
+  __syncthreads();
+  a = sm.warp[0];
+#pragma unroll
+  for (int w = 1; w < LP_T / 32; ++w) a.join(sm.warp[w]);
+  if (k > 0) {
+    // the bound: the k-th largest of the groups' maxima, any logit where there are not so many
+    if (tid < LP_TOP) sm.top[tid] = 0;
+    if (tid == 0) sm.bound = 1;
+    __syncthreads();
+    if (tid < LP_GROUPS) {
+      const LpKey g = sm.group[tid];
+      int r = 0;
+#pragma unroll 8
+      for (int j = 0; j < LP_GROUPS; ++j) r += sm.group[j] > g;
+      if (g && r == k - 1) sm.bound = g;
+    }
+    __syncthreads();
+    const LpKey bound = sm.bound;
+    bool full = a.s != a.s;                     // a NaN comes first, and no maximum saw it
+    if (!full) {
+      if (mine >= bound && held) sm.hold[atomicAdd(&sm.n_hold, 1)] = (unsigned short)tid;
+      auto keep = [&](LpKey q) {
+        if (q >= bound) {
+          const int n = atomicAdd(&sm.n_cand, 1);
+          if (n < LP_CAND) sm.cand[n] = q;
+        }
+      };
+      if (tid < singles) keep(lp_key(lp_load(z + single(tid)), single(tid)));
+      __syncthreads();
+      const int turns = (vecs + LP_T - 1) / LP_T, all = sm.n_hold * turns;
+      for (int i = tid; i < all; i += LP_T) {
+        const int h = i / turns, v = sm.hold[h] + (i - h * turns) * LP_T;
+        if (v >= vecs) continue;
+        float f[VE];
+        lp_unpack(lp_stream(body + v), f);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) keep(lp_key(f[e], col0 + v * VE + e));
+      }
+      __syncthreads();
+      full = sm.n_cand > LP_CAND;
+      if (!full) lp_rank(sm.cand, sm.n_cand, k, sm.top);
+    }
+    if (full) {
+      LpKey last = ~0ull;
+      for (int j = 0; j < k; ++j) {
+        LpKey best = 0;
+        for (int i = tid; i < vecs; i += LP_T) {
+          float f[VE];
+          lp_unpack(lp_stream(body + i), f);
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            const LpKey q = lp_key(f[e], col0 + i * VE + e);
+            if (q < last && q > best) best = q;
+          }
+        }
+        if (tid < singles) {
+          const LpKey q = lp_key(lp_load(z + single(tid)), single(tid));
+          if (q < last && q > best) best = q;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) best = lp_first(best, __shfl_xor_sync(0xffffffffu, best, o));
+        __syncthreads();
+        if (lane == 0) sm.group[warp] = best;
+        __syncthreads();
+        best = sm.group[0];
+        for (int w = 1; w < LP_T / 32; ++w) best = lp_first(best, sm.group[w]);
+        last = best;
+        if (tid == 0) sm.top[j] = best;
+      }
+    }
+    __syncthreads();
+  }
+  if (S > 1) {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (tid == 0) {
+      const uint32_t to = map_to_rank(smem_u32(&sm.part[rank]), 0);
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(a.m) : "memory");
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(a.s) : "memory");
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(a.t) : "memory");
+    }
+    if (tid < k) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(map_to_rank(smem_u32(&sm.all[0][0] + rank * k + tid), 0)), "l"(sm.top[tid]) : "memory");
+    cluster_barrier();
+    if (rank != 0) return;
+    a = sm.part[0];
+    for (int r = 1; r < S; ++r) a.join(sm.part[r]);
+    if (k > 0) {
+      lp_rank(&sm.all[0][0], S * k, k, sm.top);
+      __syncthreads();
+    }
+  }
+  const float ls = logf(a.s);
+  if (tid < k) {
+    const LpKey q = sm.top[tid];
+    ids[row * k + tid] = (long long)(uint32_t)~(uint32_t)q;
+    top[row * k + tid] = lp_value((uint32_t)(q >> 32)) - a.m - ls;
+  }
+  if (tid == 0) {
+    const float h = ls - a.t / a.s;
+    given[row] = tk >= 0 && tk < V ? zt - a.m - ls : 0.f;
+    entropy[row] = h;
+    if (stats) stats[row] = make_float4(a.m, ls, h, 0.f);
+  }
+}
+
+// One CTA for LP_U vectors a thread of a row.
 template <class Z>
 __global__ void __launch_bounds__(LP_T) logprobs_bwd_kernel(const Z* __restrict__ logits, long long ldl, int V, int cols, const long long* __restrict__ tokens,
                                                             int k, const long long* __restrict__ ids, const float4* __restrict__ stats,
                                                             const float* __restrict__ g_given, const float* __restrict__ g_entropy,
-                                                            const float* __restrict__ g_top, Z* __restrict__ dz, long long ldd) {
-  const long long row = blockIdx.x;
+                                                            const float* __restrict__ g_top, Z* __restrict__ dz, long long ldd, int chunks) {
+  constexpr int VE = 16 / sizeof(Z), CHUNK = LP_T * LP_U * VE;
+  const long long row = blockIdx.x / chunks;
+  const int chunk = (int)(blockIdx.x - row * chunks), tid = threadIdx.x;
   const Z* z = logits + row * ldl;
   Z* d = dz + row * ldd;
+  // vectors where rows of both begin alike, single columns where not, and before and behind the vectors
+  const int mis = (int)((uintptr_t)d & 15), head = min(cols, (16 - mis & 15) / (int)sizeof(Z));
+  const bool alike = (int)((uintptr_t)z & 15) == mis;
+  // columns of this CTA
+  const int c0 = chunk == 0 ? 0 : head + chunk * CHUNK, c1 = min(cols, head + (chunk + 1) * CHUNK);
+  if (c0 >= cols) return;
+  const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+  const int vb = head + chunk * CHUNK;
+  uint4 u[LP_U];
+  if (alike) {
+#pragma unroll
+    for (int j = 0; j < LP_U; ++j) {
+      const int c = vb + (tid + j * LP_T) * VE;
+      u[j] = c + VE <= cols && c < V ? lp_stream(z + c) : none;
+    }
+  }
   const float4 st = stats[row];
   const long long tk = tokens[row];
   const bool some = tk >= 0 && tk < V;
   const float g = g_given && some ? g_given[row] : 0.f, gh = g_entropy ? g_entropy[row] : 0.f;
   float pull = g;
-  if (g_top)
-    for (int j = 0; j < k; ++j) pull += g_top[row * k + j];
-  // nothing depends on this row: its gradient is 0 whatever the row holds
-  bool idle = g == 0.f && gh == 0.f;
-  if (g_top)
-    for (int j = 0; j < k; ++j) idle &= g_top[row * k + j] == 0.f;
-  if (idle) {
-    for (int c = threadIdx.x; c < cols; c += LP_T) lp_store(d + c, 0.f);
-    return;
+  bool idle = g == 0.f && gh == 0.f;            // nothing depends on this row: its gradient is 0 whatever the row holds
+  if (g_top) {
+    for (int j = 0; j < k; ++j) {
+      const float x = g_top[row * k + j];
+      pull += x;
+      idle &= x == 0.f;
+    }
   }
-  auto grad = [&](int c) {
-    const float lp = lp_load(z + c) - st.x - st.y;
-    return -expf(lp) * (pull + gh * (fmaxf(lp, -1000.f) + st.z));
+  // -p (pull + gh (log p + H)) with l = log2 p
+  const float off = -st.y * kLog2e, ca = pull + gh * st.z, cb = gh * kLn2;
+  auto grad = [&](float x) {
+    const float l = fmaf(x - st.x, kLog2e, off);
+    return -lp_exp2(l) * fmaf(cb, fmaxf(l, -1000.f), ca);
   };
-  for (int c = threadIdx.x; c < cols; c += LP_T) lp_store(d + c, c < V ? grad(c) : 0.f);
+  if (alike) {
+#pragma unroll
+    for (int j = 0; j < LP_U; ++j) {
+      const int c = vb + (tid + j * LP_T) * VE;
+      if (c + VE > cols) continue;
+      float f[VE];
+      lp_unpack(u[j], f);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) f[e] = c + e < V && !idle ? grad(f[e]) : 0.f;
+      *reinterpret_cast<uint4*>(d + c) = lp_pack(f);
+    }
+    const int full = head + (cols - head) / VE * VE;
+    auto one = [&](int c) { lp_store(d + c, c < V && !idle ? grad(lp_load(z + c)) : 0.f); };
+    if (chunk == 0 && tid < head) one(tid);
+    if (c1 == cols && tid < cols - full) one(full + tid);
+  } else {
+    for (int c = c0 + tid; c < c1; c += LP_T) lp_store(d + c, c < V && !idle ? grad(lp_load(z + c)) : 0.f);
+  }
+  if (idle) return;
   __syncthreads();
-  if ((int)threadIdx.x <= k) {
-    const bool own = (int)threadIdx.x == k;
-    if (own ? some : g_top != nullptr) {
-      const int c = (int)(own ? tk : ids[row * k + threadIdx.x]);
-      float v = grad(c);
+  if (tid <= k && (tid == k ? some : g_top != nullptr)) {
+    const long long c = tid == k ? tk : ids[row * k + tid];
+    if (c >= c0 && c < c1) {
+      float v = grad(lp_load(z + c));
       if (some && c == tk) v += g;
       if (g_top)
         for (int j = 0; j < k; ++j)
@@ -130,37 +370,62 @@ __global__ void __launch_bounds__(LP_T) logprobs_bwd_kernel(const Z* __restrict_
   }
 }
 
+// CTAs of a cluster that share a row: doubled until there are two for each SM, as long as every thread keeps a round of vectors.
+inline int lp_splits(long long rows, int V, int per, int sms) {
+  int s = 1;
+  while (s < LP_SPLIT && rows * s < 2 * sms && V >= 2 * s * LP_T * per) s *= 2;
+  return s;
+}
+
+template <class Z>
+int launch_logprobs_fwd(const void* logits, long long ldl, long long rows, int V, const long long* tokens, int k, float* given, float* entropy, float* top,
+                        long long* ids, void* stats, cudaStream_t s) {
+  static OncePerDevice once;
+  BONES_ONCE(once, BONES_CHECK(cudaFuncSetAttribute(logprobs_fwd_kernel<Z>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)););
+  int dev = 0, sms = 0;
+  BONES_CHECK(cudaGetDevice(&dev));
+  BONES_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  const int split = lp_splits(rows, V, 16 / (int)sizeof(Z), sms);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[2];
+  cfg.gridDim = dim3((unsigned)(rows * split));
+  cfg.blockDim = dim3(LP_T);
+  cfg.stream = s;
+  cfg.attrs = at;
+  cfg.numAttrs = (unsigned)dec_launch_attrs(at, split, 0);
+  return (int)cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<Z>, (const Z*)logits, ldl, V, tokens, k, given, entropy, top, ids, (float4*)stats);
+}
+template <class Z>
+int launch_logprobs_bwd(const void* logits, long long ldl, long long rows, int V, int cols, const long long* tokens, int k, const long long* ids,
+                        const void* stats, const float* g_given, const float* g_entropy, const float* g_top, void* dz, long long ldd, cudaStream_t s) {
+  const int chunk = LP_T * LP_U * (16 / (int)sizeof(Z)), chunks = (cols + chunk - 1) / chunk;
+  if (rows * chunks > 0x7fffffffll) return -2;
+  logprobs_bwd_kernel<Z><<<(unsigned)(rows * chunks), LP_T, 0, s>>>((const Z*)logits, ldl, V, cols, tokens, k, ids, (const float4*)stats, g_given, g_entropy,
+                                                                    g_top, (Z*)dz, ldd, chunks);
+  return (int)cudaGetLastError();
+}
+
 }  // namespace bones
 
 extern "C" {
 using namespace bones;
 
-// logits: rows of bf16 (fp32: `wide`), ldl values apart; the first V columns are the vocabulary.  top, ids: [rows, k], k <= 32 and <= V.
+// logits: rows of bf16 (fp32: `wide`), ldl values apart, at any multiple of their size; the first V columns are the vocabulary.
+// top, ids: [rows, k], k <= 32 and <= V; stats: [rows] float4 or null where no gradient follows
 int bones_logprobs_fwd(const void* logits, long long ldl, int wide, long long rows, int V, const long long* tokens, int k, float* given, float* entropy,
                        float* top, long long* ids, void* stats, void* stream) {
   if (rows == 0) return 0;                     // empty tensors have no address
-  if (rows < 0 || rows > 0x7fffffffll || V < 1 || k < 0 || k > LP_TOP || k > V || (k && (!top || !ids)) || ((uintptr_t)stats & 15)) return -2;
-  cudaStream_t s = (cudaStream_t)stream;
-  if (wide)
-    logprobs_fwd_kernel<float><<<(unsigned)rows, LP_T, 0, s>>>((const float*)logits, ldl, V, tokens, k, given, entropy, top, ids, (float4*)stats);
-  else
-    logprobs_fwd_kernel<__nv_bfloat16><<<(unsigned)rows, LP_T, 0, s>>>((const __nv_bfloat16*)logits, ldl, V, tokens, k, given, entropy, top, ids,
-                                                                        (float4*)stats);
-  return (int)cudaGetLastError();
+  if (rows < 0 || rows > 0x7fffffffll || V < 1 || V > (1 << 30) || k < 0 || k > LP_TOP || k > V || (k && (!top || !ids)) || ((uintptr_t)stats & 15)) return -2;
+  return wide ? launch_logprobs_fwd<float>(logits, ldl, rows, V, tokens, k, given, entropy, top, ids, stats, (cudaStream_t)stream)
+              : launch_logprobs_fwd<__nv_bfloat16>(logits, ldl, rows, V, tokens, k, given, entropy, top, ids, stats, (cudaStream_t)stream);
 }
 
 // g_given, g_entropy [rows] and g_top [rows, k]: null where there is no gradient; dz: `cols` columns, those behind the vocabulary become 0
 int bones_logprobs_bwd(const void* logits, long long ldl, int wide, long long rows, int V, int cols, const long long* tokens, int k, const long long* ids,
                        const void* stats, const float* g_given, const float* g_entropy, const float* g_top, void* dz, long long ldd, void* stream) {
   if (rows == 0) return 0;
-  if (rows < 0 || rows > 0x7fffffffll || V < 1 || cols < V || k < 0 || k > LP_TOP || (k && g_top && !ids) || !stats || ((uintptr_t)stats & 15)) return -2;
-  cudaStream_t s = (cudaStream_t)stream;
-  if (wide)
-    logprobs_bwd_kernel<float><<<(unsigned)rows, LP_T, 0, s>>>((const float*)logits, ldl, V, cols, tokens, k, ids, (const float4*)stats, g_given, g_entropy,
-                                                                g_top, (float*)dz, ldd);
-  else
-    logprobs_bwd_kernel<__nv_bfloat16><<<(unsigned)rows, LP_T, 0, s>>>((const __nv_bfloat16*)logits, ldl, V, cols, tokens, k, ids, (const float4*)stats,
-                                                                        g_given, g_entropy, g_top, (__nv_bfloat16*)dz, ldd);
-  return (int)cudaGetLastError();
+  if (rows < 0 || rows > 0x7fffffffll || V < 1 || cols < V || cols > (1 << 30) || k < 0 || k > LP_TOP || (k && g_top && !ids) || !stats || ((uintptr_t)stats & 15)) return -2;
+  return wide ? launch_logprobs_bwd<float>(logits, ldl, rows, V, cols, tokens, k, ids, stats, g_given, g_entropy, g_top, dz, ldd, (cudaStream_t)stream)
+              : launch_logprobs_bwd<__nv_bfloat16>(logits, ldl, rows, V, cols, tokens, k, ids, stats, g_given, g_entropy, g_top, dz, ldd, (cudaStream_t)stream);
 }
 }  // extern "C"
