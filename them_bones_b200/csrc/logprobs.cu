@@ -6,9 +6,9 @@
 //
 // Alternatives are ordered by their logits, equal ones by their index, a NaN before everything.
 //
-// Forward: one pass over the row.  A thread keeps a running maximum with its S and T, and where its maximum was; the alternatives come
-// out of that: among the maxima of groups of threads the k-th largest bounds the row's k-th largest from below, so only threads whose
-// maximum reaches it hold an alternative, and only their columns (a few percent of the row, still in L2) are looked at again.
+// Forward: one pass over the row.  A thread keeps a running maximum with its S and T.  The alternatives come out of that: among the maxima
+// of groups of threads the k-th largest bounds the row's k-th largest logit from below, so only threads whose maximum reaches it hold an
+// alternative, and only their columns (a few percent of the row, still in L2) are looked at again.
 // Gradient: one element-wise pass; the few columns with a gradient of their own are written once more.
 #include "decode_common.cuh"
 
@@ -58,6 +58,33 @@ __device__ __forceinline__ float lp_value(uint32_t code) {
   return code == 0xfffffffeu ? __int_as_float(0x7fc00000) : __uint_as_float((code & 0x80000000u) ? code & 0x7fffffffu : ~code);
 }
 // (logit, column) as one number: the larger comes first among alternatives; no two are equal
+// two fp32 numbers in one operation
+typedef unsigned long long LpPair;
+__device__ __forceinline__ LpPair lp_pair(float a, float b) {
+  LpPair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 lp_two(LpPair p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ LpPair lp_add2(LpPair a, LpPair b) {
+  LpPair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ LpPair lp_mul2(LpPair a, LpPair b) {
+  LpPair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ LpPair lp_fma2(LpPair a, LpPair b, LpPair c) {
+  LpPair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 typedef unsigned long long LpKey;
 __device__ __forceinline__ LpKey lp_key(float v, int c) { return (LpKey)lp_code(v) << 32 | (uint32_t)~c; }
 __device__ __forceinline__ LpKey lp_first(LpKey a, LpKey b) { return a > b ? a : b; }
@@ -86,10 +113,63 @@ struct LpSum {
   }
 };
 
+// A thread's sums over its vectors, as two sums each: the even and the odd columns.  -inf has probability 0 and no part.
+struct LpStream {
+  float m;
+  LpPair s, t;
+  __device__ __forceinline__ void raise(float n) {
+    const float d = fmaxf(m - n, -1000.f), f = lp_exp2(d * kLog2e);
+    const LpPair ff = lp_pair(f, f);
+    t = lp_mul2(ff, lp_fma2(lp_pair(d, d), s, t));
+    s = lp_mul2(ff, s);
+    m = n;
+  }
+  __device__ __forceinline__ void add(LpPair w, float w0, float w1) {                   // w = z - m, and what e^w is multiplied by for T
+    const float2 x = lp_two(lp_mul2(w, lp_pair(kLog2e, kLog2e)));
+    const LpPair e = lp_pair(lp_exp2(x.x), lp_exp2(x.y));
+    s = lp_add2(s, e);
+    t = lp_fma2(e, lp_pair(w0, w1), t);
+  }
+  __device__ __forceinline__ LpSum sum() const {
+    const float2 a = lp_two(s), b = lp_two(t);
+    return LpSum{m, a.x + a.y, b.x + b.y};
+  }
+};
+__device__ __forceinline__ float lp_most(const uint4& u, float) {
+  return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+}
+__device__ __forceinline__ float lp_most(const uint4& u, __nv_bfloat16) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+  const float2 f = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+  return fmaxf(f.x, f.y);
+}
+__device__ __forceinline__ void lp_consume(LpStream& a, const uint4& u, float) {
+  const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const LpPair w = lp_add2(lp_pair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), lp_pair(-a.m, -a.m));
+    const float2 f = lp_two(w);
+    a.add(w, fmaxf(f.x, -1000.f), fmaxf(f.y, -1000.f));
+  }
+}
+// bf16: no logit below -1e30 counts for more than that, in pairs before they are unpacked (rows of nothing larger are gone over again)
+__device__ __forceinline__ void lp_consume(LpStream& a, const uint4& u, __nv_bfloat16) {
+  const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t v;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(v) : "r"(x[i]), "r"(0xf14af14au));           // -1.0e30
+    const LpPair w = lp_add2(lp_pair(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)), lp_pair(-a.m, -a.m));
+    const float2 f = lp_two(w);
+    a.add(w, f.x, f.y);
+  }
+}
+
 struct LpShared {
-  LpKey group[LP_GROUPS], cand[LP_CAND], top[LP_TOP], bound, all[LP_SPLIT][LP_TOP];
+  LpKey cand[LP_CAND], top[LP_TOP], all[LP_SPLIT][LP_TOP], red[LP_T / 32];
+  float group[LP_GROUPS], bound;
   LpSum warp[LP_T / 32], part[LP_SPLIT];
-  int n_cand, n_hold;
+  int n_cand, n_hold, base;
   unsigned short hold[LP_T];
 };
 
@@ -98,9 +178,9 @@ __device__ __forceinline__ void lp_rank(const LpKey* keys, int n, int k, LpKey* 
   for (int i = threadIdx.x; i < n; i += LP_T) {
     const LpKey mine = keys[i];
     int r = 0;
-#pragma unroll 4
+#pragma unroll 8
     for (int j = 0; j < n; ++j) r += keys[j] > mine;
-    if (mine && r < k) out[r] = mine;
+    if (r < k) out[r] = mine;
   }
 }
 
@@ -125,136 +205,152 @@ __global__ void __launch_bounds__(LP_T, 4) logprobs_fwd_kernel(const Z* __restri
   auto single = [&](int i) { return i < head ? i : V - rest + (i - head); };             // column of single i
   const int singles = rank == 0 ? head + rest : 0;
 
-  LpSum a{-3.402823466e38f, 0.f, 0.f};
-  float best = -INFINITY;                       // of the vectors, and the round of them in which it came
-  int at = 0;
-  bool held = tid < vecs;
-  for (int i = tid, it = 0; i < vecs; i += LP_U * LP_T, ++it) {
-    uint4 u[LP_U];
+  LpSum a;
+  float best = -INFINITY;                       // of the thread's vectors
+  {
+    LpStream w{sizeof(Z) == 2 ? __uint_as_float(0xf14a0000u) : -3.402823466e38f, 0ull, 0ull};
+    for (int i = tid; i < vecs; i += LP_U * LP_T) {
+      uint4 u[LP_U];
 #pragma unroll
-    for (int j = 0; j < LP_U; ++j)
-      if (i + j * LP_T < vecs) u[j] = lp_stream(body + i + j * LP_T);
-    float f[LP_U][VE], n = -INFINITY;
+      for (int j = 0; j < LP_U; ++j)
+        if (i + j * LP_T < vecs) u[j] = lp_stream(body + i + j * LP_T);
+      float n = best;
 #pragma unroll
-    for (int j = 0; j < LP_U; ++j) {
-      lp_unpack(u[j], f[j]);
-      if (i + j * LP_T >= vecs) {
-#pragma unroll
-        for (int e = 0; e < VE; ++e) f[j][e] = -INFINITY;
-      }
-#pragma unroll
-      for (int e = 0; e < VE; ++e) n = fmaxf(n, f[j][e]);
-    }
-    if (n > best) {
+      for (int j = 0; j < LP_U; ++j)
+        if (i + j * LP_T < vecs) n = fmaxf(n, lp_most(u[j], Z()));
       best = n;
-      at = it;
-      if (n > a.m) a.raise(n);                  // (not for the lowest number)
+      if (n > w.m) w.raise(n);
+#pragma unroll
+      for (int j = 0; j < LP_U; ++j)
+        if (i + j * LP_T < vecs) lp_consume(w, u[j], Z());
     }
+    a = w.sum();
+    if (sizeof(Z) == 2 && best < -1e29f) {      // nothing but what `lp_consume` took for -1e30
+      a = LpSum{-3.402823466e38f, 0.f, 0.f};
+      if (best > a.m) a.m = best;
+      for (int i = tid; i < vecs; i += LP_T) {
+        float f[VE];
+        lp_unpack(lp_stream(body + i), f);
 #pragma unroll
-    for (int j = 0; j < LP_U; ++j)
-#pragma unroll
-      for (int e = 0; e < VE; ++e) a.add(f[j][e]);
-  }
-  // a thread's own first column of its largest logit
-  LpKey mine = 0;
-  if (k > 0 && held) {
-    for (int j = 0; j < LP_U; ++j) {
-      const int i = tid + (at * LP_U + j) * LP_T;
-      if (i >= vecs) break;
-      float f[VE];
-      lp_unpack(lp_stream(body + i), f);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) mine = lp_first(mine, lp_key(f[e], col0 + i * VE + e));
+        for (int e = 0; e < VE; ++e) a.add(f[e]);
+      }
     }
   }
   if (tid < singles) {
-    const int c = single(tid);
-    const float v = lp_load(z + c);
+    const float v = lp_load(z + single(tid));
     if (v > a.m) a.raise(v);
     a.add(v);
-    mine = lp_first(mine, lp_key(v, c));
   }
-  // the CTA's sums
+  // the CTA's sums, and the maxima of four threads each
   {
     LpSum w = a;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) w.join(LpSum{__shfl_xor_sync(0xffffffffu, w.m, o), __shfl_xor_sync(0xffffffffu, w.s, o), __shfl_xor_sync(0xffffffffu, w.t, o)});
     if (lane == 0) sm.warp[warp] = w;
-  }
-  if (k > 0) {
-    LpKey gr = mine;
-    gr = lp_first(gr, __shfl_xor_sync(0xffffffffu, gr, 1));
-    gr = lp_first(gr, __shfl_xor_sync(0xffffffffu, gr, 2));
-    if ((lane & 3) == 0) sm.group[tid >> 2] = gr;
+    if (k > 0) {
+      float g = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
+      g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 2));
+      if ((lane & 3) == 0) sm.group[tid >> 2] = g;
+    }
   }
   __syncthreads();
   a = sm.warp[0];
 #pragma unroll
   for (int w = 1; w < LP_T / 32; ++w) a.join(sm.warp[w]);
   if (k > 0) {
-    // the bound: the k-th largest of the groups' maxima, any logit where there are not so many
-    if (tid < LP_TOP) sm.top[tid] = 0;
-    if (tid == 0) sm.bound = 1;
-    __syncthreads();
+    bool one_by_one = a.s != a.s;               // a NaN comes first, and no maximum saw it
     if (tid < LP_GROUPS) {
-      const LpKey g = sm.group[tid];
+      const float g = sm.group[tid];
       int r = 0;
-#pragma unroll 8
-      for (int j = 0; j < LP_GROUPS; ++j) r += sm.group[j] > g;
-      if (g && r == k - 1) sm.bound = g;
+#pragma unroll 16
+      for (int j = 0; j < LP_GROUPS; ++j) r += sm.group[j] > g || (sm.group[j] == g && j < tid);
+      if (r == k - 1) sm.bound = g;
+    } else if (tid < LP_GROUPS + LP_TOP) {
+      sm.top[tid - LP_GROUPS] = 0;
     }
     __syncthreads();
-    const LpKey bound = sm.bound;
-    bool full = a.s != a.s;                     // a NaN comes first, and no maximum saw it
-    if (!full) {
-      if (mine >= bound && held) sm.hold[atomicAdd(&sm.n_hold, 1)] = (unsigned short)tid;
-      auto keep = [&](LpKey q) {
-        if (q >= bound) {
+    const float bound = sm.bound;
+    const int turns = (vecs + LP_T - 1) / LP_T;
+    // columns from `bound` on (or above it), of the threads that have one
+    auto collect = [&](bool above) {
+      auto keep = [&](float v, int c) {
+        if (above ? v > bound : v >= bound) {
           const int n = atomicAdd(&sm.n_cand, 1);
-          if (n < LP_CAND) sm.cand[n] = q;
+          if (n < LP_CAND) sm.cand[n] = lp_key(v, c);
         }
       };
-      if (tid < singles) keep(lp_key(lp_load(z + single(tid)), single(tid)));
-      __syncthreads();
-      const int turns = (vecs + LP_T - 1) / LP_T, all = sm.n_hold * turns;
+      if (tid < singles) keep(lp_load(z + single(tid)), single(tid));
+      const int all = sm.n_hold * turns;
       for (int i = tid; i < all; i += LP_T) {
         const int h = i / turns, v = sm.hold[h] + (i - h * turns) * LP_T;
         if (v >= vecs) continue;
         float f[VE];
         lp_unpack(lp_stream(body + v), f);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) keep(lp_key(f[e], col0 + v * VE + e));
+        for (int e = 0; e < VE; ++e) keep(f[e], col0 + v * VE + e);
       }
       __syncthreads();
-      full = sm.n_cand > LP_CAND;
-      if (!full) lp_rank(sm.cand, sm.n_cand, k, sm.top);
+    };
+    if (!one_by_one) {
+      if (tid < vecs && best >= bound) sm.hold[atomicAdd(&sm.n_hold, 1)] = (unsigned short)tid;
+      __syncthreads();
+      collect(false);
+      int n = sm.n_cand;
+      if (n > LP_CAND) {                        // many equal ones: those above the bound, then the first ones that are equal to it
+        __syncthreads();
+        if (tid == 0) sm.n_cand = 0;
+        __syncthreads();
+        collect(true);
+        n = sm.n_cand;
+        int need = max(k - n, 0);
+        one_by_one = n > LP_CAND - LP_TOP;
+        if (!one_by_one) {
+          auto first = [&](int c, float v, bool here) {        // one column a thread, columns ascending
+            const unsigned who = __ballot_sync(0xffffffffu, here && v == bound);
+            if (lane == 0) sm.red[warp] = __popc(who);
+            __syncthreads();
+            int before = __popc(who & ((1u << lane) - 1u)), total = 0;
+            for (int w = 0; w < LP_T / 32; ++w) {
+              before += w < warp ? (int)sm.red[w] : 0;
+              total += (int)sm.red[w];
+            }
+            if (here && v == bound && before < need) sm.cand[n + before] = lp_key(v, c);
+            n += min(total, need);
+            need -= min(total, need);
+            __syncthreads();
+          };
+          const int lowest = rank == 0 ? 0 : col0, highest = rank == 0 && S == 1 ? V : col0 + vecs * VE;
+          for (int c = lowest; c < highest && need > 0; c += LP_T) first(c + tid, c + tid < highest ? lp_load(z + c + tid) : 0.f, c + tid < highest);
+          if (rank == 0 && S > 1)
+            for (int c = V - rest; c < V && need > 0; c += LP_T) first(c + tid, c + tid < V ? lp_load(z + c + tid) : 0.f, c + tid < V);
+        }
+      }
+      if (!one_by_one) lp_rank(sm.cand, n, k, sm.top);
     }
-    if (full) {
+    if (one_by_one) {
       LpKey last = ~0ull;
       for (int j = 0; j < k; ++j) {
-        LpKey best = 0;
+        LpKey most = 0;
+        auto look = [&](float v, int c) {
+          const LpKey q = lp_key(v, c);
+          if (q < last && q > most) most = q;
+        };
         for (int i = tid; i < vecs; i += LP_T) {
           float f[VE];
           lp_unpack(lp_stream(body + i), f);
 #pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            const LpKey q = lp_key(f[e], col0 + i * VE + e);
-            if (q < last && q > best) best = q;
-          }
+          for (int e = 0; e < VE; ++e) look(f[e], col0 + i * VE + e);
         }
-        if (tid < singles) {
-          const LpKey q = lp_key(lp_load(z + single(tid)), single(tid));
-          if (q < last && q > best) best = q;
-        }
+        if (tid < singles) look(lp_load(z + single(tid)), single(tid));
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) best = lp_first(best, __shfl_xor_sync(0xffffffffu, best, o));
+        for (int o = 16; o > 0; o >>= 1) most = lp_first(most, __shfl_xor_sync(0xffffffffu, most, o));
         __syncthreads();
-        if (lane == 0) sm.group[warp] = best;
+        if (lane == 0) sm.red[warp] = most;
         __syncthreads();
-        best = sm.group[0];
-        for (int w = 1; w < LP_T / 32; ++w) best = lp_first(best, sm.group[w]);
-        last = best;
-        if (tid == 0) sm.top[j] = best;
+        most = sm.red[0];
+        for (int w = 1; w < LP_T / 32; ++w) most = lp_first(most, sm.red[w]);
+        last = most;
+        if (tid == 0) sm.top[j] = most;
       }
     }
     __syncthreads();
@@ -267,15 +363,27 @@ __global__ void __launch_bounds__(LP_T, 4) logprobs_fwd_kernel(const Z* __restri
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(a.s) : "memory");
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(a.t) : "memory");
     }
-    if (tid < k) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(map_to_rank(smem_u32(&sm.all[0][0] + rank * k + tid), 0)), "l"(sm.top[tid]) : "memory");
+    if (tid < k) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(map_to_rank(smem_u32(&sm.all[rank][tid]), 0)), "l"(sm.top[tid]) : "memory");
     cluster_barrier();
     if (rank != 0) return;
     a = sm.part[0];
     for (int r = 1; r < S; ++r) a.join(sm.part[r]);
-    if (k > 0) {
-      lp_rank(&sm.all[0][0], S * k, k, sm.top);
-      __syncthreads();
+    // every CTA's descend: a key's place is the sum of its places in all of them
+    for (int i = tid; i < S * k; i += LP_T) {
+      const LpKey mine = sm.all[i / k][i % k];
+      int place = 0;
+#pragma unroll 4
+      for (int r = 0; r < S; ++r) {
+        int lo = 0;                             // larger keys in list r: found by halving
+#pragma unroll
+        for (int w = LP_TOP / 2; w > 0; w >>= 1)
+          if (lo + w <= k && sm.all[r][lo + w - 1] > mine) lo += w;
+        if (lo < k && sm.all[r][lo] > mine) ++lo;
+        place += lo;
+      }
+      if (mine && place < k) sm.top[place] = mine;
     }
+    __syncthreads();
   }
   const float ls = logf(a.s);
   if (tid < k) {
