@@ -14,10 +14,11 @@
 
 namespace bones {
 
-constexpr int LP_T = 256;
+constexpr int LP_T = 128;                        // threads of a CTA
 constexpr int LP_U = 4;                         // 16-byte vectors of a thread in flight
 constexpr int LP_TOP = 32;                      // alternatives at most
-constexpr int LP_GROUPS = LP_T / 4;             // of threads, whose maxima give the bound: two for each alternative at most
+constexpr int LP_GROUPS = 64;                   // of threads, whose maxima give the bound: two for each alternative at most
+constexpr int LP_BT = 256;                       // threads of the gradient's CTAs
 constexpr int LP_CAND = 1024;                   // columns kept for the final choice; a row that needs more is gone over once for each alternative
 constexpr int LP_SPLIT = 16;                    // CTAs of a cluster, one row
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -58,33 +59,6 @@ __device__ __forceinline__ float lp_value(uint32_t code) {
   return code == 0xfffffffeu ? __int_as_float(0x7fc00000) : __uint_as_float((code & 0x80000000u) ? code & 0x7fffffffu : ~code);
 }
 // (logit, column) as one number: the larger comes first among alternatives; no two are equal
-// two fp32 numbers in one operation
-typedef unsigned long long LpPair;
-__device__ __forceinline__ LpPair lp_pair(float a, float b) {
-  LpPair r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 lp_two(LpPair p) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
-  return r;
-}
-__device__ __forceinline__ LpPair lp_add2(LpPair a, LpPair b) {
-  LpPair r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ LpPair lp_mul2(LpPair a, LpPair b) {
-  LpPair r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ LpPair lp_fma2(LpPair a, LpPair b, LpPair c) {
-  LpPair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 typedef unsigned long long LpKey;
 __device__ __forceinline__ LpKey lp_key(float v, int c) { return (LpKey)lp_code(v) << 32 | (uint32_t)~c; }
 __device__ __forceinline__ LpKey lp_first(LpKey a, LpKey b) { return a > b ? a : b; }
@@ -113,26 +87,28 @@ struct LpSum {
   }
 };
 
-// A thread's sums over its vectors, as two sums each: the even and the odd columns.  -inf has probability 0 and no part.
+// A thread's sums over its vectors, relative to 2^m2, m2 = m log2 e rounded: one operation between a logit and its exponent.  Good for
+// rows whose maximum is between -1e29 and 1e38 (`kLpFloor`, the maximum to begin with, is below); a thread that finds none goes over its
+// vectors again.  T is in units of log2.
+constexpr float kLpFloor = -1.578125f * 633825300114114700748351602688.0f;      // -1.0e30, the bf16 0xf14a
 struct LpStream {
-  float m;
-  LpPair s, t;
+  float m, m2, s, t;
+  __device__ __forceinline__ LpStream() : m(kLpFloor), m2(kLpFloor * kLog2e), s(0.f), t(0.f) {}
   __device__ __forceinline__ void raise(float n) {
-    const float d = fmaxf(m - n, -1000.f), f = lp_exp2(d * kLog2e);
-    const LpPair ff = lp_pair(f, f);
-    t = lp_mul2(ff, lp_fma2(lp_pair(d, d), s, t));
-    s = lp_mul2(ff, s);
+    const float n2 = n * kLog2e, d = fmaxf(m2 - n2, -1000.f), f = lp_exp2(d);
+    t = f * fmaf(d, s, t);
+    s *= f;
     m = n;
+    m2 = n2;
   }
-  __device__ __forceinline__ void add(LpPair w, float w0, float w1) {                   // w = z - m, and what e^w is multiplied by for T
-    const float2 x = lp_two(lp_mul2(w, lp_pair(kLog2e, kLog2e)));
-    const LpPair e = lp_pair(lp_exp2(x.x), lp_exp2(x.y));
-    s = lp_add2(s, e);
-    t = lp_fma2(e, lp_pair(w0, w1), t);
+  __device__ __forceinline__ void add(float w) {               // w = z log2 e - m2, finite
+    const float e = lp_exp2(w);
+    s += e;
+    t = fmaf(e, w, t);
   }
-  __device__ __forceinline__ LpSum sum() const {
-    const float2 a = lp_two(s), b = lp_two(t);
-    return LpSum{m, a.x + a.y, b.x + b.y};
+  __device__ __forceinline__ LpSum sum() const {               // relative to e^m: what the rounding of m2 moved goes back
+    const float r = fmaf(m, kLog2e, -m2), f = lp_exp2(-r);
+    return LpSum{m, f * s, f * kLn2 * fmaf(-r, s, t)};
   }
 };
 __device__ __forceinline__ float lp_most(const uint4& u, float) {
@@ -144,24 +120,23 @@ __device__ __forceinline__ float lp_most(const uint4& u, __nv_bfloat16) {
   return fmaxf(f.x, f.y);
 }
 __device__ __forceinline__ void lp_consume(LpStream& a, const uint4& u, float) {
-  const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+  float f[4];
+  lp_unpack(u, f);
 #pragma unroll
-  for (int i = 0; i < 4; i += 2) {
-    const LpPair w = lp_add2(lp_pair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), lp_pair(-a.m, -a.m));
-    const float2 f = lp_two(w);
-    a.add(w, fmaxf(f.x, -1000.f), fmaxf(f.y, -1000.f));
+  for (int i = 0; i < 4; ++i) {
+    float w;                                    // -inf has probability 0 and no part; a NaN stays one
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(w) : "f"(fmaf(f[i], kLog2e, -a.m2)), "f"(-1000.f));
+    a.add(w);
   }
 }
-// bf16: no logit below -1e30 counts for more than that, in pairs before they are unpacked (rows of nothing larger are gone over again)
 __device__ __forceinline__ void lp_consume(LpStream& a, const uint4& u, __nv_bfloat16) {
   const uint32_t x[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t v;
-    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(v) : "r"(x[i]), "r"(0xf14af14au));           // -1.0e30
-    const LpPair w = lp_add2(lp_pair(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)), lp_pair(-a.m, -a.m));
-    const float2 f = lp_two(w);
-    a.add(w, f.x, f.y);
+    uint32_t v;                                 // the same by twos, before they are unpacked
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(v) : "r"(x[i]), "r"(0xf14af14au));
+    a.add(fmaf(__uint_as_float(v << 16), kLog2e, -a.m2));
+    a.add(fmaf(__uint_as_float(v & 0xffff0000u), kLog2e, -a.m2));
   }
 }
 
@@ -169,8 +144,9 @@ struct LpShared {
   LpKey cand[LP_CAND], top[LP_TOP], all[LP_SPLIT][LP_TOP], red[LP_T / 32];
   float group[LP_GROUPS], bound;
   LpSum warp[LP_T / 32], part[LP_SPLIT];
-  int n_cand, n_hold, base;
-  unsigned short hold[LP_T];
+  int n_cand, n_round, n_hold;
+  int round[LP_T];                                 // thread | round << 8: columns of one round of a thread's
+  unsigned short hold[LP_T];                       // threads of which all columns are looked at
 };
 
 // Places among n keys: key i with fewer than k larger ones goes to out[that number].
@@ -187,7 +163,7 @@ __device__ __forceinline__ void lp_rank(const LpKey* keys, int n, int k, LpKey* 
 // Row r of a cluster: the columns of this CTA are `vecs` 16-byte vectors from `body` on (column `col0`), and in the first CTA up to
 // 2 * (VE - 1) single columns before and behind the row's vectors.
 template <class Z>
-__global__ void __launch_bounds__(LP_T, 4) logprobs_fwd_kernel(const Z* __restrict__ logits, long long ldl, int V, const long long* __restrict__ tokens, int k,
+__global__ void __launch_bounds__(LP_T, 10) logprobs_fwd_kernel(const Z* __restrict__ logits, long long ldl, int V, const long long* __restrict__ tokens, int k,
                                                                float* __restrict__ given, float* __restrict__ entropy, float* __restrict__ top,
                                                                long long* __restrict__ ids, float4* __restrict__ stats) {
   constexpr int VE = 16 / sizeof(Z);
@@ -198,7 +174,7 @@ __global__ void __launch_bounds__(LP_T, 4) logprobs_fwd_kernel(const Z* __restri
   const Z* z = logits + row * ldl;
   const long long tk = rank == 0 && tid == 0 ? tokens[row] : -1;
   const float zt = tk >= 0 && tk < V ? lp_load(z + tk) : 0.f;
-  if (tid == 0) sm.n_cand = sm.n_hold = 0;
+  if (tid == 0) sm.n_cand = sm.n_round = sm.n_hold = 0;
   const int head = min(V, (int)((16 - ((uintptr_t)z & 15)) & 15) / (int)sizeof(Z)), nv = (V - head) / VE, rest = V - head - nv * VE;
   const int v0 = (int)((long long)nv * rank / S), vecs = (int)((long long)nv * (rank + 1) / S) - v0, col0 = head + v0 * VE;
   const uint4* body = reinterpret_cast<const uint4*>(z + col0);
@@ -206,26 +182,31 @@ __global__ void __launch_bounds__(LP_T, 4) logprobs_fwd_kernel(const Z* __restri
   const int singles = rank == 0 ? head + rest : 0;
 
   LpSum a;
-  float best = -INFINITY;                       // of the thread's vectors
+  float best = -INFINITY, second = -INFINITY;   // of the thread's rounds of vectors
+  int at = 0;                                   // the best one
   {
-    LpStream w{sizeof(Z) == 2 ? __uint_as_float(0xf14a0000u) : -3.402823466e38f, 0ull, 0ull};
-    for (int i = tid; i < vecs; i += LP_U * LP_T) {
+    LpStream w;
+    for (int i = tid, it = 0; i < vecs; i += LP_U * LP_T, ++it) {
       uint4 u[LP_U];
 #pragma unroll
       for (int j = 0; j < LP_U; ++j)
         if (i + j * LP_T < vecs) u[j] = lp_stream(body + i + j * LP_T);
-      float n = best;
+      float n = -INFINITY;
 #pragma unroll
       for (int j = 0; j < LP_U; ++j)
         if (i + j * LP_T < vecs) n = fmaxf(n, lp_most(u[j], Z()));
-      best = n;
-      if (n > w.m) w.raise(n);
+      second = fmaxf(second, fminf(best, n));
+      if (n > best) {
+        best = n;
+        at = it;
+        if (n > w.m) w.raise(n);
+      }
 #pragma unroll
       for (int j = 0; j < LP_U; ++j)
         if (i + j * LP_T < vecs) lp_consume(w, u[j], Z());
     }
     a = w.sum();
-    if (sizeof(Z) == 2 && best < -1e29f) {      // nothing but what `lp_consume` took for -1e30
+    if (!(best > -1e29f && best < 1e38f)) {
       a = LpSum{-3.402823466e38f, 0.f, 0.f};
       if (best > a.m) a.m = best;
       for (int i = tid; i < vecs; i += LP_T) {
@@ -241,16 +222,18 @@ __global__ void __launch_bounds__(LP_T, 4) logprobs_fwd_kernel(const Z* __restri
     if (v > a.m) a.raise(v);
     a.add(v);
   }
-  // the CTA's sums, and the maxima of four threads each
+  // the CTA's sums, and the maxima of groups
   {
     LpSum w = a;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) w.join(LpSum{__shfl_xor_sync(0xffffffffu, w.m, o), __shfl_xor_sync(0xffffffffu, w.s, o), __shfl_xor_sync(0xffffffffu, w.t, o)});
     if (lane == 0) sm.warp[warp] = w;
     if (k > 0) {
-      float g = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
-      g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 2));
-      if ((lane & 3) == 0) sm.group[tid >> 2] = g;
+      constexpr int PER = LP_T / LP_GROUPS;
+      float g = best;
+#pragma unroll
+      for (int o = 1; o < PER; o *= 2) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+      if ((lane & (PER - 1)) == 0) sm.group[tid / PER] = g;
     }
   }
   __syncthreads();
@@ -280,19 +263,24 @@ __global__ void __launch_bounds__(LP_T, 4) logprobs_fwd_kernel(const Z* __restri
         }
       };
       if (tid < singles) keep(lp_load(z + single(tid)), single(tid));
-      const int all = sm.n_hold * turns;
-      for (int i = tid; i < all; i += LP_T) {
-        const int h = i / turns, v = sm.hold[h] + (i - h * turns) * LP_T;
-        if (v >= vecs) continue;
+      auto vector = [&](int v) {
+        if (v >= vecs) return;
         float f[VE];
         lp_unpack(lp_stream(body + v), f);
 #pragma unroll
         for (int e = 0; e < VE; ++e) keep(f[e], col0 + v * VE + e);
+      };
+      const int rounds = sm.n_round * LP_U, all = sm.n_hold * turns;
+      for (int i = tid; i < rounds; i += LP_T) {
+        const int r = sm.round[i / LP_U];
+        vector((r & 255) + ((r >> 8) * LP_U + i % LP_U) * LP_T);
       }
+      for (int i = tid; i < all; i += LP_T) vector(sm.hold[i / turns] + i % turns * LP_T);
       __syncthreads();
     };
     if (!one_by_one) {
-      if (tid < vecs && best >= bound) sm.hold[atomicAdd(&sm.n_hold, 1)] = (unsigned short)tid;
+      if (tid < vecs && second >= bound) sm.hold[atomicAdd(&sm.n_hold, 1)] = (unsigned short)tid;
+      else if (tid < vecs && best >= bound) sm.round[atomicAdd(&sm.n_round, 1)] = tid | at << 8;
       __syncthreads();
       collect(false);
       int n = sm.n_cand;
@@ -368,22 +356,24 @@ __global__ void __launch_bounds__(LP_T, 4) logprobs_fwd_kernel(const Z* __restri
     if (rank != 0) return;
     a = sm.part[0];
     for (int r = 1; r < S; ++r) a.join(sm.part[r]);
-    // every CTA's descend: a key's place is the sum of its places in all of them
-    for (int i = tid; i < S * k; i += LP_T) {
-      const LpKey mine = sm.all[i / k][i % k];
-      int place = 0;
-#pragma unroll 4
-      for (int r = 0; r < S; ++r) {
-        int lo = 0;                             // larger keys in list r: found by halving
-#pragma unroll
-        for (int w = LP_TOP / 2; w > 0; w >>= 1)
-          if (lo + w <= k && sm.all[r][lo + w - 1] > mine) lo += w;
-        if (lo < k && sm.all[r][lo] > mine) ++lo;
-        place += lo;
+    // every CTA's descend: a lane each, the largest of their heads k times
+    if (k > 0) {
+      if (warp == 0) {
+        LpKey cur = lane < S ? sm.all[lane][0] : 0, nxt = lane < S && k > 1 ? sm.all[lane][1] : 0;
+        int i = 2;
+        for (int j = 0; j < k; ++j) {
+          const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(cur >> 32));
+          const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(cur >> 32) == hi ? (uint32_t)cur : 0u);
+          const LpKey most = (LpKey)hi << 32 | lo;
+          if (cur == most) {
+            sm.top[j] = most;
+            cur = nxt;
+            nxt = i < k ? sm.all[lane][i++] : 0;
+          }
+        }
       }
-      if (mine && place < k) sm.top[place] = mine;
+      __syncthreads();
     }
-    __syncthreads();
   }
   const float ls = logf(a.s);
   if (tid < k) {
@@ -401,11 +391,11 @@ __global__ void __launch_bounds__(LP_T, 4) logprobs_fwd_kernel(const Z* __restri
 
 // One CTA for LP_U vectors a thread of a row.
 template <class Z>
-__global__ void __launch_bounds__(LP_T) logprobs_bwd_kernel(const Z* __restrict__ logits, long long ldl, int V, int cols, const long long* __restrict__ tokens,
+__global__ void __launch_bounds__(LP_BT) logprobs_bwd_kernel(const Z* __restrict__ logits, long long ldl, int V, int cols, const long long* __restrict__ tokens,
                                                             int k, const long long* __restrict__ ids, const float4* __restrict__ stats,
                                                             const float* __restrict__ g_given, const float* __restrict__ g_entropy,
                                                             const float* __restrict__ g_top, Z* __restrict__ dz, long long ldd, int chunks) {
-  constexpr int VE = 16 / sizeof(Z), CHUNK = LP_T * LP_U * VE;
+  constexpr int VE = 16 / sizeof(Z), CHUNK = LP_BT * LP_U * VE;
   const long long row = blockIdx.x / chunks;
   const int chunk = (int)(blockIdx.x - row * chunks), tid = threadIdx.x;
   const Z* z = logits + row * ldl;
@@ -422,7 +412,7 @@ __global__ void __launch_bounds__(LP_T) logprobs_bwd_kernel(const Z* __restrict_
   if (alike) {
 #pragma unroll
     for (int j = 0; j < LP_U; ++j) {
-      const int c = vb + (tid + j * LP_T) * VE;
+      const int c = vb + (tid + j * LP_BT) * VE;
       u[j] = c + VE <= cols && c < V ? lp_stream(z + c) : none;
     }
   }
@@ -448,7 +438,7 @@ __global__ void __launch_bounds__(LP_T) logprobs_bwd_kernel(const Z* __restrict_
   if (alike) {
 #pragma unroll
     for (int j = 0; j < LP_U; ++j) {
-      const int c = vb + (tid + j * LP_T) * VE;
+      const int c = vb + (tid + j * LP_BT) * VE;
       if (c + VE > cols) continue;
       float f[VE];
       lp_unpack(u[j], f);
@@ -461,7 +451,7 @@ __global__ void __launch_bounds__(LP_T) logprobs_bwd_kernel(const Z* __restrict_
     if (chunk == 0 && tid < head) one(tid);
     if (c1 == cols && tid < cols - full) one(full + tid);
   } else {
-    for (int c = c0 + tid; c < c1; c += LP_T) lp_store(d + c, c < V && !idle ? grad(lp_load(z + c)) : 0.f);
+    for (int c = c0 + tid; c < c1; c += LP_BT) lp_store(d + c, c < V && !idle ? grad(lp_load(z + c)) : 0.f);
   }
   if (idle) return;
   __syncthreads();
@@ -478,10 +468,11 @@ __global__ void __launch_bounds__(LP_T) logprobs_bwd_kernel(const Z* __restrict_
   }
 }
 
-// CTAs of a cluster that share a row: doubled until there are two for each SM, as long as every thread keeps a round of vectors.
+// CTAs of a cluster that share a row: doubled while there are few on an SM and every thread keeps two vectors; 16 only for a few rows.
+// us, bf16 rows of 65536, 8 alternatives: 64 rows by 8 / 16 CTAs 8.6 / 10.5, 512 rows by 1 / 2 26 / 22.
 inline int lp_splits(long long rows, int V, int per, int sms) {
   int s = 1;
-  while (s < LP_SPLIT && rows * s < 2 * sms && V >= 2 * s * LP_T * per) s *= 2;
+  while (s < LP_SPLIT && rows * s < (s < 8 ? 4 : 1) * sms && V >= 2 * s * LP_T * per) s *= 2;
   return s;
 }
 
@@ -506,9 +497,9 @@ int launch_logprobs_fwd(const void* logits, long long ldl, long long rows, int V
 template <class Z>
 int launch_logprobs_bwd(const void* logits, long long ldl, long long rows, int V, int cols, const long long* tokens, int k, const long long* ids,
                         const void* stats, const float* g_given, const float* g_entropy, const float* g_top, void* dz, long long ldd, cudaStream_t s) {
-  const int chunk = LP_T * LP_U * (16 / (int)sizeof(Z)), chunks = (cols + chunk - 1) / chunk;
+  const int chunk = LP_BT * LP_U * (16 / (int)sizeof(Z)), chunks = (cols + chunk - 1) / chunk;
   if (rows * chunks > 0x7fffffffll) return -2;
-  logprobs_bwd_kernel<Z><<<(unsigned)(rows * chunks), LP_T, 0, s>>>((const Z*)logits, ldl, V, cols, tokens, k, ids, (const float4*)stats, g_given, g_entropy,
+  logprobs_bwd_kernel<Z><<<(unsigned)(rows * chunks), LP_BT, 0, s>>>((const Z*)logits, ldl, V, cols, tokens, k, ids, (const float4*)stats, g_given, g_entropy,
                                                                     g_top, (Z*)dz, ldd, chunks);
   return (int)cudaGetLastError();
 }
