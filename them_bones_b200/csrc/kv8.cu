@@ -29,70 +29,118 @@ struct PerSeq {
 __device__ __forceinline__ float kv8_inverse(float most) { return most >= kKv8Tiny ? 127.0f / most : 0.f; }
 // the scale as it is stored; `bad`: the block holds a value that is not finite
 __device__ __forceinline__ float kv8_scale(float most, bool bad) { return copysignf(most >= kKv8Tiny ? most / 127.0f : 0.f, bad ? -1.f : 1.f); }
-__device__ __forceinline__ int kv8_code(float x, float inv) {
-  if (!(fabsf(x) <= 3.402823466e38f)) return -128;
-  return max(-127, min(127, __float2int_rn(x * inv)));
+// rint(x * inv) in the low byte: 1.5 * 2^23 is added, which rounds to whole numbers, ties to even
+__device__ __forceinline__ uint32_t kv8_code(float x, float inv) { return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.0f)); }
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
-__device__ __forceinline__ float kv8_value(int code, float scale) { return code == -128 ? __int_as_float(0x7fc00000) : (float)code * fabsf(scale); }
+__device__ __forceinline__ bool is_bad(uint32_t half) { return (half & 0x7f80u) == 0x7f80u; }         // a bf16 that is not finite
+// byte i of four codes as a number: with its sign bit turned, byte u is the end of 2^23 + u
+__device__ __forceinline__ float kv8_number(uint32_t turned, int i) {
+  return __uint_as_float(__byte_perm(turned, 0x4b000000u, 0x7440 + i)) - 8388736.0f;
+}
 
+constexpr int kTurnRow = KB + 4;                // bytes of a row on its way from [64][D] to [D][64] or back: banks 8 dimensions apart are 8 apart
 struct __align__(16) QuantShared {
   float most[8];
   int bad[8];
-  int8_t turn[128][KB + 16];                    // value codes on their way to [D][64]; rows stay 16-byte aligned
+  uint8_t turn[128 * kTurnRow];
 };
 
-// A whole block by a CTA of QT threads (256 at most): 16-byte piece i of the block is token i / (D / 8), dimensions 8 (i % (D / 8)) ..; `piece(token, dim)`
-// is its address.  Key codes go out as they lie, value codes through shared memory to be transposed.
+// A block is taken in units of four tokens by eight dimensions; 32 lanes are eight by four of them, so that rows are read and written in
+// 64-byte pieces and the words of four tokens go to shared memory without conflicts.
+template <int D>
+__device__ __forceinline__ void kv8_unit(int i, int& token, int& dim) {
+  const int lane = i & 31, w = i >> 5;
+  token = 4 * (lane >> 2) + 32 * (w & 1);
+  dim = 8 * (lane & 3) + 32 * (w >> 1);
+}
+
+// A whole block by a CTA of QT threads (256 at most); `piece(token, dim)` is the address of 16 bytes of it.  Key codes go out as they lie,
+// value codes through shared memory to be transposed.
 template <int QT, int D, bool VALUES, class Piece>
 __device__ __forceinline__ void kv8_quantise_block(Piece piece, int8_t* __restrict__ out, float* __restrict__ scale, QuantShared& sm) {
-  constexpr int PER = KB * D / 8 / QT, ROW = D / 8;
+  constexpr int UNITS = 2 * D, N = (UNITS + QT - 1) / QT;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  uint4 u[PER];
+  uint4 u[N][4];
+  __nv_bfloat162 top = __nv_bfloat162{__ushort_as_bfloat16(0), __ushort_as_bfloat16(0)};
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int p = tid + i * QT;
-    u[i] = *reinterpret_cast<const uint4*>(piece(p / ROW, p % ROW * 8));
+  for (int n = 0; n < N; ++n) {
+    int t, d;
+    kv8_unit<D>(tid + n * QT, t, d);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) u[n][r] = tid + n * QT < UNITS ? *reinterpret_cast<const uint4*>(piece(t + r, d)) : make_uint4(0u, 0u, 0u, 0u);
   }
-  float most = 0.f;
-  bool bad = false;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    float f[8];
-    unpack8(u[i], f);
+  for (int n = 0; n < N; ++n)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float a = fabsf(f[j]);
-      if (a <= 3.402823466e38f) most = fmaxf(most, a);
-      else bad = true;
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t w[4] = {u[n][r].x, u[n][r].y, u[n][r].z, u[n][r].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a = w[i] & 0x7fff7fffu;
+        top = __hmax2_nan(top, *reinterpret_cast<const __nv_bfloat162*>(&a));
+      }
     }
+  float most = fmaxf(__bfloat162float(top.x), __bfloat162float(top.y));
+  const uint32_t tops = *reinterpret_cast<const uint32_t*>(&top);
+  bool bad = is_bad(tops) || is_bad(tops >> 16);
+  if (bad) {                                    // those that are not finite do not count
+    most = 0.f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float f[8];
+        unpack8(u[n][r], f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (fabsf(f[i]) <= 3.402823466e38f) most = fmaxf(most, fabsf(f[i]));
+      }
   }
   most = warp_max(most);
-  bad = __any_sync(0xffffffffu, bad);
-  if (lane == 0) { sm.most[warp] = most; sm.bad[warp] = bad; }
+  const bool any = __any_sync(0xffffffffu, bad);
+  if (lane == 0) { sm.most[warp] = most; sm.bad[warp] = any; }
   __syncthreads();
-  bad = false;
+  bool marked = false;
 #pragma unroll
-  for (int w = 0; w < QT / 32; ++w) { most = fmaxf(most, sm.most[w]); bad |= sm.bad[w] != 0; }
+  for (int w = 0; w < QT / 32; ++w) { most = fmaxf(most, sm.most[w]); marked |= sm.bad[w] != 0; }
   const float inv = kv8_inverse(most);
-  if (tid == 0) *scale = kv8_scale(most, bad);
+  if (tid == 0) *scale = kv8_scale(most, marked);
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int p = tid + i * QT, t = p / ROW, d = p % ROW * 8;
-    float f[8];
-    unpack8(u[i], f);
-    uint32_t w[2] = {0u, 0u};
+  for (int n = 0; n < N; ++n) {
+    if (tid + n * QT >= UNITS) break;
+    int t, d;
+    kv8_unit<D>(tid + n * QT, t, d);
+    uint32_t c[4][8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = kv8_code(f[j], inv);
-      if (VALUES) sm.turn[d + j][t] = (int8_t)c;
-      else w[j >> 2] |= (uint32_t)(c & 255) << (8 * (j & 3));
+    for (int r = 0; r < 4; ++r) {
+      float f[8];
+      unpack8(u[n][r], f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[r][i] = kv8_code(f[i], inv);
+      if (bad) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (!(fabsf(f[i]) <= 3.402823466e38f)) c[r][i] = 0x80u;
+      }
     }
-    if (!VALUES) *reinterpret_cast<uint2*>(out + t * D + d) = make_uint2(w[0], w[1]);
+    if (VALUES) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(sm.turn + (d + i) * kTurnRow + t) = low_bytes(c[0][i], c[1][i], c[2][i], c[3][i]);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<uint2*>(out + (t + r) * D + d) =
+            make_uint2(low_bytes(c[r][0], c[r][1], c[r][2], c[r][3]), low_bytes(c[r][4], c[r][5], c[r][6], c[r][7]));
+    }
   }
   __syncthreads();
   if (VALUES) {
-    for (int i = tid; i < D * (KB / 16); i += QT)
-      *reinterpret_cast<uint4*>(out + i * 16) = *reinterpret_cast<const uint4*>(&sm.turn[i / (KB / 16)][i % (KB / 16) * 16]);
+    for (int i = tid; i < D * 4; i += QT) {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(sm.turn + (i >> 2) * kTurnRow + (i & 3) * 16);
+      *reinterpret_cast<uint4*>(out + i * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
     __syncthreads();
   }
 }
@@ -138,36 +186,57 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(Kv8 c, const
 // One block of one head back to bf16 rows [B, length, H, D]; zeros behind the tokens held.
 template <int D>
 __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, __nv_bfloat16* __restrict__ k, __nv_bfloat16* __restrict__ v, PerSeq held_, int length, int H, int cap) {
-  __shared__ __align__(16) int8_t turn[128][KB + 16];
-  const int b = blockIdx.z, h = blockIdx.y, blk = blockIdx.x >> 1;
+  __shared__ __align__(16) uint8_t turn[D * kTurnRow];
+  const int b = blockIdx.z, h = blockIdx.y, blk = blockIdx.x >> 1, tid = threadIdx.x;
   const bool values = blockIdx.x & 1;
   const int held = max(held_[b], 0), j0 = blk * KB;
   const long long bh = (long long)b * H + h;
   __nv_bfloat16* out = (values ? v : k) + ((long long)b * length * H + h) * D;
   const bool open = blk == held / KB, some = j0 < held && j0 < cap;
   const int8_t* codes = (values ? c.v : c.k) + (bh * cap + j0) * D;
-  const float scale = some && !open ? (values ? c.vs : c.ks)[bh * (cap / KB) + blk] : 0.f;
   const __nv_bfloat16* tail = (values ? c.vt : c.kt) + bh * KB * D;
+  const float scale = some && !open ? (values ? c.vs : c.ks)[bh * (cap / KB) + blk] : 0.f, by = fabsf(scale);
   if (values && some && !open) {
-    for (int i = threadIdx.x; i < D * 4; i += 256) *reinterpret_cast<uint4*>(&turn[i / 4][i % 4 * 16]) = *reinterpret_cast<const uint4*>(codes + i * 16);
+    for (int i = tid; i < D * 4; i += 256) {
+      const uint4 u = *reinterpret_cast<const uint4*>(codes + i * 16);
+      uint32_t* w = reinterpret_cast<uint32_t*>(turn + (i >> 2) * kTurnRow + (i & 3) * 16);
+      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  for (int p = threadIdx.x; p < KB * D / 8; p += 256) {
-    const int t = p / (D / 8), d = p % (D / 8) * 8, j = j0 + t;
-    if (j >= length) continue;
+  if (tid >= 2 * D) return;
+  int t, d;
+  kv8_unit<D>(tid, t, d);
+  uint32_t w[4][2];                             // codes of four tokens by eight dimensions: by token, or four tokens to a word
+  uint32_t x[8];
+  if (some && !open) {
+    if (values) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint32_t*>(turn + (d + i) * kTurnRow + t) ^ 0x80808080u;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint2 u = *reinterpret_cast<const uint2*>(codes + (t + r) * D + d);
+        w[r][0] = u.x ^ 0x80808080u;
+        w[r][1] = u.y ^ 0x80808080u;
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int j = j0 + t + r;
+    if (j >= length) break;
     uint4 o = make_uint4(0u, 0u, 0u, 0u);
     if (some && j < held) {
       if (open) {
-        o = *reinterpret_cast<const uint4*>(tail + t * D + d);
+        o = *reinterpret_cast<const uint4*>(tail + (t + r) * D + d);
       } else {
         float f[8];
-        if (values) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = kv8_value(turn[d + e][t], scale);
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(codes + t * D + d);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = kv8_value((int)(int8_t)((e < 4 ? u.x : u.y) >> (8 * (e & 3))), scale);
+        for (int i = 0; i < 8; ++i) {
+          const float n = values ? kv8_number(x[i], r) : kv8_number(w[r][i >> 2], i & 3);
+          f[i] = n * by;
+          if (signbit(scale) && n == -128.0f) f[i] = __int_as_float(0x7fc00000);
         }
         o = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
       }

@@ -225,24 +225,21 @@ def kv8_append(cache, k, v, pos, lens=None):
     at position ``pos[b]``, which is where its last ones ended; ``pos`` and ``lens`` are ints or int32 on the device (one value or B).
     What the cache holds does not depend on the pieces it came in.  A sequence at a negative position, without tokens or with more
     than fit is left as it was."""
-    _kv8.check_append(cache, k, v, pos, lens)
+    dims = _kv8.check_append(cache, k, v, pos, lens)
     _kv8.no_gradient(k, v)
     if native(k):
-        return _kv8.append(cache, k, v, pos, lens)
-    b = k.shape[0]
+        return _kv8.append(dims, k, v, pos, lens)
+    b = dims[0]
     RF.kv8_append(cache, k, v, _kv8.numbers(pos, b), _kv8.numbers(k.shape[1] if lens is None else lens, b))
 
 
 def kv8_read(cache, held, length):
     """``(k, v) [B, length, H, D]`` in bf16: what the cache holds of each sequence's first ``length`` positions, zeros from ``held[b]`` on
     (the number of its tokens; an int or int32 on the device)."""
-    _kv8.check_cache(cache)
-    _kv8.check_per_sequence(held, cache.k.shape[0], "held", cache.k.device)
-    if length < 0 or (isinstance(held, int) and not 0 <= held <= cache.capacity):
-        raise ValueError(f"8-bit cache: {length} positions of {held} tokens, capacity {cache.capacity}")
-    if native(cache.k):
-        return _kv8.read(cache, held, length)
-    return RF.kv8_read(cache, _kv8.numbers(held, cache.k.shape[0]), length)
+    dims = _kv8.check_read(cache, held, length)
+    if native(cache[0]):
+        return _kv8.read(dims, held, length)
+    return RF.kv8_read(cache, _kv8.numbers(held, dims[0]), length)
 
 
 def kv8_attention(qkv, cos, sin, cache, pos, scale, doc_start=None, window=0):
@@ -250,12 +247,11 @@ def kv8_attention(qkv, cos, sin, cache, pos, scale, doc_start=None, window=0):
     soft-max attention over the positions from ``doc_start[b]`` (and the band of ``window`` tokens, as in ``attention``) to ``pos[b]``
     -> ``[B, H*D]``.  A sequence at a negative position, or one past the cache or the rotary tables, is left as it was and gets
     zeros; so does a query that sees no key.  No gradient."""
-    _kv8.check_attention(qkv, cos, sin, cache, pos, doc_start, window)
+    dims = _kv8.check_attention(qkv, cos, sin, cache, pos, doc_start, window)
     _kv8.no_gradient(qkv)
     if native(qkv):
-        return _kv8.attention(qkv, cos, sin, cache, pos, scale, doc_start, window)
-    b = qkv.shape[0]
-    return RF.kv8_attention(qkv, cos, sin, cache, _kv8.numbers(pos, b), scale, None if doc_start is None else doc_start.tolist(), window)
+        return _kv8.attention(qkv, cos, sin, dims, pos, scale, doc_start, window)
+    return RF.kv8_attention(qkv, cos, sin, cache, _kv8.numbers(pos, dims[0]), scale, None if doc_start is None else doc_start.tolist(), window)
 
 
 # -- output-side hashed table ------------------------------------------------------------------------------------

@@ -70,6 +70,23 @@ def raw_stream() -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+class device:
+    """``with device(index)``: CUDA calls on that device, as ``torch.cuda.device`` but without a switch where it is the current one."""
+    __slots__ = ("_to", "_back")
+
+    def __init__(self, index: int):
+        self._to = index
+
+    def __enter__(self):
+        self._back = torch._C._cuda_getDevice()
+        if self._back != self._to:
+            torch.cuda.set_device(self._to)
+
+    def __exit__(self, *_):
+        if self._back != self._to:
+            torch.cuda.set_device(self._back)
+
+
 def ptr(t):
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
 

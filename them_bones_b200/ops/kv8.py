@@ -47,60 +47,76 @@ def cache(batch: int, max_len: int, n_head: int, head_dim: int, device=None) -> 
 
 
 def check_cache(c: KV8):
+    """``(B, H, T, D, device index, addresses)`` of a cache whose tensors are what the kernels take them for."""
     if len(c) != 6 or c[0].dim() != 4:
         raise ValueError("8-bit cache: six tensors, the first [B, H, T, D]")
     b, h, t, d = c[0].shape
     nb = t // BLOCK
-    want = ((torch.int8, (b, h, t, d)), (torch.int8, (b, h, nb, d, BLOCK)), (torch.float32, (b, h, nb)), (torch.float32, (b, h, nb)),
-            (torch.bfloat16, (b, h, BLOCK, d)), (torch.bfloat16, (b, h, BLOCK, d)))
     if d not in HEAD_DIMS or t < BLOCK or t % BLOCK or t > MAX_LEN + BLOCK or not 1 <= b <= 65535 or not 1 <= h <= 65535:
         raise ValueError(f"8-bit cache: shape {tuple(c[0].shape)}")
-    for x, (dt, shape), name in zip(c, want, KV8._fields):
-        if x.dtype != dt or x.shape != shape or x.device != c[0].device or not x.is_contiguous() or x.data_ptr() % 16:
-            raise ValueError(f"8-bit cache: {name} is {x.dtype} {tuple(x.shape)} on {x.device}, expected contiguous {dt} {shape}, 16-byte aligned")
+    k, v, ks, vs, kt, vt = c
+    dev, scales, open_ = k.get_device(), (b, h, nb), (b, h, BLOCK, d)
+    at = k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), kt.data_ptr(), vt.data_ptr()
+    # one expression: a loop over the six would be a fifth of a call's host time
+    if not (k.dtype is torch.int8 and v.dtype is torch.int8 and ks.dtype is torch.float32 and vs.dtype is torch.float32 and kt.dtype is torch.bfloat16
+            and vt.dtype is torch.bfloat16 and v.shape == (b, h, nb, d, BLOCK) and ks.shape == scales and vs.shape == scales and kt.shape == open_
+            and vt.shape == open_ and v.get_device() == dev and ks.get_device() == dev and vs.get_device() == dev and kt.get_device() == dev
+            and vt.get_device() == dev and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and kt.is_contiguous()
+            and vt.is_contiguous() and (at[0] | at[1] | at[2] | at[3] | at[4] | at[5]) % 16 == 0):
+        have = ", ".join(f"{n} {x.dtype} {tuple(x.shape)}" for n, x in zip(KV8._fields, c))
+        raise ValueError(f"8-bit cache: {have}: not six contiguous tensors of one cache on one device, each on 16 bytes")
+    return b, h, t, d, dev, at
 
 
 def check_per_sequence(x, b: int, name: str, device):
-    """An int, or int32 of one value or of one for each sequence on the cache's device."""
+    """An int, or int32 of one value or of one for each sequence on the cache's device (an index, -1 for the host)."""
     if isinstance(x, int):
         return
-    if not torch.is_tensor(x) or x.dtype != torch.int32 or x.device != device or x.numel() not in (1, b) or x.dim() > 1 or not x.is_contiguous():
-        raise ValueError(f"8-bit cache: {name} is an int or contiguous int32 of 1 or {b} values on {device}")
+    if not isinstance(x, torch.Tensor) or x.dtype is not torch.int32 or x.get_device() != device or x.numel() not in (1, b) or x.dim() > 1 or not x.is_contiguous():
+        raise ValueError(f"8-bit cache: {name} is an int or contiguous int32 of 1 or {b} values on the cache's device")
 
 
 def check_append(c: KV8, k, v, pos, lens):
-    check_cache(c)
-    b, h, t, d = c.k.shape
-    if k.dim() != 4 or v.shape != k.shape or k.shape[0] != b or k.shape[2:] != (h, d):
+    dims = b, h, t, d, dev, _ = check_cache(c)
+    if k.dim() != 4 or v.shape != k.shape or k.shape[0] != b or k.shape[2] != h or k.shape[3] != d:
         raise ValueError(f"8-bit cache: keys {tuple(k.shape)}, values {tuple(v.shape)}, cache {tuple(c.k.shape)}")
-    if k.device != c.k.device or v.device != c.k.device or k.dtype != v.dtype or not k.is_floating_point():
+    if k.get_device() != dev or v.get_device() != dev or k.dtype is not v.dtype or not k.is_floating_point():
         raise ValueError("8-bit cache: keys and values of one floating type on the cache's device")
-    check_per_sequence(pos, b, "pos", c.k.device)
+    check_per_sequence(pos, b, "pos", dev)
     if lens is not None:
-        check_per_sequence(lens, b, "lens", c.k.device)
+        check_per_sequence(lens, b, "lens", dev)
     if isinstance(lens, int) and not 0 <= lens <= k.shape[1]:
         raise ValueError(f"8-bit cache: {lens} of {k.shape[1]} tokens")
     if isinstance(pos, int) and (lens is None or isinstance(lens, int)):
         n = k.shape[1] if lens is None else lens
         if pos < 0 or pos + n > t:
             raise ValueError(f"8-bit cache: {n} of {k.shape[1]} tokens at {pos} into a capacity of {t}")
+    return dims
+
+
+def check_read(c: KV8, held, length):
+    dims = check_cache(c)
+    check_per_sequence(held, dims[0], "held", dims[4])
+    if length < 0 or length > MAX_LEN or (isinstance(held, int) and not 0 <= held <= dims[2]):
+        raise ValueError(f"8-bit cache: {length} positions of {held} tokens, capacity {dims[2]}")
+    return dims
 
 
 def check_attention(qkv, cos, sin, c: KV8, pos, doc_start, window):
-    check_cache(c)
-    b, h, t, d = c.k.shape
-    if qkv.shape != (b, 3 * h * d) or qkv.device != c.k.device or not qkv.is_floating_point():
-        raise ValueError(f"8-bit attention: qkv {tuple(qkv.shape)} on {qkv.device}, expected {(b, 3 * h * d)} on {c.k.device}")
+    dims = b, h, t, d, dev, _ = check_cache(c)
+    if qkv.shape != (b, 3 * h * d) or qkv.get_device() != dev or not qkv.is_floating_point():
+        raise ValueError(f"8-bit attention: qkv {qkv.dtype} {tuple(qkv.shape)} on {qkv.device}, expected {(b, 3 * h * d)} on {c.k.device}")
     for x in (cos, sin):
-        if x.dim() != 2 or x.shape[1] != d // 2 or x.shape != cos.shape or x.device != c.k.device or not x.is_floating_point():
+        if x.dim() != 2 or x.shape[1] != d // 2 or x.shape != cos.shape or x.get_device() != dev or not x.is_floating_point():
             raise ValueError(f"8-bit attention: rotary tables {tuple(cos.shape)}, {tuple(sin.shape)}, expected [positions, {d // 2}]")
-    check_per_sequence(pos, b, "pos", c.k.device)
+    check_per_sequence(pos, b, "pos", dev)
     if isinstance(pos, int) and not 0 <= pos < min(t, cos.shape[0]):
         raise ValueError(f"8-bit attention: position {pos}, capacity {t}, rotary tables of {cos.shape[0]}")
-    if doc_start is not None and (doc_start.dtype != torch.int32 or doc_start.shape != (b,) or doc_start.device != c.k.device or not doc_start.is_contiguous()):
+    if doc_start is not None and (doc_start.dtype is not torch.int32 or doc_start.shape != (b,) or doc_start.get_device() != dev or not doc_start.is_contiguous()):
         raise ValueError(f"8-bit attention: doc_start is contiguous int32 [{b}] on {c.k.device}")
     if window < 0 or window % 128:
         raise ValueError(f"8-bit attention: window {window} is not a multiple of 128")
+    return dims
 
 
 def no_gradient(*tensors):
@@ -132,51 +148,51 @@ def _bf16(x, what):
         raise ValueError(f"native 8-bit cache does not cover this call: {what} of {x.dtype} (bf16 only)")
 
 
-def append(c: KV8, k, v, pos, lens):
+def append(dims, k, v, pos, lens):
     _bf16(k, "keys and values")
-    b, h, t, d = c.k.shape
+    b, h, t, d, dev, at = dims
     n = k.shape[1]
     if n == 0:
         return
     k, v = _rows16(k), _rows16(v)
     (pa, ps, p0), (la, ls, l0) = _per(pos), _per(n if lens is None else lens)
-    with torch.cuda.device_of(c.k):
-        L.call("bones_kv8_append", c.k.data_ptr(), c.v.data_ptr(), c.k_scale.data_ptr(), c.v_scale.data_ptr(), c.k_open.data_ptr(), c.v_open.data_ptr(),
-               k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2), b, h, d, t, n, pa, ps, p0, la, ls, l0,
-               L.raw_stream())
+    with L.device(dev):
+        L.call("bones_kv8_append", at[0], at[1], at[2], at[3], at[4], at[5], k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.stride(0),
+               v.stride(1), v.stride(2), b, h, d, t, n, pa, ps, p0, la, ls, l0, L.raw_stream())
     COUNTS["kv8_append"] += 1
 
 
-def read(c: KV8, held, length):
-    b, h, t, d = c.k.shape
-    k, v = (torch.empty(b, length, h, d, dtype=torch.bfloat16, device=c.k.device) for _ in range(2))
+def read(dims, held, length):
+    b, h, t, d, dev, at = dims
+    k, v = (torch.empty(b, length, h, d, dtype=torch.bfloat16, device=f"cuda:{dev}") for _ in range(2))
     if length:
         ha, hs, h0 = _per(held)
-        with torch.cuda.device_of(c.k):
-            L.call("bones_kv8_read", c.k.data_ptr(), c.v.data_ptr(), c.k_scale.data_ptr(), c.v_scale.data_ptr(), c.k_open.data_ptr(), c.v_open.data_ptr(),
-                   k.data_ptr(), v.data_ptr(), b, h, d, t, length, ha, hs, h0, L.raw_stream())
+        with L.device(dev):
+            L.call("bones_kv8_read", at[0], at[1], at[2], at[3], at[4], at[5], k.data_ptr(), v.data_ptr(), b, h, d, t, length, ha, hs, h0, L.raw_stream())
         COUNTS["kv8_read"] += 1
     return k, v
 
 
-def attention(qkv, cos, sin, c: KV8, pos, scale, doc_start, window):
+def _table(x):
+    return x if x.dtype is torch.float32 and x.is_contiguous() else x.to(torch.float32).contiguous()
+
+
+def attention(qkv, cos, sin, dims, pos, scale, doc_start, window):
     _bf16(qkv, "qkv")
-    if qkv.stride(1) != 1 or (qkv.shape[0] > 1 and qkv.stride(0) % 8) or qkv.data_ptr() % 16:
+    b, h, t, d, dev, _ = dims
+    if qkv.stride(1) != 1 or (b > 1 and qkv.stride(0) % 8) or qkv.data_ptr() % 16:
         qkv = qkv.contiguous() if not qkv.is_contiguous() else qkv.clone()
-    cos, sin = (x if x.dtype == torch.float32 and x.is_contiguous() and x.data_ptr() % 8 == 0 else x.to(torch.float32, copy=True).contiguous() for x in (cos, sin))
-    b, h, _, d = c.k.shape
-    y = torch.empty(b, h * d, dtype=torch.bfloat16, device=qkv.device)
-    with torch.cuda.device_of(c.k):
-        launch(qkv, cos, sin, c, pos, scale, doc_start, window, y)
+    y = torch.empty((b, h * d), dtype=torch.bfloat16, device=qkv.device)
+    with L.device(dev):
+        launch(qkv, _table(cos), _table(sin), dims, pos, scale, doc_start, window, y)
     COUNTS["kv8_attention"] += 1
     return y
 
 
-def launch(qkv, cos, sin, c: KV8, pos, scale, doc_start, window, y, pdl=0):
+def launch(qkv, cos, sin, dims, pos, scale, doc_start, window, y, pdl=0):
     """The kernel alone, on operands that ``attention`` has checked.  ``pdl``: it may begin while the kernel before it on the stream
     still runs; what that kernel writes is not read before its end."""
-    b, h, t, d = c.k.shape
+    b, h, t, d, _, at = dims
     pa, ps, p0 = _per(pos)
-    L.call("bones_kv8_attention", qkv.data_ptr(), qkv.stride(0), cos.data_ptr(), sin.data_ptr(), cos.shape[0], c.k.data_ptr(), c.v.data_ptr(), c.k_scale.data_ptr(),
-           c.v_scale.data_ptr(), c.k_open.data_ptr(), c.v_open.data_ptr(), pa, ps, p0, 0 if doc_start is None else doc_start.data_ptr(), y.data_ptr(), b, h, d, t,
-           scale, window // 128, pdl, L.raw_stream())
+    L.call("bones_kv8_attention", qkv.data_ptr(), qkv.stride(0), cos.data_ptr(), sin.data_ptr(), cos.shape[0], at[0], at[1], at[2], at[3], at[4], at[5], pa, ps,
+           p0, 0 if doc_start is None else doc_start.data_ptr(), y.data_ptr(), b, h, d, t, scale, window // 128, pdl, L.raw_stream())

@@ -37,21 +37,24 @@ def statement(logits, tokens, topk, vocab) -> TokenLogprobs:
     return TokenLogprobs(g.view(shp), h.view(shp), t.view(*shp, topk), i.view(*shp, topk))
 
 
+def _forward(z, tokens, topk, vocab, want_stats):
+    rows, dev = z.shape[0], z.device
+    given, entropy = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
+    top, ids = torch.empty((rows, topk), dtype=torch.float32, device=dev), torch.empty((rows, topk), dtype=torch.int64, device=dev)
+    stats = torch.empty((rows, 4), dtype=torch.float32, device=dev) if want_stats else None
+    with L.device(z.get_device()):
+        L.call("bones_logprobs_fwd", z.data_ptr(), z.stride(0), int(z.dtype is torch.float32), rows, vocab, tokens.data_ptr(), topk, given.data_ptr(),
+               entropy.data_ptr(), top.data_ptr(), ids.data_ptr(), stats.data_ptr() if want_stats else 0, L.raw_stream())
+    COUNTS["token_logprobs"] += 1
+    return given, entropy, top, ids, stats
+
+
 class _LogprobsFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, z, tokens, topk, vocab, want_grad):
-        rows, dev = z.shape[0], z.device
-        given, entropy = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(2))
-        top = torch.empty(rows, topk, dtype=torch.float32, device=dev)
-        ids = torch.empty(rows, topk, dtype=torch.int64, device=dev)
-        stats = torch.empty(rows, 4, dtype=torch.float32, device=dev) if want_grad else None
-        with torch.cuda.device_of(z):
-            L.call("bones_logprobs_fwd", z.data_ptr(), z.stride(0), int(z.dtype == torch.float32), rows, vocab, tokens.data_ptr(), topk, given.data_ptr(),
-                   entropy.data_ptr(), top.data_ptr(), ids.data_ptr(), stats.data_ptr() if want_grad else 0, L.raw_stream())
-        COUNTS["token_logprobs"] += 1
-        if want_grad:
-            ctx.save_for_backward(z, tokens, ids, stats)
-            ctx.vocab = vocab
+    def forward(ctx, z, tokens, topk, vocab):
+        given, entropy, top, ids, stats = _forward(z, tokens, topk, vocab, True)
+        ctx.save_for_backward(z, tokens, ids, stats)
+        ctx.vocab = vocab
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(ids)
         return given, entropy, top, ids
@@ -63,17 +66,17 @@ class _LogprobsFn(torch.autograd.Function):
         k = ids.shape[1]
         gs = [g_given, g_entropy, g_top if k else None]
         if all(g is None for g in gs):
-            return None, None, None, None, None
+            return None, None, None, None
         if not all(_by_address(g) for g in gs + [z] if g is not None):
             # batched gradients, or a graph recorded through this one: the statement's own operators
-            return _statement_grad(z, tokens, ids, ctx.vocab, *gs), None, None, None, None
+            return _statement_grad(z, tokens, ids, ctx.vocab, *gs), None, None, None
         gs = [g.float().contiguous() if g is not None else None for g in gs]
         g0, g1, g2 = (0 if g is None else g.data_ptr() for g in gs)
         dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-        with torch.cuda.device_of(z):
+        with L.device(z.get_device()):
             L.call("bones_logprobs_bwd", z.data_ptr(), z.stride(0), int(z.dtype == torch.float32), z.shape[0], ctx.vocab, z.shape[1], tokens.data_ptr(), k,
                    ids.data_ptr(), stats.data_ptr(), g0, g1, g2, dz.data_ptr(), z.shape[1], L.raw_stream())
-        return dz, None, None, None, None
+        return dz, None, None, None
 
 
 def _statement_grad(z, tokens, ids, vocab, g_given, g_entropy, g_top):
@@ -100,11 +103,13 @@ def _statement_grad(z, tokens, ids, vocab, g_given, g_entropy, g_top):
 def native(logits, tokens, topk, vocab) -> TokenLogprobs:
     if logits.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"native token_logprobs does not cover this call: dtype {logits.dtype} (bf16 and fp32)")
-    shp = logits.shape[:-1]
-    z = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
+    rows = logits.dim() == 2
+    z = logits if rows else logits.reshape(-1, logits.shape[-1])
     if z.stride(1) != 1:
         z = z.contiguous()
-    tk = tokens.reshape(-1).to(torch.int64).contiguous()
-    want = torch.is_grad_enabled() and logits.requires_grad
-    g, h, t, i = _LogprobsFn.apply(z, tk, topk, vocab, want)
-    return TokenLogprobs(g.view(shp), h.view(shp), t.view(*shp, topk), i.view(*shp, topk))
+    tk = tokens if rows and tokens.dtype is torch.int64 and tokens.is_contiguous() else tokens.reshape(-1).to(torch.int64).contiguous()
+    r = _LogprobsFn.apply(z, tk, topk, vocab) if torch.is_grad_enabled() and logits.requires_grad else _forward(z, tk, topk, vocab, False)[:4]
+    if rows:
+        return TokenLogprobs(*r)
+    shp = logits.shape[:-1]
+    return TokenLogprobs(r[0].view(shp), r[1].view(shp), r[2].view(*shp, topk), r[3].view(*shp, topk))
