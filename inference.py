@@ -3,7 +3,9 @@
 ``load_for_eval(checkpoint_path, device)`` returns a ``ModelWrapper`` whose ``forward(input_ids)`` gives fp32 softcapped
 logits ``[B, T, V]``; ``get_eval_worker()`` treats every rank as an independent replica.  Beyond the reference (which
 scores full sequences only) the wrapper offers ``score(tokens, ctx_len, total_len)`` (continuation log-likelihoods from a
-batched prefill) and ``generate(prompts, n_new)`` (greedy decoding with a KV cache).
+batched prefill), ``report(tokens, ctx_len, total_len, topk)`` (the same token by token, with entropies and alternatives) and
+``generate(prompts, n_new)`` (greedy decoding with a KV cache in bf16 or, ``kv="int8"``, in 8 bits; ``logprobs=k`` tells what each
+new token was worth).
 """
 from __future__ import annotations
 
@@ -15,7 +17,7 @@ import torch
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 
 from them_bones_b200.utils import ckpt as CK  # noqa: E402
-from them_bones_b200.utils.evalbpb import score_continuations  # noqa: E402
+from them_bones_b200.utils.evalbpb import report_continuations, score_continuations  # noqa: E402
 from them_bones_b200.utils.decode import greedy_decode  # noqa: E402
 
 
@@ -37,8 +39,12 @@ class ModelWrapper(torch.nn.Module):
         return score_continuations(self.model, tokens, ctx_len, total_len)
 
     @torch.no_grad()
-    def generate(self, prompts: torch.Tensor, n_new: int) -> torch.Tensor:
-        return greedy_decode(self.model, prompts, n_new)
+    def report(self, tokens, ctx_len, total_len, topk: int = 0):
+        return report_continuations(self.model, tokens, ctx_len, total_len, topk)
+
+    @torch.no_grad()
+    def generate(self, prompts: torch.Tensor, n_new: int, kv: str = "bf16", logprobs: int | None = None):
+        return greedy_decode(self.model, prompts, n_new, kv, logprobs)
 
     def get_eval_worker(self):
         rank = int(os.environ.get("RANK", 0))
@@ -59,8 +65,13 @@ if __name__ == "__main__":
     ap.add_argument("checkpoint")
     ap.add_argument("--device", default="cuda" if torch.cuda.is_available() else "cpu")
     ap.add_argument("--new-tokens", type=int, default=16)
+    ap.add_argument("--kv", default="bf16", choices=["bf16", "int8"], help="how the cache holds keys and values")
+    ap.add_argument("--logprobs", type=int, default=None, help="also print each new token's log-probability and this many alternatives")
     a = ap.parse_args()
     w = load_for_eval(a.checkpoint, a.device)
     cfg = w.model.config
     prompts = torch.randint(1, cfg.vocab_size, (2, 8), device=a.device)
-    print(w.generate(prompts, a.new_tokens).tolist())
+    got = w.generate(prompts, a.new_tokens, a.kv, a.logprobs)
+    print((got if a.logprobs is None else got[0]).tolist())
+    if a.logprobs is not None:
+        print({k: v.tolist() for k, v in got[1]._asdict().items()})

@@ -721,7 +721,9 @@ struct AttnArgs {
 template <int D>
 int launch_kv8_attn(const AttnArgs& p, int B, int split, int pdl, cudaStream_t s) {
   static OncePerDevice once;
-  BONES_ONCE(once, BONES_CHECK(cudaFuncSetAttribute(kv8_attn_kernel<D>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)););
+  BONES_ONCE(once, {
+    BONES_CHECK(cudaFuncSetAttribute(kv8_attn_kernel<D>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  });
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
   cfg.gridDim = dim3((unsigned)(p.H * split), (unsigned)B);

@@ -389,12 +389,13 @@ __global__ void __launch_bounds__(LP_T, 10) logprobs_fwd_kernel(const Z* __restr
   }
 }
 
-// One CTA for LP_U vectors a thread of a row.
+// One CTA for LP_U vectors a thread of a row.  `nic2`: -1 / cap^2 where the logits are z = cap tanh(x / cap) and the gradient is wanted of x
+// (each is multiplied by 1 - (z / cap)^2), else 0.  dz may be the logits themselves.
 template <class Z>
-__global__ void __launch_bounds__(LP_BT) logprobs_bwd_kernel(const Z* __restrict__ logits, long long ldl, int V, int cols, const long long* __restrict__ tokens,
+__global__ void __launch_bounds__(LP_BT) logprobs_bwd_kernel(const Z* logits, long long ldl, int V, int cols, const long long* __restrict__ tokens,
                                                             int k, const long long* __restrict__ ids, const float4* __restrict__ stats,
                                                             const float* __restrict__ g_given, const float* __restrict__ g_entropy,
-                                                            const float* __restrict__ g_top, Z* __restrict__ dz, long long ldd, int chunks) {
+                                                            const float* __restrict__ g_top, Z* dz, long long ldd, int chunks, float nic2) {
   constexpr int VE = 16 / sizeof(Z), CHUNK = LP_BT * LP_U * VE;
   const long long row = blockIdx.x / chunks;
   const int chunk = (int)(blockIdx.x - row * chunks), tid = threadIdx.x;
@@ -435,6 +436,17 @@ __global__ void __launch_bounds__(LP_BT) logprobs_bwd_kernel(const Z* __restrict
     const float l = fmaf(x - st.x, kLog2e, off);
     return -lp_exp2(l) * fmaf(cb, fmaxf(l, -1000.f), ca);
   };
+  auto through = [&](float x) { return nic2 != 0.f ? fmaf(x * nic2, x, 1.0f) : 1.0f; };         // the soft-cap's own derivative
+  // the columns with a gradient of their own, before anything is written
+  const bool extra = !idle && tid <= k && (tid == k ? some : g_top != nullptr);
+  const long long ec = !extra ? -1 : tid == k ? tk : ids[row * k + tid];
+  const bool mine = ec >= c0 && ec < c1;
+  const float ez = mine ? lp_load(z + ec) : 0.f;
+  __syncthreads();
+  auto one = [&](int c) {
+    const float x = c < V && !idle ? lp_load(z + c) : 0.f;
+    lp_store(d + c, c < V && !idle ? grad(x) * through(x) : 0.f);
+  };
   if (alike) {
 #pragma unroll
     for (int j = 0; j < LP_U; ++j) {
@@ -443,28 +455,24 @@ __global__ void __launch_bounds__(LP_BT) logprobs_bwd_kernel(const Z* __restrict
       float f[VE];
       lp_unpack(u[j], f);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) f[e] = c + e < V && !idle ? grad(f[e]) : 0.f;
+      for (int e = 0; e < VE; ++e) f[e] = c + e < V && !idle ? grad(f[e]) * through(f[e]) : 0.f;
       *reinterpret_cast<uint4*>(d + c) = lp_pack(f);
     }
     const int full = head + (cols - head) / VE * VE;
-    auto one = [&](int c) { lp_store(d + c, c < V && !idle ? grad(lp_load(z + c)) : 0.f); };
     if (chunk == 0 && tid < head) one(tid);
     if (c1 == cols && tid < cols - full) one(full + tid);
   } else {
-    for (int c = c0 + tid; c < c1; c += LP_BT) lp_store(d + c, c < V && !idle ? grad(lp_load(z + c)) : 0.f);
+    for (int c = c0 + tid; c < c1; c += LP_BT) one(c);
   }
   if (idle) return;
   __syncthreads();
-  if (tid <= k && (tid == k ? some : g_top != nullptr)) {
-    const long long c = tid == k ? tk : ids[row * k + tid];
-    if (c >= c0 && c < c1) {
-      float v = grad(lp_load(z + c));
-      if (some && c == tk) v += g;
-      if (g_top)
-        for (int j = 0; j < k; ++j)
-          if (ids[row * k + j] == c) v += g_top[row * k + j];
-      lp_store(d + c, v);
-    }
+  if (mine) {
+    float v = grad(ez);
+    if (some && ec == tk) v += g;
+    if (g_top)
+      for (int j = 0; j < k; ++j)
+        if (ids[row * k + j] == ec) v += g_top[row * k + j];
+    lp_store(d + ec, v * through(ez));
   }
 }
 
@@ -480,7 +488,9 @@ template <class Z>
 int launch_logprobs_fwd(const void* logits, long long ldl, long long rows, int V, const long long* tokens, int k, float* given, float* entropy, float* top,
                         long long* ids, void* stats, cudaStream_t s) {
   static OncePerDevice once;
-  BONES_ONCE(once, BONES_CHECK(cudaFuncSetAttribute(logprobs_fwd_kernel<Z>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)););
+  BONES_ONCE(once, {
+    BONES_CHECK(cudaFuncSetAttribute(logprobs_fwd_kernel<Z>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  });
   int dev = 0, sms = 0;
   BONES_CHECK(cudaGetDevice(&dev));
   BONES_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
@@ -496,11 +506,11 @@ int launch_logprobs_fwd(const void* logits, long long ldl, long long rows, int V
 }
 template <class Z>
 int launch_logprobs_bwd(const void* logits, long long ldl, long long rows, int V, int cols, const long long* tokens, int k, const long long* ids,
-                        const void* stats, const float* g_given, const float* g_entropy, const float* g_top, void* dz, long long ldd, cudaStream_t s) {
+                        const void* stats, const float* g_given, const float* g_entropy, const float* g_top, void* dz, long long ldd, float nic2, cudaStream_t s) {
   const int chunk = LP_BT * LP_U * (16 / (int)sizeof(Z)), chunks = (cols + chunk - 1) / chunk;
   if (rows * chunks > 0x7fffffffll) return -2;
   logprobs_bwd_kernel<Z><<<(unsigned)(rows * chunks), LP_BT, 0, s>>>((const Z*)logits, ldl, V, cols, tokens, k, ids, (const float4*)stats, g_given, g_entropy,
-                                                                    g_top, (Z*)dz, ldd, chunks);
+                                                                    g_top, (Z*)dz, ldd, chunks, nic2);
   return (int)cudaGetLastError();
 }
 
@@ -519,12 +529,15 @@ int bones_logprobs_fwd(const void* logits, long long ldl, int wide, long long ro
               : launch_logprobs_fwd<__nv_bfloat16>(logits, ldl, rows, V, tokens, k, given, entropy, top, ids, stats, (cudaStream_t)stream);
 }
 
-// g_given, g_entropy [rows] and g_top [rows, k]: null where there is no gradient; dz: `cols` columns, those behind the vocabulary become 0
+// g_given, g_entropy [rows] and g_top [rows, k]: null where there is no gradient; dz: `cols` columns, those behind the vocabulary become 0;
+// it may be the logits.  cap > 0: the logits are soft-capped, and the gradient is that of what they were before.
 int bones_logprobs_bwd(const void* logits, long long ldl, int wide, long long rows, int V, int cols, const long long* tokens, int k, const long long* ids,
-                       const void* stats, const float* g_given, const float* g_entropy, const float* g_top, void* dz, long long ldd, void* stream) {
+                       const void* stats, const float* g_given, const float* g_entropy, const float* g_top, void* dz, long long ldd, float cap,
+                       void* stream) {
   if (rows == 0) return 0;
   if (rows < 0 || rows > 0x7fffffffll || V < 1 || cols < V || cols > (1 << 30) || k < 0 || k > LP_TOP || (k && g_top && !ids) || !stats || ((uintptr_t)stats & 15)) return -2;
-  return wide ? launch_logprobs_bwd<float>(logits, ldl, rows, V, cols, tokens, k, ids, stats, g_given, g_entropy, g_top, dz, ldd, (cudaStream_t)stream)
-              : launch_logprobs_bwd<__nv_bfloat16>(logits, ldl, rows, V, cols, tokens, k, ids, stats, g_given, g_entropy, g_top, dz, ldd, (cudaStream_t)stream);
+  const float nic2 = cap > 0.f ? -1.0f / (cap * cap) : 0.f;
+  return wide ? launch_logprobs_bwd<float>(logits, ldl, rows, V, cols, tokens, k, ids, stats, g_given, g_entropy, g_top, dz, ldd, nic2, (cudaStream_t)stream)
+              : launch_logprobs_bwd<__nv_bfloat16>(logits, ldl, rows, V, cols, tokens, k, ids, stats, g_given, g_entropy, g_top, dz, ldd, nic2, (cudaStream_t)stream);
 }
 }  // extern "C"

@@ -324,6 +324,14 @@ class GPT(nn.Module):
         stats = torch.stack([a[1] for a in moe_aux])
         return loss + aux / loss_div, stats.detach()
 
+    def token_logprobs(self, idx, tokens, topk: int = 0, doc_start=None) -> ops.TokenLogprobs:
+        """What the model says at each position of ``idx [B, T]`` about ``tokens [B, T]`` (-1: nothing is asked): log-probability, entropy and
+        ``topk`` alternatives ``[B, T, ..]``, with gradients.  The logits exist for a block of rows at a time."""
+        if self.os1 is not None:
+            raise ValueError("token_logprobs has no form with the output table")
+        x = self.trunk(idx, doc_start)
+        return ops.lmhead_logprobs(x, self.lm_head.weight, tokens, self.config.vocab_size, self.config.softcap, topk)
+
     def _plain_loss(self, x, targets, loss_reduction, loss_div, row_weights):
         cfg = self.config
         aux = self.mtp_terms(targets, loss_div) if (loss_reduction == "mean" and self.training) else None

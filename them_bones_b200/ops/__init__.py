@@ -213,6 +213,15 @@ def token_logprobs(logits, tokens, topk=0, vocab=None):
     return _logprobs.statement(logits, tokens, topk, vocab)
 
 
+def lmhead_logprobs(x, w, tokens, vocab, cap, topk=0):
+    """``token_logprobs`` of the soft-capped logits ``cap * tanh(x @ w.T / cap)`` of rows ``x [.., C]``, with gradients to ``x`` and ``w``.  The
+    logits exist for a block of rows at a time; natively in bf16, as a decode step has them."""
+    _logprobs.check_head(x, w, tokens, topk, vocab)
+    if native(x):
+        return _logprobs.head_native(x, w, tokens, topk, vocab, cap)
+    return _logprobs.head_statement(x, w, tokens, topk, vocab, cap)
+
+
 # -- key/value cache in 8 bits -----------------------------------------------------------------------------------
 def kv8_cache(batch, max_len, n_head, head_dim, device=None) -> KV8:
     """An empty cache of one layer (``ops.kv8.KV8``) for ``batch`` sequences of up to ``max_len`` tokens (rounded up to 64): int8 codes with

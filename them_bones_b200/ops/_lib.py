@@ -38,7 +38,7 @@ SIGNATURES = {
     "bones_kv8_read": [_P] * 8 + [_I] * 5 + [_P, _I, _I, _P],
     "bones_kv8_attention": [_P, _L, _P, _P, _I] + [_P] * 6 + [_P, _I, _I, _P, _P] + [_I] * 4 + [_F, _I, _I, _P],
     "bones_logprobs_fwd": [_P, _L, _I, _L, _I, _P, _I] + [_P] * 6,
-    "bones_logprobs_bwd": [_P, _L, _I, _L, _I, _I, _P, _I] + [_P] * 6 + [_L, _P],
+    "bones_logprobs_bwd": [_P, _L, _I, _L, _I, _I, _P, _I] + [_P] * 6 + [_L, _F, _P],
     "bones_mx2_quant": [_P, _L, _P, _P, _I, _P, _P, _I, _L, _L, _I, _P],
     "bones_gemm_mxfp8_pair": [_P] * 8 + [_I] + [_P] * 2 + [_I] * 5 + [_L] * 8 + [_I] * 3 + [_F] * 2 + [_I] * 3 + [_P],
 }

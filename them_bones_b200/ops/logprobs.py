@@ -31,6 +31,15 @@ def check(logits, tokens, topk, vocab):
         raise ValueError(f"token_logprobs: topk {topk}, at most {min(TOP_MAX, vocab)}")
 
 
+def check_head(x, w, tokens, topk, vocab):
+    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1] or not x.is_floating_point() or w.device != x.device:
+        raise ValueError(f"lmhead_logprobs: rows {tuple(x.shape)} on {x.device}, head {tuple(w.shape)} on {w.device}")
+    if tokens.shape != x.shape[:-1] or tokens.dtype not in (torch.int64, torch.int32) or tokens.device != x.device:
+        raise ValueError(f"lmhead_logprobs: tokens {tokens.dtype} {tuple(tokens.shape)} on {tokens.device}, expected int64 or int32 {tuple(x.shape[:-1])} on {x.device}")
+    if not 1 <= vocab <= w.shape[0] or not 0 <= topk <= min(TOP_MAX, vocab):
+        raise ValueError(f"lmhead_logprobs: a vocabulary of {vocab} in {w.shape[0]} rows, topk {topk} (at most {TOP_MAX})")
+
+
 def statement(logits, tokens, topk, vocab) -> TokenLogprobs:
     shp = logits.shape[:-1]
     g, h, t, i = RF.token_logprobs(logits.reshape(-1, logits.shape[-1]), tokens.reshape(-1).to(torch.int64), topk, vocab)
@@ -47,6 +56,17 @@ def _forward(z, tokens, topk, vocab, want_stats):
                entropy.data_ptr(), top.data_ptr(), ids.data_ptr(), stats.data_ptr() if want_stats else 0, L.raw_stream())
     COUNTS["token_logprobs"] += 1
     return given, entropy, top, ids, stats
+
+
+def _as_kernel(gs):
+    """Gradients as the kernel reads them: fp32, contiguous."""
+    return [None if g is None else g.float().contiguous() for g in gs]
+
+
+def _backward(z, tokens, ids, stats, vocab, gs, dz, cap):
+    g0, g1, g2 = (0 if g is None else g.data_ptr() for g in gs)
+    L.call("bones_logprobs_bwd", z.data_ptr(), z.stride(0), int(z.dtype is torch.float32), z.shape[0], vocab, z.shape[1], tokens.data_ptr(), ids.shape[1],
+           ids.data_ptr(), stats.data_ptr(), g0, g1, g2, dz.data_ptr(), dz.stride(0), cap, L.raw_stream())
 
 
 class _LogprobsFn(torch.autograd.Function):
@@ -70,12 +90,10 @@ class _LogprobsFn(torch.autograd.Function):
         if not all(_by_address(g) for g in gs + [z] if g is not None):
             # batched gradients, or a graph recorded through this one: the statement's own operators
             return _statement_grad(z, tokens, ids, ctx.vocab, *gs), None, None, None
-        gs = [g.float().contiguous() if g is not None else None for g in gs]
-        g0, g1, g2 = (0 if g is None else g.data_ptr() for g in gs)
+        gs = _as_kernel(gs)
         dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
         with L.device(z.get_device()):
-            L.call("bones_logprobs_bwd", z.data_ptr(), z.stride(0), int(z.dtype == torch.float32), z.shape[0], ctx.vocab, z.shape[1], tokens.data_ptr(), k,
-                   ids.data_ptr(), stats.data_ptr(), g0, g1, g2, dz.data_ptr(), z.shape[1], L.raw_stream())
+            _backward(z, tokens, ids, stats, ctx.vocab, gs, dz, 0.0)
         return dz, None, None, None
 
 
@@ -112,4 +130,82 @@ def native(logits, tokens, topk, vocab) -> TokenLogprobs:
     if rows:
         return TokenLogprobs(*r)
     shp = logits.shape[:-1]
+    return TokenLogprobs(r[0].view(shp), r[1].view(shp), r[2].view(*shp, topk), r[3].view(*shp, topk))
+
+
+# -- from the last hidden rows ---------------------------------------------------------------------------------------
+def head_statement(x, w, tokens, topk, vocab, cap) -> TokenLogprobs:
+    z = RF.softcap_logits(torch.nn.functional.linear(x, w.to(x.dtype))[..., :vocab], cap)
+    return statement(z, tokens, topk, vocab)
+
+
+class _HeadLogprobsFn(torch.autograd.Function):
+    """The head in blocks of rows: the logits of a block are made, looked at and dropped, and made again for their gradient, so that only
+    one ``[rows, V]`` block exists at a time.  A head that owns its gradient (``main_grad``) gets it by accumulation."""
+
+    @staticmethod
+    def forward(ctx, x, w, tokens, topk, vocab, cap, want_grad):
+        from . import cuda as C
+        m, dev = x.shape[0], x.device
+        given, entropy = torch.empty(m, dtype=torch.float32, device=dev), torch.empty(m, dtype=torch.float32, device=dev)
+        top, ids = torch.empty((m, topk), dtype=torch.float32, device=dev), torch.empty((m, topk), dtype=torch.int64, device=dev)
+        stats = torch.empty((m, 4), dtype=torch.float32, device=dev)
+        buf = torch.empty(min(C.LOSS_ROWS, m), w.shape[0], dtype=torch.bfloat16, device=dev)
+        for a in range(0, m, C.LOSS_ROWS):
+            n = min(C.LOSS_ROWS, m - a)
+            _capped(x[a:a + n], w, cap, buf[:n])
+            L.call("bones_logprobs_fwd", buf.data_ptr(), buf.stride(0), 0, n, vocab, tokens[a:a + n].data_ptr(), topk, given[a:a + n].data_ptr(),
+                   entropy[a:a + n].data_ptr(), top[a:a + n].data_ptr(), ids[a:a + n].data_ptr(), stats[a:a + n].data_ptr(), L.raw_stream())
+        COUNTS["lmhead_logprobs"] += 1
+        if want_grad:
+            ctx.save_for_backward(x, w, tokens, ids, stats)
+            ctx.vocab, ctx.cap, ctx.main_grad = vocab, cap, getattr(w, "main_grad", None)
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(ids)
+        return given, entropy, top, ids
+
+    @staticmethod
+    def backward(ctx, g_given, g_entropy, g_top, _g_ids):
+        from . import cuda as C
+        x, w, tokens, ids, stats = ctx.saved_tensors
+        gs = [g_given, g_entropy, g_top if ids.shape[1] else None]
+        none = (None,) * 5
+        if all(g is None for g in gs):
+            return None, None, *none
+        if not all(C._by_address(g) for g in gs + [x, w] if g is not None):
+            z = RF.softcap_logits(torch.nn.functional.linear(x.float(), w.float()), ctx.cap)
+            d = _statement_grad(z, tokens, ids, ctx.vocab, *gs) * (1 - (z / ctx.cap).square())
+            return (d @ w.float()).to(x.dtype), (d.transpose(-1, -2) @ x.float()).to(w.dtype), *none
+        gs, m = _as_kernel(gs), x.shape[0]
+        need_x, need_w = ctx.needs_input_grad[:2]
+        dx = torch.zeros(x.shape, dtype=torch.float32, device=x.device) if need_x else None
+        dw = ctx.main_grad if ctx.main_grad is not None or not need_w else torch.zeros(w.shape, dtype=torch.float32, device=w.device)
+        buf = torch.empty(min(C.LOSS_ROWS, m), w.shape[0], dtype=torch.bfloat16, device=x.device)
+        with L.device(x.get_device()):
+            for a in range(0, m, C.LOSS_ROWS):
+                n = min(C.LOSS_ROWS, m - a)
+                z = buf[:n]
+                _capped(x[a:a + n], w, ctx.cap, z)
+                _backward(z, tokens[a:a + n], ids[a:a + n], stats[a:a + n], ctx.vocab, [None if g is None else g[a:a + n] for g in gs], z, ctx.cap)
+                if need_x:
+                    C.mm_nn_acc(z, w, dx[a:a + n])
+                if need_w:
+                    C.mm_tn_acc(z, x[a:a + n], dw)
+        return dx.to(x.dtype) if need_x else None, dw.to(w.dtype) if need_w and ctx.main_grad is None else None, *none
+
+
+def _capped(x, w, cap, out):
+    from . import cuda as C
+    C.mm_nt(x, w, out=out, epi=L.EPI_SOFTCAP, alpha=1.0 / cap, beta=cap)
+
+
+def head_native(x, w, tokens, topk, vocab, cap) -> TokenLogprobs:
+    from .cuda import _c
+    if x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16 or x.shape[-1] % 8 or w.shape[0] % 8 or not cap > 0:
+        raise ValueError(f"native lmhead_logprobs does not cover this call: {x.dtype} {tuple(x.shape)}, head {w.dtype} {tuple(w.shape)}, cap {cap} "
+                         "(bf16, rows of whole 16 bytes, a soft-cap)")
+    shp, x2, tk = x.shape[:-1], _c(x).view(-1, x.shape[-1]), tokens.reshape(-1).to(torch.int64).contiguous()
+    x2, w = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (x2, w))
+    with L.device(x.get_device()):
+        r = _HeadLogprobsFn.apply(x2, w, tk, topk, vocab, float(cap), torch.is_grad_enabled() and (x.requires_grad or w.requires_grad))
     return TokenLogprobs(r[0].view(shp), r[1].view(shp), r[2].view(*shp, topk), r[3].view(*shp, topk))

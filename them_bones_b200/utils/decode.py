@@ -3,7 +3,9 @@
 The reference scores teacher-forced full sequences only (round2/submission/inference.py:26-27); autoregressive decoding
 is an added capability.  The cache stores, per layer, keys *after* RoPE and QK-norm and raw values, so a decode step
 rotates only the new token (RoPE at its absolute position) and attends over the cached prefix restricted to the current
-document and the layer's window.
+document and the layer's window.  It holds them in bf16 or, for twice the tokens in the same memory and half the bytes of a
+step, in 8 bits (``kv="int8"``: ``ops.kv8_cache``).  A decoder can also say what each of its answers was worth
+(``logprobs=k``: ``ops.token_logprobs`` of every generated token).
 """
 from __future__ import annotations
 
@@ -24,13 +26,24 @@ def L_check():
     L.check_error_word()
 
 
+KV_TYPES = ("bf16", "int8")
+
+
 class KVCache:
-    def __init__(self, model, batch: int, max_len: int):
+    """``kv="bf16"``: keys and values ``[layers, B, T, H, D]`` in the model's type; ``"int8"``: a ``KV8`` for each layer in ``kv8``."""
+
+    def __init__(self, model, batch: int, max_len: int, kv: str = "bf16"):
         cfg = model.config
         dev, dt = model.lm_head.weight.device, model.lm_head.weight.dtype
-        shape = (cfg.n_layer, batch, max_len, cfg.n_head, cfg.head_dim)
-        self.k = torch.zeros(shape, dtype=dt, device=dev)
-        self.v = torch.zeros(shape, dtype=dt, device=dev)
+        if kv not in KV_TYPES:
+            raise ValueError(f"key/value cache {kv!r} (one of {KV_TYPES})")
+        self.max_len, self.k, self.v, self.kv8 = max_len, None, None, None
+        if kv == "int8":
+            self.kv8 = [ops.kv8_cache(batch, max_len, cfg.n_head, cfg.head_dim, dev) for _ in range(cfg.n_layer)]
+        else:
+            shape = (cfg.n_layer, batch, max_len, cfg.n_head, cfg.head_dim)
+            self.k = torch.zeros(shape, dtype=dt, device=dev)
+            self.v = torch.zeros(shape, dtype=dt, device=dev)
         self.doc_start = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.len = 0
         self.tokens = None          # token history [batch, max_len], kept when the model has hashed tables
@@ -67,7 +80,7 @@ def _forward_cached(model, idx, cache: KVCache):
     if model.tables is not None:
         # rows keyed by the last `order` tokens: the cache keeps the token history for contexts that start before this call
         if cache.tokens is None:
-            cache.tokens = torch.zeros(b, cache.k.shape[2], dtype=torch.int64, device=dev)
+            cache.tokens = torch.zeros(b, cache.max_len, dtype=torch.int64, device=dev)
         cache.tokens[:, p0:p0 + t] = idx
         hist, tb = cache.tokens[:, :p0 + t], model.tables
         ids = torch.stack([RF.ngram_rows(hist, o, tb.rows, tb.seed + j, _doc_start_full(hist, cfg) if cfg.doc_mask else None)[:, p0:]
@@ -91,16 +104,26 @@ def _forward_cached(model, idx, cache: KVCache):
             v = v + blk.ve_lambda.to(v.dtype) * ve.to(v.dtype)
         q = RF.rms_norm(_rope_at(q, cos, sin))
         k = RF.rms_norm(_rope_at(k, cos, sin))
-        cache.k[i, :, p0:p0 + t] = k
-        cache.v[i, :, p0:p0 + t] = v
+        if cache.kv8 is not None:
+            # a token sees the block it is in as it came and the ones before it from their codes, as it does token by token
+            exact = [torch.cat([old, new.to(old.dtype)], 1) for old, new in zip(ops.kv8_read(cache.kv8[i], p0, p0), (k, v))]
+            ops.kv8_append(cache.kv8[i], k.to(exact[0].dtype), v.to(exact[0].dtype), p0)
+            coded = ops.kv8_read(cache.kv8[i], p0 + t, p0 + t)
+        else:
+            cache.k[i, :, p0:p0 + t] = k
+            cache.v[i, :, p0:p0 + t] = v
         ys = []
         for j in range(t):                                   # prefill is short in decode benchmarks; one row at a time
             cur = p0 + j
             lo = ds[:, j].to(torch.int64)
             if at.window:
                 lo = torch.maximum(lo, torch.full_like(lo, max(0, (cur // 128 - (at.window // 128 - 1)) * 128)))
-            ys.append(_attend(q[:, j:j + 1].transpose(1, 2), cache.k[i, :, :cur + 1], cache.v[i, :, :cur + 1],
-                              at.scale, lo))
+            if cache.kv8 is not None:
+                first = cur // RF.KV8_BLOCK * RF.KV8_BLOCK
+                keys, vals = (torch.cat([c[:, :first], e[:, first:cur + 1]], 1) for c, e in zip(coded, exact))
+            else:
+                keys, vals = cache.k[i, :, :cur + 1], cache.v[i, :, :cur + 1]
+            ys.append(_attend(q[:, j:j + 1].transpose(1, 2), keys, vals, at.scale, lo))
         y = torch.cat(ys, 1).reshape(b, t, -1).to(x.dtype)
         x = x + F.linear(y, at.c_proj.weight)
         xn = RF.rms_norm(x)
@@ -220,7 +243,9 @@ class NativeDecoder:
     advanced inside the graph, so generating ``n`` tokens is ``n`` graph replays with no host synchronisation.
     Eligible: bf16 models on CUDA whose blocks all have attention with head_dim 128.  MoE blocks run their routed experts
     inside the graph (router, slotting, grouped expert GEMMs, combine: all device-side, a decode step uses one slot per
-    sequence and expert); hashed input tables are looked up from row ids hashed on the device from the token history."""
+    sequence and expert); hashed input tables are looked up from row ids hashed on the device from the token history.
+    With a cache in 8 bits the attention is ``ops.kv8_attention``.  ``logprobs=k``: ``report`` holds, for each position of ``out``, what the
+    logits that it was chosen from say of the token there (a forced one's too), their entropy and k alternatives."""
 
     @staticmethod
     def eligible(model) -> bool:
@@ -230,10 +255,11 @@ class NativeDecoder:
         return (w.is_cuda and w.dtype == torch.bfloat16 and cfg.head_dim == 128 and tables_ok and getattr(model, "os1", None) is None
                 and not ops.reference_path() and all(blk.attn is not None for blk in model.transformer.h))
 
-    def __init__(self, model, cache: KVCache, first_tokens: torch.Tensor, out: torch.Tensor, prompt_len: int = 0):
+    def __init__(self, model, cache: KVCache, first_tokens: torch.Tensor, out: torch.Tensor, prompt_len: int = 0, logprobs: int | None = None):
         # positions below ``prompt_len`` are teacher-forced from ``out`` (stepwise prefill through the same graph)
         self.model, self.cache, self.out = model, cache, out
         dev = first_tokens.device
+        self.report = None if logprobs is None else _empty_report(first_tokens.shape[0], out.shape[1], logprobs, dev)
         self.prompt_len = torch.tensor([prompt_len], dtype=torch.int32, device=dev)
         self.tok = first_tokens.clone().to(torch.int64)
         self.pos = torch.tensor([cache.len], dtype=torch.int32, device=dev)
@@ -302,10 +328,9 @@ class NativeDecoder:
     def _step_fused(self):
         """Five kernels a layer (qkv, attention, out, c_fc, c_proj), one before the first and two after the last; the norms,
         the residual mix, ReLU^2 and the soft-cap are in the projections' epilogues."""
-        from ..ops import _lib as L
+        from ..ops import _lib as L, kv8 as KV8
         model, cache, cfg = self.model, self.cache, self.model.config
         tok, pos, b, c = self.tok, self.pos, self.tok.shape[0], cfg.n_embd
-        tmax = cache.k.shape[2]
         ds = cache.doc_start if cfg.doc_mask else None
         hs = model.transformer.h
         w = model.transformer.wte.weight
@@ -315,8 +340,12 @@ class NativeDecoder:
         for i, blk in enumerate(hs):
             at = blk.attn
             self._proj(self.xa, self.wqkv[i], self.qkv, 0, ssq=self.ssq_a, n_ssq=n_ssq, nxt=at.c_proj.weight)
-            L.call("bones_decode_attn_step", L.ptr(self.qkv), L.ptr(model.cos), L.ptr(model.sin), L.ptr(cache.k[i]), L.ptr(cache.v[i]), L.ptr(pos), L.ptr(ds),
-                   L.ptr(self.y), _I(b), _I(at.n_head), _I(tmax), ctypes.c_float(at.scale), _I(at.window // 128), L.stream())
+            if cache.kv8 is not None:
+                dims = KV8.check_attention(self.qkv, model.cos, model.sin, cache.kv8[i], pos, ds, at.window)
+                KV8.launch(self.qkv, model.cos, model.sin, dims, pos, at.scale, ds, at.window, self.y, pdl=1)
+            else:
+                L.call("bones_decode_attn_step", L.ptr(self.qkv), L.ptr(model.cos), L.ptr(model.sin), L.ptr(cache.k[i]), L.ptr(cache.v[i]), L.ptr(pos), L.ptr(ds),
+                       L.ptr(self.y), _I(b), _I(at.n_head), _I(cache.max_len), ctypes.c_float(at.scale), _I(at.window // 128), L.stream())
             n_ssq = self._proj(self.y, at.c_proj.weight, self.xb, 2, res=self.xa, ssq_out=self.ssq_b, nxt=blk.mlp.c_fc.weight)
             self._proj(self.xb, blk.mlp.c_fc.weight, self.h, 1, ssq=self.ssq_b, n_ssq=n_ssq, nxt=blk.mlp.c_proj.weight)
             nxt = hs[i + 1] if i + 1 < len(hs) else None
@@ -347,10 +376,11 @@ class NativeDecoder:
         from ..ops import _lib as L
         from ..ops import cuda as C
         if self.fused:
-            return self._step_fused()
+            self._step_fused()
+            return self._note()
         model, cache, cfg = self.model, self.cache, self.model.config
         tok, pos = self.tok, self.pos
-        b, tmax = tok.shape[0], cache.k.shape[2]
+        b, tmax = tok.shape[0], cache.max_len
         if cfg.doc_mask:
             cache.doc_start.copy_(torch.where(tok == cfg.bos_id, pos.expand(b), cache.doc_start))
         x = ops.embedding(tok, model.transformer.wte.weight, torch.bfloat16)
@@ -374,20 +404,26 @@ class NativeDecoder:
             if model.value_embeds is not None and str(i) in model.value_embeds:
                 ve = ops.embedding(tok, model.value_embeds[str(i)].weight, torch.bfloat16)
                 lam = blk.ve_lambda.detach().float()
-            L.call("bones_decode_qkv", L.ptr(qkv), L.ptr(model.cos), L.ptr(model.sin), L.ptr(ve), L.ptr(lam), L.ptr(self.qbuf),
-                   L.ptr(cache.k[i]), L.ptr(cache.v[i]), L.ptr(pos), C._I(b), C._I(at.n_head), C._I(tmax), L.stream())
-            L.call("bones_decode_attn", L.ptr(self.qbuf), L.ptr(cache.k[i]), L.ptr(cache.v[i]), L.ptr(pos),
-                   L.ptr(cache.doc_start if cfg.doc_mask else None), L.ptr(self.y), C._I(b), C._I(at.n_head), C._I(tmax),
-                   C._F(at.scale), C._I(at.window // 128), L.stream())
+            if cache.kv8 is not None:
+                if ve is not None:
+                    qkv[:, 2 * ve.shape[1]:].add_(lam.to(qkv.dtype) * ve)          # as in training: both factors and the product in bf16
+                y = ops.kv8_attention(qkv, model.cos, model.sin, cache.kv8[i], pos, at.scale, cache.doc_start if cfg.doc_mask else None, at.window)
+            else:
+                y = self.y
+                L.call("bones_decode_qkv", L.ptr(qkv), L.ptr(model.cos), L.ptr(model.sin), L.ptr(ve), L.ptr(lam), L.ptr(self.qbuf),
+                       L.ptr(cache.k[i]), L.ptr(cache.v[i]), L.ptr(pos), C._I(b), C._I(at.n_head), C._I(tmax), L.stream())
+                L.call("bones_decode_attn", L.ptr(self.qbuf), L.ptr(cache.k[i]), L.ptr(cache.v[i]), L.ptr(pos),
+                       L.ptr(cache.doc_start if cfg.doc_mask else None), L.ptr(y), C._I(b), C._I(at.n_head), C._I(tmax),
+                       C._F(at.scale), C._I(at.window // 128), L.stream())
             if self.split:
-                x = self._lin(self.y, at.c_proj.weight, 1, x)
+                x = self._lin(y, at.c_proj.weight, 1, x)
                 x, xn = ops.norm_split(x)
                 if self.dense[i]:
                     x = self._lin(self._lin(xn, blk.mlp.c_fc.weight, 2), blk.mlp.c_proj.weight, 1, x)
                 else:
                     x = blk.mlp(xn.view(b, 1, -1), residual=x.view(b, 1, -1)).view(b, -1)
             else:
-                x = ops.linear(self.y, at.c_proj.weight, residual=x)
+                x = ops.linear(y, at.c_proj.weight, residual=x)
                 x, xn = ops.norm_split(x)
                 x = blk.mlp(xn.view(b, 1, -1), residual=x.view(b, 1, -1)).view(b, -1) if not self.dense[i] else blk.mlp(xn, residual=x)
             if n_skip and i < n_skip:
@@ -402,6 +438,16 @@ class NativeDecoder:
         nxt = torch.where((pos < self.prompt_len).expand_as(nxt), forced, nxt)
         self.out.index_copy_(1, at, nxt[:, None])                         # token at position pos (after the increment)
         tok.copy_(nxt)
+        self._note()
+
+    def _note(self):
+        """What this step's logits say of the token that now stands at ``pos``; a step past the end of ``out`` leaves the last place."""
+        if self.report is None:
+            return
+        k = self.report.top_id.shape[2]
+        at = self.pos.to(torch.int64).clamp(max=self.report.logprob.shape[1] - 1)
+        for kept, new in zip(self.report, ops.token_logprobs(self.last_logits, self.tok, k, self.model.config.vocab_size)):
+            kept.index_copy_(1, at, new[:, None])
 
     @torch.no_grad()
     def run(self, n_steps: int):
@@ -424,49 +470,89 @@ class NativeDecoder:
             self.graph.replay()
 
 
+def _empty_report(b: int, length: int, k: int, dev) -> ops.TokenLogprobs:
+    """Zeros for ``length`` positions, and one place more for what a step past the end writes."""
+    z = lambda dt, *shape: torch.zeros(b, length + 1, *shape, dtype=dt, device=dev)  # noqa: E731
+    return ops.TokenLogprobs(z(torch.float32), z(torch.float32), z(torch.float32, k), z(torch.int64, k))
+
+
+def _with_report(out, report, p: int):
+    """What ``greedy_decode`` returns: the tokens, and where it was asked for what the new ones were worth."""
+    return out if report is None else (out, ops.TokenLogprobs(*(x[:, p:out.shape[1]].contiguous() for x in report)))
+
+
+def _noted(model, logits, nxt, k, report: list):
+    if k is not None:
+        report.append(ops.token_logprobs(logits, nxt, k, model.config.vocab_size))
+
+
+def _stacked(report: list, b: int, k, dev):
+    if k is None:
+        return None
+    return ops.TokenLogprobs(*(torch.stack(x, 1) for x in zip(*report))) if report else ops.TokenLogprobs(*(x[:, :0] for x in _empty_report(b, 0, k, dev)))
+
+
 @torch.no_grad()
-def greedy_decode(model, prompts: torch.Tensor, n_new: int) -> torch.Tensor:
-    """``prompts [B, P]`` -> ``[B, P + n_new]`` by arg-max decoding."""
+def greedy_decode(model, prompts: torch.Tensor, n_new: int, kv: str = "bf16", logprobs: int | None = None):
+    """``prompts [B, P]`` -> ``[B, P + n_new]`` by arg-max decoding.  ``kv``: how the cache holds keys and values, ``"bf16"`` or ``"int8"``.
+    ``logprobs=k``: ``(tokens, TokenLogprobs)`` with the log-probability, the entropy and k alternatives of each new token ``[B, n_new]``."""
     b, p = prompts.shape
     if p + n_new > model.config.sequence_len:
         raise ValueError("prompt + new tokens exceed the model's sequence length")
+    if kv not in KV_TYPES:
+        raise ValueError(f"key/value cache {kv!r} (one of {KV_TYPES})")
+    if logprobs is not None and not 0 <= logprobs <= min(ops._logprobs.TOP_MAX, model.config.vocab_size):
+        raise ValueError(f"{logprobs} alternatives (0 to {min(ops._logprobs.TOP_MAX, model.config.vocab_size)})")
     if getattr(model, "os1", None) is not None or any(blk.attn is None for blk in model.transformer.h):
-        return greedy_decode_full(model, prompts, n_new)          # output table and attention-free blocks: cache-free route
-    cache = KVCache(model, b, p + n_new)
+        if kv != "bf16":
+            raise ValueError("models with an output table or attention-free blocks decode without a cache")
+        return greedy_decode_full(model, prompts, n_new, logprobs)          # cache-free route
+    cache = KVCache(model, b, p + n_new, kv)
     if NativeDecoder.eligible(model) and n_new >= 1:
         out = torch.zeros(b, p + n_new, dtype=torch.int64, device=prompts.device)
         out[:, :p] = prompts
         if p <= 512:
             # short prompts are pre-filled token by token through the same graph (teacher-forced), then decoded
-            dec = NativeDecoder(model, cache, prompts[:, 0], out, prompt_len=p)
+            dec = NativeDecoder(model, cache, prompts[:, 0], out, prompt_len=p, logprobs=logprobs)
             dec.run(p + n_new - 1)
+            report = dec.report
         else:
             # long prompts: prefill on the cached PyTorch route, then one graph replay per generated token
             logits = _forward_cached(model, prompts, cache)
             first = logits.argmax(-1)
             out[:, p] = first
+            report = None if logprobs is None else _empty_report(b, p + n_new, logprobs, prompts.device)
             if n_new > 1:
-                dec = NativeDecoder(model, cache, first, out)
+                dec = NativeDecoder(model, cache, first, out, logprobs=logprobs)
                 dec.run(n_new - 1)
+                report = dec.report
+            if report is not None:
+                for kept, new in zip(report, ops.token_logprobs(logits, first, logprobs, model.config.vocab_size)):
+                    kept[:, p] = new
         L_check()
-        return out
-    out = [prompts]
+        return _with_report(out, report, p)
+    out, report = [prompts], []
     logits = _forward_cached(model, prompts, cache)
     for _ in range(n_new):
         nxt = logits.argmax(-1, keepdim=True)
         out.append(nxt)
+        _noted(model, logits, nxt[:, 0], logprobs, report)
         if cache.len >= p + n_new:
             break
         logits = _forward_cached(model, nxt, cache)
-    return torch.cat(out, 1)[:, :p + n_new]
+    out, report = torch.cat(out, 1)[:, :p + n_new], _stacked(report, b, logprobs, prompts.device)
+    return out if report is None else (out, report)
 
 
 @torch.no_grad()
-def greedy_decode_full(model, prompts: torch.Tensor, n_new: int) -> torch.Tensor:
+def greedy_decode_full(model, prompts: torch.Tensor, n_new: int, logprobs: int | None = None):
     """Cache-free decoding (re-runs the full forward per token); the oracle for the cached path and the route used
     when hashed tables are attached."""
-    seq = prompts
+    seq, report = prompts, []
     for _ in range(n_new):
         logits = model(seq)[:, -1]
-        seq = torch.cat([seq, logits.argmax(-1, keepdim=True)], 1)
-    return seq
+        nxt = logits.argmax(-1, keepdim=True)
+        _noted(model, logits, nxt[:, 0], logprobs, report)
+        seq = torch.cat([seq, nxt], 1)
+    report = _stacked(report, prompts.shape[0], logprobs, prompts.device)
+    return seq if report is None else (seq, report)

@@ -6,7 +6,7 @@ the reference repository; used at round2/source/train.py:23307-23318).
 * ``causality_check``  -- perturb tokens at positions > p and require the logits at positions <= p to stay put.  This
   also covers the MoE capacity count and the hashed-table lookups, which are causal by construction.
 * ``score_continuations`` -- teacher-forced log-likelihood of a continuation given a context (the scoring half of the
-  inference benchmark).
+  inference benchmark); ``report_continuations`` says the same of each token, with the entropy and the alternatives there.
 """
 from __future__ import annotations
 
@@ -65,11 +65,28 @@ def causality_check(model, vocab: int, batch: int, seq_len: int, device, seed: i
 def score_continuations(model, tokens: torch.Tensor, ctx_len: torch.Tensor, total_len: torch.Tensor) -> torch.Tensor:
     """``tokens [B, T]`` padded; request b's context is ``tokens[b, :ctx_len[b]]`` and its continuation
     ``tokens[b, ctx_len[b]:total_len[b]]``.  Returns the summed log-probability of each continuation."""
+    targets, keep = _continuation_targets(tokens, ctx_len, total_len)
+    nll = model(tokens, targets, loss_reduction="none")
+    return -(nll * keep).sum(1)
+
+
+def _continuation_targets(tokens, ctx_len, total_len):
     b, t = tokens.shape
     targets = torch.full((b, t), -1, dtype=torch.int64, device=tokens.device)
     targets[:, :-1] = tokens[:, 1:]
     pos = torch.arange(t, device=tokens.device)[None, :]
     keep = (pos + 1 >= ctx_len[:, None]) & (pos + 1 < total_len[:, None])
-    targets = torch.where(keep, targets, torch.full_like(targets, -1))
-    nll = model(tokens, targets, loss_reduction="none")
-    return -(nll * keep).sum(1)
+    return torch.where(keep, targets, torch.full_like(targets, -1)), keep
+
+
+@torch.no_grad()
+def report_continuations(model, tokens: torch.Tensor, ctx_len: torch.Tensor, total_len: torch.Tensor, topk: int = 0):
+    """``score_continuations`` token by token: ``TokenLogprobs [B, T]`` where place t tells of ``tokens[b, t]`` given what is before it;
+    zeros outside the continuations (and at the first token, which nothing precedes)."""
+    targets, keep = _continuation_targets(tokens, ctx_len, total_len)
+    r = model.token_logprobs(tokens, targets, topk)
+    out = []
+    for x in r:
+        x = torch.where(keep.view(*keep.shape, *(1,) * (x.dim() - 2)), x, torch.zeros_like(x))
+        out.append(torch.cat([torch.zeros_like(x[:, :1]), x[:, :-1]], 1))
+    return type(r)(*out)
