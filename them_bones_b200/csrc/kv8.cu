@@ -315,6 +315,28 @@ __device__ __forceinline__ T turn_and_norm(const __nv_bfloat16* __restrict__ x, 
   return r * ((T)1.5 - (T)0.5 * ss * r * r);                       // a step of Newton's: to the rounding of T
 }
 
+// The sequence with the n-th largest number of tokens to see, of 64 at most: CTAs begin in the order of their numbers, and the longest ones
+// are not to begin last (64 sequences of 1 to 2048 tokens in documents, 10 heads: 31 us for 35; 4 of 32768 to 131072: 162 for 170).  Every
+// warp works it out for itself, from what nothing writes meanwhile: not where the kernel before this one may still run.
+__device__ __forceinline__ int longest_first(int B, int n, PerSeq pos, const int* __restrict__ doc_start) {
+  const int lane = threadIdx.x & 31;
+  uint32_t key[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int b = lane + 32 * i;
+    const int p = b < B ? pos[b] : -1, lo = b < B && doc_start ? doc_start[b] : 0;
+    key[i] = b < B ? (uint32_t)min(max(p - max(lo, 0) + 1, 0), 1 << 25) << 6 | (uint32_t)(63 - b) : 0u;          // no two are equal
+  }
+  int r0 = 0, r1 = 0;
+  for (int j = 0; j < B; ++j) {
+    const uint32_t k = __shfl_sync(0xffffffffu, j < 32 ? key[0] : key[1], j & 31);
+    r0 += k > key[0];
+    r1 += k > key[1];
+  }
+  const unsigned a = __ballot_sync(0xffffffffu, lane < B && r0 == n), c = __ballot_sync(0xffffffffu, lane + 32 < B && r1 == n);
+  return a ? __ffs(a) - 1 : 31 + __ffs(c);
+}
+
 template <int D>
 struct __align__(16) AttnShared {
   float acc[2 * AW][D];                         // full blocks of each warp, then the open block's part of each
@@ -327,7 +349,7 @@ struct __align__(16) AttnShared {
 template <int D>
 __global__ void __launch_bounds__(32 * AW, D == 128 ? 3 : 4) kv8_attn_kernel(const __nv_bfloat16* __restrict__ qkv, long long ldq, const float* __restrict__ cosT,
                                                               const float* __restrict__ sinT, int rope_rows, Kv8 c, PerSeq pos_, const int* doc_start,
-                                                              __nv_bfloat16* __restrict__ y, int H, int cap, float scale2, int window_tiles) {
+                                                              __nv_bfloat16* __restrict__ y, int H, int cap, float scale2, int window_tiles, int least, int by_length) {
   constexpr int TT = 4096 / D, PER = TT / 8, VW = TT / 16;                // tokens of a turn, of a lane; words of a lane's piece of V
   constexpr int KL = D / 64, NT = D / 16, LPT = D / 8, TPI = 32 / LPT, RP = 4, PASS = KB / (AW * TPI * RP);
   __shared__ union {
@@ -337,7 +359,8 @@ __global__ void __launch_bounds__(32 * AW, D == 128 ? 3 : 4) kv8_attn_kernel(con
   AttnShared<D>& sm = sm_.at;
   pdl_launch();
   const int S = (int)cluster_size(), rank = (int)cluster_rank();
-  const int h = blockIdx.x / S, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int h = blockIdx.x / S, b = by_length ? longest_first((int)gridDim.y, (int)blockIdx.y, pos_, doc_start) : (int)blockIdx.y;
   const int g = lane >> 2, c4 = lane & 3;
   // the first kernel of a decode step may be storing a new document start: looked at again behind the wait
   int lo = doc_start ? ld_relaxed(doc_start + b) : 0;
@@ -351,7 +374,6 @@ __global__ void __launch_bounds__(32 * AW, D == 128 ? 3 : 4) kv8_attn_kernel(con
   if (S > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // waited for before the first store to another CTA
   const long long bh = (long long)b * H + h, nb = cap / KB;
   const int slot = pos % KB, last = pos / KB;
-  const bool tail_cta = rank == S - 1;          // its warps come last in the walk over the full blocks
   const int band = window_tiles > 0 ? max((pos / 128 - (window_tiles - 1)) * 128, 0) : 0;
   lo = max(lo, band);
   const int8_t *kp = c.k + bh * cap * D + PER * g * D + 16 * c4, *vp = c.v + bh * cap * D + g * KB + 4 * VW * c4;
@@ -388,19 +410,29 @@ __global__ void __launch_bounds__(32 * AW, D == 128 ? 3 : 4) kv8_attn_kernel(con
       }
     }
   };
-  const int step = S * AW, end = last * (KB / TT);
-  int u = lo / TT + rank * AW + warp;
+  // Of the cluster as many CTAs take part as get `least` turns each, and one for the open block; the others leave.  The last one has the open
+  // block (and, where there is no further CTA, its share of the full ones).
+  const int end = last * (KB / TT);
+  auto taking_part = [&](int from) { return min(S, max(0, (end - from / TT + least - 1) / least) + 1); };
+  int active = taking_part(lo), u = lo / TT + rank * AW + warp;
+  if (rank >= active) return;
+  bool tail_cta = rank == active - 1;
   if (u < end) load_k(u);
   if (tail_cta) load_tail(0);
   pdl_wait();
   if (doc_start) {
-    const int now = max(ld_relaxed(doc_start + b), band);
+    const int now = max(ld_relaxed(doc_start + b), lo);             // a document that begins with this token; none begins earlier than was seen
     if (now != lo) {
       lo = now;
+      active = taking_part(lo);
+      if (rank >= active) return;
       u = lo / TT + rank * AW + warp;
       if (u < end) load_k(u);
+      if (!tail_cta && rank == active - 1) load_tail(0);
+      tail_cta = rank == active - 1;
     }
   }
+  const int step = active * AW;
   if (warp < (tail_cta ? 3 : 1)) {
     const __nv_bfloat16* x = qkv + b * ldq + ((long long)warp * H + h) * D;
     const float *cs = cosT + (long long)pos * (D / 2), *sn = sinT + (long long)pos * (D / 2);
@@ -661,7 +693,7 @@ __global__ void __launch_bounds__(32 * AW, D == 128 ? 3 : 4) kv8_attn_kernel(con
       o += w * sm.acc[e][tid];
     }
   }
-  if (S > 1) {
+  if (active > 1) {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (tid < D) {
       const uint32_t to = map_to_rank(smem_u32(&sm.part[rank][0]), 0);
@@ -674,10 +706,10 @@ __global__ void __launch_bounds__(32 * AW, D == 128 ? 3 : 4) kv8_attn_kernel(con
     cluster_barrier();
     if (rank == 0 && tid < D) {
       M = -INFINITY;
-      for (int r = 0; r < S; ++r) M = fmaxf(M, sm.part[r][D + 1]);
+      for (int r = 0; r < active; ++r) M = fmaxf(M, sm.part[r][D + 1]);
       const float base = M == -INFINITY ? 0.f : M;
       L = o = 0.f;
-      for (int r = 0; r < S; ++r) {
+      for (int r = 0; r < active; ++r) {
         const float w = exp2_fast(sm.part[r][D + 1] - base);
         L += w * sm.part[r][D];
         o += w * sm.part[r][tid];
@@ -694,14 +726,16 @@ __global__ void __launch_bounds__(32 * AW, D == 128 ? 3 : 4) kv8_attn_kernel(con
   }
 }
 
-// CTAs of a cluster: doubled until there are one and a half for each SM, as long as the cache's length (the band's, if there is one) can give
-// every warp a turn.  us by 1 / 2 / 4 / 8 / 16 CTAs, heads of 128: 10 heads, 300 tokens 5.8 / 5.9 / 4.5 / 4.7 / 5.2, 2040 tokens 21 / 14 / 9.9 / 7.9 / 6.9;
-// 40 heads, 2040 tokens 22 / 15 / 11 / 9.4 / 14, 131000 tokens 1116 / 571 / 351 / 240 / 253; 160 heads, 2040 tokens 27 / 21 / 25 / 32 / 50; 320 heads,
-// 16000 tokens 233 / 245 / 242 / 245 / 272; 640 heads, 64 tokens 11 / 16 / 31 / 59 / 133, 2040 tokens 68 / 63 / 82 / 109 / 185.
+// CTAs of a cluster: doubled until there are one and a half for each SM (three for caches from 32768 tokens on), as long as the cache's
+// length (the band's, if there is one) can give every warp a turn.  us by 1 / 2 / 4 / 8 / 16 CTAs, heads of 128: 10 heads, 300 tokens
+// 5.8 / 6.1 / 5.0 / 5.0 / 5.4, 2040 tokens 21 / 14 / 9.8 / 7.8 / 6.9; 40 heads, 2040 tokens 22 / 15 / 12 / 10 / 14, 131000 tokens 1113 / 571 / 354 / 240 / 245;
+// 160 heads, 2040 tokens 27 / 20 / 25 / 33 / 52; 320 heads, 16000 tokens 234 / 247 / 245 / 244 / 274; 640 heads, 64 tokens 11 / 16 / 22 / 30 / 62, 2040 tokens
+// 67 / 63 / 81 / 111 / 196.  40 heads over 4 sequences of 32768 to 131072 tokens by 8 / 16 187 / 162.
 inline int kv8_splits(int B, int H, int D, int cap, int window_tiles, int sms) {
   const long long tokens = window_tiles > 0 && window_tiles < cap / 128 ? window_tiles * 128ll : cap;
+  const long long ctas = tokens >= 32768 ? 3ll * sms : 3ll * sms / 2;
   int s = 1;
-  while (s < kMaxSplit && 2ll * B * H * s < 3ll * sms && tokens >= (long long)s * AW * (4096 / D)) s *= 2;
+  while (s < kMaxSplit && (long long)B * H * s < ctas && tokens >= (long long)s * AW * (4096 / D)) s *= 2;
   return s;
 }
 
@@ -716,7 +750,7 @@ struct AttnArgs {
   __nv_bfloat16* y;
   int H, cap;
   float scale2;
-  int window_tiles;
+  int window_tiles, by_length;
 };
 template <int D>
 int launch_kv8_attn(const AttnArgs& p, int B, int split, int pdl, cudaStream_t s) {
@@ -732,7 +766,7 @@ int launch_kv8_attn(const AttnArgs& p, int B, int split, int pdl, cudaStream_t s
   cfg.attrs = at;
   cfg.numAttrs = (unsigned)dec_launch_attrs(at, split, pdl);
   return (int)cudaLaunchKernelEx(&cfg, kv8_attn_kernel<D>, p.qkv, p.ldq, p.cosT, p.sinT, p.rope_rows, p.c, p.pos, p.doc_start, p.y, p.H, p.cap, p.scale2,
-                                 p.window_tiles);
+                                 p.window_tiles, AW, p.by_length);
 }
 
 inline bool kv8_refused(const Kv8& c, int B, int H, int D, int cap) {
@@ -780,7 +814,7 @@ int bones_kv8_attention(const void* qkv, long long ldq, const float* cosT, const
   const Kv8 c{(int8_t*)k8, (int8_t*)v8, ks, vs, (__nv_bfloat16*)kt, (__nv_bfloat16*)vt};
   if (kv8_refused(c, B, H, D, cap) || !qkv || !cosT || !sinT || !y || misaligned16(qkv, y) || (B > 1 && ldq % 8) || window_tiles < 0) return -2;
   const AttnArgs p{(const __nv_bfloat16*)qkv, ldq, cosT, sinT, rope_rows, c, PerSeq{pos, pos_step, pos0}, doc_start, (__nv_bfloat16*)y, H, cap,
-                   scale * 1.4426950408889634f, window_tiles};
+                   scale * 1.4426950408889634f, window_tiles, B > 1 && B <= 64 && pos && pos_step && !pdl};
   int dev = 0, sms = 0;
   BONES_CHECK(cudaGetDevice(&dev));
   BONES_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
