@@ -364,3 +364,38 @@ def test_native_refusals():
     with pytest.raises(ValueError):
         ops.kv8_attention(torch.randn(2, 192, device="cuda").bfloat16(), cos.cpu(), cos.cpu(), c, 0, 1.0)
     assert not any(x.any() for x in c)
+
+
+def test_the_statement_s_path_on_the_gpu():
+    """The plain bodies run on the same cache and agree, within what the kernels' own tests allow."""
+    from them_bones_b200 import ops
+    from them_bones_b200.ref import functional as RF
+    torch.manual_seed(14)
+    b, h, d = 3, 2, 64
+    cos, sin = (x.cuda() for x in RF.rotary_tables(256, d, 10000.0))
+    qkv = torch.randn(b, 3 * h * d, device="cuda").bfloat16()
+    k, v = torch.randn(2, b, 70, h, d, device="cuda").bfloat16()
+    a, c = ops.kv8_cache(b, 256, h, d, "cuda"), ops.kv8_cache(b, 256, h, d, "cuda")
+    ops.kv8_append(a, k, v, 0)
+    y = ops.kv8_attention(qkv, cos, sin, a, 70, 0.1).float()
+    ops.set_reference_path(True)
+    try:
+        ops.kv8_append(c, k, v, 0)
+        w = ops.kv8_attention(qkv, cos, sin, c, 70, 0.1).float()
+        r = ops.kv8_read(c, 71, 71)
+    finally:
+        ops.set_reference_path(False)
+    # the new key may round to bf16 the other way in fp32; the rest is equal
+    assert all(torch.equal(x, z) for x, z in zip(a[:4], c[:4])) and torch.equal(a.v_open, c.v_open)
+    assert float((a.k_open.float() - c.k_open.float()).abs().max()) <= 2 ** -7 * 4 and float((y - w).abs().max()) <= 2 ** -7 * float(w.abs().max())
+    assert torch.equal(ops.kv8_read(a, 70, 70)[0], r[0][:, :70])
+
+
+def test_a_cache_as_a_plain_tuple():
+    from them_bones_b200 import ops
+    c = ops.kv8_cache(1, 64, 1, 64, "cuda")
+    k = torch.randn(1, 3, 1, 64, device="cuda").bfloat16()
+    ops.kv8_append(tuple(c), k, k, 0)
+    assert torch.equal(ops.kv8_read(tuple(c), 3, 3)[0], k)
+    with pytest.raises(ValueError):
+        ops.kv8_append(tuple(c), k[:, :, :, :32], k[:, :, :, :32], 0)

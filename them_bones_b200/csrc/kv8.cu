@@ -145,7 +145,7 @@ __device__ __forceinline__ void kv8_quantise_block(Piece piece, int8_t* __restri
   }
 }
 
-constexpr int kAppendThreads = 256;
+constexpr int kAppendThreads = 128;
 // Tokens pos .. pos + len of a sequence.  A CTA takes one block that the run touches, of the keys or of the values of one head; the first
 // one also stores what is left over for the open block, after it has read the tokens that were in it before.
 template <int D, bool VALUES>
@@ -169,7 +169,7 @@ __device__ __forceinline__ void kv8_append_block(const __nv_bfloat16* __restrict
 }
 
 template <int D>
-__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(Kv8 c, const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ v, long long kb,
+__global__ void __launch_bounds__(kAppendThreads, 8) kv8_append_kernel(Kv8 c, const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ v, long long kb,
                                                         long long kt, long long kh, long long vb, long long vt, long long vh, PerSeq pos_, PerSeq len_, int t,
                                                         int H, int cap) {
   __shared__ QuantShared sm;
@@ -205,8 +205,8 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, __nv_bfloat16* __r
     __syncthreads();
   }
   if (tid >= 2 * D) return;
-  int t, d;
-  kv8_unit<D>(tid, t, d);
+  // four tokens by eight dimensions a thread, whole rows a warp: what is written counts for more than the conflicts (four ways) of what is read
+  const int d = tid % (D / 8) * 8, t = tid / (D / 8) * 4;
   uint32_t w[4][2];                             // codes of four tokens by eight dimensions: by token, or four tokens to a word
   uint32_t x[8];
   if (some && !open) {

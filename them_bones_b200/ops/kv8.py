@@ -79,7 +79,7 @@ def check_per_sequence(x, b: int, name: str, device):
 def check_append(c: KV8, k, v, pos, lens):
     dims = b, h, t, d, dev, _ = check_cache(c)
     if k.dim() != 4 or v.shape != k.shape or k.shape[0] != b or k.shape[2] != h or k.shape[3] != d:
-        raise ValueError(f"8-bit cache: keys {tuple(k.shape)}, values {tuple(v.shape)}, cache {tuple(c.k.shape)}")
+        raise ValueError(f"8-bit cache: keys {tuple(k.shape)}, values {tuple(v.shape)}, cache {tuple(c[0].shape)}")
     if k.get_device() != dev or v.get_device() != dev or k.dtype is not v.dtype or not k.is_floating_point():
         raise ValueError("8-bit cache: keys and values of one floating type on the cache's device")
     check_per_sequence(pos, b, "pos", dev)
@@ -105,7 +105,7 @@ def check_read(c: KV8, held, length):
 def check_attention(qkv, cos, sin, c: KV8, pos, doc_start, window):
     dims = b, h, t, d, dev, _ = check_cache(c)
     if qkv.shape != (b, 3 * h * d) or qkv.get_device() != dev or not qkv.is_floating_point():
-        raise ValueError(f"8-bit attention: qkv {qkv.dtype} {tuple(qkv.shape)} on {qkv.device}, expected {(b, 3 * h * d)} on {c.k.device}")
+        raise ValueError(f"8-bit attention: qkv {qkv.dtype} {tuple(qkv.shape)} on {qkv.device}, expected {(b, 3 * h * d)} on {c[0].device}")
     for x in (cos, sin):
         if x.dim() != 2 or x.shape[1] != d // 2 or x.shape != cos.shape or x.get_device() != dev or not x.is_floating_point():
             raise ValueError(f"8-bit attention: rotary tables {tuple(cos.shape)}, {tuple(sin.shape)}, expected [positions, {d // 2}]")
@@ -113,7 +113,7 @@ def check_attention(qkv, cos, sin, c: KV8, pos, doc_start, window):
     if isinstance(pos, int) and not 0 <= pos < min(t, cos.shape[0]):
         raise ValueError(f"8-bit attention: position {pos}, capacity {t}, rotary tables of {cos.shape[0]}")
     if doc_start is not None and (doc_start.dtype is not torch.int32 or doc_start.shape != (b,) or doc_start.get_device() != dev or not doc_start.is_contiguous()):
-        raise ValueError(f"8-bit attention: doc_start is contiguous int32 [{b}] on {c.k.device}")
+        raise ValueError(f"8-bit attention: doc_start is contiguous int32 [{b}] on {c[0].device}")
     if window < 0 or window % 128:
         raise ValueError(f"8-bit attention: window {window} is not a multiple of 128")
     return dims
@@ -182,7 +182,7 @@ def attention(qkv, cos, sin, dims, pos, scale, doc_start, window):
     b, h, t, d, dev, _ = dims
     if qkv.stride(1) != 1 or (b > 1 and qkv.stride(0) % 8) or qkv.data_ptr() % 16:
         qkv = qkv.contiguous() if not qkv.is_contiguous() else qkv.clone()
-    y = torch.empty((b, h * d), dtype=torch.bfloat16, device=qkv.device)
+    y = qkv.new_empty((b, h * d))
     with L.device(dev):
         launch(qkv, _table(cos), _table(sin), dims, pos, scale, doc_start, window, y)
     COUNTS["kv8_attention"] += 1

@@ -47,10 +47,10 @@ def statement(logits, tokens, topk, vocab) -> TokenLogprobs:
 
 
 def _forward(z, tokens, topk, vocab, want_stats):
-    rows, dev = z.shape[0], z.device
-    given, entropy = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
-    top, ids = torch.empty((rows, topk), dtype=torch.float32, device=dev), torch.empty((rows, topk), dtype=torch.int64, device=dev)
-    stats = torch.empty((rows, 4), dtype=torch.float32, device=dev) if want_stats else None
+    rows = z.shape[0]
+    given = torch.empty(rows, dtype=torch.float32, device=z.device)
+    entropy, top, ids = given.new_empty(rows), given.new_empty((rows, topk)), tokens.new_empty((rows, topk))
+    stats = given.new_empty((rows, 4)) if want_stats else None
     with L.device(z.get_device()):
         L.call("bones_logprobs_fwd", z.data_ptr(), z.stride(0), int(z.dtype is torch.float32), rows, vocab, tokens.data_ptr(), topk, given.data_ptr(),
                entropy.data_ptr(), top.data_ptr(), ids.data_ptr(), stats.data_ptr() if want_stats else 0, L.raw_stream())
