@@ -6,6 +6,7 @@ required on a GPU: a missing or unloadable library raises here rather than letti
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -70,21 +71,12 @@ def raw_stream() -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
-class device:
-    """``with device(index)``: CUDA calls on that device, as ``torch.cuda.device`` but without a switch where it is the current one."""
-    __slots__ = ("_to", "_back")
+_HERE = contextlib.nullcontext()
 
-    def __init__(self, index: int):
-        self._to = index
 
-    def __enter__(self):
-        self._back = torch._C._cuda_getDevice()
-        if self._back != self._to:
-            torch.cuda.set_device(self._to)
-
-    def __exit__(self, *_):
-        if self._back != self._to:
-            torch.cuda.set_device(self._back)
+def device(index: int):
+    """``with device(index)``: CUDA calls on that device; nothing to do where it is the current one."""
+    return _HERE if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
 def ptr(t):

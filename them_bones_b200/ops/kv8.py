@@ -70,9 +70,10 @@ def check_cache(c: KV8):
 
 def check_per_sequence(x, b: int, name: str, device):
     """An int, or int32 of one value or of one for each sequence on the cache's device (an index, -1 for the host)."""
-    if isinstance(x, int):
+    if type(x) is int:
         return
-    if not isinstance(x, torch.Tensor) or x.dtype is not torch.int32 or x.get_device() != device or x.numel() not in (1, b) or x.dim() > 1 or not x.is_contiguous():
+    n = x.numel() if isinstance(x, torch.Tensor) else 0
+    if (n != b and n != 1) or x.dtype is not torch.int32 or x.get_device() != device or x.dim() > 1 or not x.is_contiguous():
         raise ValueError(f"8-bit cache: {name} is an int or contiguous int32 of 1 or {b} values on the cache's device")
 
 
@@ -106,11 +107,12 @@ def check_attention(qkv, cos, sin, c: KV8, pos, doc_start, window):
     dims = b, h, t, d, dev, _ = check_cache(c)
     if qkv.shape != (b, 3 * h * d) or qkv.get_device() != dev or not qkv.is_floating_point():
         raise ValueError(f"8-bit attention: qkv {qkv.dtype} {tuple(qkv.shape)} on {qkv.device}, expected {(b, 3 * h * d)} on {c[0].device}")
-    for x in (cos, sin):
-        if x.dim() != 2 or x.shape[1] != d // 2 or x.shape != cos.shape or x.get_device() != dev or not x.is_floating_point():
-            raise ValueError(f"8-bit attention: rotary tables {tuple(cos.shape)}, {tuple(sin.shape)}, expected [positions, {d // 2}]")
+    shape = cos.shape
+    if (len(shape) != 2 or shape[1] != d // 2 or sin.shape != shape or cos.get_device() != dev or sin.get_device() != dev or not cos.is_floating_point()
+            or not sin.is_floating_point()):
+        raise ValueError(f"8-bit attention: rotary tables {tuple(cos.shape)}, {tuple(sin.shape)}, expected [positions, {d // 2}]")
     check_per_sequence(pos, b, "pos", dev)
-    if isinstance(pos, int) and not 0 <= pos < min(t, cos.shape[0]):
+    if type(pos) is int and not 0 <= pos < min(t, shape[0]):
         raise ValueError(f"8-bit attention: position {pos}, capacity {t}, rotary tables of {cos.shape[0]}")
     if doc_start is not None and (doc_start.dtype is not torch.int32 or doc_start.shape != (b,) or doc_start.get_device() != dev or not doc_start.is_contiguous()):
         raise ValueError(f"8-bit attention: doc_start is contiguous int32 [{b}] on {c[0].device}")
@@ -119,8 +121,8 @@ def check_attention(qkv, cos, sin, c: KV8, pos, doc_start, window):
     return dims
 
 
-def no_gradient(*tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+def no_gradient(x, y=None):
+    if (x.requires_grad or (y is not None and y.requires_grad)) and torch.is_grad_enabled():
         raise ValueError("8-bit cache: its operators have no gradient; call them under torch.no_grad()")
 
 
@@ -133,7 +135,7 @@ def numbers(x, b: int):
 # -- native bodies -----------------------------------------------------------------------------------------------------
 def _per(x):
     """Address, distance from one sequence's value to the next's and the value itself where there is no address."""
-    return (0, 0, x) if isinstance(x, int) else (x.data_ptr(), 0 if x.numel() == 1 else 1, 0)
+    return (0, 0, x) if type(x) is int else (x.data_ptr(), 0 if x.numel() == 1 else 1, 0)
 
 
 def _rows16(x):
