@@ -316,22 +316,35 @@ __device__ __forceinline__ T turn_and_norm(const __nv_bfloat16* __restrict__ x, 
 }
 
 // The sequence with the n-th largest number of tokens to see, of 64 at most: CTAs begin in the order of their numbers, and the longest ones
-// are not to begin last (64 sequences of 1 to 2048 tokens in documents, 10 heads: 31 us for 35; 4 of 32768 to 131072: 162 for 170).  Every
-// warp works it out for itself, from what nothing writes meanwhile: not where the kernel before this one may still run.
+// are not to begin last (64 sequences of 1 to 2048 tokens in documents, 10 heads: 30 us for 35; 4 of 32768 to 131072: 160 for 170; where all
+// are alike it costs the look, 12.3 for 11.3 at 64 tokens each).  Every warp works it out for itself, from what nothing writes meanwhile:
+// not where the kernel before this one may still run.
 __device__ __forceinline__ int longest_first(int B, int n, PerSeq pos, const int* __restrict__ doc_start) {
   const int lane = threadIdx.x & 31;
-  uint32_t key[2];
+  uint32_t key[2], most = 0, least = ~0u;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int b = lane + 32 * i;
     const int p = b < B ? pos[b] : -1, lo = b < B && doc_start ? doc_start[b] : 0;
-    key[i] = b < B ? (uint32_t)min(max(p - max(lo, 0) + 1, 0), 1 << 25) << 6 | (uint32_t)(63 - b) : 0u;          // no two are equal
+    const uint32_t len = (uint32_t)min(max(p - max(lo, 0) + 1, 0), 1 << 25);
+    if (b < B) { most = max(most, len); least = min(least, len); }
+    key[i] = b < B ? len << 6 | (uint32_t)(63 - b) : 0u;             // no two are equal
   }
+  if (__reduce_max_sync(0xffffffffu, most) - __reduce_min_sync(0xffffffffu, least) < 2 * KB) return n;         // much the same length
   int r0 = 0, r1 = 0;
-  for (int j = 0; j < B; ++j) {
-    const uint32_t k = __shfl_sync(0xffffffffu, j < 32 ? key[0] : key[1], j & 31);
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const uint32_t k = __shfl_sync(0xffffffffu, key[0], j);
     r0 += k > key[0];
     r1 += k > key[1];
+  }
+  if (B > 32) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const uint32_t k = __shfl_sync(0xffffffffu, key[1], j);
+      r0 += k > key[0];
+      r1 += k > key[1];
+    }
   }
   const unsigned a = __ballot_sync(0xffffffffu, lane < B && r0 == n), c = __ballot_sync(0xffffffffu, lane + 32 < B && r1 == n);
   return a ? __ffs(a) - 1 : 31 + __ffs(c);
