@@ -131,8 +131,11 @@ def test_attention(b, h, d, cap, pos, start, window):
     _attend_case(b, h, d, cap, pos, start, window)
 
 
-def test_one_position_for_all():
-    _attend_case(5, 2, 128, 256, [191] * 5, None, 0, shared=True)
+@pytest.mark.parametrize("b,h,d,cap,pos,start", [(5, 2, 128, 256, 191, None), (130, 5, 64, 256, 191, None), (64, 10, 128, 320, 300, "some"), (90, 8, 128, 128, 63, None),
+                                                  (500, 1, 64, 128, 5, None), (64, 9, 64, 1024, 990, "some"), (64, 9, 64, 2048, 1990, "some")])
+def test_one_position_for_all(b, h, d, cap, pos, start):
+    """Also as many sequences as the kernel has a form of its own for."""
+    _attend_case(b, h, d, cap, [pos] * b, None if start is None else [i * pos // b for i in range(b)], 0, shared=True)
 
 
 def test_sequences_outside_and_queries_that_see_nothing():

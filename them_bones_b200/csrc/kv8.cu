@@ -258,7 +258,6 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, __nv_bfloat16* __r
 // two byte permutations and two subtractions for four of them.  The query is two fp16 numbers, hi and lo, in alternate columns of
 // B: the scores lose nothing to it.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int AW = 4;                           // warps of a CTA
 constexpr int kMaxSplit = 16;                   // CTAs of a cluster
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -350,7 +349,7 @@ __device__ __forceinline__ int longest_first(int B, int n, PerSeq pos, const int
   return a ? __ffs(a) - 1 : 31 + __ffs(c);
 }
 
-template <int D>
+template <int D, int AW>
 struct __align__(16) AttnShared {
   float acc[2 * AW][D];                         // full blocks of each warp, then the open block's part of each
   float part[kMaxSplit][D + 4];                 // every CTA's output, sum and maximum, in the first CTA
@@ -359,17 +358,17 @@ struct __align__(16) AttnShared {
   float m[2 * AW], l[2 * AW];
 };
 
-template <int D>
-__global__ void __launch_bounds__(32 * AW, D == 128 ? 3 : 4) kv8_attn_kernel(const __nv_bfloat16* __restrict__ qkv, long long ldq, const float* __restrict__ cosT,
+template <int D, int AW>
+__global__ void __launch_bounds__(32 * AW, (D == 128 ? 12 : 16) / AW) kv8_attn_kernel(const __nv_bfloat16* __restrict__ qkv, long long ldq, const float* __restrict__ cosT,
                                                               const float* __restrict__ sinT, int rope_rows, Kv8 c, PerSeq pos_, const int* doc_start,
                                                               __nv_bfloat16* __restrict__ y, int H, int cap, float scale2, int window_tiles, int least, int by_length) {
   constexpr int TT = 4096 / D, PER = TT / 8, VW = TT / 16;                // tokens of a turn, of a lane; words of a lane's piece of V
   constexpr int KL = D / 64, NT = D / 16, LPT = D / 8, TPI = 32 / LPT, RP = 4, PASS = KB / (AW * TPI * RP);
   __shared__ union {
-    AttnShared<D> at;
+    AttnShared<D, AW> at;
     QuantShared quant;
   } sm_;
-  AttnShared<D>& sm = sm_.at;
+  AttnShared<D, AW>& sm = sm_.at;
   pdl_launch();
   const int S = (int)cluster_size(), rank = (int)cluster_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -381,7 +380,8 @@ __global__ void __launch_bounds__(32 * AW, D == 128 ? 3 : 4) kv8_attn_kernel(con
   __nv_bfloat16* out = y + ((long long)b * H + h) * D;
   if (pos < 0 || pos >= min(cap, rope_rows)) {
     pdl_wait();
-    if (rank == 0 && tid < D / 2) reinterpret_cast<uint32_t*>(out)[tid] = 0u;
+    if (rank == 0)
+      for (int i = tid; i < D / 2; i += 32 * AW) reinterpret_cast<uint32_t*>(out)[i] = 0u;
     return;
   }
   if (S > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // waited for before the first store to another CTA
@@ -446,10 +446,10 @@ __global__ void __launch_bounds__(32 * AW, D == 128 ? 3 : 4) kv8_attn_kernel(con
     }
   }
   const int step = active * AW;
-  if (warp < (tail_cta ? 3 : 1)) {
-    const __nv_bfloat16* x = qkv + b * ldq + ((long long)warp * H + h) * D;
+  for (int role = warp; role < (tail_cta ? 3 : 1); role += AW) {      // query, new key, new value
+    const __nv_bfloat16* x = qkv + b * ldq + ((long long)role * H + h) * D;
     const float *cs = cosT + (long long)pos * (D / 2), *sn = sinT + (long long)pos * (D / 2);
-    if (warp == 0) {
+    if (role == 0) {
       float a[D / 64], e[D / 64];
       const float r = turn_and_norm<D, float>(x, cs, sn, a, e);
 #pragma unroll
@@ -458,8 +458,8 @@ __global__ void __launch_bounds__(32 * AW, D == 128 ? 3 : 4) kv8_attn_kernel(con
         sm.q[lane + 32 * i + D / 2] = e[i] * r;
       }
     } else {
-      __nv_bfloat16 *tail = (warp == 1 ? c.kt : c.vt) + (bh * KB + slot) * D, v0[D / 64], v1[D / 64];
-      if (warp == 1) {                          // in 64 bits: the key's rounding to bf16 is the only one, and it stays
+      __nv_bfloat16 *tail = (role == 1 ? c.kt : c.vt) + (bh * KB + slot) * D, v0[D / 64], v1[D / 64];
+      if (role == 1) {                          // in 64 bits: the key's rounding to bf16 is the only one, and it stays
         double a[D / 64], e[D / 64];
         const double r = turn_and_norm<D, double>(x, cs, sn, a, e);
 #pragma unroll
@@ -477,8 +477,8 @@ __global__ void __launch_bounds__(32 * AW, D == 128 ? 3 : 4) kv8_attn_kernel(con
 #pragma unroll
       for (int i = 0; i < D / 64; ++i) {
         const int d = lane + 32 * i;
-        sm.fresh[warp - 1][d] = v0[i];
-        sm.fresh[warp - 1][d + D / 2] = v1[i];
+        sm.fresh[role - 1][d] = v0[i];
+        sm.fresh[role - 1][d + D / 2] = v1[i];
         tail[d] = v0[i];
         tail[d + D / 2] = v1[i];
       }
@@ -695,41 +695,47 @@ __global__ void __launch_bounds__(32 * AW, D == 128 ? 3 : 4) kv8_attn_kernel(con
   __syncthreads();
 
   // The CTA's own parts, then the cluster's.  A part without a token has -inf and 0.
+  constexpr int OUT = (D + 32 * AW - 1) / (32 * AW);                      // dimensions of a thread
   const int parts = tail_cta ? 2 * AW : AW;
-  float M = -INFINITY, L = 0.f, o = 0.f;
-  if (tid < D) {
-    for (int e = 0; e < parts; ++e) M = fmaxf(M, sm.m[e]);
+  float M = -INFINITY, L = 0.f, o[OUT] = {};
+  auto sum_up = [&](int n, auto maximum, auto sum, auto values) {
+    M = -INFINITY;
+    for (int e = 0; e < n; ++e) M = fmaxf(M, maximum(e));
     const float base = M == -INFINITY ? 0.f : M;
-    for (int e = 0; e < parts; ++e) {
-      const float w = exp2_fast(sm.m[e] - base);
-      L += w * sm.l[e];
-      o += w * sm.acc[e][tid];
+    L = 0.f;
+#pragma unroll
+    for (int i = 0; i < OUT; ++i) o[i] = 0.f;
+    for (int e = 0; e < n; ++e) {
+      const float w = exp2_fast(maximum(e) - base);
+      L += w * sum(e);
+#pragma unroll
+      for (int i = 0; i < OUT; ++i)
+        if (tid + 32 * AW * i < D) o[i] += w * values(e)[tid + 32 * AW * i];
     }
-  }
+  };
+  sum_up(parts, [&](int e) { return sm.m[e]; }, [&](int e) { return sm.l[e]; }, [&](int e) { return sm.acc[e]; });
   if (active > 1) {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (tid < D) {
-      const uint32_t to = map_to_rank(smem_u32(&sm.part[rank][0]), 0);
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4u * (uint32_t)tid), "f"(o) : "memory");
-      if (tid == 0) {
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4u * D), "f"(L) : "memory");
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4u * D + 4u), "f"(M) : "memory");
-      }
+    const uint32_t to = map_to_rank(smem_u32(&sm.part[rank][0]), 0);
+#pragma unroll
+    for (int i = 0; i < OUT; ++i) {
+      const int d = tid + 32 * AW * i;
+      if (d < D) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4u * (uint32_t)d), "f"(o[i]) : "memory");
+    }
+    if (tid == 0) {
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4u * D), "f"(L) : "memory");
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4u * D + 4u), "f"(M) : "memory");
     }
     cluster_barrier();
-    if (rank == 0 && tid < D) {
-      M = -INFINITY;
-      for (int r = 0; r < active; ++r) M = fmaxf(M, sm.part[r][D + 1]);
-      const float base = M == -INFINITY ? 0.f : M;
-      L = o = 0.f;
-      for (int r = 0; r < active; ++r) {
-        const float w = exp2_fast(sm.part[r][D + 1] - base);
-        L += w * sm.part[r][D];
-        o += w * sm.part[r][tid];
-      }
+    if (rank == 0) sum_up(active, [&](int r) { return sm.part[r][D + 1]; }, [&](int r) { return sm.part[r][D]; }, [&](int r) { return sm.part[r]; });
+  }
+  if (rank == 0) {
+#pragma unroll
+    for (int i = 0; i < OUT; ++i) {
+      const int d = tid + 32 * AW * i;
+      if (d < D) out[d] = __float2bfloat16(L != 0.f ? o[i] / L : 0.f);
     }
   }
-  if (rank == 0 && tid < D) out[tid] = __float2bfloat16(L != 0.f ? o / L : 0.f);
   if (tail_cta && slot == KB - 1) {
     // the block is full: its last token is in memory since the first barrier of the CTA
     __syncthreads();
@@ -744,7 +750,7 @@ __global__ void __launch_bounds__(32 * AW, D == 128 ? 3 : 4) kv8_attn_kernel(con
 // 5.8 / 6.1 / 5.0 / 5.0 / 5.4, 2040 tokens 21 / 14 / 9.8 / 7.8 / 6.9; 40 heads, 2040 tokens 22 / 15 / 12 / 10 / 14, 131000 tokens 1113 / 571 / 354 / 240 / 245;
 // 160 heads, 2040 tokens 27 / 20 / 25 / 33 / 52; 320 heads, 16000 tokens 234 / 247 / 245 / 244 / 274; 640 heads, 64 tokens 11 / 16 / 22 / 30 / 62, 2040 tokens
 // 67 / 63 / 81 / 111 / 196.  40 heads over 4 sequences of 32768 to 131072 tokens by 8 / 16 187 / 162.
-inline int kv8_splits(int B, int H, int D, int cap, int window_tiles, int sms) {
+inline int kv8_splits(int B, int H, int D, int AW, int cap, int window_tiles, int sms) {
   const long long tokens = window_tiles > 0 && window_tiles < cap / 128 ? window_tiles * 128ll : cap;
   const long long ctas = tokens >= 32768 ? 3ll * sms : 3ll * sms / 2;
   int s = 1;
@@ -765,11 +771,11 @@ struct AttnArgs {
   float scale2;
   int window_tiles, by_length;
 };
-template <int D>
+template <int D, int AW>
 int launch_kv8_attn(const AttnArgs& p, int B, int split, int pdl, cudaStream_t s) {
   static OncePerDevice once;
   BONES_ONCE(once, {
-    BONES_CHECK(cudaFuncSetAttribute(kv8_attn_kernel<D>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    BONES_CHECK(cudaFuncSetAttribute(kv8_attn_kernel<D, AW>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   });
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
@@ -778,7 +784,7 @@ int launch_kv8_attn(const AttnArgs& p, int B, int split, int pdl, cudaStream_t s
   cfg.stream = s;
   cfg.attrs = at;
   cfg.numAttrs = (unsigned)dec_launch_attrs(at, split, pdl);
-  return (int)cudaLaunchKernelEx(&cfg, kv8_attn_kernel<D>, p.qkv, p.ldq, p.cosT, p.sinT, p.rope_rows, p.c, p.pos, p.doc_start, p.y, p.H, p.cap, p.scale2,
+  return (int)cudaLaunchKernelEx(&cfg, kv8_attn_kernel<D, AW>, p.qkv, p.ldq, p.cosT, p.sinT, p.rope_rows, p.c, p.pos, p.doc_start, p.y, p.H, p.cap, p.scale2,
                                  p.window_tiles, AW, p.by_length);
 }
 
@@ -831,8 +837,13 @@ int bones_kv8_attention(const void* qkv, long long ldq, const float* cosT, const
   int dev = 0, sms = 0;
   BONES_CHECK(cudaGetDevice(&dev));
   BONES_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  const int split = kv8_splits(B, H, D, cap, window_tiles, sms);
+  // Two warps a CTA where sequences of one length make more CTAs of four than the SMs hold (three each) and the cache is short: twice as many,
+  // smaller ones fit at once, but the longest take twice the time.  640 heads, us by four / two: alone, 64 tokens 11.8 / 8.2, lengths from 1 to
+  // 2048 37 / 53; a step of 20 layers at 64 tokens 715 / 645, at 500 948 / 944, at 1900 1730 / 1866.
+  const int aw = (long long)B * H > 3ll * sms && !(pos && pos_step) && cap <= 1024 ? 2 : 4;
+  const int split = kv8_splits(B, H, D, aw, cap, window_tiles, sms);
   cudaStream_t s = (cudaStream_t)stream;
-  return D == 128 ? launch_kv8_attn<128>(p, B, split, pdl, s) : launch_kv8_attn<64>(p, B, split, pdl, s);
+  if (aw == 2) return D == 128 ? launch_kv8_attn<128, 2>(p, B, split, pdl, s) : launch_kv8_attn<64, 2>(p, B, split, pdl, s);
+  return D == 128 ? launch_kv8_attn<128, 4>(p, B, split, pdl, s) : launch_kv8_attn<64, 4>(p, B, split, pdl, s);
 }
 }  // extern "C"
