@@ -177,6 +177,29 @@ def test_head_gradient_that_the_weight_owns():
         assert not ops.lmhead_logprobs(x, w, tokens, 250, 15.0).logprob.requires_grad
 
 
+def test_head_rows_and_weights_that_lie_anywhere():
+    from them_bones_b200 import ops
+    torch.manual_seed(2)
+    x, w = torch.randn(2, 9, 65, device="cuda").bfloat16(), (0.3 * torch.randn(65, 129, device="cuda")).bfloat16()
+    tokens = torch.randint(0, 120, (2, 9), device="cuda")
+    for xv, wv in ((x[:, ::2, 1:], w[:64, :128].T), (x[..., :64].transpose(0, 1).transpose(0, 1), w[1:, 1:].T), (x[:, :, :64], w.T[:128, 1:])):
+        leaves = [t.detach().requires_grad_() for t in (xv, wv)]
+        plain = [t.detach().clone(memory_format=torch.contiguous_format).requires_grad_() for t in (xv, wv)]
+        tk = tokens[:, :xv.shape[1]]
+        a, b = (ops.lmhead_logprobs(*t, tk, 120, 15.0, 3) for t in (leaves, plain))
+        assert a.logprob.shape == tk.shape and all(torch.equal(p, q) for p, q in zip(a, b))
+        for p, q in zip(torch.autograd.grad(a.logprob.sum(), leaves), torch.autograd.grad(b.logprob.sum(), plain)):
+            assert p.shape == q.shape and float((p.float() - q.float()).norm()) <= 2 ** -8 * float(q.float().norm())
+
+
+def test_head_of_no_rows():
+    from them_bones_b200 import ops
+    x, w = torch.randn(0, 64, device="cuda").bfloat16().requires_grad_(), torch.randn(128, 64, device="cuda").bfloat16().requires_grad_()
+    r = ops.lmhead_logprobs(x, w, torch.zeros(0, dtype=torch.int64, device="cuda"), 120, 15.0, 2)
+    dx, dw = torch.autograd.grad(r.entropy.sum(), [x, w])
+    assert r.top_id.shape == (0, 2) and dx.shape == (0, 64) and not dw.any()
+
+
 def test_head_batched_and_recorded_gradients():
     from them_bones_b200 import ops
     torch.manual_seed(1)

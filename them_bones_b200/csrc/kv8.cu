@@ -146,6 +146,8 @@ __device__ __forceinline__ void kv8_quantise_block(Piece piece, int8_t* __restri
 }
 
 constexpr int kAppendThreads = 128;
+// Bound by bytes: 2 read and 1 written for each value.  4 x 16384 tokens of 10 heads of 128, keys and values, 84 us (6.0 TB/s, 0.91 of the copy
+// rate); CTAs of 256 threads, which wait for their slowest load twice as often, 95 to 107.
 // Tokens pos .. pos + len of a sequence.  A CTA takes one block that the run touches, of the keys or of the values of one head; the first
 // one also stores what is left over for the open block, after it has read the tokens that were in it before.
 template <int D, bool VALUES>
@@ -183,7 +185,8 @@ __global__ void __launch_bounds__(kAppendThreads, 8) kv8_append_kernel(Kv8 c, co
     kv8_append_block<D, false>(k + b * kb + h * kh, kt, c.k + bh * cap * D, c.ks + bh * nb, c.kt + bh * KB * D, pos, len, i, sm);
 }
 
-// One block of one head back to bf16 rows [B, length, H, D]; zeros behind the tokens held.
+// One block of one head back to bf16 rows [B, length, H, D]; zeros behind the tokens held.  Bound by bytes, two thirds of them written:
+// 4 x 16384 tokens of 10 heads of 128 in 96 us (0.80 of the copy rate).
 template <int D>
 __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, __nv_bfloat16* __restrict__ k, __nv_bfloat16* __restrict__ v, PerSeq held_, int length, int H, int cap) {
   __shared__ __align__(16) uint8_t turn[D * kTurnRow];
@@ -256,7 +259,15 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, __nv_bfloat16* __r
 // tcgen05 would want its operands in shared memory and 64 rows of queries, and there is one): the codes' rows are the MMA's rows,
 // and a lane's consecutive bytes of a row are its columns of several MMAs, so that codes go from memory to the operands with
 // two byte permutations and two subtractions for four of them.  The query is two fp16 numbers, hi and lo, in alternate columns of
-// B: the scores lose nothing to it.
+// B: the scores lose nothing to it.  Probabilities are rounded to fp16 for the second product: half of 2^-10 of each at most, in both
+// directions, far below the rounding of the result to bf16; the sum that the result is divided by is of the unrounded ones in fp32.
+//
+// Bound by the bytes of the codes where there are enough turns for every warp: 4 sequences of 131000 tokens, 10 heads, 232 to 240 us (5.6 to 5.8
+// TB/s, 0.86 to 0.88 of the copy rate), 32 of 16000 228 to 234 (0.87).  A turn is 2000 clocks of a warp that is alone on its scheduler: 575
+// instructions, the two loads' latencies between them; three to a scheduler hide that.  Few or short sequences are bound by one turn after
+// the other and by the way in and out (4.8 us for 300 tokens).  Taken before it: a block of 64 tokens a turn and two CTAs an SM (4 x 131000
+// 273 us, 64 sequences of 64 tokens 17.4 for 10.3); the codes through shared memory, by each warp's own cp.async (250) or by bulk copies for
+// the CTA (259), which cost the walk more instructions than the deeper prefetch saved; four CTAs an SM, whose 128 registers spill (248).
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int kMaxSplit = 16;                   // CTAs of a cluster
 

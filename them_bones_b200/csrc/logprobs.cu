@@ -10,15 +10,21 @@
 // of groups of threads the k-th largest bounds the row's k-th largest logit from below, so only threads whose maximum reaches it hold an
 // alternative, and only their columns (a few percent of the row, still in L2) are looked at again.
 // Gradient: one element-wise pass; the few columns with a gradient of their own are written once more.
+//
+// Bound by bytes, and in bf16 nearly as much by the exponentials (64 % of the special-function units' rate): 4096 rows of 65536, forward 98 us
+// in bf16 (0.83 of the copy rate) and 158 in fp32 (1.03), with five alternatives 106 and 167; gradient 183 (0.90) and 326 (1.0).  One row takes 3.4 us,
+// with 20 alternatives 6.9: latencies of the choice, which has a barrier between any two of its steps.  Before, 4096 rows with five alternatives:
+// a pass for the maximum, one for the sums and one for each alternative 1580 us in fp32; one pass, and every thread's best column looked for
+// again 214 (146 in bf16); the columns of all rounds of the threads that hold one looked at again 193 (109).
 #include "decode_common.cuh"
 
 namespace bones {
 
-constexpr int LP_T = 128;                        // threads of a CTA
+constexpr int LP_T = 128;                       // threads of a CTA (256: as fast for long rows, 37 us for 27 where 4096 rows have 8192 columns)
 constexpr int LP_U = 4;                         // 16-byte vectors of a thread in flight
 constexpr int LP_TOP = 32;                      // alternatives at most
 constexpr int LP_GROUPS = 64;                   // of threads, whose maxima give the bound: two for each alternative at most
-constexpr int LP_BT = 256;                       // threads of the gradient's CTAs
+constexpr int LP_BT = 256;                      // threads of the gradient's CTAs
 constexpr int LP_CAND = 1024;                   // columns kept for the final choice; a row that needs more is gone over once for each alternative
 constexpr int LP_SPLIT = 16;                    // CTAs of a cluster, one row
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -145,8 +151,8 @@ struct LpShared {
   float group[LP_GROUPS], bound;
   LpSum warp[LP_T / 32], part[LP_SPLIT];
   int n_cand, n_round, n_hold;
-  int round[LP_T];                                 // thread | round << 8: columns of one round of a thread's
-  unsigned short hold[LP_T];                       // threads of which all columns are looked at
+  int round[LP_T];                              // thread | round << 8: columns of one round of a thread's
+  unsigned short hold[LP_T];                    // threads of which all columns are looked at
 };
 
 // Places among n keys: key i with fewer than k larger ones goes to out[that number].
@@ -477,7 +483,7 @@ __global__ void __launch_bounds__(LP_BT) logprobs_bwd_kernel(const Z* logits, lo
 }
 
 // CTAs of a cluster that share a row: doubled while there are few on an SM and every thread keeps two vectors; 16 only for a few rows.
-// us, bf16 rows of 65536, 8 alternatives: 64 rows by 8 / 16 CTAs 8.6 / 10.5, 512 rows by 1 / 2 26 / 22.
+// us, bf16 rows of 65536, 8 alternatives: 64 rows by 8 / 16 CTAs 9.5 / 10.5, 512 rows by 1 / 2 26 / 22.
 inline int lp_splits(long long rows, int V, int per, int sms) {
   int s = 1;
   while (s < LP_SPLIT && rows * s < (s < 8 ? 4 : 1) * sms && V >= 2 * s * LP_T * per) s *= 2;

@@ -59,14 +59,20 @@ def _forward(z, tokens, topk, vocab, want_stats):
 
 
 def _as_kernel(gs):
-    """Gradients as the kernel reads them: fp32, contiguous."""
-    return [None if g is None else g.float().contiguous() for g in gs]
+    """Gradients as the kernel reads them, fp32 and contiguous, and their addresses (0: none); None where one has no address (a batched
+    gradient) or a graph is being recorded: then the statement's own operators."""
+    if torch.is_grad_enabled():
+        return None
+    try:
+        gs = [g if g is None or (g.dtype is torch.float32 and g.is_contiguous()) else g.float().contiguous() for g in gs]
+        return gs, [0 if g is None else g.data_ptr() for g in gs]
+    except RuntimeError:
+        return None
 
 
-def _backward(z, tokens, ids, stats, vocab, gs, dz, cap):
-    g0, g1, g2 = (0 if g is None else g.data_ptr() for g in gs)
+def _backward(z, tokens, ids, stats, vocab, at, dz, cap):
     L.call("bones_logprobs_bwd", z.data_ptr(), z.stride(0), int(z.dtype is torch.float32), z.shape[0], vocab, z.shape[1], tokens.data_ptr(), ids.shape[1],
-           ids.data_ptr(), stats.data_ptr(), g0, g1, g2, dz.data_ptr(), dz.stride(0), cap, L.raw_stream())
+           ids.data_ptr(), stats.data_ptr(), at[0], at[1], at[2], dz.data_ptr(), dz.stride(0), cap, L.raw_stream())
 
 
 class _LogprobsFn(torch.autograd.Function):
@@ -81,19 +87,16 @@ class _LogprobsFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_given, g_entropy, g_top, _g_ids):
-        from .cuda import _by_address
         z, tokens, ids, stats = ctx.saved_tensors
-        k = ids.shape[1]
-        gs = [g_given, g_entropy, g_top if k else None]
-        if all(g is None for g in gs):
+        gs = [g_given, g_entropy, g_top if ids.shape[1] else None]
+        if g_given is None and g_entropy is None and gs[2] is None:
             return None, None, None, None
-        if not all(_by_address(g) for g in gs + [z] if g is not None):
-            # batched gradients, or a graph recorded through this one: the statement's own operators
+        ready = _as_kernel(gs)
+        if ready is None:
             return _statement_grad(z, tokens, ids, ctx.vocab, *gs), None, None, None
-        gs = _as_kernel(gs)
         dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
         with L.device(z.get_device()):
-            _backward(z, tokens, ids, stats, ctx.vocab, gs, dz, 0.0)
+            _backward(z, tokens, ids, stats, ctx.vocab, ready[1], dz, 0.0)
         return dz, None, None, None
 
 
@@ -172,11 +175,12 @@ class _HeadLogprobsFn(torch.autograd.Function):
         none = (None,) * 5
         if all(g is None for g in gs):
             return None, None, *none
-        if not all(C._by_address(g) for g in gs + [x, w] if g is not None):
+        ready, m = _as_kernel(gs), x.shape[0]
+        if ready is None:
             z = RF.softcap_logits(torch.nn.functional.linear(x.float(), w.float()), ctx.cap)
             d = _statement_grad(z, tokens, ids, ctx.vocab, *gs) * (1 - (z / ctx.cap).square())
             return (d @ w.float()).to(x.dtype), (d.transpose(-1, -2) @ x.float()).to(w.dtype), *none
-        gs, m = _as_kernel(gs), x.shape[0]
+        gs = ready[0]
         need_x, need_w = ctx.needs_input_grad[:2]
         dx = torch.zeros(x.shape, dtype=torch.float32, device=x.device) if need_x else None
         dw = ctx.main_grad if ctx.main_grad is not None or not need_w else torch.zeros(w.shape, dtype=torch.float32, device=w.device)
@@ -186,7 +190,7 @@ class _HeadLogprobsFn(torch.autograd.Function):
                 n = min(C.LOSS_ROWS, m - a)
                 z = buf[:n]
                 _capped(x[a:a + n], w, ctx.cap, z)
-                _backward(z, tokens[a:a + n], ids[a:a + n], stats[a:a + n], ctx.vocab, [None if g is None else g[a:a + n] for g in gs], z, ctx.cap)
+                _backward(z, tokens[a:a + n], ids[a:a + n], stats[a:a + n], ctx.vocab, [0 if g is None else g[a:a + n].data_ptr() for g in gs], z, ctx.cap)
                 if need_x:
                     C.mm_nn_acc(z, w, dx[a:a + n])
                 if need_w:
@@ -205,7 +209,9 @@ def head_native(x, w, tokens, topk, vocab, cap) -> TokenLogprobs:
         raise ValueError(f"native lmhead_logprobs does not cover this call: {x.dtype} {tuple(x.shape)}, head {w.dtype} {tuple(w.shape)}, cap {cap} "
                          "(bf16, rows of whole 16 bytes, a soft-cap)")
     shp, x2, tk = x.shape[:-1], _c(x).view(-1, x.shape[-1]), tokens.reshape(-1).to(torch.int64).contiguous()
-    x2, w = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (x2, w))
+    x2 = x2 if x2.data_ptr() % 16 == 0 else x2.clone()
+    if w.stride(1) != 1 or w.stride(0) % 8 or w.data_ptr() % 16:
+        w = w.clone(memory_format=torch.contiguous_format)
     with L.device(x.get_device()):
         r = _HeadLogprobsFn.apply(x2, w, tk, topk, vocab, float(cap), torch.is_grad_enabled() and (x.requires_grad or w.requires_grad))
     return TokenLogprobs(r[0].view(shp), r[1].view(shp), r[2].view(*shp, topk), r[3].view(*shp, topk))
