@@ -160,6 +160,49 @@ def test_columns_masked_with_the_lowest_number(rows, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 300])
+@pytest.mark.parametrize("mask", [-1e4, -1e7, -2e7, -9e7, -2e8, -1e9, -1e10, -1e20, -1e30, -3e38])
+def test_masks_of_any_depth(mask, rows, dtype):
+    """Threads that find nothing but masked columns for a while, and then others."""
+    from them_bones_b200 import ops
+    z = _logits(rows, 65536, dtype, seed=4)
+    z[:, :40000] = mask
+    z[:, 50000:65000] = mask
+    tokens = torch.full((rows,), 41000, device="cuda")
+    r = ops.token_logprobs(z, tokens, 5)
+    given, h, top, ids, _, _, _ = _exact(z, tokens, 5, 65536)
+    assert torch.equal(r.top_id, ids)
+    tol = 30 * 2 ** -24 * 2 + 2 ** 10 * 2 ** -24                           # as in `test_forward`
+    for got, want in ((r.logprob, given), (r.entropy, h), (r.top_logprob, top)):
+        assert float((got.double() - want).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 300])
+@pytest.mark.parametrize("size", [1e3, 3e6, 1.1e7, 1e8, 1e9, 1e12, 1e25, 1e30, 3e37, -1e3, -3e6, -1.1e7, -1e9, -1e12, -1e30, -3e37])
+def test_logits_of_any_size(size, rows, dtype):
+    """Rows around a large number: what counts is the distance from the largest, whatever it is."""
+    from them_bones_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(1)
+    step = 2.0 ** (torch.tensor(abs(size), dtype=torch.float64).log2().floor() - (7 if dtype == torch.bfloat16 else 23))       # of the type there
+    k = torch.randint(0, 9, (rows, 20000), device="cuda", generator=g)
+    z = (size - step * k).to(dtype)
+    assert torch.equal(z.double(), (size - step * k).to(dtype).double())
+    tokens = torch.randint(0, 20000, (rows,), device="cuda", generator=g)
+    x = z.clone().requires_grad_()
+    r = ops.token_logprobs(x, tokens, 5)
+    given, h, top, ids, _, _, _ = _exact(z, tokens, 5, 20000)
+    assert torch.equal(r.top_id, ids)
+    tol = 2 ** 10 * 2 ** -24 + 2 ** -18                                     # sums as in `test_forward`; distances are exact, and beyond 20 their exponentials count for nothing
+    for got, want in ((r.logprob, given), (r.entropy, h), (r.top_logprob, top)):
+        got, want = got.detach().double(), want
+        assert bool(((got - want).abs() <= tol + 2 ** -22 * want.abs()).all()), float((got - want).abs().max())
+    d, = torch.autograd.grad(r.logprob.sum() + r.entropy.sum(), [x])
+    want, p = _exact_grad(z, tokens, 0, 20000, [torch.ones(rows, device="cuda"), torch.ones(rows, device="cuda"), None])
+    assert bool(d.isfinite().all()) and bool(((d.double() - want).abs() <= torch.finfo(dtype).eps / 2 * want.abs() + 2 ** -12 * 31 * p + 2 ** -20).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_rows_that_lie_anywhere(dtype):
     from them_bones_b200 import ops
     big = _logits(12, 2011, dtype)

@@ -93,13 +93,14 @@ struct LpSum {
   }
 };
 
-// A thread's sums over its vectors, relative to 2^m2, m2 = m log2 e rounded: one operation between a logit and its exponent.  Good for
-// rows whose maximum is between -1e29 and 1e38 (`kLpFloor`, the maximum to begin with, is below); a thread that finds none goes over its
-// vectors again.  T is in units of log2.
-constexpr float kLpFloor = -1.578125f * 633825300114114700748351602688.0f;      // -1.0e30, the bf16 0xf14a
+// A thread's sums over its vectors, relative to 2^m2, m2 = m log2 e rounded: one operation between a logit and its exponent.  The rounding
+// of m2 moves all of a thread's exponents alike, by up to |m| 2^-24 log2 e: less than 1.5 for maxima within 2^24, which is what it is for
+// (from 2^30 on it would be more than an exponent holds).  The maximum begins at -2^24, so that a masked stretch never becomes one; a
+// thread whose own lies outside goes over its vectors again.  T is in units of log2.
+constexpr float kLpMost = 16777216.0f;
 struct LpStream {
   float m, m2, s, t;
-  __device__ __forceinline__ LpStream() : m(kLpFloor), m2(kLpFloor * kLog2e), s(0.f), t(0.f) {}
+  __device__ __forceinline__ LpStream() : m(-kLpMost), m2(-kLpMost * kLog2e), s(0.f), t(0.f) {}
   __device__ __forceinline__ void raise(float n) {
     const float n2 = n * kLog2e, d = fmaxf(m2 - n2, -1000.f), f = lp_exp2(d);
     t = f * fmaf(d, s, t);
@@ -139,7 +140,7 @@ __device__ __forceinline__ void lp_consume(LpStream& a, const uint4& u, __nv_bfl
   const uint32_t x[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t v;                                 // the same by twos, before they are unpacked
+    uint32_t v;                                 // the same by twos, before they are unpacked: -1e30
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(v) : "r"(x[i]), "r"(0xf14af14au));
     a.add(fmaf(__uint_as_float(v << 16), kLog2e, -a.m2));
     a.add(fmaf(__uint_as_float(v & 0xffff0000u), kLog2e, -a.m2));
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(LP_T, 10) logprobs_fwd_kernel(const Z* __restr
         if (i + j * LP_T < vecs) lp_consume(w, u[j], Z());
     }
     a = w.sum();
-    if (!(best > -1e29f && best < 1e38f)) {
+    if (!(best > -kLpMost && best < kLpMost)) {
       a = LpSum{-3.402823466e38f, 0.f, 0.f};
       if (best > a.m) a.m = best;
       for (int i = tid; i < vecs; i += LP_T) {
