@@ -170,6 +170,29 @@ def test_scales(scale):
 
 
 @pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bits", [10.5, 17.5, 25.5, 30.5])
+def test_many_small_probabilities_beside_a_large_one(bits, d):
+    """One key with a score `bits` above all others' and value 0, the others' value 1: the result is what the others weigh together."""
+    from them_bones_b200 import ops
+    b, h, n = 32, 10, 1990
+    eye, none = torch.ones(n + 1, d // 2, device="cuda"), torch.zeros(n + 1, d // 2, device="cuda")           # a rotation by nothing
+    k, v = torch.zeros(b, n, h, d, device="cuda", dtype=torch.bfloat16), torch.ones(b, n, h, d, device="cuda", dtype=torch.bfloat16)
+    k[..., d // 2:] = 1
+    peak = [(61 * i) % 1900 for i in range(b)]
+    for i, p in enumerate(peak):
+        k[i, p, :, :d // 2], k[i, p, :, d // 2:], v[i, p] = 1, 0, 0
+    cache = ops.kv8_cache(b, n + 1, h, d, "cuda")
+    ops.kv8_append(cache, k, v, 0)
+    qkv = torch.zeros(b, 3, h, d, device="cuda", dtype=torch.bfloat16)
+    qkv[:, 0, :, :d // 2], qkv[:, 1, :, d // 2:], qkv[:, 2] = 1, 1, 1
+    top = d // 2 * 2 ** 0.5                                                                # the query's norm makes its ones sqrt(2); a query sees its own key as the others
+    y = ops.kv8_attention(qkv.view(b, -1), eye, none, cache, n, bits * 0.6931471805599453 / top)
+    w = n * 2.0 ** -bits
+    # rounding to bf16 2^-8 at most; scores of 31 bits with 2^-20 of them 2^-15; probabilities by 2^-11 at most as fp16 (2^(15 - 30.5) is 362.04 of its smallest steps)
+    assert float((y.double() / (w / (1 + w)) - 1).abs().max()) <= 2 ** -8 + 2 ** -11 + 2 ** -14
+
+
+@pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_values_that_are_not_finite_reach_who_sees_them_only(d, bad):
     from them_bones_b200 import ops

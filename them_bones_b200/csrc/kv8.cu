@@ -259,8 +259,10 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, __nv_bfloat16* __r
 // tcgen05 would want its operands in shared memory and 64 rows of queries, and there is one): the codes' rows are the MMA's rows,
 // and a lane's consecutive bytes of a row are its columns of several MMAs, so that codes go from memory to the operands with
 // two byte permutations and two subtractions for four of them.  The query is two fp16 numbers, hi and lo, in alternate columns of
-// B: the scores lose nothing to it.  Probabilities are rounded to fp16 for the second product: half of 2^-10 of each at most, in both
-// directions, far below the rounding of the result to bf16; the sum that the result is divided by is of the unrounded ones in fp32.
+// B: the scores lose nothing to it.  Probabilities go into the second product as fp16, times 2^15, so that the largest is in
+// its top range: rounded by half of 2^-10 of each at most, in both directions, far below the rounding of the result to bf16, down to 2^-29
+// of the largest, and gone below 2^-40 (unscaled 2^-25: with one key far above 2000 others a quarter of what they weigh was lost); the
+// sum that the result is divided by is of the unrounded ones in fp32.
 //
 // Bound by the bytes of the codes where there are enough turns for every warp: 4 sequences of 131000 tokens, 10 heads, 232 to 240 us (5.6 to 5.8
 // TB/s, 0.86 to 0.88 of the copy rate), 32 of 16000 228 to 234 (0.87).  A turn is 2000 clocks of a warp that is alone on its scheduler: 575
@@ -270,6 +272,7 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, __nv_bfloat16* __r
 // the CTA (259), which cost the walk more instructions than the deeper prefetch saved; four CTAs an SM, whose 128 registers spill (248).
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int kMaxSplit = 16;                   // CTAs of a cluster
+constexpr float kLift = 15.f, kDrop = 1.f / 32768.f;       // of probabilities while they are fp16, and back
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -643,7 +646,7 @@ __global__ void __launch_bounds__(32 * AW, (D == 128 ? 12 : 16) / AW) kv8_attn_k
         }
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-        const float base = mn == -INFINITY ? 0.f : mn, corr = exp2_fast(m - base);
+        const float top = mn == -INFINITY ? 0.f : mn, corr = exp2_fast(m - top), base = top - kLift;
         m = mn;
         l *= corr;
         uint32_t pr[VW], pf[VW][2];
@@ -658,7 +661,7 @@ __global__ void __launch_bounds__(32 * AW, (D == 128 ? 12 : 16) / AW) kv8_attn_k
         for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int i = 0; i < VW; ++i) pf[(k * VW + i) >> 1][(k * VW + i) & 1] = __shfl_sync(0xffffffffu, pr[i], 4 * (2 * c4 + k));
-        const float fv = fabsf(vs);
+        const float fv = fabsf(vs) * kDrop;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           float d[4] = {0.f, 0.f, 0.f, 0.f};
@@ -694,6 +697,7 @@ __global__ void __launch_bounds__(32 * AW, (D == 128 ? 12 : 16) / AW) kv8_attn_k
     }
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    l *= kDrop;
     if (c4 == 0) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
