@@ -62,3 +62,14 @@ def test_refusals():
                  (torch.tensor(1.0), torch.tensor(0))):
         with pytest.raises(ValueError):
             ops.token_logprobs(*args)
+
+
+def test_head_refusals():
+    from them_bones_b200 import ops
+    x, w, t = torch.randn(3, 16), torch.randn(40, 16), torch.zeros(3, dtype=torch.int64)
+    assert ops.lmhead_logprobs(x, w, t, 40, 15.0, 2).top_id.shape == (3, 2)
+    for args in ((x, w, t[:2], 40, 15.0), (x, w, t.float(), 40, 15.0), (x[:, :8], w, t, 40, 15.0), (x.int(), w, t, 40, 15.0), (x, w[0], t, 40, 15.0), (x, w, t, 41, 15.0),
+                 (x, w, t, 0, 15.0), (x, w, t, 40, 15.0, 33), (x, w, t, 4, 15.0, 5), (x, w, t, 40, 0.0), (x, w, t, 40, -15.0), (x, w, t, 40, float("inf")),
+                 (x, w, t, 40, float("nan"))):
+        with pytest.raises(ValueError):
+            ops.lmhead_logprobs(*args)

@@ -217,7 +217,7 @@ def token_logprobs(logits, tokens, topk=0, vocab=None):
 def lmhead_logprobs(x, w, tokens, vocab, cap, topk=0):
     """``token_logprobs`` of the soft-capped logits ``cap * tanh(x @ w.T / cap)`` of rows ``x [.., C]``, with gradients to ``x`` and ``w``.  The
     logits exist for a block of rows at a time; natively in bf16, as a decode step has them."""
-    _logprobs.check_head(x, w, tokens, topk, vocab)
+    _logprobs.check_head(x, w, tokens, topk, vocab, cap)
     if native(x):
         return _logprobs.head_native(x, w, tokens, topk, vocab, cap)
     return _logprobs.head_statement(x, w, tokens, topk, vocab, cap)

@@ -31,13 +31,15 @@ def check(logits, tokens, topk, vocab):
         raise ValueError(f"token_logprobs: topk {topk}, at most {min(TOP_MAX, vocab)}")
 
 
-def check_head(x, w, tokens, topk, vocab):
+def check_head(x, w, tokens, topk, vocab, cap):
     if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1] or not x.is_floating_point() or w.device != x.device:
         raise ValueError(f"lmhead_logprobs: rows {tuple(x.shape)} on {x.device}, head {tuple(w.shape)} on {w.device}")
     if tokens.shape != x.shape[:-1] or tokens.dtype not in (torch.int64, torch.int32) or tokens.device != x.device:
         raise ValueError(f"lmhead_logprobs: tokens {tokens.dtype} {tuple(tokens.shape)} on {tokens.device}, expected int64 or int32 {tuple(x.shape[:-1])} on {x.device}")
     if not 1 <= vocab <= w.shape[0] or not 0 <= topk <= min(TOP_MAX, vocab):
         raise ValueError(f"lmhead_logprobs: a vocabulary of {vocab} in {w.shape[0]} rows, topk {topk} (at most {TOP_MAX})")
+    if not 0 < cap < float("inf"):
+        raise ValueError(f"lmhead_logprobs: a soft-cap of {cap}")
 
 
 def statement(logits, tokens, topk, vocab) -> TokenLogprobs:
@@ -205,9 +207,9 @@ def _capped(x, w, cap, out):
 
 def head_native(x, w, tokens, topk, vocab, cap) -> TokenLogprobs:
     from .cuda import _c
-    if x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16 or x.shape[-1] % 8 or w.shape[0] % 8 or not cap > 0:
-        raise ValueError(f"native lmhead_logprobs does not cover this call: {x.dtype} {tuple(x.shape)}, head {w.dtype} {tuple(w.shape)}, cap {cap} "
-                         "(bf16, rows of whole 16 bytes, a soft-cap)")
+    if x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16 or x.shape[-1] % 8 or w.shape[0] % 8:
+        raise ValueError(f"native lmhead_logprobs does not cover this call: {x.dtype} {tuple(x.shape)}, head {w.dtype} {tuple(w.shape)} "
+                         "(bf16, rows of whole 16 bytes)")
     shp, x2, tk = x.shape[:-1], _c(x).view(-1, x.shape[-1]), tokens.reshape(-1).to(torch.int64).contiguous()
     x2 = x2 if x2.data_ptr() % 16 == 0 else x2.clone()
     if w.stride(1) != 1 or w.stride(0) % 8 or w.data_ptr() % 16:
