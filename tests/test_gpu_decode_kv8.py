@@ -117,6 +117,33 @@ def test_steps_past_the_end_and_two_decoders():
     assert torch.equal(alone[:, :16], outs[0][:, :16]) and all(torch.equal(x[:, :16], y[:, :16]) for x, y in zip(dec.report, kept))
 
 
+def test_long_cache_step(monkeypatch):
+    """The step over a cache in which all heads share the CTAs, against the same step with a cluster for each: a document that begins within the
+    step is seen by both, and later tokens see no other document's."""
+    from them_bones_b200 import ops
+    from them_bones_b200.utils import decode as D
+    model, b, n = _model(seq=16384), 3, 140
+    toks = _tokens(b, n)
+    toks[0, 70], toks[1, 128], toks[2, n - 1] = 0, 0, 0
+    logits, caches = [], []
+    for long in (ops._kv8.LONG, 1 << 40):
+        monkeypatch.setattr(ops._kv8, "LONG", long)
+        out = torch.cat([toks, torch.zeros(b, 1, dtype=torch.int64, device="cuda")], 1)
+        with torch.no_grad():
+            cache = D.KVCache(model, b, 16384, "int8")
+            dec = D.NativeDecoder(model, cache, toks[:, 0], out, prompt_len=n)
+            assert dec.fused
+            dec.run(n)
+        logits.append(dec.last_logits[:, :1024].float())
+        caches.append(cache)
+    D.L_check()
+    # two orders of summation, rounded to bf16: a step of it here and there, through two layers
+    assert float((logits[0] - logits[1]).norm() / logits[1].norm()) < 2e-2
+    for x, y in zip(caches[0].kv8[0], caches[1].kv8[0]):                     # the first layer's keys and values do not depend on it
+        assert torch.equal(x, y)
+    assert torch.equal(caches[0].doc_start, caches[1].doc_start)
+
+
 def test_moe_step():
     from them_bones_b200.config import moe_capacity_for
     from them_bones_b200.utils import decode as D

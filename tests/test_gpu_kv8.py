@@ -131,6 +131,60 @@ def test_attention(b, h, d, cap, pos, start, window):
     _attend_case(b, h, d, cap, pos, start, window)
 
 
+@pytest.mark.parametrize("b,h,d,cap,pos,start,window", [
+    (1, 2, 128, 32768, [32767], None, 0), (1, 10, 64, 32768, [40], None, 0), (1, 1, 128, 32832, [0], None, 0), (1, 3, 128, 65536, [65000], [64001], 0),
+    (2, 3, 64, 16384, [16383, 16320], None, 0), (4, 3, 128, 16384, [5, 16383, 9000, 16384], [0, 16000, 9001, 0], 0), (6, 2, 64, 16384, [-1, -1, 63, 64, 16000, 1 << 30], None, 0),
+    (32, 1, 128, 16384, [500 * i + 63 for i in range(32)], [i * i for i in range(32)], 0), (33, 1, 64, 16384, [500 * i for i in range(32)] + [16383], None, 0),
+    (3, 10, 128, 40960, [40000, 39935, 127], None, 32768), (2, 2, 64, 32768, [30000, 200], [0, 100], 128), (16, 10, 64, 16384, [1000 * i + 300 for i in range(16)], None, 0),
+    (17, 10, 64, 16384, [900 * i for i in range(17)], None, 0)])
+def test_long_caches(b, h, d, cap, pos, start, window):
+    """On both sides of where all heads and sequences share the CTAs in equal parts."""
+    _attend_case(b, h, d, cap, pos, start, window)
+
+
+def test_long_caches_one_position():
+    _attend_case(1, 3, 128, 40000, 39990, None, 0)
+    _attend_case(3, 2, 64, 20000 // 64 * 64, 19000, [0, 18999, 19000], 0)
+    y = _attend_case(2, 2, 128, 16384, [-1, 16384], None, 0)
+    assert not y.any()
+
+
+def test_long_caches_captured_replayed_and_on_two_streams():
+    """Each call's parts are its own: two graphs over two caches replayed side by side, and calls on two streams, give the bits of calls alone."""
+    from them_bones_b200 import ops
+    from them_bones_b200.ref import functional as RF
+    torch.manual_seed(17)
+    b, h, d, cap, n = 2, 4, 128, 32768, 40
+    cos, sin = (x.cuda() for x in RF.rotary_tables(cap, d, 10000.0))
+    qkv = torch.randn(n, b, 3 * h * d, device="cuda").bfloat16()
+    at = _i32([[30000 + i, 20000 + 64 * i] for i in range(n)])
+    start = _random_cache(b, h, d, cap, 5)
+    caches = [_ref(start) for _ in range(4)]
+    want = [ops.kv8_attention(qkv[i], cos, sin, caches[0], at[i].clone(), 0.1) for i in range(n)]
+    graphs = []
+    for c in caches[1:3]:
+        pos, x = at[0].clone(), qkv[0].clone()
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            y = ops.kv8_attention(x, cos, sin, c, pos, 0.1)
+        graphs.append((g, pos, x, y))
+    streams, outs = [torch.cuda.Stream() for _ in range(3)], [[], [], []]
+    torch.cuda.synchronize()
+    for i in range(n):
+        for (g, pos, x, y), s, out in zip(graphs, streams, outs):
+            with torch.cuda.stream(s):
+                x.copy_(qkv[i])
+                pos.copy_(at[i])
+                g.replay()
+                out.append(y.clone())
+        with torch.cuda.stream(streams[2]):
+            outs[2].append(ops.kv8_attention(qkv[i], cos, sin, caches[3], at[i].clone(), 0.1))
+    torch.cuda.synchronize()
+    for out, c in zip(outs, caches[1:]):
+        assert all(torch.equal(a, w) for a, w in zip(out, want)) and _same(c, caches[0])
+
+
 @pytest.mark.parametrize("b,h,d,cap,pos,start", [(5, 2, 128, 256, 191, None), (130, 5, 64, 256, 191, None), (64, 10, 128, 320, 300, "some"), (90, 8, 128, 128, 63, None),
                                                   (500, 1, 64, 128, 5, None), (64, 9, 64, 1024, 990, "some"), (64, 9, 64, 2048, 1990, "some")])
 def test_one_position_for_all(b, h, d, cap, pos, start):

@@ -272,6 +272,8 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, __nv_bfloat16* __r
 // the CTA (259), which cost the walk more instructions than the deeper prefetch saved; four CTAs an SM, whose 128 registers spill (248).
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int kMaxSplit = 16;                   // CTAs of a cluster
+constexpr int kFlatFrom = 16384;                // tokens
+constexpr int kFlatPlaces = 1024, kFlatTurns = 2;   // CTAs of equal shares, and turns of each of their warps at least
 constexpr float kLift = 15.f, kDrop = 1.f / 32768.f;       // of probabilities while they are fp16, and back
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -372,10 +374,47 @@ struct __align__(16) AttnShared {
   float m[2 * AW], l[2 * AW];
 };
 
-template <int D, int AW>
+// Long caches (`FLAT`): as many CTAs as the SMs hold share all turns of all heads and sequences, and a second kernel joins what they have,
+// instead of a cluster for each.  CTAs of each head that sequence `lane` gets (32 sequences at most); 0 for a sequence outside, and
+// `places` in all at most: a head gets one CTA more than its part of places - B H.  Warps of both kernels work it out alike.  us by
+// clusters / shares, 10 heads: 131000 tokens 93 / 59 (0.87 of the copy rate), 32700 27 / 22, 3000 in a cache of 32768 8.0 / 10.1; 4 sequences of
+// 131000 248 / 213 (0.96), of 32768 to 131072 157 / 148; 16 of 16300 128 / 129, of 1000 to 16000 90 / 68; 4 heads of 64, 131000 tokens 44 / 20.
+// A CTA takes every n-th turn: a stretch for each is 3 to 7 % slower.  Two turns of each warp at least: four, 12.7 us for 10.1 of those 3000.
+template <int TT, int AW>
+__device__ __forceinline__ int flat_ctas(int B, int H, int places, PerSeq pos_, const int* __restrict__ doc_start, int limit, int window_tiles) {
+  const int b = threadIdx.x & 31, p = b < B ? pos_[b] : -1;
+  int turns = -1;
+  if (p >= 0 && p < limit) {
+    const int lo = max(doc_start ? ld_relaxed(doc_start + b) : 0, window_tiles > 0 ? max((p / 128 - (window_tiles - 1)) * 128, 0) : 0);
+    turns = max(p / KB * (KB / TT) - lo / TT, 0);
+  }
+  long long all = max(turns, 0);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+  const long long room = (long long)(places - B * H) * AW;
+  const int share = (int)max((all * H + room - 1) / room, (long long)kFlatTurns) * AW;
+  return turns < 0 ? 0 : max((turns + share - 1) / share, 1);
+}
+// CTA `n` of all: its sequence in `b` (none: B), its number among that sequence's CTAs in `n`, their number for each head in `ctas`.
+__device__ __forceinline__ void flat_place(int mine, int H, int B, int& n, int& b, int& ctas) {
+  const int lane = threadIdx.x & 31;
+  int upto = mine * H;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
+  }
+  const unsigned who = __ballot_sync(0xffffffffu, upto > n);
+  b = who ? __ffs(who) - 1 : B;
+  ctas = __shfl_sync(0xffffffffu, mine, b & 31);
+  n -= __shfl_sync(0xffffffffu, upto, b & 31) - ctas * H;
+}
+
+template <int D, int AW, bool FLAT>
 __global__ void __launch_bounds__(32 * AW, (D == 128 ? 12 : 16) / AW) kv8_attn_kernel(const __nv_bfloat16* __restrict__ qkv, long long ldq, const float* __restrict__ cosT,
                                                               const float* __restrict__ sinT, int rope_rows, Kv8 c, PerSeq pos_, const int* doc_start,
-                                                              __nv_bfloat16* __restrict__ y, int H, int cap, float scale2, int window_tiles, int least, int by_length) {
+                                                              __nv_bfloat16* __restrict__ y, int H, int cap, float scale2, int window_tiles, int least, int by_length,
+                                                              float* __restrict__ flat, int B) {
   constexpr int TT = 4096 / D, PER = TT / 8, VW = TT / 16;                // tokens of a turn, of a lane; words of a lane's piece of V
   constexpr int KL = D / 64, NT = D / 16, LPT = D / 8, TPI = 32 / LPT, RP = 4, PASS = KB / (AW * TPI * RP);
   __shared__ union {
@@ -384,9 +423,22 @@ __global__ void __launch_bounds__(32 * AW, (D == 128 ? 12 : 16) / AW) kv8_attn_k
   } sm_;
   AttnShared<D, AW>& sm = sm_.at;
   pdl_launch();
-  const int S = (int)cluster_size(), rank = (int)cluster_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int h = blockIdx.x / S, b = by_length ? longest_first((int)gridDim.y, (int)blockIdx.y, pos_, doc_start) : (int)blockIdx.y;
+  int S, rank, h, b, ctas = 0;
+  if (FLAT) {
+    pdl_wait();
+    S = 1;
+    rank = (int)blockIdx.x;
+    flat_place(flat_ctas<TT, AW>(B, H, (int)gridDim.x, pos_, doc_start, min(cap, rope_rows), window_tiles), H, B, rank, b, ctas);
+    if (b == B) return;
+    h = rank / ctas;
+    rank -= h * ctas;
+  } else {
+    S = (int)cluster_size();
+    rank = (int)cluster_rank();
+    h = blockIdx.x / S;
+    b = by_length ? longest_first((int)gridDim.y, (int)blockIdx.y, pos_, doc_start) : (int)blockIdx.y;
+  }
   const int g = lane >> 2, c4 = lane & 3;
   // the first kernel of a decode step may be storing a new document start: looked at again behind the wait
   int lo = doc_start ? ld_relaxed(doc_start + b) : 0;
@@ -440,14 +492,14 @@ __global__ void __launch_bounds__(32 * AW, (D == 128 ? 12 : 16) / AW) kv8_attn_k
   // Of the cluster as many CTAs take part as get `least` turns each, and one for the open block; the others leave.  The last one has the open
   // block (and, where there is no further CTA, its share of the full ones).
   const int end = last * (KB / TT);
-  auto taking_part = [&](int from) { return min(S, max(0, (end - from / TT + least - 1) / least) + 1); };
+  auto taking_part = [&](int from) { return FLAT ? ctas : min(S, max(0, (end - from / TT + least - 1) / least) + 1); };
   int active = taking_part(lo), u = lo / TT + rank * AW + warp;
   if (rank >= active) return;
   bool tail_cta = rank == active - 1;
   if (u < end) load_k(u);
   if (tail_cta) load_tail(0);
-  pdl_wait();
-  if (doc_start) {
+  if (!FLAT) pdl_wait();
+  if (!FLAT && doc_start) {
     const int now = max(ld_relaxed(doc_start + b), lo);             // a document that begins with this token; none begins earlier than was seen
     if (now != lo) {
       lo = now;
@@ -729,7 +781,15 @@ __global__ void __launch_bounds__(32 * AW, (D == 128 ? 12 : 16) / AW) kv8_attn_k
     }
   };
   sum_up(parts, [&](int e) { return sm.m[e]; }, [&](int e) { return sm.l[e]; }, [&](int e) { return sm.acc[e]; });
-  if (active > 1) {
+  if (FLAT) {
+    float* to = flat + (long long)blockIdx.x * (D + 4);
+#pragma unroll
+    for (int i = 0; i < OUT; ++i) {
+      const int d = tid + 32 * AW * i;
+      if (d < D) to[d] = o[i];
+    }
+    if (tid == 0) *reinterpret_cast<float2*>(to + D) = make_float2(L, M);
+  } else if (active > 1) {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     const uint32_t to = map_to_rank(smem_u32(&sm.part[rank][0]), 0);
 #pragma unroll
@@ -744,7 +804,7 @@ __global__ void __launch_bounds__(32 * AW, (D == 128 ? 12 : 16) / AW) kv8_attn_k
     cluster_barrier();
     if (rank == 0) sum_up(active, [&](int r) { return sm.part[r][D + 1]; }, [&](int r) { return sm.part[r][D]; }, [&](int r) { return sm.part[r]; });
   }
-  if (rank == 0) {
+  if (!FLAT && rank == 0) {
 #pragma unroll
     for (int i = 0; i < OUT; ++i) {
       const int d = tid + 32 * AW * i;
@@ -758,6 +818,47 @@ __global__ void __launch_bounds__(32 * AW, (D == 128 ? 12 : 16) / AW) kv8_attn_k
     kv8_quantise_block<32 * AW, D, false>(tail_of(c.kt + bh * KB * D), c.k + (bh * cap + (long long)last * KB) * D, c.ks + bh * nb + last, sm_.quant);
     kv8_quantise_block<32 * AW, D, true>(tail_of(c.vt + bh * KB * D), c.v + (bh * cap + (long long)last * KB) * D, c.vs + bh * nb + last, sm_.quant);
   }
+}
+
+// What the CTAs of a head and sequence have, together: eight groups of threads, each some of the CTAs.  It begins while they run.
+template <int D, int AW>
+__global__ void __launch_bounds__(8 * D) kv8_join_kernel(const float* parts, PerSeq pos_, const int* doc_start, __nv_bfloat16* __restrict__ y, int B, int H,
+                                                        int places, int limit, int window_tiles) {
+  __shared__ float acc[8][D], ml[8][2];
+  const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x % D, group = threadIdx.x / D, lane = threadIdx.x & 31;
+  pdl_launch();
+  pdl_wait();
+  const int mine = flat_ctas<4096 / D, AW>(B, H, places, pos_, doc_start, limit, window_tiles), n = __shfl_sync(0xffffffffu, mine, b);
+  int before = lane < b ? mine * H : 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  const float* p = parts + (long long)(before + h * n) * (D + 4);
+  float M = -INFINITY, L = 0.f, o = 0.f;
+#pragma unroll 8
+  for (int e = group; e < n; e += 8) {
+    const float2 lm = __ldcg(reinterpret_cast<const float2*>(p + e * (D + 4) + D));
+    const float v = __ldcg(p + e * (D + 4) + d), top = fmaxf(M, lm.y), base = top == -INFINITY ? 0.f : top;
+    const float f = exp2_fast(M - base), w = exp2_fast(lm.y - base);
+    L = L * f + w * lm.x;
+    o = o * f + w * v;
+    M = top;
+  }
+  acc[group][d] = o;
+  if (d == 0) { ml[group][0] = L; ml[group][1] = M; }
+  __syncthreads();
+  if (group) return;
+  M = ml[0][1];
+#pragma unroll
+  for (int e = 1; e < 8; ++e) M = fmaxf(M, ml[e][1]);
+  const float base = M == -INFINITY ? 0.f : M;
+  L = o = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float w = exp2_fast(ml[e][1] - base);
+    L += w * ml[e][0];
+    o += w * acc[e][d];
+  }
+  y[((long long)b * H + h) * D + d] = __float2bfloat16(L != 0.f ? o / L : 0.f);
 }
 
 // CTAs of a cluster: doubled until there are one and a half for each SM (three for caches from 32768 tokens on), as long as the cache's
@@ -785,12 +886,13 @@ struct AttnArgs {
   int H, cap;
   float scale2;
   int window_tiles, by_length;
+  float* parts;
 };
 template <int D, int AW>
 int launch_kv8_attn(const AttnArgs& p, int B, int split, int pdl, cudaStream_t s) {
   static OncePerDevice once;
   BONES_ONCE(once, {
-    BONES_CHECK(cudaFuncSetAttribute(kv8_attn_kernel<D, AW>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    BONES_CHECK(cudaFuncSetAttribute(kv8_attn_kernel<D, AW, false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   });
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
@@ -799,8 +901,24 @@ int launch_kv8_attn(const AttnArgs& p, int B, int split, int pdl, cudaStream_t s
   cfg.stream = s;
   cfg.attrs = at;
   cfg.numAttrs = (unsigned)dec_launch_attrs(at, split, pdl);
-  return (int)cudaLaunchKernelEx(&cfg, kv8_attn_kernel<D, AW>, p.qkv, p.ldq, p.cosT, p.sinT, p.rope_rows, p.c, p.pos, p.doc_start, p.y, p.H, p.cap, p.scale2,
-                                 p.window_tiles, AW, p.by_length);
+  return (int)cudaLaunchKernelEx(&cfg, kv8_attn_kernel<D, AW, false>, p.qkv, p.ldq, p.cosT, p.sinT, p.rope_rows, p.c, p.pos, p.doc_start, p.y, p.H, p.cap, p.scale2,
+                                 p.window_tiles, AW, p.by_length, (float*)nullptr, B);
+}
+template <int D>
+int launch_kv8_flat(const AttnArgs& p, int B, int places, int pdl, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[2];
+  cfg.gridDim = dim3((unsigned)places);
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cfg.attrs = at;
+  cfg.numAttrs = (unsigned)dec_launch_attrs(at, 1, pdl);
+  BONES_CHECK(cudaLaunchKernelEx(&cfg, kv8_attn_kernel<D, 4, true>, p.qkv, p.ldq, p.cosT, p.sinT, p.rope_rows, p.c, p.pos, p.doc_start, p.y, p.H, p.cap, p.scale2,
+                                 p.window_tiles, 4, 0, p.parts, B));
+  cfg.gridDim = dim3((unsigned)p.H, (unsigned)B);
+  cfg.blockDim = dim3(8 * D);
+  cfg.numAttrs = (unsigned)dec_launch_attrs(at, 1, 1);
+  return (int)cudaLaunchKernelEx(&cfg, kv8_join_kernel<D, 4>, (const float*)p.parts, p.pos, p.doc_start, p.y, B, p.H, places, min(p.cap, p.rope_rows), p.window_tiles);
 }
 
 inline bool kv8_refused(const Kv8& c, int B, int H, int D, int cap) {
@@ -841,14 +959,15 @@ int bones_kv8_read(void* k8, void* v8, float* ks, float* vs, void* kt, void* vt,
   return (int)cudaGetLastError();
 }
 
-// qkv: bf16 rows of 3 * H * D, ldq apart; cosT, sinT: fp32 [rope_rows, D / 2]; y: bf16 [B, H * D]; window_tiles: of 128 tokens, 0 for all.
+// qkv: bf16 rows of 3 * H * D, ldq apart; cosT, sinT: fp32 [rope_rows, D / 2]; y: bf16 [B, H * D]; window_tiles: of 128 tokens, 0 for all;
+// parts: room for 1024 * (D + 4) floats on 16 bytes, of this call alone until it ends, or null (where no more than 16383 tokens are seen none is used).
 int bones_kv8_attention(const void* qkv, long long ldq, const float* cosT, const float* sinT, int rope_rows, void* k8, void* v8, float* ks, float* vs, void* kt,
                         void* vt, const int* pos, int pos_step, int pos0, const int* doc_start, void* y, int B, int H, int D, int cap, float scale,
-                        int window_tiles, int pdl, void* stream) {
+                        int window_tiles, int pdl, float* parts, void* stream) {
   const Kv8 c{(int8_t*)k8, (int8_t*)v8, ks, vs, (__nv_bfloat16*)kt, (__nv_bfloat16*)vt};
-  if (kv8_refused(c, B, H, D, cap) || !qkv || !cosT || !sinT || !y || misaligned16(qkv, y) || (B > 1 && ldq % 8) || window_tiles < 0) return -2;
+  if (kv8_refused(c, B, H, D, cap) || !qkv || !cosT || !sinT || !y || misaligned16(qkv, y, parts) || (B > 1 && ldq % 8) || window_tiles < 0) return -2;
   const AttnArgs p{(const __nv_bfloat16*)qkv, ldq, cosT, sinT, rope_rows, c, PerSeq{pos, pos_step, pos0}, doc_start, (__nv_bfloat16*)y, H, cap,
-                   scale * 1.4426950408889634f, window_tiles, B > 1 && B <= 64 && pos && pos_step && !pdl};
+                   scale * 1.4426950408889634f, window_tiles, B > 1 && B <= 64 && pos && pos_step && !pdl, parts};
   int dev = 0, sms = 0;
   BONES_CHECK(cudaGetDevice(&dev));
   BONES_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
@@ -858,6 +977,13 @@ int bones_kv8_attention(const void* qkv, long long ldq, const float* cosT, const
   const int aw = (long long)B * H > 3ll * sms && !(pos && pos_step) && cap <= 1024 ? 2 : 4;
   const int split = kv8_splits(B, H, D, aw, cap, window_tiles, sms);
   cudaStream_t s = (cudaStream_t)stream;
+  // Equal shares for long caches where they pay for the second kernel (3 us of latencies): a cluster leaves SMs idle where heads are few, or where
+  // lengths differ.  With many heads a share is most of one's turns, and the parts come out unequal: 4 sequences of 7000 to 28000 tokens, 32 heads,
+  // 104 / 114, 6 of 5000 to 30000 150 / 165.  One position for all is known here where it comes as a number.
+  const int places = min((D == 128 ? 3 : 4) * sms, kFlatPlaces);
+  const long long seen = pos ? cap : min((long long)cap, pos0 + 1ll), tokens = window_tiles > 0 ? min(seen, window_tiles * 128ll) : seen;
+  if (parts && B <= 32 && 8ll * B * H <= 3ll * places && tokens >= (B > 1 ? kFlatFrom : 2 * kFlatFrom))
+    return D == 128 ? launch_kv8_flat<128>(p, B, places, pdl, s) : launch_kv8_flat<64>(p, B, places, pdl, s);
   if (aw == 2) return D == 128 ? launch_kv8_attn<128, 2>(p, B, split, pdl, s) : launch_kv8_attn<64, 2>(p, B, split, pdl, s);
   return D == 128 ? launch_kv8_attn<128, 4>(p, B, split, pdl, s) : launch_kv8_attn<64, 4>(p, B, split, pdl, s);
 }
