@@ -264,8 +264,8 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, __nv_bfloat16* __r
 // of the largest, and gone below 2^-40 (unscaled 2^-25: with one key far above 2000 others a quarter of what they weigh was lost); the
 // sum that the result is divided by is of the unrounded ones in fp32.
 //
-// Bound by the bytes of the codes where there are enough turns for every warp: 4 sequences of 131000 tokens, 10 heads, 232 to 240 us (5.6 to 5.8
-// TB/s, 0.86 to 0.88 of the copy rate), 32 of 16000 228 to 234 (0.87).  A turn is 2000 clocks of a warp that is alone on its scheduler: 575
+// Bound by the bytes of the codes where there are enough turns for every warp: 4 sequences of 131000 tokens, 10 heads, 213 us (6.3
+// TB/s, 0.96 of the copy rate; before the CTAs shared all of it equally 240), 64 of 8192 224 (0.91).  A turn is 2000 clocks of a warp that is alone on its scheduler: 575
 // instructions, the two loads' latencies between them; three to a scheduler hide that.  Few or short sequences are bound by one turn after
 // the other and by the way in and out (4.8 us for 300 tokens).  Taken before it: a block of 64 tokens a turn and two CTAs an SM (4 x 131000
 // 273 us, 64 sequences of 64 tokens 17.4 for 10.3); the codes through shared memory, by each warp's own cp.async (250) or by bulk copies for
@@ -331,7 +331,7 @@ __device__ __forceinline__ T turn_and_norm(const __nv_bfloat16* __restrict__ x, 
 }
 
 // The sequence with the n-th largest number of tokens to see, of 64 at most: CTAs begin in the order of their numbers, and the longest ones
-// are not to begin last (64 sequences of 1 to 2048 tokens in documents, 10 heads: 30 us for 35; 4 of 32768 to 131072: 160 for 170; where all
+// are not to begin last (64 sequences of 1 to 2048 tokens in documents, 10 heads: 30 us for 35; where all
 // are alike it costs the look, 12.3 for 11.3 at 64 tokens each).  Every warp works it out for itself, from what nothing writes meanwhile:
 // not where the kernel before this one may still run.
 __device__ __forceinline__ int longest_first(int B, int n, PerSeq pos, const int* __restrict__ doc_start) {
@@ -861,16 +861,18 @@ __global__ void __launch_bounds__(8 * D) kv8_join_kernel(const float* parts, Per
   y[((long long)b * H + h) * D + d] = __float2bfloat16(L != 0.f ? o / L : 0.f);
 }
 
-// CTAs of a cluster: doubled until there are one and a half for each SM (three for caches from 32768 tokens on), as long as the cache's
-// length (the band's, if there is one) can give every warp a turn.  us by 1 / 2 / 4 / 8 / 16 CTAs, heads of 128: 10 heads, 300 tokens
+// CTAs of a cluster: doubled until there are one and a half for each SM, as long as the cache's length (the band's, if there is one) can give
+// every warp a turn; where sequences have positions of their own until there are three, as long as each gets 2048 tokens.  us by 1 / 2 / 4 / 8 / 16 CTAs, heads of 128: 10 heads, 300 tokens
 // 5.8 / 6.1 / 5.0 / 5.0 / 5.4, 2040 tokens 21 / 14 / 9.8 / 7.8 / 6.9; 40 heads, 2040 tokens 22 / 15 / 12 / 10 / 14, 131000 tokens 1113 / 571 / 354 / 240 / 245;
 // 160 heads, 2040 tokens 27 / 20 / 25 / 33 / 52; 320 heads, 16000 tokens 234 / 247 / 245 / 244 / 274; 640 heads, 64 tokens 11 / 16 / 22 / 30 / 62, 2040 tokens
-// 67 / 63 / 81 / 111 / 196.  40 heads over 4 sequences of 32768 to 131072 tokens by 8 / 16 187 / 162.
-inline int kv8_splits(int B, int H, int D, int AW, int cap, int window_tiles, int sms) {
+// 67 / 63 / 81 / 111 / 196.  192 heads, 32700 tokens 357 / 282 / 267 / 276.  16 sequences of 10 heads, random lengths up to 2048 22 / 15.6 / 17.5,
+// up to 8192 74 / 46 / 34 (all of 8192: 92 / 62 / 68); 40 sequences up to 8192 87 / 58 / 69 (140 / 147 / 148); 4 sequences up to 8192 by 8 / 16 15.6 / 20.9.
+inline int kv8_splits(int B, int H, int D, int AW, int cap, int window_tiles, bool own, int sms) {
   const long long tokens = window_tiles > 0 && window_tiles < cap / 128 ? window_tiles * 128ll : cap;
-  const long long ctas = tokens >= 32768 ? 3ll * sms : 3ll * sms / 2;
+  const long long heads = (long long)B * H;
   int s = 1;
-  while (s < kMaxSplit && (long long)B * H * s < ctas && tokens >= (long long)s * AW * (4096 / D)) s *= 2;
+  while (s < kMaxSplit && heads * s < 3ll * sms / 2 && tokens >= (long long)s * AW * (4096 / D)) s *= 2;
+  while (own && s < kMaxSplit && heads * s < 3ll * sms && tokens >= s * 4096ll) s *= 2;
   return s;
 }
 
@@ -975,7 +977,7 @@ int bones_kv8_attention(const void* qkv, long long ldq, const float* cosT, const
   // smaller ones fit at once, but the longest take twice the time.  640 heads, us by four / two: alone, 64 tokens 11.8 / 8.2, lengths from 1 to
   // 2048 37 / 53; a step of 20 layers at 64 tokens 715 / 645, at 500 948 / 944, at 1900 1730 / 1866.
   const int aw = (long long)B * H > 3ll * sms && !(pos && pos_step) && cap <= 1024 ? 2 : 4;
-  const int split = kv8_splits(B, H, D, aw, cap, window_tiles, sms);
+  const int split = kv8_splits(B, H, D, aw, cap, window_tiles, B > 1 && pos && pos_step, sms);
   cudaStream_t s = (cudaStream_t)stream;
   // Equal shares for long caches where they pay for the second kernel (3 us of latencies): a cluster leaves SMs idle where heads are few, or where
   // lengths differ.  With many heads a share is most of one's turns, and the parts come out unequal: 4 sequences of 7000 to 28000 tokens, 32 heads,
