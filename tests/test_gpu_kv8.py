@@ -149,6 +149,34 @@ def test_long_caches_one_position():
     assert not y.any()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_long_caches_values_that_are_not_finite(d, bad):
+    """A key and a value of head 1 somewhere in the middle: who sees them has no number, others the bits they had without."""
+    from them_bones_b200 import ops
+    from them_bones_b200.ref import functional as RF
+    torch.manual_seed(6)
+    b, h, n = 4, 2, 16384
+    k, v = torch.randn(2, b, 9000, h, d, device="cuda").bfloat16()
+    cos, sin = (x.cuda() for x in RF.rotary_tables(n, d, 10000.0))
+    qkv = torch.randn(b, 3 * h * d, device="cuda").bfloat16()
+    at, start = _i32([8990, 8990, 8990, 70]), _i32([8000, 7000, 4097, 0])
+    out = []
+    for dirty in (False, True):
+        if dirty:
+            k[:, 7000, 1, 3], v[:, 4096, 1, 5] = bad, bad
+        cache = ops.kv8_cache(b, n, h, d, "cuda")
+        ops.kv8_append(cache, k, v, 0)
+        out.append(ops.kv8_attention(qkv, cos, sin, cache, at, 0.1, start).view(b, h, d))
+    clean, y = out
+    assert torch.equal(y[:, 0], clean[:, 0]) and torch.equal(y[[0, 3]], clean[[0, 3]])
+    assert bool(y[1:3, 1].isnan().all())
+    cache.k[:, 1].view(b, n // 64, 64, d)[:, 7000 // 64, 7000 % 64] = 1           # the value alone
+    cache.k_scale[:, 1, 7000 // 64] = 0.02
+    y = ops.kv8_attention(qkv, cos, sin, cache, at, 0.1, _i32([4096] * 4)).view(b, h, d)
+    assert bool(y[:3, 1, 5].isnan().all()) and bool(y[:3, 1, :5].isfinite().all()) and bool(y[:3, 1, 6:].isfinite().all())
+
+
 def test_long_caches_captured_replayed_and_on_two_streams():
     """Each call's parts are its own: two graphs over two caches replayed side by side, and calls on two streams, give the bits of calls alone."""
     from them_bones_b200 import ops
