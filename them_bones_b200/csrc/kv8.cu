@@ -935,13 +935,15 @@ inline bool kv8_refused(const Kv8& c, int B, int H, int D, int cap) {
 extern "C" {
 using namespace bones;
 
-// k, v: bf16, distances of sequences, tokens and heads in values (multiples of 8); pos, len: an address and the distance between two
+// k, v: bf16, distances of sequences, tokens and heads in values (multiples of 8 where there are two or more); pos, len: an address and the distance between two
 // sequences' values, or a value for all.  A sequence at a negative position, without tokens or with more than fit is left as it was.
 int bones_kv8_append(void* k8, void* v8, float* ks, float* vs, void* kt, void* vt, const void* k, const void* v, long long kb, long long kst, long long kh,
                      long long vb, long long vst, long long vh, int B, int H, int D, int cap, int t, const int* pos, int pos_step, int pos0, const int* len,
                      int len_step, int len0, void* stream) {
   const Kv8 c{(int8_t*)k8, (int8_t*)v8, ks, vs, (__nv_bfloat16*)kt, (__nv_bfloat16*)vt};
-  if (kv8_refused(c, B, H, D, cap) || t < 0 || !k || !v || misaligned16(k, v) || ((kst | vst | (B > 1 ? kb | vb : 0) | (H > 1 ? kh | vh : 0)) % 8)) return -2;
+  if (kv8_refused(c, B, H, D, cap) || t < 0 || !k || !v || misaligned16(k, v) ||
+      (((t > 1 ? kst | vst : 0) | (B > 1 ? kb | vb : 0) | (H > 1 ? kh | vh : 0)) % 8))
+    return -2;
   if (t == 0) return 0;
   // t tokens touch this many blocks at most; none lies past the capacity
   const long long blocks = min(((long long)t + KB - 2) / KB + 1, (long long)cap / KB);
