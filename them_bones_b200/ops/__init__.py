@@ -206,7 +206,7 @@ def token_logprobs(logits, tokens, topk=0, vocab=None):
     of the row's token in ``tokens [..]`` (0 where that is outside the vocabulary, as -1), the entropy in nats and the ``topk`` (32 at
     most) most probable tokens, equal logits in the order of their index, with their log-probabilities.  All but the ids have gradients.
     A row that holds a NaN or +inf, or nothing but -inf, has NaN for results (and no gradient where nothing depends on it).  Logits in bf16 or
-    fp32, sums in fp32.  A backward pass that is captured into a CUDA graph needs, as any, leaves without a living eager graph."""
+    fp32, sums in fp32.  Natively there is no forward-mode differentiation: a dual tensor is refused.  A backward pass that is captured into a CUDA graph needs, as any, leaves without a living eager graph."""
     vocab = logits.shape[-1] if vocab is None and logits.dim() else vocab
     _logprobs.check(logits, tokens, topk, vocab)
     if native(logits):

@@ -5,6 +5,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from . import COUNTS
@@ -60,10 +61,15 @@ def _forward(z, tokens, topk, vocab, want_stats):
     return given, entropy, top, ids, stats
 
 
+def has_tangent(*xs) -> bool:
+    """Whether one of the tensors (or None) carries a tangent of forward-mode differentiation; kernels that go by address would drop it."""
+    return forward_ad._current_level >= 0 and any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in xs)
+
+
 def _as_kernel(gs):
     """Gradients as the kernel reads them, fp32 and contiguous, and their addresses (0: none); None where one has no address (a batched
-    gradient) or a graph is being recorded: then the statement's own operators."""
-    if torch.is_grad_enabled():
+    gradient) or a tangent, or a graph is being recorded: then the statement's own operators."""
+    if torch.is_grad_enabled() or has_tangent(*gs):
         return None
     try:
         gs = [g if g is None or (g.dtype is torch.float32 and g.is_contiguous()) else g.float().contiguous() for g in gs]
@@ -131,7 +137,9 @@ def native(logits, tokens, topk, vocab) -> TokenLogprobs:
     if z.stride(1) != 1:
         z = z.contiguous()
     tk = tokens if rows and tokens.dtype is torch.int64 and tokens.is_contiguous() else tokens.reshape(-1).to(torch.int64).contiguous()
-    r = _LogprobsFn.apply(z, tk, topk, vocab) if torch.is_grad_enabled() and logits.requires_grad else _forward(z, tk, topk, vocab, False)[:4]
+    # a tangent goes to the function too, which has no forward mode and says so
+    recorded = (torch.is_grad_enabled() and logits.requires_grad) or has_tangent(logits)
+    r = _LogprobsFn.apply(z, tk, topk, vocab) if recorded else _forward(z, tk, topk, vocab, False)[:4]
     if rows:
         return TokenLogprobs(*r)
     shp = logits.shape[:-1]
