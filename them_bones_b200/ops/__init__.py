@@ -256,7 +256,8 @@ def kv8_attention(qkv, cos, sin, cache, pos, scale, doc_start=None, window=0):
     """One token a sequence: ``qkv [B, 3*H*D]`` -> RoPE and norm of the query and the key, key and value appended at ``pos[b]`` (in place),
     soft-max attention over the positions from ``doc_start[b]`` (and the band of ``window`` tokens, as in ``attention``) to ``pos[b]``
     -> ``[B, H*D]``.  A sequence at a negative position, or one past the cache or the rotary tables, is left as it was and gets
-    zeros; so does a query that sees no key.  No gradient."""
+    zeros; so does a query that sees no key.  No gradient: tensors that ask for one, and dual tensors, are refused, as by
+    ``kv8_append``."""
     dims = _kv8.check_attention(qkv, cos, sin, cache, pos, doc_start, window)
     _kv8.no_gradient(qkv)
     if native(qkv):

@@ -13,6 +13,7 @@ import torch
 
 from . import _lib as L
 from . import COUNTS
+from .logprobs import has_tangent
 
 BLOCK = 64
 HEAD_DIMS = (128, 64)
@@ -125,6 +126,8 @@ def check_attention(qkv, cos, sin, c: KV8, pos, doc_start, window):
 def no_gradient(x, y=None):
     if (x.requires_grad or (y is not None and y.requires_grad)) and torch.is_grad_enabled():
         raise ValueError("8-bit cache: its operators have no gradient; call them under torch.no_grad()")
+    if has_tangent(x, y):
+        raise ValueError("8-bit cache: its operators have no forward-mode differentiation")
 
 
 def numbers(x, b: int):
