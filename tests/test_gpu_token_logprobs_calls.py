@@ -31,3 +31,40 @@ def test_a_tangent_of_the_gradient():
     want, = torch.autograd.grad(r.logprob, [z], t)
     # the gradient is linear in what comes from above: p of it, p off by a few roundings of exponents up to 30
     assert float((tangent - want).abs().max()) < float(t.abs().max()) * 30 * 2 ** -22
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("how", ["plain", "recorded", "batched", "plain operators"])
+def test_rows_without_a_number_that_nothing_depends_on(how, dtype):
+    """Zeros for them however the gradient is taken, and NaN for one that something depends on."""
+    from them_bones_b200 import ops
+    inf, nan = float("inf"), float("nan")
+    torch.manual_seed(2)
+    z = torch.randn(7, 520, device="cuda").to(dtype)
+    z[0, 3], z[1, 4], z[2], z[3], z[4, 1], z[4, 2] = nan, inf, -inf, nan, inf, nan
+    z[5, :300] = -inf
+    z.requires_grad_()
+    tokens = torch.tensor([0, 4, 1, -1, 1, 505, 2], device="cuda")
+    keep = torch.tensor([0, 0, 0, 0, 0, 1.0, 2.0], device="cuda")
+    gs = [keep, -keep, torch.stack([keep, 3 * keep], 1)]
+    gs[0] = keep.clone()
+    gs[0][3] = 1.0                                                  # row 3 has no token: this counts for nothing
+    ops.set_reference_path(how == "plain operators")
+    try:
+        r = ops.token_logprobs(z, tokens, 2, 515)
+        outs = [r.logprob, r.entropy, r.top_logprob]
+        if how == "batched":
+            d = torch.autograd.grad(outs, [z], [torch.stack([0 * g, g]) for g in gs], is_grads_batched=True, retain_graph=True)[0][1]
+        else:
+            d, = torch.autograd.grad(outs, [z], gs, create_graph=how == "recorded", retain_graph=True)
+        gs[1] = gs[1].clone()
+        gs[1][2] = 1.0
+        e, = torch.autograd.grad(outs, [z], gs, create_graph=how != "plain")
+    finally:
+        ops.set_reference_path(False)
+    d, e = d.detach(), e.detach()
+    want, = torch.autograd.grad(ops.token_logprobs(z, tokens, 2, 515)[:3], [z], [gs[0], -keep, gs[2]])
+    assert not d[:5].any() and not d[:5].isnan().any() and not d[:, 515:].any()
+    # fp32 products and sums of numbers of size 20 at most, and a rounding to the type that may fall the other way
+    assert bool(((d - want)[5:].float().abs() <= torch.finfo(dtype).eps * want[5:].float().abs() + 20 * 2 ** -18).all())
+    assert bool(e[2, :515].isnan().all()) and not e[[0, 1, 3, 4]].any() and bool(e[5:].isfinite().all())

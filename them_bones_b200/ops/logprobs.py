@@ -101,31 +101,42 @@ class _LogprobsFn(torch.autograd.Function):
             return None, None, None, None
         ready = _as_kernel(gs)
         if ready is None:
-            return _statement_grad(z, tokens, ids, ctx.vocab, *gs), None, None, None
+            return _statement_grad(*_settled(z, ctx.vocab), tokens, ids, ctx.vocab, *gs), None, None, None
         dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
         with L.device(z.get_device()):
             _backward(z, tokens, ids, stats, ctx.vocab, ready[1], dz, 0.0)
         return dz, None, None, None
 
 
-def _statement_grad(z, tokens, ids, vocab, g_given, g_entropy, g_top):
-    """The gradient in PyTorch operators (differentiable, batchable); ``z`` is the saved input itself."""
+def _settled(z, vocab):
+    """``z`` with zeros for its rows without a number, and which ones they are."""
+    bad = RF.rows_without_number(z[:, :vocab].float())
+    return torch.where(bad[:, None], torch.zeros_like(z), z), bad
+
+
+def _statement_grad(z, bad, tokens, ids, vocab, g_given, g_entropy, g_top):
+    """The gradient in PyTorch operators (differentiable, batchable); ``z`` is the saved input itself, but for ``_settled``: a row without a
+    number has NaN for its gradient where something depends on it, and 0 where nothing does, not NaN times 0."""
     logp = torch.log_softmax(z[:, :vocab].float(), -1)
     gone = logp == float("-inf")
     p, logp0 = logp.exp(), logp.masked_fill(gone, 0.0)
     some = (tokens >= 0) & (tokens < vocab)
-    d = torch.zeros_like(p)
+    d, used = torch.zeros_like(p), torch.zeros_like(bad)
     if g_given is not None:
-        g = (g_given * some)[:, None]
+        g = torch.where(some, g_given, torch.zeros_like(g_given))
+        used = used | (g != 0)
         one = torch.zeros_like(p).scatter(1, torch.where(some, tokens, torch.zeros_like(tokens))[:, None], 1.0)
-        d = d + g * (one - p)
+        d = d + g[:, None] * (one - p)
     if g_entropy is not None:
+        used = used | (g_entropy != 0)
         entropy = -(p * logp0).sum(-1)
         d = d - g_entropy[:, None] * p * (logp0 + entropy[:, None])
     if g_top is not None:
+        used = used | (g_top != 0).any(-1)
         d = d - p * g_top.sum(-1, keepdim=True)
         for j in range(ids.shape[1]):
             d = d + g_top[:, j:j + 1] * torch.zeros_like(p).scatter(1, ids[:, j:j + 1], 1.0)
+    d = torch.where((bad & used)[:, None], torch.full_like(p, float("nan")), d)
     return torch.nn.functional.pad(d, (0, z.shape[1] - vocab)).to(z.dtype)
 
 
@@ -187,8 +198,8 @@ class _HeadLogprobsFn(torch.autograd.Function):
             return None, None, *none
         ready, m = _as_kernel(gs), x.shape[0]
         if ready is None:
-            z = RF.softcap_logits(torch.nn.functional.linear(x.float(), w.float()), ctx.cap)
-            d = _statement_grad(z, tokens, ids, ctx.vocab, *gs) * (1 - (z / ctx.cap).square())
+            z, bad = _settled(RF.softcap_logits(torch.nn.functional.linear(x.float(), w.float()), ctx.cap), ctx.vocab)
+            d = _statement_grad(z, bad, tokens, ids, ctx.vocab, *gs) * (1 - (z / ctx.cap).square())
             return (d @ w.float()).to(x.dtype), (d.transpose(-1, -2) @ x.float()).to(w.dtype), *none
         gs = ready[0]
         need_x, need_w = ctx.needs_input_grad[:2]

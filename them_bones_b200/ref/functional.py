@@ -691,13 +691,41 @@ def kv8_attention(qkv, cos, sin, cache, pos, scale: float, doc_start=None, windo
 def token_logprobs(logits, tokens, topk: int, vocab: int):
     """``(logprob, entropy, top_logprob, top_id)`` of the soft-max over the first ``vocab`` columns of ``logits [n, C]``; fp32.
     Differentiable.  A token outside the vocabulary has log-probability 0; alternatives descend, equal logits in the order of
-    their index, a NaN before everything; a row with a NaN, with +inf or with nothing but -inf has NaN for results."""
+    their index, a NaN before everything; a row with a NaN, with +inf or with nothing but -inf has NaN for results and no
+    gradient where nothing depends on them."""
     z = logits[:, :vocab].float()
     logp = torch.log_softmax(z, -1)
     gone = logp == float("-inf")                       # probability 0: no part in the entropy or its gradient
     entropy = -(logp.exp() * logp.masked_fill(gone, 0.0)).masked_fill(gone, 0.0).sum(-1)
     some = (tokens >= 0) & (tokens < vocab)
     given = logp.gather(1, torch.where(some, tokens, torch.zeros_like(tokens))[:, None])[:, 0]
-    given = torch.where(some, given, torch.zeros_like(given))
     ids = torch.sort(z.detach(), dim=-1, descending=True, stable=True).indices[:, :topk]
-    return given, entropy, logp.gather(1, ids), ids
+    top = logp.gather(1, ids)
+    if z.requires_grad:
+        _no_gradient_from_nothing(z, given, entropy, top)
+    return torch.where(some, given, torch.zeros_like(given)), entropy, top, ids
+
+
+def rows_without_number(z: torch.Tensor) -> torch.Tensor:
+    """Rows of logits that hold a NaN or +inf, or nothing but -inf: none of them has a probability."""
+    return ~torch.logsumexp(z.detach(), -1).isfinite()
+
+
+def _no_gradient_from_nothing(z, *outs):
+    """A row without a number gets no gradient from outputs whose gradients are zero: the formula's would be NaN times 0."""
+    bad, used = rows_without_number(z), []
+
+    def note(g):
+        u = g != 0
+        used.append(u if u.dim() == 1 else u.any(1))
+
+    def settle(g):
+        if not used:                                   # a second derivative: it does not come through the outputs
+            return None
+        some = used.pop()
+        while used:
+            some = some | used.pop()
+        return g.masked_fill((bad & ~some)[:, None], 0.0)
+    for x in outs:
+        x.register_hook(note)
+    z.register_hook(settle)
