@@ -311,25 +311,42 @@ __device__ __forceinline__ void ld_stream(uint32_t (&w)[2], const void* p) {
 // bytes of `w` that are -128, as the top bits of theirs
 __device__ __forceinline__ uint32_t bad_codes(uint32_t w) { return __vcmpeq4(w, 0x80808080u) & 0x80808080u; }
 
+// 1 / sqrt(x), by Newton's steps to the rounding of the type (two where it is 64 bits), of what fits fp32 or is brought there by an even power of 2
+__device__ __forceinline__ float inverse_root(float x) {
+  const float r = rsqrtf(x);
+  return r * (1.5f - 0.5f * x * r * r);
+}
+__device__ __forceinline__ double inverse_root(double x) {
+  const bool far = x > 1e30;
+  const double y = far ? x * 7.174648137343064e-43 : x;
+  double r = (double)rsqrtf((float)y);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) r *= 1.5 - 0.5 * y * r * r;
+  return far ? r * 8.470329472543003e-22 : r;
+}
 // RoPE of a row by a warp, and what norm multiplies it by: dimensions lane + 32 i of the first half in `a`, their partners in `e`.
 template <int D, class T>
 __device__ __forceinline__ T turn_and_norm(const __nv_bfloat16* __restrict__ x, const float* __restrict__ cs, const float* __restrict__ sn, T (&a)[D / 64],
                                            T (&e)[D / 64]) {
   const int lane = threadIdx.x & 31;
-  T ss = 0;
+  auto turn = [&](T by) {                                          // the mean of the squares of `by` times the row
+    T ss = 0;
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    const int d = lane + 32 * i;
-    const T x0 = (T)__bfloat162float(x[d]), x1 = (T)__bfloat162float(x[d + D / 2]), c = (T)cs[d], s = (T)sn[d];
-    a[i] = x0 * c + x1 * s;
-    e[i] = x1 * c - x0 * s;
-    ss += a[i] * a[i] + e[i] * e[i];
-  }
+    for (int i = 0; i < D / 64; ++i) {
+      const int d = lane + 32 * i;
+      const T x0 = (T)__bfloat162float(x[d]) * by, x1 = (T)__bfloat162float(x[d + D / 2]) * by, c = (T)cs[d], s = (T)sn[d];
+      a[i] = x0 * c + x1 * s;
+      e[i] = x1 * c - x0 * s;
+      ss += a[i] * a[i] + e[i] * e[i];
+    }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  ss = ss * (T)(1.0 / D) + (T)1.1920928955078125e-07;
-  const T r = (T)rsqrtf((float)ss);
-  return r * ((T)1.5 - (T)0.5 * ss * r * r);                       // a step of Newton's: to the rounding of T
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    return ss * (T)(1.0 / D);
+  };
+  T ss = turn((T)1) + (T)1.1920928955078125e-07;
+  // squares beyond fp32 (values from 1e18 on): 2^-70 of the row, beside which the epsilon counts for nothing; 64 bits hold them
+  if (sizeof(T) == 4 && !(ss <= (T)3.402823466e38f)) ss = turn((T)8.470329472543003e-22);
+  return inverse_root(ss);
 }
 
 // The sequence with the n-th largest number of tokens to see, of 64 at most: CTAs begin in the order of their numbers, and the longest ones

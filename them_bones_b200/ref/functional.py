@@ -657,8 +657,8 @@ def kv8_read(cache, held, length: int):
 
 @torch.no_grad()
 def kv8_attention(qkv, cos, sin, cache, pos, scale: float, doc_start=None, window: int = 0):
-    """One token a sequence: RoPE and norm of ``q`` and ``k`` from the packed ``qkv [B, 3*H*D]`` in fp32, ``k`` and ``v``
-    appended at ``pos[b]``, ``q`` against the keys from ``max(doc_start[b], band)`` on -> ``[B, H*D]``.  Sequences at a
+    """One token a sequence: RoPE and norm of ``q`` and ``k`` from the packed ``qkv [B, 3*H*D]`` in fp64 (squares of large values leave fp32),
+    ``k`` and ``v`` appended at ``pos[b]``, ``q`` against the keys from ``max(doc_start[b], band)`` on -> ``[B, H*D]``.  Sequences at a
     position outside the cache or the rotary tables get zeros and their cache is left as it was; a query that sees no key gets zeros."""
     k8 = cache[0]
     b, h, cap, d = k8.shape
@@ -666,10 +666,11 @@ def kv8_attention(qkv, cos, sin, cache, pos, scale: float, doc_start=None, windo
     for i, p in enumerate(pos):
         if p < 0 or p >= min(cap, cos.shape[0]):
             continue
-        q, k, v = qkv[i].float().view(3, h, d).unbind(0)
-        c, s = cos[p].float(), sin[p].float()
-        q, k = (torch.cat([x[:, :d // 2] * c + x[:, d // 2:] * s, -x[:, :d // 2] * s + x[:, d // 2:] * c], -1) for x in (q, k))
+        q, k, v = qkv[i].view(3, h, d).unbind(0)
+        c, s = cos[p].double(), sin[p].double()
+        q, k = (torch.cat([x[:, :d // 2] * c + x[:, d // 2:] * s, -x[:, :d // 2] * s + x[:, d // 2:] * c], -1) for x in (q.double(), k.double()))
         q, k = (x * torch.rsqrt(x.square().mean(-1, keepdim=True) + RMS_EPS) for x in (q, k))
+        q, v = q.float(), v.float()
         lo = max(doc_start[i] if doc_start is not None else 0, (p // 128 - (window // 128 - 1)) * 128 if window else 0, 0)
         first = p // KV8_BLOCK * KV8_BLOCK
         keys, vals = (torch.cat([line, tail[i, :, :p - first].float(), new.to(tail.dtype).float()[:, None]], 1)
