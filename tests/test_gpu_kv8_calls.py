@@ -91,3 +91,28 @@ def test_rows_that_are_not_finite(bad):
         qkv[1, part, 1, 5] = bad
         y = ops.kv8_attention(qkv.view(2, -1), cos, 0 * cos, cache, 0, 0.1).view(2, 2, 64)
         assert bool(y[0].isfinite().all()) and bool(y[1, 0].isfinite().all()) and bool(y[1, 1].isnan().all())
+
+
+def _nearest_bf16(x):
+    """fp64 to the nearest bf16 in one rounding: of the neighbours of what two roundings give, the nearest one."""
+    b = x.float().bfloat16()
+    near = [b] + [(b.view(torch.int16) + i).view(torch.bfloat16) for i in (-1, 1)]
+    off = torch.stack([(n.double() - x).abs().nan_to_num(float("inf")) for n in near])
+    return torch.stack(near).gather(0, off.argmin(0, keepdim=True))[0]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_the_new_key_is_rounded_once(d):
+    """16 million keys' values: where fp32 lies between, one in 2^17 falls to the wrong side of the middle of two bf16 numbers."""
+    from tests import kv8_oracle as O
+    from them_bones_b200 import ops
+    torch.manual_seed(9)
+    b, h, n = 64, 16, 16 * 2 ** 20 // (64 * 16 * d)
+    cache = ops.kv8_cache(b, 64, h, d, "cuda")
+    cos, sin = torch.rand(2, 1, d // 2, device="cuda")
+    for i in range(n):
+        qkv = torch.randn(b, 3 * h * d, device="cuda").bfloat16()
+        ops.kv8_attention(qkv, cos, sin, cache, 0, 0.1)
+        want = O.new_rows(qkv.view(b, 3, h, d).transpose(0, 1).reshape(1, -1)[0], cos, sin, 0, b * h, d)[1].view(b, h, d)
+        # a tie of two bf16 numbers to the last bits of fp64 is not met here
+        assert torch.equal(cache.k_open[:, :, 0], _nearest_bf16(want)), i

@@ -549,8 +549,8 @@ __global__ void __launch_bounds__(32 * AW, (D == 128 ? 12 : 16) / AW) kv8_attn_k
         const double r = turn_and_norm<D, double>(x, cs, sn, a, e);
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) {
-          v0[i] = __float2bfloat16((float)(a[i] * r));
-          v1[i] = __float2bfloat16((float)(e[i] * r));
+          v0[i] = __double2bfloat16(a[i] * r);
+          v1[i] = __double2bfloat16(e[i] * r);
         }
       } else {
 #pragma unroll
