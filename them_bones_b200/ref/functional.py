@@ -603,13 +603,22 @@ def kv8_values(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     return torch.where(codes == -128, torch.full_like(x, float("nan")), x)
 
 
-def _kv8_line(cache, b: int, blocks: int):
-    """Keys and values ``[H, blocks * 64, D]`` (fp32) of sequence ``b`` from its full blocks."""
+def kv8_coded(cache, blocks: int, more: int = 0):
+    """Keys and values ``[B, H, blocks * 64 + more, D]`` (fp32) of the first full blocks: codes times scales, not rounded further.  The ``more``
+    rows behind them are for the caller to fill."""
     k8, v8, ks, vs = cache[:4]
-    _, h, _, d = k8.shape
-    k = kv8_values(k8[b, :, :blocks * KV8_BLOCK].reshape(h, blocks, KV8_BLOCK, d), ks[b, :, :blocks])
-    v = kv8_values(v8[b, :, :blocks].transpose(-1, -2), vs[b, :, :blocks])
-    return k.reshape(h, -1, d), v.reshape(h, -1, d)
+    b, h, _, d = k8.shape
+    n, out = blocks * KV8_BLOCK, []
+    for codes, scale in ((k8[:, :, :n].view(b, h, blocks, KV8_BLOCK, d), ks), (v8[:, :, :blocks].transpose(-1, -2), vs)):
+        x = torch.empty(b, h, n + more, d, dtype=torch.float32, device=codes.device)
+        x[:, :, :n].unflatten(2, (blocks, KV8_BLOCK)).copy_(codes).mul_(scale[:, :, :blocks, None, None].abs()).masked_fill_(codes == -128, float("nan"))
+        out.append(x)
+    return out
+
+
+def _kv8_line(cache, b: int, blocks: int):
+    """``kv8_coded`` of sequence ``b`` alone, ``[H, blocks * 64, D]``."""
+    return tuple(x[0] for x in kv8_coded([t[b:b + 1] for t in cache[:4]], blocks))
 
 
 @torch.no_grad()

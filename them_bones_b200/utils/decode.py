@@ -106,24 +106,31 @@ def _forward_cached(model, idx, cache: KVCache):
         k = RF.rms_norm(_rope_at(k, cos, sin))
         if cache.kv8 is not None:
             # a token sees the block it is in as it came and the ones before it from their codes, as it does token by token
-            exact = [torch.cat([old, new.to(old.dtype)], 1) for old, new in zip(ops.kv8_read(cache.kv8[i], p0, p0), (k, v))]
-            ops.kv8_append(cache.kv8[i], k.to(exact[0].dtype), v.to(exact[0].dtype), p0)
-            coded = ops.kv8_read(cache.kv8[i], p0 + t, p0 + t)
+            c8, b0 = cache.kv8[i], p0 // RF.KV8_BLOCK * RF.KV8_BLOCK
+            new = [x.to(c8.k_open.dtype) for x in (k, v)]
+            exact = [torch.cat([old[:, :, :p0 - b0], x.transpose(1, 2)], 2) for old, x in zip((c8.k_open, c8.v_open), new)]       # from b0 on
+            ops.kv8_append(c8, *new, p0)
+            lines = RF.kv8_coded(c8, b0 // RF.KV8_BLOCK, p0 + t - b0)
+            held = [x.transpose(1, 2) for x in lines]
         else:
             cache.k[i, :, p0:p0 + t] = k
             cache.v[i, :, p0:p0 + t] = v
+            held = cache.k[i], cache.v[i]
         ys = []
         for j in range(t):                                   # prefill is short in decode benchmarks; one row at a time
             cur = p0 + j
             lo = ds[:, j].to(torch.int64)
             if at.window:
                 lo = torch.maximum(lo, torch.full_like(lo, max(0, (cur // 128 - (at.window // 128 - 1)) * 128)))
-            if cache.kv8 is not None:
+            if cache.kv8 is not None and (j == 0 or cur % RF.KV8_BLOCK == 0):       # a block's tokens as they came, the one before it from its codes
                 first = cur // RF.KV8_BLOCK * RF.KV8_BLOCK
-                keys, vals = (torch.cat([c[:, :first], e[:, first:cur + 1]], 1) for c, e in zip(coded, exact))
-            else:
-                keys, vals = cache.k[i, :, :cur + 1], cache.v[i, :, :cur + 1]
-            ys.append(_attend(q[:, j:j + 1].transpose(1, 2), keys, vals, at.scale, lo))
+                for line, own in zip(lines, exact):
+                    line[:, :, first:first + RF.KV8_BLOCK] = own[:, :, first - b0:first - b0 + RF.KV8_BLOCK]
+                if j and first:
+                    n8, full = first // RF.KV8_BLOCK - 1, slice(first - RF.KV8_BLOCK, first)
+                    lines[0][:, :, full] = RF.kv8_values(c8.k[:, :, full], c8.k_scale[:, :, n8])
+                    lines[1][:, :, full] = RF.kv8_values(c8.v[:, :, n8].transpose(-1, -2), c8.v_scale[:, :, n8])
+            ys.append(_attend(q[:, j:j + 1].transpose(1, 2), *(x[:, :cur + 1] for x in held), at.scale, lo))
         y = torch.cat(ys, 1).reshape(b, t, -1).to(x.dtype)
         x = x + F.linear(y, at.c_proj.weight)
         xn = RF.rms_norm(x)
