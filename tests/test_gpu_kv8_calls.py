@@ -116,3 +116,28 @@ def test_the_new_key_is_rounded_once(d):
         want = O.new_rows(qkv.view(b, 3, h, d).transpose(0, 1).reshape(1, -1)[0], cos, sin, 0, b * h, d)[1].view(b, h, d)
         # a tie of two bf16 numbers to the last bits of fp64 is not met here
         assert torch.equal(cache.k_open[:, :, 0], _nearest_bf16(want)), i
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("places", [0, 5, 16, 17, 100, 1024])
+def test_long_caches_take_no_more_room_than_there_is(places, d):
+    """Parts of the result go to as many places as the call was given, whatever the SMs hold; behind them nothing is written."""
+    from them_bones_b200 import ops
+    from them_bones_b200.ops import _lib as L
+    from them_bones_b200.ref import functional as RF
+    torch.manual_seed(3)
+    b, h, cap = 2, 3, 16384
+    cos, sin = (x.cuda() for x in RF.rotary_tables(cap, d, 10000.0))
+    qkv, pos = torch.randn(b, 3 * h * d, device="cuda").bfloat16(), torch.tensor([16000, 9000], dtype=torch.int32, device="cuda")
+    cache = ops.kv8_cache(b, cap, h, d, "cuda")
+    k, v = torch.randn(2, b, 16000, h, d, device="cuda").bfloat16()
+    ops.kv8_append(cache, k, v, 0, pos)
+    want = ops.kv8_attention(qkv, cos, sin, cache, pos, 0.1)
+    y, room = torch.empty_like(want), torch.full((1024 * (d + 4),), 12345.0, device="cuda")
+    c = cache
+    L.call("bones_kv8_attention", qkv.data_ptr(), qkv.stride(0), cos.data_ptr(), sin.data_ptr(), cap, c.k.data_ptr(), c.v.data_ptr(), c.k_scale.data_ptr(), c.v_scale.data_ptr(),
+           c.k_open.data_ptr(), c.v_open.data_ptr(), pos.data_ptr(), 1, 0, 0, y.data_ptr(), b, h, d, cap, 0.1, 0, 0, room.data_ptr(), places, L.raw_stream())
+    assert bool((room[places * (d + 4):] == 12345.0).all())
+    assert bool((room != 12345.0).any()) == (places >= 16)          # 8 * 6 heads in 3 of them; with fewer, clusters
+    # other orders of the same sum: probabilities of 11 bits whose largest differs, and a rounding to bf16 of a result of size 1 at most
+    assert float((y.float() - want.float()).abs().max()) <= 2 ** -8 + 2 ** -11 * 6

@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, __nv_bfloat16* __r
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int kMaxSplit = 16;                   // CTAs of a cluster
 constexpr int kFlatFrom = 16384;                // tokens
-constexpr int kFlatPlaces = 1024, kFlatTurns = 2;   // CTAs of equal shares, and turns of each of their warps at least
+constexpr int kFlatTurns = 2;                   // turns of each warp of a CTA of equal shares, at least
 constexpr float kLift = 15.f, kDrop = 1.f / 32768.f;       // of probabilities while they are fp16, and back
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -983,12 +983,13 @@ int bones_kv8_read(void* k8, void* v8, float* ks, float* vs, void* kt, void* vt,
 }
 
 // qkv: bf16 rows of 3 * H * D, ldq apart; cosT, sinT: fp32 [rope_rows, D / 2]; y: bf16 [B, H * D]; window_tiles: of 128 tokens, 0 for all;
-// parts: room for 1024 * (D + 4) floats on 16 bytes, of this call alone until it ends, or null (where no more than 16383 tokens are seen none is used).
+// parts: room for part_places * (D + 4) floats on 16 bytes, of this call alone until it ends, or null; no more CTAs than it has places share a
+// long cache (where no more than 16383 tokens are seen none is used).
 int bones_kv8_attention(const void* qkv, long long ldq, const float* cosT, const float* sinT, int rope_rows, void* k8, void* v8, float* ks, float* vs, void* kt,
                         void* vt, const int* pos, int pos_step, int pos0, const int* doc_start, void* y, int B, int H, int D, int cap, float scale,
-                        int window_tiles, int pdl, float* parts, void* stream) {
+                        int window_tiles, int pdl, float* parts, int part_places, void* stream) {
   const Kv8 c{(int8_t*)k8, (int8_t*)v8, ks, vs, (__nv_bfloat16*)kt, (__nv_bfloat16*)vt};
-  if (kv8_refused(c, B, H, D, cap) || !qkv || !cosT || !sinT || !y || misaligned16(qkv, y, parts) || (B > 1 && ldq % 8) || window_tiles < 0) return -2;
+  if (kv8_refused(c, B, H, D, cap) || !qkv || !cosT || !sinT || !y || misaligned16(qkv, y, parts) || (B > 1 && ldq % 8) || window_tiles < 0 || part_places < 0) return -2;
   const AttnArgs p{(const __nv_bfloat16*)qkv, ldq, cosT, sinT, rope_rows, c, PerSeq{pos, pos_step, pos0}, doc_start, (__nv_bfloat16*)y, H, cap,
                    scale * 1.4426950408889634f, window_tiles, B > 1 && B <= 64 && pos && pos_step && !pdl, parts};
   int dev = 0, sms = 0;
@@ -1003,9 +1004,9 @@ int bones_kv8_attention(const void* qkv, long long ldq, const float* cosT, const
   // Equal shares for long caches where they pay for the second kernel (3 us of latencies): a cluster leaves SMs idle where heads are few, or where
   // lengths differ.  With many heads a share is most of one's turns, and the parts come out unequal: 4 sequences of 7000 to 28000 tokens, 32 heads,
   // 104 / 114, 6 of 5000 to 30000 150 / 165.  One position for all is known here where it comes as a number.
-  const int places = min((D == 128 ? 3 : 4) * sms, kFlatPlaces);
+  const int places = parts ? min((D == 128 ? 3 : 4) * sms, part_places) : 0;
   const long long seen = pos ? cap : min((long long)cap, pos0 + 1ll), tokens = window_tiles > 0 ? min(seen, window_tiles * 128ll) : seen;
-  if (parts && B <= 32 && 8ll * B * H <= 3ll * places && tokens >= (B > 1 ? kFlatFrom : 2 * kFlatFrom))
+  if (B <= 32 && 8ll * B * H <= 3ll * places && tokens >= (B > 1 ? kFlatFrom : 2 * kFlatFrom))
     return D == 128 ? launch_kv8_flat<128>(p, B, places, pdl, s) : launch_kv8_flat<64>(p, B, places, pdl, s);
   if (aw == 2) return D == 128 ? launch_kv8_attn<128, 2>(p, B, split, pdl, s) : launch_kv8_attn<64, 2>(p, B, split, pdl, s);
   return D == 128 ? launch_kv8_attn<128, 4>(p, B, split, pdl, s) : launch_kv8_attn<64, 4>(p, B, split, pdl, s);

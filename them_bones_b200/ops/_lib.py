@@ -37,7 +37,7 @@ SIGNATURES = {
     "bones_attention_bwd": [_P] * 13 + [_I] * 4 + [_F, _I, _P],
     "bones_kv8_append": [_P] * 8 + [_L] * 6 + [_I] * 5 + [_P, _I, _I] * 2 + [_P],
     "bones_kv8_read": [_P] * 8 + [_I] * 5 + [_P, _I, _I, _P],
-    "bones_kv8_attention": [_P, _L, _P, _P, _I] + [_P] * 6 + [_P, _I, _I, _P, _P] + [_I] * 4 + [_F, _I, _I, _P, _P],
+    "bones_kv8_attention": [_P, _L, _P, _P, _I] + [_P] * 6 + [_P, _I, _I, _P, _P] + [_I] * 4 + [_F, _I, _I, _P, _I, _P],
     "bones_logprobs_fwd": [_P, _L, _I, _L, _I, _P, _I] + [_P] * 6,
     "bones_logprobs_bwd": [_P, _L, _I, _L, _I, _I, _P, _I] + [_P] * 6 + [_L, _F, _P],
     "bones_mx2_quant": [_P, _L, _P, _P, _I, _P, _P, _I, _L, _L, _I, _P],

@@ -18,7 +18,7 @@ from .logprobs import has_tangent
 BLOCK = 64
 HEAD_DIMS = (128, 64)
 MAX_LEN = (1 << 31) - 2 * BLOCK        # positions are 32-bit
-LONG, PARTS = 16384, 1024              # tokens from which the attention may want room for parts of its result, and how many
+LONG, PARTS = 16384, 1024              # capacity from which the attention gets room for parts of its result, and for how many (it takes no more)
 
 
 class KV8(NamedTuple):
@@ -202,4 +202,5 @@ def launch(qkv, cos, sin, dims, pos, scale, doc_start, window, y, pdl=0):
     pa, ps, p0 = _per(pos)
     parts = torch.empty(PARTS * (d + 4), dtype=torch.float32, device=y.device) if t >= LONG and b <= 32 else None
     L.call("bones_kv8_attention", qkv.data_ptr(), qkv.stride(0), cos.data_ptr(), sin.data_ptr(), cos.shape[0], at[0], at[1], at[2], at[3], at[4], at[5], pa, ps,
-           p0, 0 if doc_start is None else doc_start.data_ptr(), y.data_ptr(), b, h, d, t, scale, window // 128, pdl, 0 if parts is None else parts.data_ptr(), L.raw_stream())
+           p0, 0 if doc_start is None else doc_start.data_ptr(), y.data_ptr(), b, h, d, t, scale, window // 128, pdl, 0 if parts is None else parts.data_ptr(), PARTS,
+           L.raw_stream())
