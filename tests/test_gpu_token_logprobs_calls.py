@@ -68,3 +68,21 @@ def test_rows_without_a_number_that_nothing_depends_on(how, dtype):
     # fp32 products and sums of numbers of size 20 at most, and a rounding to the type that may fall the other way
     assert bool(((d - want)[5:].float().abs() <= torch.finfo(dtype).eps * want[5:].float().abs() + 20 * 2 ** -18).all())
     assert bool(e[2, :515].isnan().all()) and not e[[0, 1, 3, 4]].any() and bool(e[5:].isfinite().all())
+
+
+@pytest.mark.parametrize("form", ["turned", "odd rows", "odd address"])
+def test_a_head_that_owns_its_gradient_and_lies_anywhere(form):
+    """The kernels take a copy of such a weight; its gradient goes where the weight's owner wants it all the same."""
+    from them_bones_b200 import ops
+    torch.manual_seed(0)
+    x, flat = torch.randn(40, 64, device="cuda").bfloat16(), (0.3 * torch.randn(256 * 64 + 256, device="cuda")).bfloat16()
+    w = {"turned": lambda: flat[:256 * 64].view(64, 256).T, "odd rows": lambda: flat[:256 * 65].view(256, 65)[:, :64], "odd address": lambda: flat[3:256 * 64 + 3].view(256, 64)}[form]()
+    tokens = torch.randint(0, 250, (40,), device="cuda")
+    own, plain = w.detach().requires_grad_(), w.detach().clone(memory_format=torch.contiguous_format).requires_grad_()
+    own.main_grad = torch.ones(256, 64, device="cuda")
+    a, b = (ops.lmhead_logprobs(x, t, tokens, 250, 15.0) for t in (own, plain))
+    assert torch.equal(a.logprob, b.logprob)
+    a.logprob.sum().backward()
+    b.logprob.sum().backward()
+    # one is fp32, the other rounded to bf16
+    assert own.grad is None and float((own.main_grad - 1 - plain.grad.float()).norm()) < 2 ** -7 * float(plain.grad.float().norm())

@@ -232,7 +232,9 @@ def head_native(x, w, tokens, topk, vocab, cap) -> TokenLogprobs:
     shp, x2, tk = x.shape[:-1], _c(x).view(-1, x.shape[-1]), tokens.reshape(-1).to(torch.int64).contiguous()
     x2 = x2 if x2.data_ptr() % 16 == 0 else x2.clone()
     if w.stride(1) != 1 or w.stride(0) % 8 or w.data_ptr() % 16:
-        w = w.clone(memory_format=torch.contiguous_format)
+        own, w = getattr(w, "main_grad", None), w.clone(memory_format=torch.contiguous_format)
+        if own is not None:
+            w.main_grad = own
     with L.device(x.get_device()):
         r = _HeadLogprobsFn.apply(x2, w, tk, topk, vocab, float(cap), torch.is_grad_enabled() and (x.requires_grad or w.requires_grad))
     return TokenLogprobs(r[0].view(shp), r[1].view(shp), r[2].view(*shp, topk), r[3].view(*shp, topk))
