@@ -3,7 +3,7 @@
 ``load_for_eval(checkpoint_path, device)`` returns a ``ModelWrapper`` whose ``forward(input_ids)`` gives fp32 softcapped
 logits ``[B, T, V]``; ``get_eval_worker()`` treats every rank as an independent replica.  Beyond the reference (which
 scores full sequences only) the wrapper offers ``score(tokens, ctx_len, total_len)`` (continuation log-likelihoods from a
-batched prefill), ``report(tokens, ctx_len, total_len, topk)`` (the same token by token, with entropies and alternatives) and
+batched prefill), ``report(tokens, ctx_len, total_len, topk)`` (token by token, with entropies and alternatives; natively of logits in bf16) and
 ``generate(prompts, n_new)`` (greedy decoding with a KV cache in bf16 or, ``kv="int8"``, in 8 bits; ``logprobs=k`` tells what each
 new token was worth).
 """

@@ -147,7 +147,7 @@ __device__ __forceinline__ void kv8_quantise_block(Piece piece, int8_t* __restri
 
 constexpr int kAppendThreads = 128;
 // Bound by bytes: 2 read and 1 written for each value.  4 x 16384 tokens of 10 heads of 128, keys and values, 84 us (6.0 TB/s, 0.91 of the copy
-// rate); CTAs of 256 threads, which wait for their slowest load twice as often, 95 to 107.
+// rate); CTAs of 256 threads, which wait for their slowest load twice as often, 95 to 107.  64 registers a thread, 8 bytes spilled with heads of 128.
 // Tokens pos .. pos + len of a sequence.  A CTA takes one block that the run touches, of the keys or of the values of one head; the first
 // one also stores what is left over for the open block, after it has read the tokens that were in it before.
 template <int D, bool VALUES>
@@ -186,7 +186,8 @@ __global__ void __launch_bounds__(kAppendThreads, 8) kv8_append_kernel(Kv8 c, co
 }
 
 // One block of one head back to bf16 rows [B, length, H, D]; zeros behind the tokens held.  Bound by bytes, two thirds of them written:
-// 4 x 16384 tokens of 10 heads of 128 in 95 us (0.80 of the copy rate; filling the outputs alone takes PyTorch 86).
+// 4 x 16384 tokens of 10 heads of 128 in 95 us (0.80 of the copy rate; filling the outputs alone takes PyTorch 86).  Heads of 64 are further from
+// it (24 x up to 1357 tokens of 4 heads, 13.5 us for 7.6): half of the 256 threads only bring codes to shared memory, and a row is one line.
 template <int D>
 __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, __nv_bfloat16* __restrict__ k, __nv_bfloat16* __restrict__ v, PerSeq held_, int length, int H, int cap) {
   __shared__ __align__(16) uint8_t turn[D * kTurnRow];
@@ -265,11 +266,13 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8 c, __nv_bfloat16* __r
 // sum that the result is divided by is of the unrounded ones in fp32.
 //
 // Bound by the bytes of the codes where there are enough turns for every warp: 4 sequences of 131000 tokens, 10 heads, 213 us (6.3
-// TB/s, 0.96 of the copy rate; before the CTAs shared all of it equally 240), 64 of 8192 224 (0.91).  A turn is 2000 clocks of a warp that is alone on its scheduler: 575
-// instructions, the two loads' latencies between them; three to a scheduler hide that.  Few or short sequences are bound by one turn after
-// the other and by the way in and out (4.8 us for 300 tokens).  Taken before it: a block of 64 tokens a turn and two CTAs an SM (4 x 131000
-// 273 us, 64 sequences of 64 tokens 17.4 for 10.3); the codes through shared memory, by each warp's own cp.async (250) or by bulk copies for
-// the CTA (259), which cost the walk more instructions than the deeper prefetch saved; four CTAs an SM, whose 128 registers spill (248); equal
+// TB/s, 0.96 of the copy rate; before the CTAs shared all of it equally 240), 64 of 8192 224 (0.91).  A turn is about 2000 clocks of a warp
+// that is alone on its scheduler (one CTA takes 21 us for 2040 tokens, 5.8 for 300) and 600 instructions, the two loads' latencies between
+// them; three to a scheduler hide that.  Few or short sequences are bound by one turn after the other and by the way in and out (4.9 us for 300 tokens).
+// The token that fills a block costs 4 us more (32 sequences of up to 1536 tokens, 10 heads: 26.7 for 22.6): its codes are made last, those of the
+// keys before those of the values, by one CTA a head.  Heads of 128 take 161 or 163 of 168 registers; two of the three forms for heads of 64 spill
+// 8 and 16 bytes at 128.  Taken before it: a block of 64 tokens a turn and two CTAs an SM (4 x 131000 273 us, 64 sequences of 64 tokens
+// 17.4 for 10.3); the codes through shared memory, by each warp's own cp.async (250) or by bulk copies for the CTA (259), which cost the walk more instructions than the deeper prefetch saved; four CTAs an SM, whose 128 registers spill (248); equal
 // runs of turns for one CTA after the other over the ends of heads, for many heads (64 sequences up to 2048 tokens, 10 heads: 48 for 40, all of
 // 2048 72 for 75: each CTA's heads wait for one another's way in and out, where CTAs of one head overlap).
 // ---------------------------------------------------------------------------------------------------------------
@@ -839,7 +842,8 @@ __global__ void __launch_bounds__(32 * AW, (D == 128 ? 12 : 16) / AW) kv8_attn_k
   }
 }
 
-// What the CTAs of a head and sequence have, together: eight groups of threads, each some of the CTAs.  It begins while they run.
+// What the CTAs of a head and sequence have, together: eight groups of threads, each some of the CTAs.  It is launched before they end, so that
+// its CTAs come to the SMs as those leave; its 8 D threads find no room beside three of them.
 template <int D, int AW>
 __global__ void __launch_bounds__(8 * D) kv8_join_kernel(const float* parts, PerSeq pos_, const int* doc_start, __nv_bfloat16* __restrict__ y, int B, int H,
                                                         int places, int limit, int window_tiles) {

@@ -11,7 +11,7 @@
 // alternative, and only their columns (a few percent of the row, still in L2) are looked at again.
 // Gradient: one element-wise pass; the few columns with a gradient of their own are written once more.
 //
-// Bound by bytes, and in bf16 nearly as much by the exponentials (64 % of the special-function units' rate): 4096 rows of 65536, forward 98 us
+// Bound by bytes, and in bf16 nearly as much by the exponentials (65 % of the special-function units' rate): 4096 rows of 65536, forward 98 us
 // in bf16 (0.83 of the copy rate) and 158 in fp32 (1.03), with five alternatives 106 and 167; gradient 183 (0.90) and 326 (1.0).  One row takes 3.4 us,
 // with 20 alternatives 6.9: latencies of the choice, which has a barrier between any two of its steps.  Before, 4096 rows with five alternatives:
 // a pass for the maximum, one for the sums and one for each alternative 1580 us in fp32; one pass, and every thread's best column looked for

@@ -3,9 +3,14 @@
 The reference scores teacher-forced full sequences only (round2/submission/inference.py:26-27); autoregressive decoding
 is an added capability.  The cache stores, per layer, keys *after* RoPE and QK-norm and raw values, so a decode step
 rotates only the new token (RoPE at its absolute position) and attends over the cached prefix restricted to the current
-document and the layer's window.  It holds them in bf16 or, for twice the tokens in the same memory and half the bytes of a
-step, in 8 bits (``kv="int8"``: ``ops.kv8_cache``).  A decoder can also say what each of its answers was worth
+document and the layer's window.  It holds them in bf16 or, with close to half the memory and half the bytes of a step in long
+caches, in 8 bits (``kv="int8"``: ``ops.kv8_cache``).  A decoder can also say what each of its answers was worth
 (``logprobs=k``: ``ops.token_logprobs`` of every generated token).
+
+When 8 bits pay: the tokens of the open block are held in bf16 beside the codes, so a cache of 64 tokens takes 1.5 times the bf16 one's
+memory, one of 128 as much, one of 2048 0.53 of it.  ``NativeDecoder``'s step reads the codes themselves and is the faster one from a few hundred
+tokens on (at 64 tokens it costs 0.5 to 2 us a layer).  The plain route (``_forward_cached``: prompts of more than 512 tokens, models whose heads
+are not of 128, models on the CPU) turns the codes into fp32 numbers at every call: there only the memory is saved.
 """
 from __future__ import annotations
 
@@ -501,7 +506,8 @@ def _stacked(report: list, b: int, k, dev):
 
 @torch.no_grad()
 def greedy_decode(model, prompts: torch.Tensor, n_new: int, kv: str = "bf16", logprobs: int | None = None):
-    """``prompts [B, P]`` -> ``[B, P + n_new]`` by arg-max decoding.  ``kv``: how the cache holds keys and values, ``"bf16"`` or ``"int8"``.
+    """``prompts [B, P]`` -> ``[B, P + n_new]`` by arg-max decoding.  ``kv``: how the cache holds keys and values, ``"bf16"`` or ``"int8"`` (for
+    long answers; see the module's text).
     ``logprobs=k``: ``(tokens, TokenLogprobs)`` with the log-probability, the entropy and k alternatives of each new token ``[B, n_new]``."""
     b, p = prompts.shape
     if p + n_new > model.config.sequence_len:

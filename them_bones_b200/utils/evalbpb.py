@@ -6,7 +6,8 @@ the reference repository; used at round2/source/train.py:23307-23318).
 * ``causality_check``  -- perturb tokens at positions > p and require the logits at positions <= p to stay put.  This
   also covers the MoE capacity count and the hashed-table lookups, which are causal by construction.
 * ``score_continuations`` -- teacher-forced log-likelihood of a continuation given a context (the scoring half of the
-  inference benchmark); ``report_continuations`` says the same of each token, with the entropy and the alternatives there.
+  inference benchmark); ``report_continuations`` tells of each token, with the entropy and the alternatives there (natively from
+  logits in bf16, as a decode step has them).
 """
 from __future__ import annotations
 
@@ -82,7 +83,8 @@ def _continuation_targets(tokens, ctx_len, total_len):
 @torch.no_grad()
 def report_continuations(model, tokens: torch.Tensor, ctx_len: torch.Tensor, total_len: torch.Tensor, topk: int = 0):
     """``score_continuations`` token by token: ``TokenLogprobs [B, T]`` where place t tells of ``tokens[b, t]`` given what is before it;
-    zeros outside the continuations (and at the first token, which nothing precedes)."""
+    zeros outside the continuations (and at the first token, which nothing precedes).  Natively the logits are rounded to bf16, by up to
+    2^-5 each where they are 8 to 15; those of ``score_continuations`` are not, and its sums differ by that."""
     targets, keep = _continuation_targets(tokens, ctx_len, total_len)
     r = model.token_logprobs(tokens, targets, topk)
     out = []
