@@ -141,3 +141,26 @@ def test_long_caches_take_no_more_room_than_there_is(places, d):
     assert bool((room != 12345.0).any()) == (places >= 16)          # 8 * 6 heads in 3 of them; with fewer, clusters
     # other orders of the same sum: probabilities of 11 bits whose largest differs, and a rounding to bf16 of a result of size 1 at most
     assert float((y.float() - want.float()).abs().max()) <= 2 ** -8 + 2 ** -11 * 6
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_key_that_is_not_finite_is_kept_as_the_formula_has_it(d):
+    """Behind an infinite norm the finite values are zeros and the infinite ones have no number; a NaN leaves nothing."""
+    from tests import kv8_oracle as O
+    from them_bones_b200 import ops
+    from them_bones_b200.ref import functional as RF
+    torch.manual_seed(10)
+    inf, nan = float("inf"), float("nan")
+    cos, sin = (x.cuda() for x in RF.rotary_tables(64, d, 10000.0))
+    qkv = torch.randn(4, 3, 2, d, device="cuda").bfloat16()
+    qkv[0, 1, 0, 3], qkv[1, 1, 1, d - 1], qkv[2, 1, 0, 5], qkv[3, 1, 0, 7], qkv[3, 1, 1, 7] = inf, -inf, nan, inf, nan
+    plain, kernel = (ops.kv8_cache(4, 64, 2, d, "cuda") for _ in range(2))
+    ops.kv8_attention(qkv.view(4, -1), cos, sin, kernel, 63, 0.1)
+    RF.kv8_attention(qkv.view(4, -1), cos, sin, plain, [63] * 4, 0.1)
+    for i in range(4):
+        want = O.new_rows(qkv[i].view(-1), cos, sin, 63, 2, d)[1]
+        for c in (kernel, plain):
+            got = c.k_open[i, :, 63].double()
+            assert torch.equal(got.isnan(), want.isnan()) and not (got - want)[(want == 0) & ~want.isnan()].any()
+            assert torch.equal(c.k[i, :, 63] == -128, want.isnan())
+    assert int(kernel.k_open[0, 0, 63].isnan().sum()) == 2 and int(kernel.k_open[2, 0, 63].isnan().sum()) == d

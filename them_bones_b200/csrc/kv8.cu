@@ -325,7 +325,7 @@ __device__ __forceinline__ double inverse_root(double x) {
   double r = (double)rsqrtf((float)y);
 #pragma unroll
   for (int i = 0; i < 2; ++i) r *= 1.5 - 0.5 * y * r * r;
-  return far ? r * 8.470329472543003e-22 : r;
+  return y > 3.4e38 ? 0.0 : far ? r * 8.470329472543003e-22 : r;           // of an infinite value: a step of Newton's would make it NaN
 }
 // RoPE of a row by a warp, and what norm multiplies it by: dimensions lane + 32 i of the first half in `a`, their partners in `e`.
 template <int D, class T>
