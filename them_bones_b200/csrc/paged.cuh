@@ -1,0 +1,55 @@
+// A paged key/value cache: what the kernels that write and read it share.
+#pragma once
+#include "common.cuh"
+
+namespace bones {
+
+// The new tokens of B sequences lie one after another in N rows: sequence b's are starts[b] .. starts[b + 1], the first at position pos[b].
+// Position p of sequence b is slot p % P of page table[b * ldt + p / P]; k, v: [pages, H, P, D].
+struct Paged {
+  const int* starts;   // [B + 1], ascending
+  const int* pos;      // [B]
+  const int* table;    // [B, M], rows ldt apart
+  long long ldt;
+  int B, N, M, H;
+  int shift;           // log2 P
+  int pages;
+  int cap;             // positions with a place in the table: M * P
+};
+
+struct Piece {
+  int row, len, pos;   // its rows, and the position of the first
+  int live;            // rows whose position is inside the table: the others are left out
+};
+
+__device__ __forceinline__ Piece paged_piece(const Paged& p, int b) {
+  Piece s;
+  s.row = min(max(p.starts[b], 0), p.N);
+  s.len = min(max(p.starts[b + 1], s.row), p.N) - s.row;
+  s.pos = p.pos[b];
+  s.live = s.pos < 0 || s.pos >= p.cap ? 0 : min(s.len, p.cap - s.pos);
+  return s;
+}
+
+// The sequence that row r belongs to, by a warp: the number of starts at or before r, less one (-1 in front of the first, B behind the last).
+__device__ __forceinline__ int paged_owner(const int* starts, int B, int r) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = B + 1;                         // how many starts are <= r lies in [lo, hi]
+  while (hi - lo > 32) {
+    const int step = (hi - lo + 31) / 32;
+    const int i = lo + (lane + 1) * step - 1;     // the last one of the lane's share
+    const int full = __popc(__ballot_sync(0xffffffffu, i < hi && starts[min(i, B)] <= r));
+    const int from = lo + full * step;
+    hi = min(hi, from + step);
+    lo = min(from, hi);
+  }
+  const int i = lo + lane;
+  return lo + __popc(__ballot_sync(0xffffffffu, i < hi && starts[min(i, B)] <= r)) - 1;
+}
+
+// First row's offset of page `id`, head h; -1 where there is no such page.
+__device__ __forceinline__ long long paged_at(const Paged& p, int id, int h) {
+  return id < 0 || id >= p.pages ? -1 : ((long long)id * p.H + h) << p.shift;
+}
+
+}  // namespace bones

@@ -42,9 +42,11 @@ def _cuda():
     return cuda
 
 
-from . import kv8 as _kv8, logprobs as _logprobs  # noqa: E402  (they read COUNTS)
+from . import kv8 as _kv8, logprobs as _logprobs, paged as _paged, verify as _verify  # noqa: E402  (they read COUNTS)
 from .kv8 import KV8  # noqa: E402
 from .logprobs import TokenLogprobs  # noqa: E402,F401
+from .paged import PagedKV  # noqa: E402
+from .verify import Verified  # noqa: E402
 
 
 # --------------------------------------------------------------------------------------------------------------
@@ -263,6 +265,58 @@ def kv8_attention(qkv, cos, sin, cache, pos, scale, doc_start=None, window=0):
     if native(qkv):
         return _kv8.attention(qkv, cos, sin, dims, pos, scale, doc_start, window)
     return RF.kv8_attention(qkv, cos, sin, cache, _kv8.numbers(pos, dims[0]), scale, None if doc_start is None else doc_start.tolist(), window)
+
+
+# -- key/value cache in pages ------------------------------------------------------------------------------------
+def paged_cache(pages, n_head, head_dim, page=64, device=None, dtype=torch.bfloat16) -> PagedKV:
+    """An empty cache of one layer (``ops.paged.PagedKV``): ``pages`` pages of ``page`` tokens (16, 32, 64 or 128) that any sequences share."""
+    return _paged.cache(pages, n_head, head_dim, page, device, dtype)
+
+
+def paged_append(qkv, cos, sin, cache, table, starts, pos):
+    """Pieces of new tokens into the cache, in place: ``qkv [N, 3*H*D]`` -> RoPE and norm of queries and keys, keys and values to their pages,
+    the queries back ``[N, H*D]``.  Rows ``starts[b] .. starts[b + 1]`` (int32 ``[B + 1]``, ascending, on the device) are sequence b's, at
+    the positions from ``pos[b]`` (int32 ``[B]``) on; position p is in page ``table[b, p // P]`` (int32 ``[B, M]``).  Left out, with zeros for
+    their queries: the tokens of a sequence at a negative position, those past the table or the rotary tables, and rows outside all
+    pieces.  A token whose page is not one of the cache's (as -1) is not stored.  No page may be written by two sequences.  No gradient:
+    tensors that ask for one, and dual tensors, are refused."""
+    dims = _paged.check_append(qkv, cos, sin, cache, table, starts, pos)
+    _paged.no_gradient(qkv)
+    if native(qkv):
+        return _paged.append(dims, qkv, cos, sin, cache, table, starts, pos)
+    return RF.paged_append(qkv, cos, sin, cache, table, starts, pos)
+
+
+def paged_attention(q, cache, table, starts, pos, scale, doc_start=None, window=0, longest=None):
+    """Pieces of new tokens against the cache: ``q [N, H*D]`` as ``paged_append`` returned it, with its ``table``, ``starts`` and ``pos`` -> ``[N, H*D]``.
+    Token i of the N sees its sequence's positions from ``doc_start[i]`` (int32 ``[N]``) and the band of ``window`` tokens (as in ``attention``) to its
+    own, as far as they have pages.  One token a sequence, drafts, pieces of prompts and whole prompts in one call.  ``longest``: the length of the
+    longest piece as far as the host knows (default: the mean); it picks a kernel, not the result.  Tokens that were left out, rows outside all pieces and
+    queries that see no key get zeros.  Queries and keys are behind the norm (``|q . k|`` about D at most): natively the soft-max has a
+    fixed shift, and ``|scale| * D`` up to 32.  No gradient."""
+    dims = _paged.check_attention(q, cache, table, starts, pos, scale, doc_start, window, longest)
+    _paged.no_gradient(q, *cache)
+    if native(q):
+        return _paged.attention(dims, q, cache, table, starts, pos, scale, doc_start, window, longest)
+    return RF.paged_attention(q, cache, table, starts, pos, scale, doc_start, window)
+
+
+# -- drafted tokens ----------------------------------------------------------------------------------------------
+def verify_drafts(logits, ids, starts, uniforms=None, draft_logits=None, temperature=1.0, vocab=None) -> Verified:
+    """Which drafted tokens the target's logits let stand, and the token behind them.  Rows ``starts[b] .. starts[b + 1]`` (int32 ``[B + 1]``, ascending) of
+    ``logits [N, C]`` (its first ``vocab`` columns; bf16 or fp32) are what the target says behind each of sequence b's tokens ``ids [N]`` (int64), of
+    which the first is given and the others are drafts.  Row by row, with ``p = softmax(logits / temperature)`` and ``q`` what the drafts were
+    drawn from, the soft-max of ``draft_logits [N, C']`` (the row in front of a draft's; a sequence's last row is not read) or, without
+    them, certainty: the draft x behind row r stands while ``uniforms[r, 0] * q(x) < p(x)`` (fp32 ``[N, 2]`` in [0, 1)).  At the first that does not the
+    token is drawn from ``max(p - q, 0)``, behind the last draft from p: the first one whose cumulated weight is above ``uniforms[r, 1]`` of the
+    total.  ``temperature=0``: the arg-max (the lowest index of equals) throughout, no ``uniforms``.  -> ``Verified(accepted [B], token [B])``.  Sums in 64
+    bits.  A draft outside the vocabulary falls; so does one whose draft row has no number (NaN, +inf or nothing but -inf), and the token is then drawn from p.
+    A target row without a number ends a sequence with token -1, as does a sequence without rows.  No gradient."""
+    vocab = logits.shape[-1] if vocab is None and logits.dim() else vocab
+    _verify.check(logits, ids, starts, uniforms, draft_logits, temperature, vocab)
+    if native(logits):
+        return _verify.native(logits, ids, starts, uniforms, draft_logits, temperature, vocab)
+    return Verified(*RF.verify_drafts(logits, ids, starts, uniforms, draft_logits, temperature, vocab))
 
 
 # -- output-side hashed table ------------------------------------------------------------------------------------

@@ -695,6 +695,124 @@ def kv8_attention(qkv, cos, sin, cache, pos, scale: float, doc_start=None, windo
 
 
 # ----------------------------------------------------------------------------------------------------------------
+# Keys and values in pages; drafted tokens
+# ----------------------------------------------------------------------------------------------------------------
+
+def paged_pieces(starts, pos, n: int, capacity: int):
+    """``[(first row, rows, position of the first, rows whose position is below the capacity)]`` of each sequence's piece."""
+    st, out = starts.tolist(), []
+    for b, p in enumerate(pos.tolist()):
+        a = min(max(st[b], 0), n)
+        m = min(max(st[b + 1], a), n) - a
+        out.append((a, m, p, 0 if p < 0 else min(m, max(0, capacity - p))))
+    return out
+
+
+@torch.no_grad()
+def paged_append(qkv, cos, sin, cache, table, starts, pos):
+    """RoPE and norm in fp64 (squares of large values leave fp32); see ``ops.paged_append``."""
+    k, v = cache
+    pages, h, page, d = k.shape
+    n = qkv.shape[0]
+    q_out = torch.zeros(n, h * d, dtype=qkv.dtype, device=qkv.device)
+    for b, (a, _, p0, live) in enumerate(paged_pieces(starts, pos, n, min(table.shape[1] * page, cos.shape[0]))):
+        if not live:
+            continue
+        q, kk, vv = qkv[a:a + live].view(live, 3, h, d).unbind(1)
+        c, s = (x[p0:p0 + live, None].double() for x in (cos, sin))
+        q, kk = (torch.cat([x[..., :d // 2] * c + x[..., d // 2:] * s, -x[..., :d // 2] * s + x[..., d // 2:] * c], -1) for x in (q.double(), kk.double()))
+        q, kk = (x * torch.rsqrt(x.square().mean(-1, keepdim=True) + RMS_EPS) for x in (q, kk))
+        q_out[a:a + live] = q.reshape(live, h * d).to(q_out.dtype)
+        at = torch.arange(p0, p0 + live, device=k.device)
+        ids = table[b, at // page].long()
+        ok = (ids >= 0) & (ids < pages)
+        k[ids[ok], :, at[ok] % page] = kk[ok].to(k.dtype)
+        v[ids[ok], :, at[ok] % page] = vv[ok].to(v.dtype)
+    return q_out
+
+
+@torch.no_grad()
+def paged_attention(q, cache, table, starts, pos, scale: float, doc_start=None, window: int = 0):
+    """See ``ops.paged_attention``; rows of 512 queries at a time."""
+    k, v = cache
+    pages, h, page, d = k.shape
+    n = q.shape[0]
+    y = torch.zeros(n, h * d, dtype=q.dtype, device=q.device)
+    for b, (a, _, p0, live) in enumerate(paged_pieces(starts, pos, n, table.shape[1] * page)):
+        if not live:
+            continue
+        ids = table[b, :-(-(p0 + live) // page)].long()
+        there = ((ids >= 0) & (ids < pages)).repeat_interleave(page)[:p0 + live]
+        keys, values = (x[ids.clamp(0, pages - 1)].transpose(0, 1).reshape(h, -1, d)[:, :p0 + live].float() for x in (k, v))
+        j = torch.arange(p0 + live, device=q.device)
+        for r in range(0, live, 512):
+            e = min(r + 512, live)
+            at = torch.arange(p0 + r, p0 + e, device=q.device)
+            lo = torch.zeros_like(at) if doc_start is None else doc_start[a + r:a + e].long()
+            if window:
+                lo = torch.maximum(lo, (at // 128 - (window // 128 - 1)) * 128)
+            seen = (j <= at[:, None]) & (j >= lo[:, None]) & there
+            s = torch.einsum("thd,hnd->htn", q[a + r:a + e].view(e - r, h, d).float(), keys) * scale
+            s = s.masked_fill(~seen, float("-inf"))
+            w = torch.softmax(s, -1).masked_fill(~seen, 0.0)          # a row without a key has zeros
+            fine = torch.isfinite(values)
+            out = torch.einsum("htn,hnd->thd", w, torch.where(fine, values, torch.zeros_like(values)))
+            for jj in torch.nonzero(~fine.all(-1).all(0) & seen.any(0))[:, 0].tolist():      # 0 times a value that is not finite would not be nothing
+                x = values[:, jj]
+                out += torch.where(seen[:, jj, None, None] & ~torch.isfinite(x), x, torch.zeros_like(x))
+            y[a + r:a + e] = out.reshape(e - r, h * d).to(y.dtype)
+    return y
+
+
+def _law(row, temperature: float):
+    """The soft-max of a row of logits in fp64, or None for a row without a number."""
+    z = row.double()
+    if bool(torch.isnan(z).any()) or float(z.max()) in (float("inf"), float("-inf")):
+        return None
+    e = torch.exp((z - z.max()) / temperature)
+    return e / e.sum()
+
+
+@torch.no_grad()
+def verify_drafts(logits, ids, starts, uniforms, draft_logits, temperature: float, vocab: int):
+    """``(accepted [B], token [B])``, sequence by sequence; see ``ops.verify_drafts``."""
+    n, seq = logits.shape[0], ids.tolist()
+    accepted, tokens = [], []
+    for a, m, _, _ in paged_pieces(starts, starts[:-1], n, 1 << 40):
+        i, token = 0, -1
+        while i < m:
+            r, more = a + i, i + 1 < m
+            x = seq[r + 1] if more else -1
+            p = _law(logits[r, :vocab], temperature or 1.0)
+            if p is None:
+                break
+            if temperature == 0:
+                token = int(torch.nonzero(logits[r, :vocab] == logits[r, :vocab].max())[0])
+                if more and token == x:
+                    i, token = i + 1, -1
+                    continue
+                break
+            u, w = uniforms[r].tolist(), p
+            if more:
+                q = torch.zeros_like(p) if draft_logits is None else _law(draft_logits[r, :vocab], temperature)
+                if 0 <= x < vocab and q is not None:
+                    if draft_logits is None:
+                        q[x] = 1.0
+                    if u[0] * float(q[x]) < float(p[x]):
+                        i += 1
+                        continue
+                if q is not None:
+                    w = (p - q).clamp_min(0.0)
+            w = w if bool((w > 0).any()) else p                    # p and q the same but for rounding
+            c = w.cumsum(0)
+            token = min(int((c <= u[1] * float(c[-1])).sum()), int(torch.nonzero(w)[-1]))      # by rounding none: the last one that has weight
+            break
+        accepted.append(min(i, max(m - 1, 0)))
+        tokens.append(token)
+    return torch.tensor(accepted, dtype=torch.int32, device=logits.device), torch.tensor(tokens, dtype=torch.int64, device=logits.device)
+
+
+# ----------------------------------------------------------------------------------------------------------------
 # Log-probabilities of given tokens, entropy, alternatives
 # ----------------------------------------------------------------------------------------------------------------
 
