@@ -7,6 +7,13 @@ from tests import paged_oracle as O
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def _no_wait_ran_out():
+    yield
+    from them_bones_b200.ops import _lib as L
+    L.check_error_word()
+
+
 def _close(got, want, tol):
     far = ((got.double() - want).abs() - tol).max()
     assert bool(((got.double() - want).abs() <= tol).all()), f"{float(far)} beyond the tolerance"
@@ -285,6 +292,23 @@ def _far(q, c, table, starts, pos, scale):
     from them_bones_b200 import ops
     small = ops.PagedKV(c.k[ids].clone(), c.v[ids].clone())
     return O.attend(q, small, O.i32([[ids.index(x) for x in row] for row in table.tolist()], "cuda"), starts, pos, scale, None, 0)
+
+
+def test_the_same_bits_every_time():
+    """Items of all kinds beside one another, often: what depended on which role came first would show."""
+    from them_bones_b200 import ops
+    lens, pos = [1, 300, 17, 128, 0, 5, 129, 64] * 4, [37 * i * (i % 5) for i in range(32)]
+    c, table, starts, at = O.world(32, 5, 128, 16, lens, pos, "cuda")
+    q = O.queries(sum(lens), 5, 128, "cuda")
+    junk = torch.randint(-2 ** 31, 2 ** 31 - 1, (1 << 22,), dtype=torch.int32, device="cuda")
+    want = {k: ops.paged_attention(q, c, table, starts, at, 0.1, longest=k) for k in (1, 4096)}
+    y, tol = O.attend(q, c, table, starts, at, 0.1, None, 0)
+    for k in (1, 4096):
+        _close(want[k], y, tol)
+    for i in range(300):
+        junk += 1                                       # other kernels' leftovers in shared memory
+        assert torch.equal(ops.paged_attention(q, c, table, starts, at, 0.1, longest=4096), want[4096])
+        assert i % 10 or torch.equal(ops.paged_attention(q, c, table, starts, at, 0.1, longest=1), want[1])
 
 
 def test_native_refusals():

@@ -451,13 +451,6 @@ static int launch_rows(const RowsArgs& p, int S, bool parts, cudaStream_t s) {
   return (int)cudaLaunchKernelEx(&cfg, paged_join_kernel<D>, p, S);
 }
 
-static bool paged_refused(const Paged& p, int D, const void* k, const void* v) {
-  const int page = 1 << p.shift;
-  return (D != 128 && D != 64) || p.B < 1 || p.B > 65534 || p.N < 0 || p.M < 1 || p.H < 1 || p.H > 65535 || p.pages < 1 || p.shift < 4 || p.shift > 7 ||
-         p.ldt < p.M || (long long)p.M * page > 0x7fffff00ll || (long long)p.pages * p.H * page > 0x7fffffffll || !k || !v || !p.starts || !p.pos || !p.table ||
-         (((uintptr_t)k | (uintptr_t)v) & 31);
-}
-
 }  // namespace bones
 
 extern "C" {
@@ -467,8 +460,8 @@ using namespace bones;
 // rows ldt apart; starts: int32 [B + 1]; pos: int32 [B]; q: bf16 [N, H * D].
 int bones_paged_append(const void* qkv, long long ldq, const float* cosT, const float* sinT, int rope_rows, void* k, void* v, int pages, const int* table,
                        long long ldt, const int* starts, const int* pos, int B, int N, int M, int H, int D, int shift, void* q, void* stream) {
-  const Paged p{starts, pos, table, ldt, B, N, M, H, shift, pages, (int)min((long long)M << shift, 0x7fffff00ll)};
-  if (paged_refused(p, D, k, v) || !qkv || !q || !cosT || !sinT || rope_rows < 0 || misaligned16(qkv, q, cosT, sinT) || (N > 1 && ldq % 8)) return -2;
+  const Paged p{starts, pos, table, ldt, B, N, M, H, shift, pages, (int)min((long long)M << shift, 0x7fffff00ll), v};
+  if (paged_refused(B, N, M, H, D, shift, pages, ldt, k, v, starts, pos, table) || !qkv || !q || !cosT || !sinT || rope_rows < 0 || misaligned16(qkv, q, cosT, sinT) || (N > 1 && ldq % 8)) return -2;
   if (N == 0) return 0;
   const long long warps = (long long)N * ((H + 512 / D - 1) / (512 / D));
   if (warps > 0x3fffffffll) return -2;
@@ -485,8 +478,8 @@ int bones_paged_append(const void* qkv, long long ldq, const float* cosT, const 
 int bones_paged_rows(const void* q, const void* k, const void* v, int pages, const int* table, long long ldt, const int* starts, const int* pos,
                      const int* doc_start, void* y, int B, int N, int M, int H, int D, int shift, float scale, int window_tiles, float* parts,
                      long long part_floats, void* stream) {
-  const Paged p{starts, pos, table, ldt, B, N, M, H, shift, pages, (int)min((long long)M << shift, 0x7fffff00ll)};
-  if (paged_refused(p, D, k, v) || !q || !y || (((uintptr_t)q | (uintptr_t)y) & 31) || window_tiles < 0 || misaligned16(parts)) return -2;
+  const Paged p{starts, pos, table, ldt, B, N, M, H, shift, pages, (int)min((long long)M << shift, 0x7fffff00ll), v};
+  if (paged_refused(B, N, M, H, D, shift, pages, ldt, k, v, starts, pos, table) || !q || !y || (((uintptr_t)q | (uintptr_t)y) & 31) || window_tiles < 0 || misaligned16(parts)) return -2;
   if (N == 0) return 0;
   const float log2e = 1.4426950408889634f;
   RowsArgs a{(const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, p, (__nv_bfloat16*)y, doc_start, window_tiles, scale * log2e,

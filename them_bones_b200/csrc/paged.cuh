@@ -15,6 +15,7 @@ struct Paged {
   int shift;           // log2 P
   int pages;
   int cap;             // positions with a place in the table: M * P
+  const void* values;  // the cache's v
 };
 
 struct Piece {
@@ -50,6 +51,15 @@ __device__ __forceinline__ int paged_owner(const int* starts, int B, int r) {
 // First row's offset of page `id`, head h; -1 where there is no such page.
 __device__ __forceinline__ long long paged_at(const Paged& p, int id, int h) {
   return id < 0 || id >= p.pages ? -1 : ((long long)id * p.H + h) << p.shift;
+}
+
+// Host: whether a call is not one that the kernels are made for.
+inline bool paged_refused(int B, int N, int M, int H, int D, int shift, int pages, long long ldt, const void* k, const void* v, const int* starts, const int* pos,
+                          const int* table) {
+  if (shift < 4 || shift > 7) return true;
+  const long long page = 1ll << shift;
+  return (D != 128 && D != 64) || B < 1 || B > 65534 || N < 0 || M < 1 || H < 1 || H > 65535 || pages < 1 || ldt < M || M * page > 0x7fffff00ll ||
+         pages * page * H > 0x7fffff00ll || !k || !v || !starts || !pos || !table || (((uintptr_t)k | (uintptr_t)v) & 31);
 }
 
 }  // namespace bones

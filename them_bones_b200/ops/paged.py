@@ -1,4 +1,4 @@
-"""A key/value cache in pages: its layout, the checks of its calls and the native bodies (``csrc/paged.cu``).
+"""A key/value cache in pages: its layout, the checks of its calls and the native bodies (``csrc/paged.cu``, ``csrc/paged_pieces.cu``).
 
 A cache is two tensors (``PagedKV``) of pages of 16 to 128 tokens; a table says which page each stretch of a sequence is in, so
 sequences of any lengths share one pool and may share pages that they only read.  New tokens come as pieces, packed one after another:
@@ -7,6 +7,7 @@ device and are never read by the host.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
@@ -18,6 +19,8 @@ from .logprobs import has_tangent
 
 PAGES = (16, 32, 64, 128)              # tokens of a page
 SHIFT = 32.0                           # largest |scale| * head_dim: the kernels' soft-max has this fixed shift, and its smallest weights, exp(-2 * 32), stay normal in fp32
+MOST_ROWS = (1 << 31) - 256             # rows of [D] in a cache
+FEW = 16                               # pieces of up to this many tokens go by tiles of 16 rows, longer ones by tiles of 128
 PART_FLOATS = 8 << 20                  # room for the parts of a result (32 MiB at most)
 
 
@@ -33,7 +36,7 @@ class PagedKV(NamedTuple):
 def cache(pages: int, n_head: int, head_dim: int, page: int, device, dtype) -> PagedKV:
     if head_dim not in HEAD_DIMS or page not in PAGES:
         raise ValueError(f"paged cache: head_dim {head_dim} (supported: {HEAD_DIMS}), {page} tokens a page (supported: {PAGES})")
-    if pages < 1 or not 1 <= n_head <= 65535 or pages * n_head * page >= 1 << 31:
+    if pages < 1 or not 1 <= n_head <= 65535 or pages * n_head * page > MOST_ROWS:
         raise ValueError(f"paged cache: {pages} pages, {n_head} heads")
     k, v = (torch.zeros(pages, n_head, page, head_dim, dtype=dtype, device=device) for _ in range(2))
     return PagedKV(k, v)
@@ -48,7 +51,7 @@ def _check(c: PagedKV, table, starts, pos):
     dev = k.get_device()
     if d not in HEAD_DIMS or page not in PAGES or not (
             k.dtype is v.dtype and k.is_floating_point() and v.shape == k.shape and v.get_device() == dev and k.is_contiguous() and v.is_contiguous()
-            and (k.data_ptr() | v.data_ptr()) % 32 == 0 and 1 <= pages and 1 <= h <= 65535 and pages * h * page < 1 << 31):
+            and (k.data_ptr() | v.data_ptr()) % 32 == 0 and 1 <= pages and 1 <= h <= 65535 and pages * h * page <= MOST_ROWS):
         raise ValueError(f"paged cache: k {k.dtype} {tuple(k.shape)}, v {v.dtype} {tuple(v.shape)}: not two contiguous tensors of one cache on one device, each on 32 bytes")
     if not (table.dtype is torch.int32 and table.get_device() == dev and table.stride(1) == 1 and 1 <= b <= 65534 and 1 <= m and m * page <= MAX_LEN
             and (b == 1 or table.stride(0) >= m)):
@@ -130,12 +133,20 @@ def attention(dims, q, c, table, starts, pos, scale, doc_start, window, longest)
     q = _aligned(q, 32)
     y = torch.empty(n, h * d, dtype=q.dtype, device=q.device)
     if n:
+        if longest is None:
+            longest = -(-n // b)
         with L.device(dev):
-            room = parts_room(b, n, m * page, h, d, window)
-            parts = torch.empty(room, dtype=torch.float32, device=q.device) if room else None
-            L.call("bones_paged_rows", q.data_ptr(), c[0].data_ptr(), c[1].data_ptr(), c[0].shape[0], table.data_ptr(), max(table.stride(0), m), starts.data_ptr(),
-                   pos.data_ptr(), 0 if doc_start is None else doc_start.data_ptr(), y.data_ptr(), b, n, m, h, d, page.bit_length() - 1, scale, window // 128,
-                   0 if parts is None else parts.data_ptr(), room, L.raw_stream())
+            common = (q.data_ptr(), c[0].data_ptr(), c[1].data_ptr(), c[0].shape[0], table.data_ptr(), max(table.stride(0), m), starts.data_ptr(), pos.data_ptr(),
+                      0 if doc_start is None else doc_start.data_ptr(), y.data_ptr(), b, n, m, h, d, page.bit_length() - 1, scale, window // 128)
+            if longest > FEW:
+                slots = part_slots(n, m * page, h, window, dev)
+                ints = torch.empty(3 * b + 16, dtype=torch.int32, device=q.device)
+                parts = torch.empty(slots * 128 * (d + 1), dtype=torch.float32, device=q.device) if slots else None
+                L.call("bones_paged_pieces", *common, ints.data_ptr(), 0 if parts is None else parts.data_ptr(), slots, L.raw_stream(), launches=3 if slots else 2)
+            else:
+                room = parts_room(b, n, m * page, h, d, window)
+                parts = torch.empty(room, dtype=torch.float32, device=q.device) if room else None
+                L.call("bones_paged_rows", *common, 0 if parts is None else parts.data_ptr(), room, L.raw_stream(), launches=2 if room else 1)
         COUNTS["paged_attention"] += 1
     return y
 
@@ -144,3 +155,14 @@ def parts_room(b, n, capacity, h, d, window):
     """Floats for the parts of a step's result: what caches of more than 8192 tokens and few heads are given."""
     seen = min(capacity, window + 128) if window else capacity
     return min(PART_FLOATS, n * h * (d + 4) * (seen // 1024)) if seen > 8192 and b * h < 512 else 0
+
+
+@functools.lru_cache(maxsize=None)
+def _sms(dev: int) -> int:
+    return torch.cuda.get_device_properties(dev).multi_processor_count
+
+
+def part_slots(n, capacity, h, window, dev):
+    """Places for parts of a tile of 128 queries: four an SM, none where the tiles alone are two an SM or see a few tiles of keys at most."""
+    seen = min(capacity, window + 128) if window else capacity
+    return 4 * _sms(dev) if seen > 768 and n // 128 * h < 2 * _sms(dev) else 0
