@@ -96,7 +96,7 @@ def _ok():
     dict(ids=torch.zeros(4, dtype=torch.int64)), dict(ids=torch.zeros(5, dtype=torch.int32)), dict(starts=torch.zeros(1, dtype=torch.int32)),
     dict(starts=torch.zeros(3, dtype=torch.int64)), dict(uniforms=None), dict(uniforms=torch.zeros(5)), dict(uniforms=torch.zeros(5, 2, dtype=torch.float64)),
     dict(draft_logits=torch.zeros(5, 15)), dict(draft_logits=torch.zeros(5, 16).bfloat16()), dict(temperature=-1.0), dict(temperature=1e-9),
-    dict(temperature=float("inf")), dict(temperature=float("nan")), dict(vocab=0), dict(vocab=17)])
+    dict(temperature=float("inf")), dict(temperature=1e7), dict(temperature=float("nan")), dict(vocab=0), dict(vocab=17)])
 def test_calls_that_are_refused(change):
     with pytest.raises(ValueError):
         ops.verify_drafts(**{**_ok(), **change})

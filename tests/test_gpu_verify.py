@@ -93,10 +93,9 @@ def test_masked_columns_and_drafts_outside():
             z[:, 55] = 1.0
             u = torch.tensor([[0.5, 0.999], [0.5, 0.0]], device="cuda")
             for x, want in ((55, (1, 55)), (-1, (0, 55)), (300, (0, 55)), (1 << 40, (0, 55)), (3, (0, 55))):
-                for t in (1.0, 0.0, 1e-6, 1e30):
+                for t in (1.0, 0.0, 1e-6, 1e6):
                     got = ops.verify_drafts(z, torch.tensor([0, x], device="cuda"), O.i32([0, 2], "cuda"), u, temperature=t)
-                    if t != 1e30 or low == float("-inf"):
-                        assert (int(got.accepted), int(got.token)) == want, (dtype, low, x, t)
+                    assert (int(got.accepted), int(got.token)) == want, (dtype, low, x, t)
 
 
 def test_ties_go_to_the_lowest_index():

@@ -118,13 +118,20 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __nv_bfloat16* 
 // 16 consecutive dimensions of key g as its share of four steps (32 bytes a load), with the queries laid out alike; of the values it takes
 // D / 8 consecutive dimensions of keys 2c, 2c + 1, 2c + 8, 2c + 9, whose pairs two byte permutations make into operands.
 // Probabilities enter the second product in bf16, the type of the values: each is off by 2^-8 of itself at most.
+//
+// The turns of all tiles of all heads, one after another, are shared equally by as many warps as the SMs hold: a step's sequences have any lengths,
+// and with a CTA or a cluster a head the way in and out of each was longer than its turns.  A warp that has all turns of a tile writes its
+// rows; of the at most two tiles that it shares with others it leaves sums, which a second kernel adds in order.  A tile counts as RC turns more than it
+// has, the way to its first keys: without them a warp got as many tiles of a turn or two as others got turns of one.
 constexpr int RW = 4;                       // warps of a CTA
 constexpr int RT = 16;                      // rows of a tile, keys of a turn
+constexpr int RB = 512;                     // sequences of a call
+constexpr int RC = 3;                       // turns that getting to a tile counts for
 
 __device__ __forceinline__ void mma_bf16_16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ bool pair_not_finite(uint32_t u) { return (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u; }
 
@@ -136,8 +143,10 @@ struct RowsArgs {
   const int* doc_start;       // [N] or null
   int window_tiles;
   float c1, c2;               // scale log2 e, |scale| D log2 e
-  float* parts;               // PARTS: [N, H, gridDim.x, D + 4]
-  int turns;                  // PARTS: turns of a part
+  long long* before;          // [B + 1]: turns of the sequences before
+  int* first;                 // [B]: the first key that one of the sequence's rows sees, a multiple of 16
+  float* parts;               // [warps][2][RT][D + 4]: sums of the tile that a warp's turns begin in and of the one that they end in
+  int warps;
 };
 
 __device__ __forceinline__ int paged_first_key(const RowsArgs& p, int row, int pos) {
@@ -145,310 +154,348 @@ __device__ __forceinline__ int paged_first_key(const RowsArgs& p, int row, int p
   if (p.window_tiles > 0) lo = max(lo, ((pos >> 7) - (p.window_tiles - 1)) * 128);
   return lo;
 }
+// What tile t of a piece whose first row is `ahead` keys behind the first key counts for: RC and its turns, to the end of its last row; 0 without keys.
+__device__ __forceinline__ int tile_turns(int ahead, int live, int t) {
+  const int n = max(ahead + min(live, (t + 1) * RT) + RT - 1, 0) / RT;
+  return n ? n + RC : 0;
+}
+// and of all tiles in front of t
+__device__ __forceinline__ int turns_before(int ahead, int live, int t) {
+  int n = 0;
+  for (int i = 0; i < t; ++i) n += tile_turns(ahead, live, i);
+  return n;
+}
+// A warp's turns: from w * share to below (w + 1) * share
+__device__ __forceinline__ int turn_share(long long total, int warps) { return (int)max((total + warps - 1) / warps, (long long)RC + 1); }
 
-// Where a tile's keys lie: `first` (a multiple of 16) and `turns` of 16 keys.
-struct TileKeys {
-  int first, turns;
-};
-
+__device__ __forceinline__ void ld_32(uint32_t* r, const __nv_bfloat16* p) {
+  uint4 a, b;
+  ld_global_v8(p, a, b);
+  r[0] = a.x; r[1] = a.y; r[2] = a.z; r[3] = a.w; r[4] = b.x; r[5] = b.y; r[6] = b.z; r[7] = b.w;
+}
 template <int D>
-__device__ __forceinline__ void ld_row(uint32_t* r, const __nv_bfloat16* p) {          // D / 8 consecutive values, 32 bytes (16 of heads of 64)
+__device__ __forceinline__ void ld_value(uint32_t* r, const __nv_bfloat16* p) {          // D / 8 consecutive values
   if (D == 128) {
-    uint4 a, b;
-    ld_global_v8(p, a, b);
-    r[0] = a.x; r[1] = a.y; r[2] = a.z; r[3] = a.w; r[4] = b.x; r[5] = b.y; r[6] = b.z; r[7] = b.w;
+    ld_32(r, p);
   } else {
     const uint4 a = *reinterpret_cast<const uint4*>(p);
     r[0] = a.x; r[1] = a.y; r[2] = a.z; r[3] = a.w;
   }
 }
 
-// grid: (CTAs of a head, H, B + 1): the last layer clears the rows that belong to no sequence.  PARTS: each CTA of a head takes `turns` turns of
-// its keys and leaves sums; else the CTAs are a cluster that shares the turns equally and joins its sums through distributed shared memory.
-template <int D, bool PARTS>
-__global__ void __launch_bounds__(32 * RW, 3) paged_rows_kernel(const RowsArgs p) {
-  constexpr int KC = D / 64;                // 32-byte pieces of a key a lane has
-  constexpr int NV = D / 8;                 // dimensions of a value a lane has: tiles of eight output columns
-  constexpr int LD = D + 4;                 // a row of sums: column d at d + d / 32, so that a warp's stores meet no bank twice
-  extern __shared__ __align__(16) float red[];   // [RW][RT][LD] sums, [RW][RT] sums of weights, the CTA's own [RT][LD] and [RT], the queries
-  float* red_l = red + RW * RT * LD;
-  float* own = red_l + RW * RT;
-  float* own_l = own + RT * LD;
-  uint4* qs = reinterpret_cast<uint4*>(own_l + RT);        // [KC][4][32]: the A operand's registers, lane by lane
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-  const int h = blockIdx.y, seq = blockIdx.z;
-  const long long A = (long long)p.p.H * D;
-  const int S = gridDim.x, rank = blockIdx.x;
-  if (seq == p.p.B) {                       // (the whole cluster is here)
-    const int head = min(max(p.p.starts[0], 0), p.p.N), tail = min(max(p.p.starts[p.p.B], head), p.p.N);
-    for (int r = rank; r < head + p.p.N - tail; r += S) {
-      const int row = r < head ? r : tail + r - head;
-      for (int d = threadIdx.x; d < D; d += 32 * RW) p.y[row * A + (long long)h * D + d] = __float2bfloat16(0.f);
+// What the CTAs' threads agree on: turns before each sequence.  At most RB sequences.
+__device__ __forceinline__ long long rows_plan(const RowsArgs& p, long long* before, int* first, Piece* pieces, long long* box) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long total = 0;
+  for (int b0 = 0; b0 < p.p.B; b0 += 32 * RW) {
+    const int b = b0 + threadIdx.x;
+    long long n = 0;
+    int f = 0;
+    if (b < p.p.B) {
+      const Piece s = paged_piece(p.p, b);
+      pieces[b] = s;
+      if (s.live) {
+        int lo = 0x7fffffff;
+        if (p.doc_start) {
+#pragma unroll 4
+          for (int i = 0; i < s.live; ++i) lo = min(lo, paged_first_key(p, s.row + i, s.pos + i));
+        } else {
+          lo = paged_first_key(p, s.row, s.pos);
+        }
+        f = lo & ~(RT - 1);
+        const int tiles = (s.live + RT - 1) / RT;
+        n = (long long)p.p.H * turns_before(s.pos - f, s.live, tiles);
+      }
     }
-    return;
-  }
-  const Piece s = paged_piece(p.p, seq);
-  const int* table = p.p.table + seq * p.p.ldt;
-  const int mask = (1 << p.p.shift) - 1;
-  for (int t0 = 0; t0 < s.len; t0 += RT) {
-    const int n = min(RT, s.len - t0), live = min(max(s.live - t0, 0), n), row0 = s.row + t0, pos0 = s.pos + t0;
-    // rows g and g + 8 of the tile: their positions and first keys
-    const int pos_a = g < live ? pos0 + g : -1, pos_b = g + 8 < live ? pos0 + g + 8 : -1;
-    const int lo_a = g < live ? paged_first_key(p, row0 + g, pos_a) : 0x7fffffff, lo_b = g + 8 < live ? paged_first_key(p, row0 + g + 8, pos_b) : 0x7fffffff;
-    const int lo = __reduce_min_sync(0xffffffffu, min(lo_a, lo_b)), hi_lo = __reduce_max_sync(0xffffffffu, max(g < live ? lo_a : 0, g + 8 < live ? lo_b : 0));
-    const int first = lo & ~(RT - 1), end = live ? pos0 + live : 0;       // keys first .. end
-    const int turns = end > first ? (end - first + RT - 1) / RT : 0;
-    // this warp's turns: `from`, from + step, ... below `to`
-    const int from = PARTS ? rank * p.turns + warp : rank * RW + warp, step = PARTS ? RW : S * RW, to = PARTS ? min(turns, (rank + 1) * p.turns) : turns;
-    // queries: step (j, i) takes rows g, g + 8 at dimensions 16 (4 j + c) + 4 i + {0, 1} and + {2, 3}; the registers of all steps would leave no room
-    // for the keys and values on their way
-    for (int i = warp; i < KC * 4; i += RW) {
-      const int r = g + (i & 1) * 8;
-      qs[i * 32 + lane] = r < live ? *reinterpret_cast<const uint4*>(p.q + (long long)(row0 + r) * A + (long long)h * D + (i >> 2) * 64 + c * 16 + ((i >> 1) & 1) * 8)
-                                   : make_uint4(0, 0, 0, 0);
+    long long up = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += x;
+    }
+    if (lane == 31) box[warp] = up;
+    __syncthreads();
+    long long front = total;
+    for (int w = 0; w < RW; ++w) {
+      if (w < warp) front += box[w];
+      total += box[w];
+    }
+    if (b < p.p.B) {
+      before[b] = front + up - n;
+      first[b] = f;
     }
     __syncthreads();
+  }
+  if (threadIdx.x == 0) before[p.p.B] = total;
+  __syncthreads();
+  return total;
+}
+
+template <int D>
+__global__ void __launch_bounds__(32 * RW, D == 128 ? 3 : 4) paged_rows_kernel(const RowsArgs p) {
+  constexpr int KC = D / 64;                // 32-byte pieces of a key that a lane has
+  constexpr int NV = D / 8;                 // dimensions of a value that a lane has: tiles of eight output columns
+  __shared__ long long before[RB + 1], box[RW];
+  __shared__ int first_of[RB];
+  __shared__ Piece piece_of[RB];
+  __shared__ uint4 qs_all[RW][KC * 4 * 32];        // a warp's queries: the A operand's registers, lane by lane
+  pdl_launch();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const long long A = (long long)p.p.H * D;
+  const int mask = (1 << p.p.shift) - 1;
+  const long long total = rows_plan(p, before, first_of, piece_of, box);
+  if (blockIdx.x == 0) {                     // for the join
+    for (int b = threadIdx.x; b <= p.p.B; b += 32 * RW) {
+      p.before[b] = before[b];
+      if (b < p.p.B) p.first[b] = first_of[b];
+    }
+  }
+  const int share = turn_share(total, p.warps), me = blockIdx.x * RW + warp;
+  long long at_turn = (long long)me * share;
+  const long long end_turn = min(at_turn + share, total);
+  uint4* qs = qs_all[warp];
+  const uint32_t qs_at = smem_u32(qs + lane);
+  while (at_turn < end_turn) {
+    // the sequence, head and tile of the turn
+    int b = 0;
+    for (int n = p.p.B; n > 1;) {
+      const int half = n >> 1;
+      if (before[b + half] <= at_turn) b += half;
+      n -= half;
+    }
+    const Piece s = piece_of[b];
+    const int key0 = first_of[b], ahead = s.pos - key0, tiles = (s.live + RT - 1) / RT, a_head = turns_before(ahead, s.live, tiles);
+    const long long in_seq = at_turn - before[b];
+    const int h = (int)(in_seq / a_head);
+    int from = (int)(in_seq % a_head), t = 0, turns = tile_turns(ahead, s.live, 0);
+    while (from >= turns) {
+      from -= turns;
+      turns = tile_turns(ahead, s.live, ++t);
+    }
+    int to = (int)min((long long)turns, from + end_turn - at_turn);
+    at_turn += to - from;
+    // without what getting there counts for
+    from = max(from - RC, 0);
+    to -= RC;
+    turns -= RC;
+    if (to <= from) continue;
+    const int live = min(RT, s.live - t * RT), row0 = s.row + t * RT, pos0 = s.pos + t * RT;
+    const int* table = p.p.table + b * p.p.ldt;
+    uint32_t kr[2][KC][8], vr[4][NV / 2];
+    auto page_of = [&](int turn) { return turn < to ? table[(key0 + turn * RT) >> p.p.shift] : -1; };
+    auto place = [&](int turn, int id) {
+      const long long at = paged_at(p.p, id, h);
+      return at < 0 ? at : (at + ((key0 + turn * RT) & mask)) * D;
+    };
+    auto load_k = [&](long long at) {
+      if (at < 0) return;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < KC; ++j) ld_32(kr[i][j], p.k + at + (long long)(8 * i + g) * D + (4 * j + c) * 16);
+    };
+    auto load_v = [&](long long at) {
+      if (at < 0) return;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ld_value<D>(vr[i], p.v + at + (long long)(2 * c + (i & 1) + 8 * (i >> 1)) * D + g * NV);
+    };
+    // All that comes from memory is asked for before any of it is waited for, but for the keys and values, which wait for their page.
+    const int id_first = page_of(from);
+    int id_next = page_of(from + 1);
+    // rows g and g + 8: their positions and first keys
+    const int pos_a = g < live ? pos0 + g : -1, pos_b = g + 8 < live ? pos0 + g + 8 : -1;
+    const int lo_a = g < live ? paged_first_key(p, row0 + g, pos_a) : 0x7fffffff, lo_b = g + 8 < live ? paged_first_key(p, row0 + g + 8, pos_b) : 0x7fffffff;
+    // queries: step (j, i) takes rows g, g + 8 at dimensions 16 (4 j + c) + 4 i + {0, 1} and + {2, 3}; the registers of all steps would leave no room
+    // for the keys and values on their way
+    uint4 qr[KC * 4];
+#pragma unroll
+    for (int i = 0; i < KC * 4; ++i) {
+      const int r = g + (i & 1) * 8;
+      qr[i] = r < live ? *reinterpret_cast<const uint4*>(p.q + (long long)(row0 + r) * A + (long long)h * D + (i >> 2) * 64 + c * 16 + ((i >> 1) & 1) * 8)
+                       : make_uint4(0, 0, 0, 0);
+    }
+    long long at = place(from, id_first);
+    load_k(at);
+    load_v(at);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < KC * 4; ++i) qs[i * 32 + lane] = qr[i];
+    __syncwarp();
+    const int far = __reduce_max_sync(0xffffffffu, max(g < live ? lo_a : 0, g + 8 < live ? lo_b : 0));
     float o[NV][4], l_a = 0.f, l_b = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    if (from < to) {
-      uint32_t kr[2][KC][8], vr[4][NV / 2];
-      auto page_of = [&](int turn) { return turn < to ? table[(first + turn * RT) >> p.p.shift] : -1; };
-      auto place = [&](int turn, int id) {
-        const long long at = paged_at(p.p, id, h);
-        return at < 0 ? at : (at + ((first + turn * RT) & mask)) * D;
-      };
-      auto load_k = [&](long long at) {
-        if (at < 0) return;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int j = 0; j < KC; ++j) ld_row<128>(kr[t][j], p.k + at + (long long)(8 * t + g) * D + (4 * j + c) * 16);
-      };
-      auto load_v = [&](long long at) {
-        if (at < 0) return;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) ld_row<D>(vr[t], p.v + at + (long long)(2 * c + (t & 1) + 8 * (t >> 1)) * D + g * NV);
-      };
-      const uint32_t qs_at = smem_u32(qs + lane);
-      long long at = place(from, page_of(from));
-      load_k(at);
-      load_v(at);
-      int id_next = page_of(from + step);
-      for (int turn = from; turn < to; turn += step) {
-        const int k0 = first + turn * RT;
-        const long long at_next = place(turn + step, id_next), now = at;
-        id_next = page_of(turn + 2 * step);
-        at = at_next;
-        if (now < 0) {                              // no such page: its positions are not seen
-          load_k(at);
-          load_v(at);
-          continue;
-        }
-        float sc[2][4] = {};
-#pragma unroll
-        for (int j = 0; j < KC; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; i += 2) {
-            uint32_t x[2][4];                        // rows g and g + 8
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[r][0]), "=r"(x[r][1]), "=r"(x[r][2]), "=r"(x[r][3]) : "r"(qs_at + (j * 4 + i + r) * 512));
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t a[4] = {x[0][2 * e], x[1][2 * e], x[0][2 * e + 1], x[1][2 * e + 1]};
-              mma_bf16_16816(sc[0], a, kr[0][j][2 * (i + e)], kr[0][j][2 * (i + e) + 1]);
-              mma_bf16_16816(sc[1], a, kr[1][j][2 * (i + e)], kr[1][j][2 * (i + e) + 1]);
-            }
-          }
+    for (int turn = from; turn < to; ++turn) {
+      const int k0 = key0 + turn * RT;
+      const long long at_next = place(turn + 1, id_next), now = at;
+      id_next = page_of(turn + 2);
+      at = at_next;
+      if (now < 0) {                              // no such page: its positions are not seen
         load_k(at);
-        // columns 2 c, 2 c + 1 of both halves
+        load_v(at);
+        continue;
+      }
+      float sc[2][4] = {};
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+      for (int j = 0; j < KC; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          uint32_t x[2][4];                        // rows g and g + 8
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[r][0]), "=r"(x[r][1]), "=r"(x[r][2]), "=r"(x[r][3]) : "r"(qs_at + (j * 4 + i + r) * 512));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t a[4] = {x[0][2 * e], x[1][2 * e], x[0][2 * e + 1], x[1][2 * e + 1]};
+            mma_bf16_16816(sc[0], a, kr[0][j][2 * (i + e)], kr[0][j][2 * (i + e) + 1]);
+            mma_bf16_16816(sc[1], a, kr[1][j][2 * (i + e)], kr[1][j][2 * (i + e) + 1]);
+          }
+        }
+      load_k(at);
+      // columns 2 c, 2 c + 1 of both halves
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = fmaf(sc[i][e], p.c1, -p.c2);
+          asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(sc[i][e]) : "f"(x));
+        }
+      const bool masked = k0 + RT - 1 > pos0 || k0 < far;      // some row does not see some key
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float x = fmaf(sc[t][e], p.c1, -p.c2);
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(sc[t][e]) : "f"(x));
+            const int key = k0 + 8 * i + 2 * c + (e & 1);
+            if (key > (e < 2 ? pos_a : pos_b) || key < (e < 2 ? lo_a : lo_b)) sc[i][e] = 0.f;
           }
-        const bool masked = k0 + RT - 1 > pos0 || k0 < hi_lo;      // some row does not see some key
-        if (masked) {
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int key = k0 + 8 * t + 2 * c + (e & 1);
-              if (key > (e < 2 ? pos_a : pos_b) || key < (e < 2 ? lo_a : lo_b)) sc[t][e] = 0.f;
-            }
-        }
-        l_a += (sc[0][0] + sc[0][1]) + (sc[1][0] + sc[1][1]);
-        l_b += (sc[0][2] + sc[0][3]) + (sc[1][2] + sc[1][3]);
-        const uint32_t pr[4] = {pack_bf16(sc[0][0], sc[0][1]), pack_bf16(sc[0][2], sc[0][3]), pack_bf16(sc[1][0], sc[1][1]), pack_bf16(sc[1][2], sc[1][3])};
-        if (masked) {
-          // a value that is not finite would make NaN of the zeros of rows that do not see it (behind the sequence's end lies what the page held before)
-          uint32_t odd = 0;
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int i = 0; i < NV / 2; ++i) odd |= pair_not_finite(vr[t][i]);
-          if (__any_sync(0xffffffffu, odd)) {
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-              for (int i = 0; i < NV / 2; ++i) {
-                uint32_t u = vr[t][i];
-                if ((u & 0x7f80u) == 0x7f80u) u &= 0xffff0000u;
-                if ((u & 0x7f800000u) == 0x7f800000u) u &= 0xffffu;
-                vr[t][i] = u;
-              }
-            for (int j = 0; j < RT; ++j) {          // and goes to those that do
-              const int key = k0 + j;
-              const bool in_a = key <= pos_a && key >= lo_a, in_b = key <= pos_b && key >= lo_b;
-              const __nv_bfloat16* val = p.v + now + (long long)j * D;
-#pragma unroll
-              for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const float x = __bfloat162float(val[(2 * c + e) * NV + i]);
-                  if (!isfinite(x)) {
-                    if (in_a) o[i][e] += x;
-                    if (in_b) o[i][2 + e] += x;
-                  }
-                }
-            }
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < NV / 2; ++i) {
-          // dimensions 2 i and 2 i + 1 of this lane's: pairs of keys
-          mma_bf16_16816(o[2 * i], pr, __byte_perm(vr[0][i], vr[1][i], 0x5410), __byte_perm(vr[2][i], vr[3][i], 0x5410));
-          mma_bf16_16816(o[2 * i + 1], pr, __byte_perm(vr[0][i], vr[1][i], 0x7632), __byte_perm(vr[2][i], vr[3][i], 0x7632));
-        }
-        load_v(at);
       }
+      l_a += (sc[0][0] + sc[0][1]) + (sc[1][0] + sc[1][1]);
+      l_b += (sc[0][2] + sc[0][3]) + (sc[1][2] + sc[1][3]);
+      const uint32_t pr[4] = {pack_bf16(sc[0][0], sc[0][1]), pack_bf16(sc[0][2], sc[0][3]), pack_bf16(sc[1][0], sc[1][1]), pack_bf16(sc[1][2], sc[1][3])};
+      if (masked) {
+        // a value that is not finite would make NaN of the zeros of rows that do not see it (behind the sequence's end lies what the page held before)
+        uint32_t odd = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < NV / 2; ++i) odd |= pair_not_finite(vr[j][i]);
+        if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < NV / 2; ++i) {
+              uint32_t u = vr[j][i];
+              if ((u & 0x7f80u) == 0x7f80u) u &= 0xffff0000u;
+              if ((u & 0x7f800000u) == 0x7f800000u) u &= 0xffffu;
+              vr[j][i] = u;
+            }
+          for (int j = 0; j < RT; ++j) {          // and goes to those that do
+            const int key = k0 + j;
+            const bool in_a = key <= pos_a && key >= lo_a, in_b = key <= pos_b && key >= lo_b;
+            const __nv_bfloat16* val = p.v + now + (long long)j * D;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float x = __bfloat162float(val[(2 * c + e) * NV + i]);
+                if (!isfinite(x)) {
+                  if (in_a) o[i][e] += x;
+                  if (in_b) o[i][2 + e] += x;
+                }
+              }
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NV / 2; ++i) {
+        // dimensions 2 i and 2 i + 1 of this lane's: pairs of keys
+        mma_bf16_16816(o[2 * i], pr, __byte_perm(vr[0][i], vr[1][i], 0x5410), __byte_perm(vr[2][i], vr[3][i], 0x5410));
+        mma_bf16_16816(o[2 * i + 1], pr, __byte_perm(vr[0][i], vr[1][i], 0x7632), __byte_perm(vr[2][i], vr[3][i], 0x7632));
+      }
+      load_v(at);
     }
     l_a += __shfl_xor_sync(0xffffffffu, l_a, 1);
     l_a += __shfl_xor_sync(0xffffffffu, l_a, 2);
     l_b += __shfl_xor_sync(0xffffffffu, l_b, 1);
     l_b += __shfl_xor_sync(0xffffffffu, l_b, 2);
-    // warps of the CTA, in their order
+    // a lane has dimensions 2 c NV .. 2 (c + 1) NV of rows g and g + 8
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int half = 0; half < 2; ++half) {
+      const int r = g + 8 * half;
+      const float l = half ? l_b : l_a;
+      if (r >= live) continue;
+      if (from == 0 && to == turns) {                // all of the tile's
+        const float inv = l == 0.f ? 0.f : 1.0f / l;       // a row that sees no key has zeros
+        __nv_bfloat16* y = p.y + (long long)(row0 + r) * A + (long long)h * D + 2 * c * NV;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int d = (2 * c + e) * NV + i;
-        if (g < live) red[(warp * RT + g) * LD + d + (d >> 5)] = o[i][e];
-        if (g + 8 < live) red[(warp * RT + g + 8) * LD + d + (d >> 5)] = o[i][2 + e];
-      }
-    if (c == 0) {
-      red_l[warp * RT + g] = l_a;
-      red_l[warp * RT + g + 8] = l_b;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < live * D; i += 32 * RW) {
-      const int d = i % D, at = i / D * LD + d + (d >> 5);
-      float x = 0.f;
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
-      for (int w = 0; w < RW; ++w) x += red[w * RT * LD + at];
-      if (PARTS) {
-        if (rank * p.turns < turns) p.parts[(((long long)(row0 + i / D) * p.p.H + h) * S + rank) * (D + 4) + d] = x;
-      } else {
-        own[at] = x;
-      }
-    }
-    if (threadIdx.x < live) {
-      float x = 0.f;
+          for (int i = 0; i < NV; i += 8) {
+            uint32_t u[4];
 #pragma unroll
-      for (int w = 0; w < RW; ++w) x += red_l[w * RT + threadIdx.x];
-      if (PARTS) {
-        if (rank * p.turns < turns) p.parts[(((long long)(row0 + threadIdx.x) * p.p.H + h) * S + rank) * (D + 4) + D] = x;
-      } else {
-        own_l[threadIdx.x] = x;
-      }
-    }
-    if (!PARTS) {
-      __syncthreads();
-      if (S > 1) cluster_barrier();
-      // the cluster's CTAs each finish some of the values
-      for (int i = rank * 32 * RW + threadIdx.x; i < n * D; i += S * 32 * RW) {
-        const int d = i % D;
-        float x = 0.f, l = 0.f;
-        if (i < live * D) {
-          if (S > 1) {
-            const uint32_t at_x = smem_u32(own + i / D * LD + d + (d >> 5)), at_l = smem_u32(own_l + i / D);
-            for (int r = 0; r < S; ++r) {
-              float a, b;
-              asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(a) : "r"(map_to_rank(at_x, r)));
-              asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(b) : "r"(map_to_rank(at_l, r)));
-              x += a;
-              l += b;
-            }
-          } else {
-            x = own[i / D * LD + d + (d >> 5)];
-            l = own_l[i / D];
+            for (int k = 0; k < 4; ++k) u[k] = pack_bf16(o[i + 2 * k][2 * half + e] * inv, o[i + 2 * k + 1][2 * half + e] * inv);
+            *reinterpret_cast<uint4*>(y + e * NV + i) = make_uint4(u[0], u[1], u[2], u[3]);
           }
-        }
-        // a row that sees no key has zeros
-        p.y[(long long)(row0 + i / D) * A + (long long)h * D + d] = __float2bfloat16(l == 0.f ? 0.f : x / l);
+      } else {
+        float* part = p.parts + (((long long)me * 2 + (from > 0 ? 0 : 1)) * RT + r) * (D + 4);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int i = 0; i < NV; i += 4)
+            *reinterpret_cast<float4*>(part + (2 * c + e) * NV + i) =
+                make_float4(o[i][2 * half + e], o[i + 1][2 * half + e], o[i + 2][2 * half + e], o[i + 3][2 * half + e]);
+        if (c == 0) part[D] = l;
       }
-      __syncwarp();
-      if (S > 1) cluster_barrier();             // nobody's sums change or go before all have read them
     }
-    __syncthreads();
   }
 }
 
-// Joins the parts of a row and head in their order.  grid: (N, H), D threads.
+// Adds a row's sums where several warps have some, in their order; zeros for rows without a result.  grid: (N, H), D threads.
 template <int D>
-__global__ void __launch_bounds__(D) paged_join_kernel(const RowsArgs p, int S) {
+__global__ void __launch_bounds__(D) paged_rows_join_kernel(const RowsArgs p) {
   pdl_wait();
   const int row = blockIdx.x, h = blockIdx.y, d = threadIdx.x;
-  const int seq = paged_owner(p.p.starts, p.p.B, row);
-  if (seq < 0 || seq >= p.p.B) return;              // cleared already
-  const Piece s = paged_piece(p.p, seq);
-  const int i = row - s.row;
-  if (i < 0 || i >= s.len) return;
-  // the turns of the tile that the row was in
-  const int t0 = i / RT * RT, live = min(max(s.live - t0, 0), RT), lane = d & 31;
-  int lo = 0x7fffffff;
-  if (lane < live) lo = paged_first_key(p, s.row + t0 + lane, s.pos + t0 + lane);
-  lo = __reduce_min_sync(0xffffffffu, lo);
-  const int first = lo & ~(RT - 1), end = live ? s.pos + t0 + live : 0;
-  const int turns = end > first ? (end - first + RT - 1) / RT : 0, parts = min((turns + p.turns - 1) / p.turns, S);
+  __nv_bfloat16* y = p.y + ((long long)row * p.p.H + h) * D + d;
+  const int b = paged_owner(p.p.starts, p.p.B, row);
   float x = 0.f, l = 0.f;
-  if (i < s.live) {
-    const float* at = p.parts + ((long long)row * p.p.H + h) * S * (D + 4);
+  if (b >= 0 && b < p.p.B) {
+    const Piece s = paged_piece(p.p, b);
+    const int i = row - s.row;
+    if (i >= 0 && i < s.live) {
+      const int ahead = s.pos - p.first[b], tiles = (s.live + RT - 1) / RT, turns = tile_turns(ahead, s.live, i / RT);
+      if (turns > 0) {
+        const long long from = p.before[b] + (long long)h * turns_before(ahead, s.live, tiles) + turns_before(ahead, s.live, i / RT);
+        const int share = turn_share(p.before[p.p.B], p.warps), w0 = (int)((from + RC) / share), w1 = (int)((from + turns - 1) / share);
+        if (w0 == w1) return;                      // written
+        const float* at = p.parts + (((long long)w0 * 2 + 1) * RT + i % RT) * (D + 4);
+        x = at[d];
+        l = at[D];
+        at += RT * (D + 4);                        // the next warp's first
 #pragma unroll 8
-    for (int r = 0; r < parts; ++r) {
-      x += at[r * (D + 4) + d];
-      l += at[r * (D + 4) + D];
+        for (int w = w0 + 1; w <= w1; ++w, at += 2 * RT * (D + 4)) {
+          x += at[d];
+          l += at[D];
+        }
+      }
     }
   }
-  p.y[(long long)row * p.p.H * D + (long long)h * D + d] = __float2bfloat16(l == 0.f ? 0.f : x / l);
+  *y = __float2bfloat16(l == 0.f ? 0.f : x / l);
 }
 
 template <int D>
-static int launch_rows(const RowsArgs& p, int S, bool parts, cudaStream_t s) {
-  constexpr size_t smem = sizeof(float) * (RW * RT * (D + 4) + RW * RT + RT * (D + 4) + RT) + D / 64 * 4 * 32 * 16;
-  static OncePerDevice limit;
-  BONES_ONCE(limit, {
-    BONES_CHECK(cudaFuncSetAttribute(paged_rows_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    BONES_CHECK(cudaFuncSetAttribute(paged_rows_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  });
+static int launch_rows(RowsArgs& p, int ctas, cudaStream_t s) {
+  p.warps = ctas * RW;
+  paged_rows_kernel<D><<<(unsigned)ctas, 32 * RW, 0, s>>>(p);
+  BONES_CHECK(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
-  cfg.gridDim = dim3((unsigned)S, (unsigned)p.p.H, (unsigned)p.p.B + 1);
-  cfg.blockDim = dim3(32 * RW);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cfg.attrs = at;
-  cfg.numAttrs = (unsigned)dec_launch_attrs(at, parts ? 1 : S, 0);
-  if (!parts) return (int)cudaLaunchKernelEx(&cfg, paged_rows_kernel<D, false>, p);
-  BONES_CHECK(cudaLaunchKernelEx(&cfg, paged_rows_kernel<D, true>, p));
   cfg.gridDim = dim3((unsigned)p.p.N, (unsigned)p.p.H);
   cfg.blockDim = dim3(D);
-  cfg.dynamicSmemBytes = 0;
+  cfg.stream = s;
+  cfg.attrs = at;
   cfg.numAttrs = (unsigned)dec_launch_attrs(at, 1, 1);
-  return (int)cudaLaunchKernelEx(&cfg, paged_join_kernel<D>, p, S);
+  return (int)cudaLaunchKernelEx(&cfg, paged_rows_join_kernel<D>, p);
 }
 
 }  // namespace bones
@@ -474,29 +521,27 @@ int bones_paged_append(const void* qkv, long long ldq, const float* cosT, const 
   return (int)cudaGetLastError();
 }
 
-// q, y: bf16 [N, H * D]; doc_start: int32 [N] or null; parts: room for part_floats floats on 16 bytes, of this call alone until it ends, or null.
+// CTAs that share a step's turns, for a device of `sms` SMs; what `work` has to have room for goes by them.
+int bones_paged_rows_ctas(int D, int sms) { return (D == 128 ? 3 : 4) * sms; }
+
+// q, y: bf16 [N, H * D]; doc_start: int32 [N] or null; at most 512 sequences.  work: of this call alone until it ends, 32-byte aligned: with C =
+// bones_paged_rows_ctas, 8 C tiles of 16 * (D + 4) floats and then B + 1 64-bit and B 32-bit whole numbers.
 int bones_paged_rows(const void* q, const void* k, const void* v, int pages, const int* table, long long ldt, const int* starts, const int* pos,
-                     const int* doc_start, void* y, int B, int N, int M, int H, int D, int shift, float scale, int window_tiles, float* parts,
-                     long long part_floats, void* stream) {
-  const Paged p{starts, pos, table, ldt, B, N, M, H, shift, pages, (int)min((long long)M << shift, 0x7fffff00ll), v};
-  if (paged_refused(B, N, M, H, D, shift, pages, ldt, k, v, starts, pos, table) || !q || !y || (((uintptr_t)q | (uintptr_t)y) & 31) || window_tiles < 0 || misaligned16(parts)) return -2;
+                     const int* doc_start, void* y, int B, int N, int M, int H, int D, int shift, float scale, int window_tiles, void* work, void* stream) {
+  if (paged_refused(B, N, M, H, D, shift, pages, ldt, k, v, starts, pos, table) || B > RB || !q || !y || (((uintptr_t)q | (uintptr_t)y | (uintptr_t)work) & 31) ||
+      window_tiles < 0 || !work)
+    return -2;
   if (N == 0) return 0;
   const float log2e = 1.4426950408889634f;
-  RowsArgs a{(const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, p, (__nv_bfloat16*)y, doc_start, window_tiles, scale * log2e,
-             (scale < 0 ? -scale : scale) * D * log2e, parts, 0};
   int dev = 0, sms = 0;
   BONES_CHECK(cudaGetDevice(&dev));
   BONES_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  const long long heads = (long long)B * H, seen = window_tiles > 0 ? min((long long)p.cap, (window_tiles + 1) * 128ll) : p.cap;
-  const long long turns = (seen + RT - 1) / RT;
-  // few heads and long caches: parts of their own, ten rounds of CTAs so that unequal lengths even out
-  long long S = min(30ll * sms / heads, turns / 64);
-  if (parts && S > 8 && (long long)N * H * S * (D + 4) <= part_floats && N <= 65535) {
-    a.turns = (int)((turns + S - 1) / S);
-    return D == 128 ? launch_rows<128>(a, (int)S, true, (cudaStream_t)stream) : launch_rows<64>(a, (int)S, true, (cudaStream_t)stream);
-  }
-  int C = 1;
-  while (C < 8 && heads * C < 6ll * sms && turns >= 2 * RW * C) C *= 2;
-  return D == 128 ? launch_rows<128>(a, C, false, (cudaStream_t)stream) : launch_rows<64>(a, C, false, (cudaStream_t)stream);
+  const int ctas = bones_paged_rows_ctas(D, sms);
+  float* parts = (float*)work;
+  long long* before = (long long*)(parts + (long long)ctas * RW * 2 * RT * (D + 4));
+  RowsArgs a{(const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v,
+             Paged{starts, pos, table, ldt, B, N, M, H, shift, pages, (int)min((long long)M << shift, 0x7fffff00ll), v}, (__nv_bfloat16*)y, doc_start, window_tiles,
+             scale * log2e, (scale < 0 ? -scale : scale) * D * log2e, before, (int*)(before + B + 1), parts, 0};
+  return D == 128 ? launch_rows<128>(a, ctas, (cudaStream_t)stream) : launch_rows<64>(a, ctas, (cudaStream_t)stream);
 }
 }  // extern "C"

@@ -159,41 +159,129 @@ __global__ void verify_stats_kernel(const VerifyArgs p) {
 // ---------------------------------------------------------------------------------------------------------------
 // a sequence: which drafts stand, and the token.  grid: (VC CTAs of a cluster, B)
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int VC = 8, VT = 256, VW = VC * VT / 32;       // CTAs, threads of one, warps of a cluster
-static_assert(VW == 64, "a lane has two warps' sums");
+constexpr int VC = 8, VT = 128, VW = VC * VT / 32;       // CTAs, threads of one, warps of a cluster
+constexpr int VS = 8;                                    // steps of a warp at most
+static_assert(VW == 32, "a lane has a warp's sums");
 
-template <typename E>
-struct Law {                  // exp((z - most) / T), 64 bits
-  const E* z;
-  double most, inv;
-  __device__ __forceinline__ double operator()(double x) const { return exp((x - most) * inv); }
-};
-
-// eight columns from `at` on, -inf behind the last
-template <typename E>
-__device__ __forceinline__ void load8(const E* z, int at, int V, float* f) {
-  if (at + 8 <= V && ((uintptr_t)(z + at) & 15) == 0) {
-    load_vec(z + at, f);
-    if constexpr (sizeof(E) == 4) load_vec(z + at + 4, f + 4);
-  } else {
+// A row's law, exp((z - most) / T), in 64 bits, by a table of powers of two (the method of Tang, "Table-driven implementation of the exponential
+// function in IEEE floating-point arithmetic", 1989): x = (64 m + j) ln 2 / 64 + r with |r| <= ln 2 / 128, exp(x) = 2^m 2^(j/64) (1 + r + .. + r^5 / 120),
+// whose remainder r^6 / 720 is 2^-54.6.  One constant for ln 2 / 64: its rounding is 2^-53 of x, and x is -40 at most where the result counts beside the
+// row's largest, 1.  Twenty instructions, half of them in 64 bits:
+//  - what is a multiple of all values does not matter, so z / T - most / T is one operation whose second part is rounded;
+//  - a conversion to 64 bits runs at 16 a clock and SM, so it is made of the value's bits: the exponent's other bias, the fraction moved;
+//  - the table has a column for each lane of a half-warp (with a common one their reads met in the same banks, 6 clocks a warp), and its high words are
+//    short of j 2^14, so that adding n 2^14 for n = 64 m + j makes 2^m of them;
+//  - x stays above -690: what lies below counts as kNothing at most instead of 0.
+constexpr int EXP_COLS = 16;
+constexpr double kNothing = 1e-280;
+struct Law {
+  double inv, shift;
+  float least;
+  const double* powers;                                      // at this lane's column
+  __device__ __forceinline__ Law(float most, double T, const double* powers_) : inv(1.0 / T), shift(-(double)most * (1.0 / T)), powers(powers_) {
+    least = (float)fmax((double)most - 690.0 * T, -3e38);
+  }
+  // W values side by side: an operation in 64 bits takes 25 clocks, so one value's chain of twelve leaves the pipe idle
+  template <int W>
+  __device__ __forceinline__ void of(const float* z, double* e) const {
+    const double magic = 6755399441055744.0;                 // 1.5 * 2^52: a sum's low word is the whole number
+    double r[W], q[W];
+    int n[W];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = at + i < V ? logit(z + at + i) : -__int_as_float(0x7f800000);
+    for (int i = 0; i < W; ++i) {
+      const uint32_t u = __float_as_uint(fmaxf(z[i], least));
+      const double x = fma(__hiloint2double((int)(((uint32_t)((int)u >> 3) & 0x8fffffffu) + (896u << 20)), (int)(u << 29)), inv, shift);
+      const double t = fma(x, 0x1.71547652b82fep+6, magic);
+      n[i] = __double2loint(t);
+      r[i] = fma(t - magic, -0x1.62e42fefa39efp-7, x);
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) q[i] = fma(r[i], 1.0 / 120, 1.0 / 24);
+#pragma unroll
+    for (int i = 0; i < W; ++i) q[i] = fma(r[i], q[i], 1.0 / 6);
+#pragma unroll
+    for (int i = 0; i < W; ++i) q[i] = fma(r[i], q[i], 0.5);
+#pragma unroll
+    for (int i = 0; i < W; ++i) q[i] = fma(r[i], q[i], 1.0);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const double j = powers[(n[i] & 63) * EXP_COLS], w = __hiloint2double(__double2hiint(j) + n[i] * 16384, __double2loint(j));
+      e[i] = fma(w, r[i] * q[i], w);
+    }
+  }
+  __device__ __forceinline__ double operator()(float z) const {
+    double e;
+    of<1>(&z, &e);
+    return e;
+  }
+};
+__device__ __forceinline__ void fill_powers(double* table) {
+  if (threadIdx.x < 64) {
+    const double x = exp2(threadIdx.x * (1.0 / 64));
+    for (int i = 0; i < EXP_COLS; ++i) table[threadIdx.x * EXP_COLS + i] = __hiloint2double(__double2hiint(x) - (int)threadIdx.x * 16384, __double2loint(x));
   }
 }
 
-// A double of each warp to all: lane l gets those of warps 2 l and 2 l + 1 of the cluster.
-struct Both {
-  double a, b;
+// Eight consecutive columns as they lie in memory
+template <typename E>
+struct Eight {
+  uint4 v[sizeof(E) / 2];
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (sizeof(E) == 2) {
+      const uint32_t pair = (&v[0].x)[i >> 1];
+      return __uint_as_float(i & 1 ? pair & 0xffff0000u : pair << 16);
+    } else {
+      return __uint_as_float((&v[i >> 2].x)[i & 3]);
+    }
+  }
 };
-__device__ __forceinline__ Both share(double mine, double* box) {
+// Columns at .. at + 7; -inf behind the last
+template <typename E>
+__device__ __forceinline__ Eight<E> load8(const E* z, int at, int V) {
+  Eight<E> f;
+  if (((uintptr_t)(z + at) & 15) == 0 && at + 8 <= V) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(E) / 2; ++i) f.v[i] = reinterpret_cast<const uint4*>(z + at)[i];
+  } else {
+    uint32_t w[2 * sizeof(E)];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool in = at + i < V;
+      if constexpr (sizeof(E) == 2) {
+        const uint32_t x = in ? reinterpret_cast<const unsigned short*>(z)[at + i] : 0xff80u;
+        if (i & 1) w[i >> 1] |= x << 16;
+        else w[i >> 1] = x;
+      } else {
+        w[i] = in ? reinterpret_cast<const uint32_t*>(z)[at + i] : 0xff800000u;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(E) / 2; ++i) f.v[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  }
+  return f;
+}
+
+// A warp's columns: consecutive steps, of which each lane has 8 * wide consecutive columns
+struct Cut {
+  int from, to, wide;
+  __device__ __forceinline__ int column(int step, int lane) const { return (step * 32 + lane) * wide * 8; }
+};
+
+// Four doubles of each warp to all: lane l gets those of warp l of the cluster.
+struct Sums {
+  double p, q;         // of the law's own terms
+  double p_up, q_up;   // of those columns' where p is above q
+};
+__device__ __forceinline__ Sums share(const Sums& s, Sums* box) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (lane == 0) box[warp] = mine;
+  if (lane == 0) box[warp] = s;
   __syncthreads();
   cluster_barrier();
-  const uint32_t at = map_to_rank(smem_u32(box + (2 * lane) % (VT / 32)), (2 * lane) / (VT / 32));
-  Both r;
-  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(r.a) : "r"(at));
-  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(r.b) : "r"(at + 8));
+  const uint32_t at = map_to_rank(smem_u32(box + lane % (VT / 32)), lane / (VT / 32));
+  Sums r;
+  double* v = &r.p;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v[i]) : "r"(at + 8 * i));
   __syncwarp();
   cluster_barrier();
   return r;
@@ -204,10 +292,78 @@ __device__ __forceinline__ double warp_sum64(double v) {
   return v;
 }
 
+// A warp's sums over its columns; p_up and q_up those of the columns where p's law is above `ratio` times q's (without q: p's but for column `without`), in
+// `parts` also lane by lane for each step.  Not unrolled over columns: with four tiles' exponentials written out the kernel waited for its
+// instructions more than for anything else.
+template <typename E, bool BOTH>
+__device__ __noinline__ Sums row_sums(const E* z, const E* q, const Law lp, const Law lq, double ratio, int without, const Cut cut, int V, double2* parts) {
+  const int lane = threadIdx.x & 31, n = (cut.to - cut.from) * cut.wide;
+  Sums s = {};
+  if (n > 0) {
+    int at = cut.column(cut.from, lane), k = 0;
+    double up = 0.0, q_up = 0.0;
+    Eight<E> f = load8(z, at, V), g;
+    if (BOTH) g = load8(q, at, V);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      float u[8];
+      double x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] = f[j];
+      const int here = at, next = k + 1 == cut.wide ? at + 8 + 31 * 8 * cut.wide : at + 8;
+      if (i + 1 < n) f = load8(z, next, V);
+      lp.of<8>(u, x);
+      s.p += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+      if (BOTH) {
+        double y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = g[j];
+        if (i + 1 < n) g = load8(q, next, V);
+        lq.of<8>(u, y);
+        s.q += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool above = x[j] > ratio * y[j];
+          x[j] = above ? x[j] : 0.0;
+          y[j] = above ? y[j] : 0.0;
+        }
+        q_up += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (here + j == without) x[j] = 0.0;
+      }
+      up += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+      at = next;
+      if (++k == cut.wide) {
+        k = 0;
+        parts[i / cut.wide * 32 + lane] = make_double2(up, q_up);
+        s.p_up += up;
+        s.q_up += q_up;
+        up = q_up = 0.0;
+      }
+    }
+  }
+  s.p = warp_sum64(s.p);
+  s.q = warp_sum64(s.q);
+  s.p_up = warp_sum64(s.p_up);
+  s.q_up = warp_sum64(s.q_up);
+  return s;
+}
+
+// Whether p_up - ratio q_up is weight, and not what rounding leaves of columns where p and q are the same
+__device__ __forceinline__ bool weighs(double w, double p_up) { return w > fmax(kNothing, 1e-12 * p_up); }
+
 template <typename E>
-__global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT) verify_draw_kernel(const VerifyArgs p) {
-  __shared__ double box[VT / 32];
+__global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT, 4) verify_draw_kernel(const VerifyArgs p) {
+  __shared__ Sums box[VT / 32];
+  __shared__ double table[64 * EXP_COLS];
+  __shared__ double2 parts_all[VT / 32][VS * 32];
+  double2* parts = parts_all[threadIdx.x >> 5];
+  const double* powers = table + threadIdx.x % EXP_COLS;
+  fill_powers(table);
   pdl_wait();
+  __syncthreads();
   const int seq = blockIdx.y, lane = threadIdx.x & 31, gw = (int)cluster_rank() * (VT / 32) + (threadIdx.x >> 5);
   const int a = min(max(p.starts[seq], 0), p.N), e = min(max(p.starts[seq + 1], a), p.N);
   const bool writer = cluster_rank() == 0 && threadIdx.x == 0;
@@ -218,21 +374,9 @@ __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT) verify_draw_ker
     }
     return;
   }
-  const double inv = 1.0 / p.T;
-  // this warp's columns: whole tiles of 256, consecutive warps consecutive columns
-  const int tiles = (p.V + 255) / 256, mine = (tiles + VW - 1) / VW, t0 = min(gw * mine, tiles), t1 = min(t0 + mine, tiles);
-  auto total = [&](const E* z, double most) {
-    const Law<E> law{z, most, inv};
-    double s = 0.0;
-    for (int t = t0; t < t1; ++t) {
-      float f[8];
-      load8(z, t * 256 + lane * 8, p.V, f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s += law(f[i]);
-    }
-    const Both r = share(warp_sum64(s), box);
-    return warp_sum64(r.a + r.b);
-  };
+  // consecutive warps have consecutive columns; VS steps at most (one of 256 columns or more each)
+  const int wide = (p.V + VW * VS * 256 - 1) / (VW * VS * 256), steps = (p.V + 256 * wide - 1) / (256 * wide), mine = (steps + VW - 1) / VW;
+  const Cut cut{min(gw * mine, steps), min(gw * mine + mine, steps), wide};
   auto target = [&](int r) { return (const E*)p.z + r * p.ldz; };
   auto draft = [&](int r) { return (const E*)p.q + r * p.ldq; };
 
@@ -249,8 +393,8 @@ __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT) verify_draw_ker
         const long long x = p.ids[r + 1];
         const RowStat sq = p.q ? p.stats[r * 2ll + 1] : RowStat{1.0, 0.f, 0};
         if (x >= 0 && x < p.V && sq.sum > 0.0) {
-          const double px = exp(((double)logit(target(r) + x) - st.most) * inv) / st.sum;
-          const double qx = p.q ? exp(((double)logit(draft(r) + x) - sq.most) * inv) / sq.sum : 1.0, need = p.u[2ll * r] * qx;
+          const double px = Law(st.most, p.T, powers)(logit(target(r) + x)) / st.sum;
+          const double qx = p.q ? Law(sq.most, p.T, powers)(logit(draft(r) + x)) / sq.sum : 1.0, need = p.u[2ll * r] * qx;
           is = fabs(need - px) <= 1e-4 * (need + px) ? CLOSE : need < px ? STANDS : FALLS;
         }
       }
@@ -263,9 +407,12 @@ __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT) verify_draw_ker
         const int rr = r0 + l;
         const float mp = p.stats[rr * 2ll].most, mq = p.q ? p.stats[rr * 2ll + 1].most : 0.f;
         const long long x = p.ids[rr + 1];
-        const double sp = total(target(rr), mp), sq = p.q ? total(draft(rr), mq) : 1.0;
-        const double px = exp(((double)logit(target(rr) + x) - mp) * inv) / sp;
-        const double qx = p.q ? exp(((double)logit(draft(rr) + x) - mq) * inv) / sq : 1.0;
+        const Law lp(mp, p.T, powers), lq(mq, p.T, powers);
+        const Sums both = share(p.q ? row_sums<E, true>(target(rr), draft(rr), lp, lq, 0.0, -1, cut, p.V, parts)
+                                    : row_sums<E, false>(target(rr), nullptr, lp, lq, 0.0, -1, cut, p.V, parts), box);
+        const double sum_p = warp_sum64(both.p), sum_q = warp_sum64(both.q);
+        const double px = lp(logit(target(rr) + x)) / sum_p;
+        const double qx = p.q ? lq(logit(draft(rr) + x)) / sum_q : 1.0;
         if (p.u[2ll * rr] * qx < px) {
           open &= open - 1;
           continue;
@@ -288,85 +435,78 @@ __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT) verify_draw_ker
   const RowStat st = p.stats[row * 2ll], sq = refused && p.q ? p.stats[row * 2ll + 1] : RowStat{0.0, 0.f, 0};
   const E *z = target(row), *zq = sq.sum > 0.0 ? draft(row) : nullptr;
   const long long without = refused && !p.q ? p.ids[row + 1] : -1;
-  const Law<E> lp{z, st.most, inv}, lq{zq, sq.most, inv};
-  double sp = 1.0, sd = 1.0;
-  if (zq) {                                    // p's and q's scales matter only beside one another
-    sp = 1.0 / total(z, st.most);
-    sd = 1.0 / total(zq, sq.most);
-  }
-  bool plain = false;                          // of p alone
-  auto weights = [&](int t, double* w) {
-    const int at = t * 256 + lane * 8;
-    float f[8], g[8];
-    load8(z, at, p.V, f);
-    if (zq && !plain) load8(zq, at, p.V, g);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      double x = lp(f[i]) * sp;
-      if (zq && !plain) x = fmax(x - lq(g[i]) * sd, 0.0);
-      if (at + i == without && !plain) x = 0.0;
-      w[i] = x;
-    }
-  };
+  const Law lp(st.most, p.T, powers), lq(sq.most, p.T, powers);
+  // One pass for both laws' sums and those of the columns where p is above q, with the first kernel's 32-bit sums for the ratio of the scales: where that
+  // errs about a column, p and q are the same to seven digits there.  The weights' sums follow with the ratio in 64 bits.
+  const E* other = zq;
+  double ratio = zq ? st.sum / sq.sum : 0.0;
+  int skip = without >= 0 && without < p.V ? (int)without : -1;
   for (int round = 0; round < 2; ++round) {
-    double s = 0.0;
-    for (int t = t0; t < t1; ++t) {
-      double w[8];
-      weights(t, w);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s += w[i];
-    }
-    const Both r = share(warp_sum64(s), box);
-    // sums up to and with each warp's
-    double up = r.a + r.b;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double x = __shfl_up_sync(0xffffffffu, up, o);
-      if (lane >= o) up += x;
-    }
-    const double all = __shfl_sync(0xffffffffu, up, 31);
-    double prev = __shfl_up_sync(0xffffffffu, up, 1);
-    if (lane == 0) prev = 0.0;
-    if (!(all > 0.0) && !plain) {              // p and q the same but for rounding: of p
-      plain = true;
+    const Sums r = share(other ? row_sums<E, true>(z, other, lp, lq, ratio, -1, cut, p.V, parts)
+                               : row_sums<E, false>(z, nullptr, lp, lq, 0.0, skip, cut, p.V, parts), box);
+    if (other) ratio = warp_sum64(r.p) / warp_sum64(r.q);
+    const double w = r.p_up - ratio * r.q_up;                 // of warp `lane`
+    const uint32_t some = __ballot_sync(0xffffffffu, weighs(w, r.p_up));
+    if (!some && round == 0) {                                // p and q the same: of p alone
+      other = nullptr;
+      ratio = 0.0;
+      skip = -1;
       continue;
     }
-    const double need = (double)p.u[2ll * row + 1] * all;
-    // the first warp with weight whose sum reaches above; by rounding there may be none: the last with weight
-    const double first = prev + r.a;
-    int w = r.a > 0.0 && first > need ? 2 * lane : r.b > 0.0 && up > need ? 2 * lane + 1 : VW;
-    w = __reduce_min_sync(0xffffffffu, w);
-    if (w == VW) w = __reduce_max_sync(0xffffffffu, r.b > 0.0 ? 2 * lane + 1 : r.a > 0.0 ? 2 * lane : 0);
-    if (w == gw) {
-      double before = __shfl_sync(0xffffffffu, (w & 1) ? first : prev, w >> 1);
-      int found = -1, last = -1;
-      for (int t = t0; t < t1 && found < 0; ++t) {
-        double x[8], sum = 0.0;
-        weights(t, x);
+    auto up_to = [&](double x) {                              // sums up to and with each lane's
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += x[i];
-        double to = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double y = __shfl_up_sync(0xffffffffu, to, o);
-          if (lane >= o) to += y;
-        }
-        double at = before + to - sum;
-        int hit = 0x7fffffff, tail = -1;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          at += x[i];
-          if (x[i] > 0.0) {
-            tail = t * 256 + lane * 8 + i;
-            if (at > need && hit == 0x7fffffff) hit = tail;
-          }
-        }
-        hit = __reduce_min_sync(0xffffffffu, hit);
-        last = max(last, __reduce_max_sync(0xffffffffu, tail));
-        if (hit != 0x7fffffff) found = hit;
-        before += __shfl_sync(0xffffffffu, to, 31);
+      for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
       }
-      if (lane == 0) p.token[seq] = found >= 0 ? found : last;
+      return x;
+    };
+    // the first with weight whose sum reaches above; by rounding there may be none: the last with weight
+    auto pick = [&](bool heavy, double upto, double need) {
+      const uint32_t has = __ballot_sync(0xffffffffu, heavy), above = __ballot_sync(0xffffffffu, heavy && upto > need);
+      return above ? __ffs(above) - 1 : has ? 31 - __clz(has) : -1;
+    };
+    const double up = up_to(w), need = (double)p.u[2ll * row + 1] * __shfl_sync(0xffffffffu, up, 31);
+    const int owner = pick(weighs(w, r.p_up), up, need);
+    double before = __shfl_sync(0xffffffffu, up - w, max(owner, 0));
+    if (owner == gw) {
+      // its step (a lane a step), the lane in it, the column
+      double mine_w = 0.0, mine_p = 0.0, lane_w = 0.0, lane_p = 0.0;
+#pragma unroll
+      for (int j = 0; j < VS; ++j) {
+        if (cut.from + j >= cut.to) break;
+        const double2 part = parts[j * 32 + lane];
+        const double a_w = warp_sum64(part.x - ratio * part.y), a_p = warp_sum64(part.x);
+        if (lane == j) {
+          mine_w = a_w;
+          mine_p = a_p;
+        }
+      }
+      const double step_up = before + up_to(mine_w);
+      const int step = max(pick(weighs(mine_w, mine_p), step_up, need), 0);
+      before = __shfl_sync(0xffffffffu, step_up - mine_w, step);
+      lane_p = parts[step * 32 + lane].x;
+      lane_w = lane_p - ratio * parts[step * 32 + lane].y;
+      const double lane_up = before + up_to(lane_w);
+      const int from = max(pick(weighs(lane_w, lane_p), lane_up, need), 0);
+      before = __shfl_sync(0xffffffffu, lane_up - lane_w, from);
+      const int at = cut.column(cut.from + step, from);
+      int found = -1, last = at;
+      for (int k = 0; k < wide && found < 0; ++k) {
+        const int col = at + k * 8 + lane;
+        double x = 0.0, y = 0.0;
+        if (lane < 8 && col < p.V) {
+          x = lp(logit(z + col));
+          if (other) y = lq(logit(other + col));
+        }
+        const double weight = col == skip ? 0.0 : fmax(x - ratio * y, 0.0), upto = before + up_to(weight);
+        const bool heavy = weighs(weight, x);
+        const uint32_t has = __ballot_sync(0xffffffffu, heavy), above = __ballot_sync(0xffffffffu, heavy && upto > need);
+        if (has) last = at + k * 8 + 31 - __clz(has);
+        if (above) found = at + k * 8 + __ffs(above) - 1;
+        before = __shfl_sync(0xffffffffu, upto, 31);
+      }
+      if (lane == 0) p.token[seq] = min(found >= 0 ? found : last, p.V - 1);
     }
     break;
   }
@@ -407,7 +547,7 @@ template <typename E>
 static int launch_verify(const VerifyArgs& p, cudaStream_t s) {
   const dim3 grid((unsigned)p.N, p.q ? 2 : 1);
   // few rows: many threads for each, so that all of a row is on its way at once
-  const unsigned threads = (long long)p.N * grid.y <= 296 ? 1024 : 256;
+  const unsigned threads = (long long)p.N * grid.y <= 296 ? 1024 : (long long)p.N * grid.y <= 592 ? 512 : 256;
   if (p.N) {
     if (p.T == 0.0) verify_stats_kernel<E, true><<<grid, threads, 0, s>>>(p);
     else verify_stats_kernel<E, false><<<grid, threads, 0, s>>>(p);

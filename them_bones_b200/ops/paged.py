@@ -21,7 +21,7 @@ PAGES = (16, 32, 64, 128)              # tokens of a page
 SHIFT = 32.0                           # largest |scale| * head_dim: the kernels' soft-max has this fixed shift, and its smallest weights, exp(-2 * 32), stay normal in fp32
 MOST_ROWS = (1 << 31) - 256             # rows of [D] in a cache
 FEW = 16                               # pieces of up to this many tokens go by tiles of 16 rows, longer ones by tiles of 128
-PART_FLOATS = 8 << 20                  # room for the parts of a result (32 MiB at most)
+MOST_FEW = 512                         # as do those of more sequences than this
 
 
 class PagedKV(NamedTuple):
@@ -138,28 +138,26 @@ def attention(dims, q, c, table, starts, pos, scale, doc_start, window, longest)
         with L.device(dev):
             common = (q.data_ptr(), c[0].data_ptr(), c[1].data_ptr(), c[0].shape[0], table.data_ptr(), max(table.stride(0), m), starts.data_ptr(), pos.data_ptr(),
                       0 if doc_start is None else doc_start.data_ptr(), y.data_ptr(), b, n, m, h, d, page.bit_length() - 1, scale, window // 128)
-            if longest > FEW:
+            if longest > FEW or b > MOST_FEW:
                 slots = part_slots(n, m * page, h, window, dev)
                 ints = torch.empty(3 * b + 16, dtype=torch.int32, device=q.device)
                 parts = torch.empty(slots * 128 * (d + 1), dtype=torch.float32, device=q.device) if slots else None
                 L.call("bones_paged_pieces", *common, ints.data_ptr(), 0 if parts is None else parts.data_ptr(), slots, L.raw_stream(), launches=3 if slots else 2)
             else:
-                room = parts_room(b, n, m * page, h, d, window)
-                parts = torch.empty(room, dtype=torch.float32, device=q.device) if room else None
-                L.call("bones_paged_rows", *common, 0 if parts is None else parts.data_ptr(), room, L.raw_stream(), launches=2 if room else 1)
+                work = torch.empty(rows_work(b, d, dev), dtype=torch.uint8, device=q.device)
+                L.call("bones_paged_rows", *common, work.data_ptr(), L.raw_stream(), launches=2)
         COUNTS["paged_attention"] += 1
     return y
-
-
-def parts_room(b, n, capacity, h, d, window):
-    """Floats for the parts of a step's result: what caches of more than 8192 tokens and few heads are given."""
-    seen = min(capacity, window + 128) if window else capacity
-    return min(PART_FLOATS, n * h * (d + 4) * (seen // 1024)) if seen > 8192 and b * h < 512 else 0
 
 
 @functools.lru_cache(maxsize=None)
 def _sms(dev: int) -> int:
     return torch.cuda.get_device_properties(dev).multi_processor_count
+
+
+def rows_work(b, d, dev):
+    """Bytes that ``bones_paged_rows`` works with."""
+    return L.load().bones_paged_rows_ctas(d, _sms(dev)) * 8 * 16 * (d + 4) * 4 + 12 * b + 16
 
 
 def part_slots(n, capacity, h, window, dev):

@@ -9,7 +9,7 @@ from . import _lib as L
 from . import COUNTS
 from .logprobs import has_tangent
 
-COLDEST = 1e-6                # smallest temperature but 0
+COLDEST, WARMEST = 1e-6, 1e6  # temperatures but 0
 
 
 class Verified(NamedTuple):
@@ -27,8 +27,8 @@ def check(logits, ids, starts, uniforms, draft, temperature, vocab):
         raise ValueError(f"verify_drafts: starts {starts.dtype} {tuple(starts.shape)} on {starts.device}, expected contiguous int32 [B + 1] on {dev}, B from 1 to 65535")
     if not 1 <= vocab <= logits.shape[1] or vocab > 1 << 30:
         raise ValueError(f"verify_drafts: a vocabulary of {vocab} in {logits.shape[1]} columns")
-    if temperature != 0 and not COLDEST <= temperature < float("inf"):
-        raise ValueError(f"verify_drafts: temperature {temperature} (0, or {COLDEST} and more)")
+    if temperature != 0 and not COLDEST <= temperature <= WARMEST:
+        raise ValueError(f"verify_drafts: temperature {temperature} (0, or {COLDEST} to {WARMEST})")
     if temperature != 0 and (uniforms is None or uniforms.shape != (n, 2) or uniforms.dtype is not torch.float32 or uniforms.device != dev or not uniforms.is_contiguous()):
         have = None if uniforms is None else f"{uniforms.dtype} {tuple(uniforms.shape)} on {uniforms.device}"
         raise ValueError(f"verify_drafts: uniforms {have}, expected contiguous fp32 [{n}, 2] on {dev}")
