@@ -145,12 +145,14 @@ def verify(logits, ids, starts, uniforms, draft, t, vocab):
                 if q is not None and 0 <= x < vocab:
                     if draft is None:
                         q[x] = 1.0
-                    close = min(close, abs(u[r][0] * q[x] - p[x]) / max(u[r][0] * q[x], p[x], 1e-300))
+                    most = max(u[r][0] * q[x], p[x])
+                    close = min(close, abs(u[r][0] * q[x] - p[x]) / most if most > 0 else 1.0)
                     if u[r][0] * q[x] < p[x]:
                         got += 1
                         continue
                 if q is not None:
                     w = [max(pp - qq, 0.0) for pp, qq in zip(p, q)]
+                    w = w if any(w) else p                      # q is p
             total, c = math.fsum(w), 0.0
             for i, x in enumerate(w):
                 c += x

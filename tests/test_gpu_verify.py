@@ -31,16 +31,16 @@ def test_it_is_the_definition(lens, vocab, cols, dtype, model, t):
 
 
 @pytest.mark.parametrize("dtype,cols,model,t", [(torch.bfloat16, 65536, True, 1.0), (torch.float32, 65536, True, 0.7), (torch.bfloat16, 65531, False, 1.0),
-                                                (torch.bfloat16, 65536, True, 0.0), (torch.float32, 50001, False, 1.3)])
+                                                (torch.bfloat16, 65536, True, 0.0), (torch.float32, 50001, False, 1.3), (torch.float32, 200003, True, 1.0)])
 def test_large_vocabularies_agree_with_the_statement(dtype, cols, model, t):
     """Some hundred draws: a border in 32 bits would miss one of them."""
     from them_bones_b200 import ops
     from them_bones_b200.ref import functional as RF
-    z, ids, starts, u, q = _cuda(*problem([1 + i % 6 for i in range(200)], cols, cols, dtype, model, seed=5, spread=1.5))
+    z, ids, starts, u, q = _cuda(*problem([1 + i % 6 for i in range(200 if cols < 100000 else 60)], cols, cols, dtype, model, seed=5, spread=1.5))
     got = ops.verify_drafts(z, ids, starts, u if t else None, q, t)
     want = RF.verify_drafts(z, ids, starts, u, q, t, cols)
     assert torch.equal(got.accepted, want[0]) and torch.equal(got.token, want[1])
-    assert 100 < int(got.accepted.sum()) < 500 or not t or not model          # without a model no draft is likely here
+    assert 25 < int(got.accepted.sum()) < 500 or not t or not model          # without a model no draft is likely here
     again = ops.verify_drafts(z, ids, starts, u if t else None, q, t)
     assert torch.equal(got.accepted, again.accepted) and torch.equal(got.token, again.token)
 
@@ -55,6 +55,17 @@ def test_drafts_next_to_their_border():
         edge = torch.tensor(min(p[x] / d[x], 0.999))
         u[r, 0] = torch.nextafter(edge, torch.tensor(float(i % 2)))
     _check(z, ids, starts, u, q, 1.0, 1000)
+
+
+def test_logits_far_from_zero_and_cold_temperatures():
+    """Whole numbers of steps that the law's scale is cut into: large logits, and differences that are large multiples of the temperature."""
+    for far, t in ((0.0, 1e-6), (1e4, 1.0), (-1e4, 0.01), (3e37, 1.0), (-3e38, 1e-6), (1e-3, 1e6), (2.0 ** 20, 0.5)):
+        for dtype in (torch.float32, torch.bfloat16):
+            z, ids, starts, u, q = problem([3, 2, 4], 700, 704, torch.float32, True, seed=3)
+            z, q = (z + far).to(dtype), (q + far).to(dtype)
+            ids[1], ids[4] = int(z[0, :700].float().argmax()), int(z[3, :700].float().argmax())
+            _check(z, ids, starts, u, q, t, 700)
+            _check(z, ids, starts, u, None, t, 700)
 
 
 def test_the_ends_of_the_numbers():

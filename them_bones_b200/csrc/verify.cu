@@ -105,14 +105,18 @@ __global__ void verify_stats_kernel(const VerifyArgs p) {
     const float f = logit(z + threadIdx.x);
     row_step<GREEDY, 1>(r, &f, threadIdx.x, c);
   }
-  constexpr int U = 4;                               // loads of a thread in flight
+  constexpr int U = 8;                               // loads of a thread in flight
   int i = threadIdx.x;
   for (; i + (U - 1) * (int)blockDim.x < vecs; i += U * blockDim.x) {
-    float f[U][W];
+    uint4 raw[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) load_vec(z + head + (long long)(i + j * blockDim.x) * W, f[j]);
+    for (int j = 0; j < U; ++j) raw[j] = *reinterpret_cast<const uint4*>(z + head + (long long)(i + j * blockDim.x) * W);
 #pragma unroll
-    for (int j = 0; j < U; ++j) row_step<GREEDY, W>(r, f[j], head + (i + j * blockDim.x) * W, c);
+    for (int j = 0; j < U; ++j) {
+      float f[W];
+      load_vec(reinterpret_cast<const E*>(&raw[j]), f);
+      row_step<GREEDY, W>(r, f, head + (i + j * blockDim.x) * W, c);
+    }
   }
   for (; i < vecs; i += blockDim.x) {
     float f[W];
@@ -164,49 +168,50 @@ constexpr int VS = 8;                                    // steps of a warp at m
 static_assert(VW == 32, "a lane has a warp's sums");
 
 // A row's law, exp((z - most) / T), in 64 bits, by a table of powers of two (the method of Tang, "Table-driven implementation of the exponential
-// function in IEEE floating-point arithmetic", 1989): x = (64 m + j) ln 2 / 64 + r with |r| <= ln 2 / 128, exp(x) = 2^m 2^(j/64) (1 + r + .. + r^5 / 120),
-// whose remainder r^6 / 720 is 2^-54.6.  One constant for ln 2 / 64: its rounding is 2^-53 of x, and x is -40 at most where the result counts beside the
-// row's largest, 1.  Twenty instructions, half of them in 64 bits:
-//  - what is a multiple of all values does not matter, so z / T - most / T is one operation whose second part is rounded;
+// function in IEEE floating-point arithmetic", 1989): with K = 256 / ln 2, z K / T - S = 256 m + j + f, |f| <= 1/2, the law is 2^m 2^(j/256)
+// (1 + a f + a^2 f^2 / 2 + a^3 f^3 / 6), a = ln 2 / 256, whose remainder is 1.4e-13 at most.  Seven operations in 64 bits, which run at half the rate of those in 32
+// and take 25 clocks each:
+//  - what is a multiple of all values does not matter (the row's largest comes out as 1 to 0.2 %), so S is most K / T to a whole number, and z K / T - S
+//    needs no more than the two sums with it;
 //  - a conversion to 64 bits runs at 16 a clock and SM, so it is made of the value's bits: the exponent's other bias, the fraction moved;
 //  - the table has a column for each lane of a half-warp (with a common one their reads met in the same banks, 6 clocks a warp), and its high words are
-//    short of j 2^14, so that adding n 2^14 for n = 64 m + j makes 2^m of them;
-//  - x stays above -690: what lies below counts as kNothing at most instead of 0.
-constexpr int EXP_COLS = 16;
+//    short of j 2^12, so that adding n 2^12 for n = 256 m + j makes 2^m of them;
+//  - a value far below the largest (-inf, masks) is first raised to where the whole number has 31 bits, and that to -256000: it counts as 2^-1000, below
+//    kNothing, instead of 0.
+constexpr int EXP_ROWS = 256, EXP_COLS = 16;
 constexpr double kNothing = 1e-280;
+constexpr double kMagic = 6755399441055744.0;                // 1.5 * 2^52: a sum's low word is the whole number
 struct Law {
-  double inv, shift;
+  double scale, offset;                                      // K / T, kMagic - S
   float least;
   const double* powers;                                      // at this lane's column
-  __device__ __forceinline__ Law(float most, double T, const double* powers_) : inv(1.0 / T), shift(-(double)most * (1.0 / T)), powers(powers_) {
-    least = (float)fmax((double)most - 690.0 * T, -3e38);
+  __device__ __forceinline__ Law(float most, double T, const double* powers_) : powers(powers_) {
+    // S stays below 2^49: there the next value of fp32 is 90000 T away from the largest, and any scale does
+    scale = fmin(0x1.71547652b82fep+8 / T, 0x1p49 / fmax(fabs((double)most), 1e-300));
+    offset = kMagic - rint((double)most * scale);
+    least = (float)((double)most - 0x1p30 / scale);          // -inf where that leaves fp32: from there -inf itself, as 2^128, is as near
   }
-  // W values side by side: an operation in 64 bits takes 25 clocks, so one value's chain of twelve leaves the pipe idle
+  // W values side by side: one value's chain would leave the pipe idle
   template <int W>
   __device__ __forceinline__ void of(const float* z, double* e) const {
-    const double magic = 6755399441055744.0;                 // 1.5 * 2^52: a sum's low word is the whole number
-    double r[W], q[W];
+    double f[W], q[W];
     int n[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) {
       const uint32_t u = __float_as_uint(fmaxf(z[i], least));
-      const double x = fma(__hiloint2double((int)(((uint32_t)((int)u >> 3) & 0x8fffffffu) + (896u << 20)), (int)(u << 29)), inv, shift);
-      const double t = fma(x, 0x1.71547652b82fep+6, magic);
-      n[i] = __double2loint(t);
-      r[i] = fma(t - magic, -0x1.62e42fefa39efp-7, x);
+      const double v = __hiloint2double((int)(((uint32_t)((int)u >> 3) & 0x8fffffffu) + (896u << 20)), (int)(u << 29));
+      const double t = fma(v, scale, offset);
+      n[i] = max(__double2loint(t), -1000 * EXP_ROWS);
+      f[i] = fma(v, scale, offset - t);                      // offset - t = -(S + 256 m + j)
     }
 #pragma unroll
-    for (int i = 0; i < W; ++i) q[i] = fma(r[i], 1.0 / 120, 1.0 / 24);
+    for (int i = 0; i < W; ++i) q[i] = fma(f[i], 0x1.c6b08d704a0bfp-29, 0x1.ebfbdff82c58ep-19);
 #pragma unroll
-    for (int i = 0; i < W; ++i) q[i] = fma(r[i], q[i], 1.0 / 6);
-#pragma unroll
-    for (int i = 0; i < W; ++i) q[i] = fma(r[i], q[i], 0.5);
-#pragma unroll
-    for (int i = 0; i < W; ++i) q[i] = fma(r[i], q[i], 1.0);
+    for (int i = 0; i < W; ++i) q[i] = fma(f[i], q[i], 0x1.62e42fefa39efp-9);
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      const double j = powers[(n[i] & 63) * EXP_COLS], w = __hiloint2double(__double2hiint(j) + n[i] * 16384, __double2loint(j));
-      e[i] = fma(w, r[i] * q[i], w);
+      const double j = powers[(n[i] & (EXP_ROWS - 1)) * EXP_COLS], w = __hiloint2double(__double2hiint(j) + n[i] * 4096, __double2loint(j));
+      e[i] = fma(w, f[i] * q[i], w);
     }
   }
   __device__ __forceinline__ double operator()(float z) const {
@@ -216,9 +221,9 @@ struct Law {
   }
 };
 __device__ __forceinline__ void fill_powers(double* table) {
-  if (threadIdx.x < 64) {
-    const double x = exp2(threadIdx.x * (1.0 / 64));
-    for (int i = 0; i < EXP_COLS; ++i) table[threadIdx.x * EXP_COLS + i] = __hiloint2double(__double2hiint(x) - (int)threadIdx.x * 16384, __double2loint(x));
+  for (int j = threadIdx.x; j < EXP_ROWS; j += blockDim.x) {
+    const double x = exp2(j * (1.0 / EXP_ROWS)), y = __hiloint2double(__double2hiint(x) - j * 4096, __double2loint(x));
+    for (int i = 0; i < EXP_COLS; ++i) table[j * EXP_COLS + (i + j) % EXP_COLS] = y;          // (all columns; threads in different banks)
   }
 }
 
@@ -323,9 +328,9 @@ __device__ __noinline__ Sums row_sums(const E* z, const E* q, const Law lp, cons
         s.q += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const bool above = x[j] > ratio * y[j];
-          x[j] = above ? x[j] : 0.0;
-          y[j] = above ? y[j] : 0.0;
+          const bool above = __double2hiint(fma(-ratio, y[j], x[j])) > 0;              // by the difference's sign
+          x[j] = __hiloint2double(above ? __double2hiint(x[j]) : 0, __double2loint(x[j]));        // (what is left without the high word is below 1e-310)
+          y[j] = __hiloint2double(above ? __double2hiint(y[j]) : 0, __double2loint(y[j]));
         }
         q_up += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
       } else {
@@ -357,16 +362,35 @@ __device__ __forceinline__ bool weighs(double w, double p_up) { return w > fmax(
 template <typename E>
 __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT, 4) verify_draw_kernel(const VerifyArgs p) {
   __shared__ Sums box[VT / 32];
-  __shared__ double table[64 * EXP_COLS];
-  __shared__ double2 parts_all[VT / 32][VS * 32];
-  double2* parts = parts_all[threadIdx.x >> 5];
+  extern __shared__ __align__(16) double table[];                // the powers, and behind them the warps' parts
+  double2* parts = reinterpret_cast<double2*>(table + EXP_ROWS * EXP_COLS) + (threadIdx.x >> 5) * VS * 32;
   const double* powers = table + threadIdx.x % EXP_COLS;
   fill_powers(table);
-  pdl_wait();
-  __syncthreads();
+  // What does not come from the first kernel is read before its end (it began behind all that came before): of the first 32 rows the draft behind each,
+  // its logits and its number.
   const int seq = blockIdx.y, lane = threadIdx.x & 31, gw = (int)cluster_rank() * (VT / 32) + (threadIdx.x >> 5);
   const int a = min(max(p.starts[seq], 0), p.N), e = min(max(p.starts[seq + 1], a), p.N);
   const bool writer = cluster_rank() == 0 && threadIdx.x == 0;
+  struct Draft {
+    bool is;
+    float p, q, u;
+  };
+  auto draft_behind = [&](int r) {
+    Draft d{false, 0.f, 0.f, 0.f};
+    if (r + 1 < e) {
+      const long long x = p.ids[r + 1];
+      d.is = x >= 0 && x < p.V;
+      if (d.is) {
+        d.p = logit((const E*)p.z + r * p.ldz + x);
+        if (p.q) d.q = logit((const E*)p.q + r * p.ldq + x);
+        d.u = p.u[2ll * r];
+      }
+    }
+    return d;
+  };
+  Draft next = draft_behind(a + lane);
+  pdl_wait();
+  __syncthreads();
   if (a == e) {
     if (writer) {
       p.accepted[seq] = 0;
@@ -389,12 +413,10 @@ __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT, 4) verify_draw_
     if (r < e) {
       const RowStat st = p.stats[r * 2ll];
       if (!(st.sum > 0.0)) is = GONE;
-      else if (r + 1 < e) {
-        const long long x = p.ids[r + 1];
+      else if (next.is) {
         const RowStat sq = p.q ? p.stats[r * 2ll + 1] : RowStat{1.0, 0.f, 0};
-        if (x >= 0 && x < p.V && sq.sum > 0.0) {
-          const double px = Law(st.most, p.T, powers)(logit(target(r) + x)) / st.sum;
-          const double qx = p.q ? Law(sq.most, p.T, powers)(logit(draft(r) + x)) / sq.sum : 1.0, need = p.u[2ll * r] * qx;
+        if (sq.sum > 0.0) {
+          const double px = exp(((double)next.p - st.most) / p.T) / st.sum, qx = p.q ? exp(((double)next.q - sq.most) / p.T) / sq.sum : 1.0, need = next.u * qx;
           is = fabs(need - px) <= 1e-4 * (need + px) ? CLOSE : need < px ? STANDS : FALLS;
         }
       }
@@ -411,8 +433,8 @@ __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT, 4) verify_draw_
         const Sums both = share(p.q ? row_sums<E, true>(target(rr), draft(rr), lp, lq, 0.0, -1, cut, p.V, parts)
                                     : row_sums<E, false>(target(rr), nullptr, lp, lq, 0.0, -1, cut, p.V, parts), box);
         const double sum_p = warp_sum64(both.p), sum_q = warp_sum64(both.q);
-        const double px = lp(logit(target(rr) + x)) / sum_p;
-        const double qx = p.q ? lq(logit(draft(rr) + x)) / sum_q : 1.0;
+        const double px = exp(((double)logit(target(rr) + x) - mp) / p.T) * lp(mp) / sum_p;
+        const double qx = p.q ? exp(((double)logit(draft(rr) + x) - mq) / p.T) * lq(mq) / sum_q : 1.0;
         if (p.u[2ll * rr] * qx < px) {
           open &= open - 1;
           continue;
@@ -423,6 +445,7 @@ __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT, 4) verify_draw_
       break;
     }
     if (open) break;
+    next = draft_behind(r0 + 32 + lane);
   }
   row = min(row, e - 1);
   if (writer) p.accepted[seq] = row - a;
@@ -439,7 +462,7 @@ __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT, 4) verify_draw_
   // One pass for both laws' sums and those of the columns where p is above q, with the first kernel's 32-bit sums for the ratio of the scales: where that
   // errs about a column, p and q are the same to seven digits there.  The weights' sums follow with the ratio in 64 bits.
   const E* other = zq;
-  double ratio = zq ? st.sum / sq.sum : 0.0;
+  double ratio = zq ? st.sum * lp(st.most) / (sq.sum * lq(sq.most)) : 0.0;
   int skip = without >= 0 && without < p.V ? (int)without : -1;
   for (int round = 0; round < 2; ++round) {
     const Sums r = share(other ? row_sums<E, true>(z, other, lp, lq, ratio, -1, cut, p.V, parts)
@@ -557,14 +580,18 @@ static int launch_verify(const VerifyArgs& p, cudaStream_t s) {
   cudaLaunchAttribute at[2];
   cfg.stream = s;
   cfg.attrs = at;
-  cfg.numAttrs = (unsigned)dec_launch_attrs(at, 1, 1);
+  cfg.numAttrs = (unsigned)dec_launch_attrs(at, 1, p.N > 0);        // (without a first kernel, what comes before is not the one that it may overlap)
   if (p.T == 0.0) {
     cfg.gridDim = dim3((unsigned)((p.B + 3) / 4));
     cfg.blockDim = dim3(128);
     return (int)cudaLaunchKernelEx(&cfg, verify_greedy_kernel, p);
   }
+  constexpr size_t smem = (EXP_ROWS * EXP_COLS + VT / 32 * VS * 32 * 2) * sizeof(double);
+  static OncePerDevice limit;
+  BONES_ONCE(limit, { BONES_CHECK(cudaFuncSetAttribute(verify_draw_kernel<E>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); });
   cfg.gridDim = dim3(VC, (unsigned)p.B);
   cfg.blockDim = dim3(VT);
+  cfg.dynamicSmemBytes = smem;
   return (int)cudaLaunchKernelEx(&cfg, verify_draw_kernel<E>, p);
 }
 
