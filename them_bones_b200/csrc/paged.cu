@@ -12,7 +12,6 @@ namespace bones {
 
 constexpr float kPagedEps = 1.1920928955078125e-07f;   // 2^-23
 
-__device__ __forceinline__ void paged_ld8(const __nv_bfloat16* p, float* f) { unpack8(*reinterpret_cast<const uint4*>(p), f); }
 __device__ __forceinline__ void paged_st8(__nv_bfloat16* p, const float* f) {
   *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
 }
@@ -54,58 +53,87 @@ __device__ __forceinline__ void paged_turn(const float* a, const float* b, const
   }
 }
 
-// A warp takes 512 / D heads of one row, so the row's sequence, page and angles are looked up once a warp.
+__device__ __forceinline__ void paged_unpack(const uint4* raw, float* a, float* b) {
+  unpack8(raw[0], a);
+  unpack8(raw[1], b);
+}
+
+// A CTA takes up to AR rows with all their heads, D / 16 lanes a head: a row's sequence, page and angles are looked up once a CTA, and no lane is left
+// over whatever the number of heads.  What a lane takes stays packed until it is worked on: 96 bytes on their way in 24 registers (unpacked, the kernel had room for
+// half the warps and ran at two thirds of the rate).
+constexpr int AT = 256, AR = 16;
 template <int D>
-__global__ void __launch_bounds__(256) paged_append_kernel(const __nv_bfloat16* __restrict__ qkv, long long ldq, const float* __restrict__ cosT,
-                                                           const float* __restrict__ sinT, int rope_rows, const Paged p, __nv_bfloat16* __restrict__ k,
-                                                           __nv_bfloat16* __restrict__ v, __nv_bfloat16* __restrict__ q) {
-  constexpr int LANES = D / 16, HEADS = 32 / LANES, HALF = D / 2;
-  const int parts = (p.H + HEADS - 1) / HEADS;
-  const long long w = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31, l8 = lane % LANES;
-  if (w >= (long long)p.N * parts) return;
-  const int row = (int)(w / parts), h = (int)(w % parts) * HEADS + lane / LANES;
-  const bool on = h < p.H;
-  const long long A = (long long)p.H * D, col = (long long)(on ? h : 0) * D + l8 * 8;
-  // the row itself is on its way while its place is looked up
-  const __nv_bfloat16* src = qkv + row * ldq + col;
-  float a[3][8], b[3][8];
+__global__ void __launch_bounds__(AT, 3) paged_append_kernel(const __nv_bfloat16* __restrict__ qkv, long long ldq, const float* __restrict__ cosT,
+                                                             const float* __restrict__ sinT, int rope_rows, int rows, const Paged p, __nv_bfloat16* __restrict__ k,
+                                                             __nv_bfloat16* __restrict__ v, __nv_bfloat16* __restrict__ q) {
+  constexpr int LANES = D / 16, HALF = D / 2;
+  __shared__ int pos_of[AR];                 // -1: no new token, or one that is left out
+  __shared__ long long place_of[AR];         // of head 0, in rows of D; -1 without a page
+  const int row0 = blockIdx.x * rows, items = min(rows, p.N - row0) * p.H;
+  const int l8 = threadIdx.x % LANES, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long A = (long long)p.H * D;
+  uint4 raw[3][2];
+  auto load = [&](int item) {
+    if (item >= items) return;
+    const int r = item / p.H;
+    const __nv_bfloat16* src = qkv + (row0 + r) * ldq + (long long)(item - r * p.H) * D + l8 * 8;
 #pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    paged_ld8(src + i * A, a[i]);
-    paged_ld8(src + i * A + HALF, b[i]);
-  }
-  const int seq = paged_owner(p.starts, p.B, row);
-  long long at = -1;
-  int t = -1;
-  if (seq >= 0 && seq < p.B) {
-    const Piece s = paged_piece(p, seq);
-    const int i = row - s.row;
-    if (i >= 0 && i < s.live && s.pos + i < rope_rows) {
-      t = s.pos + i;
-      at = paged_at(p, p.table[seq * p.ldt + (t >> p.shift)], on ? h : 0);
+    for (int i = 0; i < 3; ++i) {
+      raw[i][0] = *reinterpret_cast<const uint4*>(src + i * A);
+      raw[i][1] = *reinterpret_cast<const uint4*>(src + i * A + HALF);
+    }
+  };
+  int item = threadIdx.x / LANES;
+  load(item);                                // on its way while the rows are looked up
+  for (int r = warp; r < rows && row0 + r < p.N; r += AT / 32) {
+    const int b = paged_owner(p.starts, p.B, row0 + r);
+    int t = -1;
+    long long at = -1;
+    if (b >= 0 && b < p.B) {
+      const Piece s = paged_piece(p, b);
+      const int i = row0 + r - s.row;
+      if (i >= 0 && i < s.live && s.pos + i < rope_rows) {
+        t = s.pos + i;
+        at = paged_at(p, p.table[b * p.ldt + (t >> p.shift)], 0);
+        if (at >= 0) at += t & ((1 << p.shift) - 1);
+      }
+    }
+    if (lane == 0) {
+      pos_of[r] = t;
+      place_of[r] = at;
     }
   }
-  __nv_bfloat16* out = q + row * A + col;
-  if (t < 0) {                                       // not a new token, or left out
-    if (on) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<uint4*>(out + HALF) = make_uint4(0, 0, 0, 0);
-    return;
-  }
-  float cs[8], sn[8], y1[8], y2[8];
-  paged_ld8f(cosT + (long long)t * HALF + l8 * 8, cs);
-  paged_ld8f(sinT + (long long)t * HALF + l8 * 8, sn);
-  paged_turn<D>(a[0], b[0], cs, sn, y1, y2);
-  if (on) {
-    paged_st8(out, y1);
-    paged_st8(out + HALF, y2);
-  }
-  paged_turn<D>(a[1], b[1], cs, sn, y1, y2);
-  if (on && at >= 0) {
-    const long long o = (at + (t & ((1 << p.shift) - 1))) * D + l8 * 8;
-    paged_st8(k + o, y1);
-    paged_st8(k + o + HALF, y2);
-    paged_st8(v + o, a[2]);
-    paged_st8(v + o + HALF, b[2]);
+  __syncthreads();
+  // all lanes of a warp make the same rounds
+  for (int first = (int)(threadIdx.x & ~31u) / LANES; first < items; first += AT / LANES, item += AT / LANES) {
+    const bool on = item < items;
+    const int r = on ? item / p.H : 0, h = on ? item - r * p.H : 0, t = on ? pos_of[r] : -1;
+    const long long at = on ? place_of[r] : -1;
+    __nv_bfloat16* out = q + (row0 + r) * A + (long long)h * D + l8 * 8;
+    float cs[8], sn[8], y1[8], y2[8], a[8], b[8];
+    const long long angle = (long long)max(t, 0) * HALF + l8 * 8;
+    if (rope_rows > 0) {
+      paged_ld8f(cosT + angle, cs);
+      paged_ld8f(sinT + angle, sn);
+    }
+    paged_unpack(raw[0], a, b);
+    paged_turn<D>(a, b, cs, sn, y1, y2);
+    if (on && t >= 0) {
+      paged_st8(out, y1);
+      paged_st8(out + HALF, y2);
+    } else if (on) {
+      *reinterpret_cast<uint4*>(out) = *reinterpret_cast<uint4*>(out + HALF) = make_uint4(0, 0, 0, 0);
+    }
+    paged_unpack(raw[1], a, b);
+    paged_turn<D>(a, b, cs, sn, y1, y2);
+    if (on && at >= 0) {
+      const long long o = (at + ((long long)h << p.shift)) * D + l8 * 8;
+      paged_st8(k + o, y1);
+      paged_st8(k + o + HALF, y2);
+      *reinterpret_cast<uint4*>(v + o) = raw[2][0];
+      *reinterpret_cast<uint4*>(v + o + HALF) = raw[2][1];
+    }
+    load(item + AT / LANES);
   }
 }
 
@@ -451,36 +479,74 @@ __global__ void __launch_bounds__(32 * RW, D == 128 ? 3 : 4) paged_rows_kernel(c
   }
 }
 
-// Adds a row's sums where several warps have some, in their order; zeros for rows without a result.  grid: (N, H), D threads.
-template <int D>
-__global__ void __launch_bounds__(D) paged_rows_join_kernel(const RowsArgs p) {
+// Adds a row's sums where several warps have some, in their order; zeros for rows without a result.  256 threads take D / 4 threads' worth of rows and
+// heads, G groups of threads for each: eight where there are few (44 warps share a head of a long cache).
+template <int D, int G>
+__global__ void __launch_bounds__(256) paged_rows_join_kernel(const RowsArgs p) {
+  constexpr int T = D / 4, PAIRS = 256 / (T * G);
+  __shared__ float4 box[G > 1 ? G : 1][PAIRS][T];
+  __shared__ float box_l[G > 1 ? G : 1][PAIRS];
+  const int pair = threadIdx.x / (T * G), group = threadIdx.x / T % G, d = threadIdx.x % T;
+  const long long item = (long long)blockIdx.x * PAIRS + pair;
+  const bool on = item < (long long)p.p.N * p.p.H;
+  // (a warp's two rows are looked up one after the other where a row has less than a warp's threads)
+  const int row = on ? (int)(item / p.p.H) : -1, h = on ? (int)(item % p.p.H) : 0;
+  int b = -1;
+#pragma unroll
+  for (int i = 0; i < 32; i += min(T * G, 32)) {
+    const int x = paged_owner(p.p.starts, p.p.B, __shfl_sync(0xffffffffu, row, i));
+    if ((int)(threadIdx.x & 31) >= i) b = x;
+  }
+  Piece s = {};
+  if (on && b >= 0 && b < p.p.B) s = paged_piece(p.p, b);
+  const int i = row - s.row, tile = i / RT;
+  const bool live = on && s.live && i >= 0 && i < s.live;
   pdl_wait();
-  const int row = blockIdx.x, h = blockIdx.y, d = threadIdx.x;
-  __nv_bfloat16* y = p.y + ((long long)row * p.p.H + h) * D + d;
-  const int b = paged_owner(p.p.starts, p.p.B, row);
-  float x = 0.f, l = 0.f;
-  if (b >= 0 && b < p.p.B) {
-    const Piece s = paged_piece(p.p, b);
-    const int i = row - s.row;
-    if (i >= 0 && i < s.live) {
-      const int ahead = s.pos - p.first[b], tiles = (s.live + RT - 1) / RT, turns = tile_turns(ahead, s.live, i / RT);
-      if (turns > 0) {
-        const long long from = p.before[b] + (long long)h * turns_before(ahead, s.live, tiles) + turns_before(ahead, s.live, i / RT);
-        const int share = turn_share(p.before[p.p.B], p.warps), w0 = (int)((from + RC) / share), w1 = (int)((from + turns - 1) / share);
-        if (w0 == w1) return;                      // written
-        const float* at = p.parts + (((long long)w0 * 2 + 1) * RT + i % RT) * (D + 4);
-        x = at[d];
-        l = at[D];
-        at += RT * (D + 4);                        // the next warp's first
-#pragma unroll 8
-        for (int w = w0 + 1; w <= w1; ++w, at += 2 * RT * (D + 4)) {
-          x += at[d];
-          l += at[D];
+  bool written = !on;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  if (live) {
+    const long long in_front = p.before[b], total = p.before[p.p.B];
+    const int ahead = s.pos - p.first[b], turns = tile_turns(ahead, s.live, tile);
+    if (turns > 0) {
+      const long long from = in_front + (long long)h * turns_before(ahead, s.live, (s.live + RT - 1) / RT) + turns_before(ahead, s.live, tile);
+      const int share = turn_share(total, p.warps), w0 = (int)((from + RC) / share), w1 = (int)((from + turns - 1) / share);
+      written = w0 == w1;
+      if (!written) {
+        // the first warp's second place, the others' first
+        const float* at = p.parts + (long long)(i % RT) * (D + 4);
+        constexpr int STEP = RT * (D + 4);
+#pragma unroll 4
+        for (int w = w0 + group; w <= w1; w += G) {
+          const float* y = at + (long long)(2 * w + (w == w0)) * STEP;
+          const float4 z = *reinterpret_cast<const float4*>(y + 4 * d);
+          x.x += z.x;
+          x.y += z.y;
+          x.z += z.z;
+          x.w += z.w;
+          l += y[D];
         }
       }
     }
   }
-  *y = __float2bfloat16(l == 0.f ? 0.f : x / l);
+  if (G > 1) {
+    box[group][pair][d] = x;
+    if (d == 0) box_l[group][pair] = l;
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int k = 1; k < G; ++k) {
+      const float4 z = box[k][pair][d];
+      x.x += z.x;
+      x.y += z.y;
+      x.z += z.z;
+      x.w += z.w;
+      l += box_l[k][pair];
+    }
+  }
+  if (written) return;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  *reinterpret_cast<uint2*>(p.y + ((long long)row * p.p.H + h) * D + 4 * d) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
 }
 
 template <int D>
@@ -490,12 +556,15 @@ static int launch_rows(RowsArgs& p, int ctas, cudaStream_t s) {
   BONES_CHECK(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
-  cfg.gridDim = dim3((unsigned)p.p.N, (unsigned)p.p.H);
-  cfg.blockDim = dim3(D);
+  const long long pairs = (long long)p.p.N * p.p.H;
+  const bool few = pairs <= 8 * ctas;
+  const int a_cta = 256 / (D / 4 * (few ? 8 : 1));
+  cfg.gridDim = dim3((unsigned)((pairs + a_cta - 1) / a_cta));
+  cfg.blockDim = dim3(256);
   cfg.stream = s;
   cfg.attrs = at;
   cfg.numAttrs = (unsigned)dec_launch_attrs(at, 1, 1);
-  return (int)cudaLaunchKernelEx(&cfg, paged_rows_join_kernel<D>, p);
+  return (int)(few ? cudaLaunchKernelEx(&cfg, paged_rows_join_kernel<D, 8>, p) : cudaLaunchKernelEx(&cfg, paged_rows_join_kernel<D, 1>, p));
 }
 
 }  // namespace bones
@@ -510,14 +579,16 @@ int bones_paged_append(const void* qkv, long long ldq, const float* cosT, const 
   const Paged p{starts, pos, table, ldt, B, N, M, H, shift, pages, (int)min((long long)M << shift, 0x7fffff00ll), v};
   if (paged_refused(B, N, M, H, D, shift, pages, ldt, k, v, starts, pos, table) || !qkv || !q || !cosT || !sinT || rope_rows < 0 || misaligned16(qkv, q, cosT, sinT) || (N > 1 && ldq % 8)) return -2;
   if (N == 0) return 0;
-  const long long warps = (long long)N * ((H + 512 / D - 1) / (512 / D));
-  if (warps > 0x3fffffffll) return -2;
-  const unsigned grid = (unsigned)((warps + 7) / 8);
+  int dev = 0, sms = 0;
+  BONES_CHECK(cudaGetDevice(&dev));
+  BONES_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  const int rows = (int)max(1ll, min((long long)AR, N / (4ll * sms)));
+  const unsigned grid = (unsigned)((N + rows - 1) / rows);
   const auto* x = (const __nv_bfloat16*)qkv;
   auto *kc = (__nv_bfloat16*)k, *vc = (__nv_bfloat16*)v, *out = (__nv_bfloat16*)q;
   cudaStream_t s = (cudaStream_t)stream;
-  if (D == 128) paged_append_kernel<128><<<grid, 256, 0, s>>>(x, ldq, cosT, sinT, rope_rows, p, kc, vc, out);
-  else paged_append_kernel<64><<<grid, 256, 0, s>>>(x, ldq, cosT, sinT, rope_rows, p, kc, vc, out);
+  if (D == 128) paged_append_kernel<128><<<grid, AT, 0, s>>>(x, ldq, cosT, sinT, rope_rows, rows, p, kc, vc, out);
+  else paged_append_kernel<64><<<grid, AT, 0, s>>>(x, ldq, cosT, sinT, rope_rows, rows, p, kc, vc, out);
   return (int)cudaGetLastError();
 }
 

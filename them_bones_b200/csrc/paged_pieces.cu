@@ -30,7 +30,7 @@ struct PiecesArgs {
 // ---------------------------------------------------------------------------------------------------------------
 // plan
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int PLAN_T = 1024;
+constexpr int PLAN_T = 256;
 
 __device__ __forceinline__ int plan_tiles(const PiecesArgs& a, const Piece& s) {       // key tiles of the longest row of tiles
   const int last = (s.pos + s.live - 1) >> 7;
@@ -48,9 +48,11 @@ __device__ __forceinline__ int plan_scan(int v, int* box, int* all) {
   if (lane == 31) box[warp] = up;
   __syncthreads();
   int before = 0, total = 0;
+#pragma unroll
   for (int w = 0; w < PLAN_T / 32; ++w) {
-    if (w < warp) before += box[w];
-    total += box[w];
+    const int x = box[w];
+    if (w < warp) before += x;
+    total += x;
   }
   __syncthreads();
   *all = total;
@@ -59,7 +61,8 @@ __device__ __forceinline__ int plan_scan(int v, int* box, int* all) {
 
 __global__ void __launch_bounds__(PLAN_T) paged_plan_kernel(const PiecesArgs a) {
   __shared__ int box[PLAN_T / 32], rows_of[PLAN_T], tiles_of[PLAN_T], part;
-  __shared__ float cost[64];
+  __shared__ float cost[2];
+  __shared__ int cut[2];
   const Paged& p = a.p;
   pdl_launch();
   if (blockIdx.x > 0) {                          // rows without a result: outside all pieces, or left out
@@ -75,7 +78,7 @@ __global__ void __launch_bounds__(PLAN_T) paged_plan_kernel(const PiecesArgs a) 
     return;
   }
   if (threadIdx.x == 0) *a.next = 0;
-  // Parts only where the tiles of queries alone leave SMs without work, and only of up to 1024 sequences
+  // Parts only where the tiles of queries alone leave SMs without work, and only of up to PLAN_T sequences
   part = 0x7fffffff;
   if (a.slots > 0 && p.B <= PLAN_T) {
     int rows = 0, tiles = 0, items;
@@ -96,24 +99,35 @@ __global__ void __launch_bounds__(PLAN_T) paged_plan_kernel(const PiecesArgs a) 
       if (threadIdx.x < 64) {
         const int len = (most + threadIdx.x) / ((int)threadIdx.x + 1);
         float work = 0.f, n = 0.f, used = 0.f;
-        if (len > 0)
+        if (len > 0) {
+          const float inv = 1.0f / len;
           for (int b = 0; b < p.B; ++b) {
-            const int s = (tiles_of[b] + len - 1) / len;
-            work += (float)rows_of[b] * tiles_of[b];
-            n += (float)rows_of[b] * s;
-            if (s > 1) used += (float)rows_of[b] * s;
+            const float rows_b = (float)rows_of[b], s = ceilf(tiles_of[b] * inv);          // (as estimates go)
+            work += rows_b * tiles_of[b];
+            n += rows_b * s;
+            if (s > 1.f) used += rows_b * (s + 1.f);
           }
+        }
         const float waves = ceilf(n / a.sms);
-        cost[threadIdx.x] = used > a.slots || (threadIdx.x > 0 && len < 3) ? 1e30f : fmaxf(fminf(waves * (len + 1.f), (work + n) / a.sms + 0.5f * len), len + 1.f);
+        float c = used > a.slots || (threadIdx.x > 0 && len < 3) ? 1e30f : fmaxf(fminf(waves * (len + 1.f), (work + n) / a.sms + 0.5f * len), len + 1.f);
+        int best = threadIdx.x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          const float x = __shfl_xor_sync(0xffffffffu, c, o);
+          const int i = __shfl_xor_sync(0xffffffffu, best, o);
+          if (x < c || (x == c && i < best)) {
+            c = x;
+            best = i;
+          }
+        }
+        if ((threadIdx.x & 31) == 0) {
+          cost[threadIdx.x >> 5] = c;
+          cut[threadIdx.x >> 5] = best;
+        }
       }
       __syncthreads();
-      if (threadIdx.x == 0) {
-        int best = 0;
-        for (int s = 1; s < 64; ++s)
-          if (cost[s] < cost[best]) best = s;
-        part = best ? (most + best) / (best + 1) : 0x7fffffff;
-      }
-      __syncthreads();
+      const int best = cost[1] < cost[0] ? cut[1] : cut[0];
+      if (threadIdx.x == 0 && best) part = (most + best) / (best + 1);
     }
   }
   __syncthreads();
@@ -607,30 +621,45 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   }
 }
 
-// Adds the parts of a row and head in their order.  grid: (rows, heads), D threads.
+// Adds the parts of a row and head in their order.  D / 4 threads a row and head.
 template <int D>
-__global__ void __launch_bounds__(D) paged_pieces_join_kernel(const PiecesArgs a) {
-  pdl_wait();
+__global__ void __launch_bounds__(256) paged_pieces_join_kernel(const PiecesArgs a) {
+  constexpr int T = D / 4, PAIRS = 256 / T;
   const Paged& p = a.p;
-  const int row = blockIdx.x, h = blockIdx.y, d = threadIdx.x;
-  const int b = paged_owner(p.starts, p.B, row);
-  if (b < 0 || b >= p.B) return;
-  const int splits = a.splits[b];
-  if (splits == 1) return;
-  const Piece s = paged_piece(p, b);
+  const long long item = (long long)blockIdx.x * PAIRS + threadIdx.x / T;
+  const int d = threadIdx.x % T;
+  const bool on = item < (long long)p.N * p.H;
+  const int row = on ? (int)(item / p.H) : -1, h = on ? (int)(item % p.H) : 0;
+  int b = -1;
+#pragma unroll
+  for (int i = 0; i < 32; i += T) {
+    const int x = paged_owner(p.starts, p.B, __shfl_sync(0xffffffffu, row, i));
+    if ((int)(threadIdx.x & 31) >= i) b = x;
+  }
+  Piece s = {};
+  if (on && b >= 0 && b < p.B) s = paged_piece(p, b);
+  pdl_wait();
   const int i = row - s.row;
-  if (i < 0 || i >= s.live) return;
+  if (!on || !s.live || i < 0 || i >= s.live) return;
+  const int splits = a.splits[b], place0 = a.places[b];
+  if (splits == 1) return;
   const int rows = (s.live + PT - 1) / PT, qt = i / PT, g = h * rows + ((rows - 1 - qt - h) % rows + rows) % rows;
-  const long long place = a.places[b] + (long long)g * splits;
-  const float* parts = a.parts + (place * PT + i % PT) * D;
+  const long long place = place0 + (long long)g * splits;
+  const float* parts = a.parts + (place * PT + i % PT) * D + 4 * d;
   const float* sums = a.parts + (long long)a.slots * PT * D + place * PT + i % PT;
-  float x = 0.f, l = 0.f;
-#pragma unroll 8
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+#pragma unroll 4
   for (int k = 0; k < splits; ++k) {
-    x += parts[(long long)k * PT * D + d];
+    const float4 z = *reinterpret_cast<const float4*>(parts + (long long)k * PT * D);
+    x.x += z.x;
+    x.y += z.y;
+    x.z += z.z;
+    x.w += z.w;
     l += sums[(long long)k * PT];
   }
-  a.y[((long long)row * p.H + h) * D + d] = __float2bfloat16(l == 0.f ? 0.f : x / l);
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  *reinterpret_cast<uint2*>(a.y + ((long long)row * p.H + h) * D + 4 * d) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
 }
 
 static int tmap_rows_2d(CUtensorMap* out, const void* ptr, long long rows, long long cols, int box_rows) {
@@ -660,8 +689,9 @@ static int launch_pieces(const CUtensorMap& tq, const CUtensorMap& tk, const CUt
   cfg.numAttrs = (unsigned)dec_launch_attrs(at, 1, 1);
   BONES_CHECK(cudaLaunchKernelEx(&cfg, paged_pieces_kernel<D>, tq, tk, tv, a));
   if (a.slots == 0) return 0;
-  cfg.gridDim = dim3((unsigned)p.N, (unsigned)p.H);
-  cfg.blockDim = dim3(D);
+  const long long pairs = (long long)p.N * p.H;
+  cfg.gridDim = dim3((unsigned)((pairs + 1024 / D - 1) / (1024 / D)));
+  cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
   return (int)cudaLaunchKernelEx(&cfg, paged_pieces_join_kernel<D>, a);
 }
