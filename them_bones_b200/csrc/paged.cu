@@ -549,6 +549,9 @@ __global__ void __launch_bounds__(256) paged_rows_join_kernel(const RowsArgs p) 
   *reinterpret_cast<uint2*>(p.y + ((long long)row * p.p.H + h) * D + 4 * d) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
 }
 
+// CTAs that share a step's turns: what the SMs hold
+static int rows_ctas(int D, int sms) { return (D == 128 ? 3 : 4) * sms; }
+
 template <int D>
 static int launch_rows(RowsArgs& p, int ctas, cudaStream_t s) {
   p.warps = ctas * RW;
@@ -572,6 +575,8 @@ static int launch_rows(RowsArgs& p, int ctas, cudaStream_t s) {
 extern "C" {
 using namespace bones;
 
+long long bones_paged_room(int B, int N, int cap, int H, int D, int window_tiles, int tall, int sms);
+
 // qkv: bf16 rows of 3 * H * D, ldq apart; cosT, sinT: fp32 [rope_rows, D / 2]; k, v: bf16 [pages, H, 1 << shift, D] on 32 bytes; table: int32 [B, M],
 // rows ldt apart; starts: int32 [B + 1]; pos: int32 [B]; q: bf16 [N, H * D].
 int bones_paged_append(const void* qkv, long long ldq, const float* cosT, const float* sinT, int rope_rows, void* k, void* v, int pages, const int* table,
@@ -592,27 +597,33 @@ int bones_paged_append(const void* qkv, long long ldq, const float* cosT, const 
   return (int)cudaGetLastError();
 }
 
-// CTAs that share a step's turns, for a device of `sms` SMs; what `work` has to have room for goes by them.
-int bones_paged_rows_ctas(int D, int sms) { return (D == 128 ? 3 : 4) * sms; }
-
-// q, y: bf16 [N, H * D]; doc_start: int32 [N] or null; at most 512 sequences.  work: of this call alone until it ends, 32-byte aligned: with C =
-// bones_paged_rows_ctas, 8 C tiles of 16 * (D + 4) floats and then B + 1 64-bit and B 32-bit whole numbers.
-int bones_paged_rows(const void* q, const void* k, const void* v, int pages, const int* table, long long ldt, const int* starts, const int* pos,
-                     const int* doc_start, void* y, int B, int N, int M, int H, int D, int shift, float scale, int window_tiles, void* work, void* stream) {
-  if (paged_refused(B, N, M, H, D, shift, pages, ldt, k, v, starts, pos, table) || B > RB || !q || !y || (((uintptr_t)q | (uintptr_t)y | (uintptr_t)work) & 31) ||
+// q, y: bf16 [N, H * D]; doc_start: int32 [N] or null; window_tiles: of 128 tokens, 0 for all; tall: by tiles of 128 rows (pieces of more than a few tokens),
+// which calls of more than 512 sequences take in any case; work: of this call alone until it ends, on 32 bytes, as many as bones_paged_room says.
+int bones_paged_attention(const void* q, const void* k, const void* v, int pages, const int* table, long long ldt, const int* starts, const int* pos,
+                          const int* doc_start, void* y, int B, int N, int M, int H, int D, int shift, float scale, int window_tiles, int tall, void* work,
+                          long long room, void* stream) {
+  if (paged_refused(B, N, M, H, D, shift, pages, ldt, k, v, starts, pos, table) || !q || !y || (((uintptr_t)q | (uintptr_t)y | (uintptr_t)work) & 31) ||
       window_tiles < 0 || !work)
     return -2;
   if (N == 0) return 0;
-  const float log2e = 1.4426950408889634f;
   int dev = 0, sms = 0;
   BONES_CHECK(cudaGetDevice(&dev));
   BONES_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  const int ctas = bones_paged_rows_ctas(D, sms);
+  const Paged p{starts, pos, table, ldt, B, N, M, H, shift, pages, (int)min((long long)M << shift, 0x7fffff00ll), v};
+  if (room < bones_paged_room(B, N, p.cap, H, D, window_tiles, tall, sms)) return -2;
+  if (tall || B > RB) return paged_pieces(q, k, p, doc_start, y, D, scale, window_tiles, sms, work, stream);
+  const float log2e = 1.4426950408889634f;
+  const int ctas = rows_ctas(D, sms);
   float* parts = (float*)work;
   long long* before = (long long*)(parts + (long long)ctas * RW * 2 * RT * (D + 4));
-  RowsArgs a{(const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v,
-             Paged{starts, pos, table, ldt, B, N, M, H, shift, pages, (int)min((long long)M << shift, 0x7fffff00ll), v}, (__nv_bfloat16*)y, doc_start, window_tiles,
+  RowsArgs a{(const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, p, (__nv_bfloat16*)y, doc_start, window_tiles,
              scale * log2e, (scale < 0 ? -scale : scale) * D * log2e, before, (int*)(before + B + 1), parts, 0};
   return D == 128 ? launch_rows<128>(a, ctas, (cudaStream_t)stream) : launch_rows<64>(a, ctas, (cudaStream_t)stream);
+}
+
+// Bytes of bones_paged_attention's `work` on a device of `sms` SMs, for caches of `cap` tokens a sequence.
+long long bones_paged_room(int B, int N, int cap, int H, int D, int window_tiles, int tall, int sms) {
+  if (tall || B > RB) return paged_pieces_room(B, N, cap, H, D, window_tiles, sms);
+  return (long long)rows_ctas(D, sms) * RW * 2 * RT * (D + 4) * 4 + 12ll * B + 16;
 }
 }  // extern "C"

@@ -33,7 +33,8 @@ __device__ __forceinline__ Piece paged_piece(const Paged& p, int b) {
 }
 
 // The sequence that row r belongs to, by a warp: the number of starts at or before r, less one (-1 in front of the first, B behind the last).
-__device__ __forceinline__ int paged_owner(const int* starts, int B, int r) {
+template <typename I, typename R>
+__device__ __forceinline__ int paged_owner(const I* starts, int B, R r) {
   const int lane = threadIdx.x & 31;
   int lo = 0, hi = B + 1;                         // how many starts are <= r lies in [lo, hi]
   while (hi - lo > 32) {
@@ -52,6 +53,10 @@ __device__ __forceinline__ int paged_owner(const int* starts, int B, int r) {
 __device__ __forceinline__ long long paged_at(const Paged& p, int id, int h) {
   return id < 0 || id >= p.pages ? -1 : ((long long)id * p.H + h) << p.shift;
 }
+
+// Host: attention of longer pieces (paged_pieces.cu) and the bytes that it works with.
+int paged_pieces(const void* q, const void* k, const Paged& p, const int* doc_start, void* y, int D, float scale, int window_tiles, int sms, void* work, void* stream);
+long long paged_pieces_room(int B, int N, int cap, int H, int D, int window_tiles, int sms);
 
 // Host: whether a call is not one that the kernels are made for.
 inline bool paged_refused(int B, int N, int M, int H, int D, int shift, int pages, long long ldt, const void* k, const void* v, const int* starts, const int* pos,

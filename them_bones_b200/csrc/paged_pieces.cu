@@ -1,9 +1,9 @@
 // Attention of pieces of new tokens over a paged cache, in tiles of 128 queries and 128 keys: `tcgen05` products with TMEM accumulators,
 // keys and values brought page by page by TMA.  The formula stands with the kernels for pieces of a few tokens (paged.cu).
 //
-// Three kernels.  A plan (one CTA; others clear the rows that get no result): how many items each sequence has.  An item is a head's tile of
-// queries against its visible tiles of keys, or, where there are too few of those for all SMs, a part of these, whose sums go to memory.
-// The attention itself, persistent.  A join of parts, where there may be some.
+// Three kernels.  A plan (one CTA; others clear the rows that get no result).  The attention itself, persistent: an item is a head's tile of
+// queries against its visible tiles of keys.  Where these are fewer than two an SM, the CTAs share all key tiles equally instead, and what they have of a tile that is
+// not theirs alone goes to memory.  A join of such parts, where there may be some.
 #include "decode_common.cuh"
 #include "paged.cuh"
 
@@ -20,10 +20,10 @@ struct PiecesArgs {
   __nv_bfloat16* y;           // [N, H * D]
   int* err;
   int* next;                  // items drawn
-  int* prefix;                // [B + 1]: items of the sequences before
-  int* splits;                // [B]: parts of a tile of queries
-  int* places;                // [B]: the first of its parts' places, where there are parts
-  float* parts;               // [slots][128][D], and behind them [slots][128] sums of weights
+  int* tiles;                 // [B + 1]: tiles of queries, heads' one after another, of the sequences before
+  long long* before;          // [B + 1]: what the sequences before count for, in tiles of keys; behind that a CTA's share, 0 where items are drawn
+  float* parts;               // [slots][D][128], and behind them [slots][128] sums of weights: two places a CTA, of the tile that its share begins in and of
+                              // the one that it ends in
   int slots, sms, row_bytes;
 };
 
@@ -37,20 +37,20 @@ __device__ __forceinline__ int plan_tiles(const PiecesArgs& a, const Piece& s) {
   return a.window_tiles > 0 ? min(last + 1, a.window_tiles + 1) : last + 1;
 }
 // Sums of `v` over the threads in front; the total in *all.
-__device__ __forceinline__ int plan_scan(int v, int* box, int* all) {
+__device__ __forceinline__ long long plan_scan(long long v, long long* box, long long* all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int up = v;
+  long long up = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, up, o);
+    const long long x = __shfl_up_sync(0xffffffffu, up, o);
     if (lane >= o) up += x;
   }
   if (lane == 31) box[warp] = up;
   __syncthreads();
-  int before = 0, total = 0;
+  long long before = 0, total = 0;
 #pragma unroll
   for (int w = 0; w < PLAN_T / 32; ++w) {
-    const int x = box[w];
+    const long long x = box[w];
     if (w < warp) before += x;
     total += x;
   }
@@ -59,10 +59,11 @@ __device__ __forceinline__ int plan_scan(int v, int* box, int* all) {
   return before + up - v;
 }
 
+constexpr int PIECE_WAY = 2;                     // tiles of keys that a tile of queries' way in and out counts for
+constexpr int PIECE_LEAST = 4;                   // tiles of keys that are worth a part
+
 __global__ void __launch_bounds__(PLAN_T) paged_plan_kernel(const PiecesArgs a) {
-  __shared__ int box[PLAN_T / 32], rows_of[PLAN_T], tiles_of[PLAN_T], part;
-  __shared__ float cost[2];
-  __shared__ int cut[2];
+  __shared__ long long box[PLAN_T / 32];
   const Paged& p = a.p;
   pdl_launch();
   if (blockIdx.x > 0) {                          // rows without a result: outside all pieces, or left out
@@ -77,82 +78,32 @@ __global__ void __launch_bounds__(PLAN_T) paged_plan_kernel(const PiecesArgs a) 
     }
     return;
   }
-  if (threadIdx.x == 0) *a.next = 0;
-  // Parts only where the tiles of queries alone leave SMs without work, and only of up to PLAN_T sequences
-  part = 0x7fffffff;
-  if (a.slots > 0 && p.B <= PLAN_T) {
-    int rows = 0, tiles = 0, items;
-    if ((int)threadIdx.x < p.B) {
-      const Piece s = paged_piece(p, threadIdx.x);
-      if (s.live) {
-        rows = (s.live + PT - 1) / PT * p.H;
-        tiles = plan_tiles(a, s);
-      }
-    }
-    rows_of[threadIdx.x] = rows;
-    tiles_of[threadIdx.x] = tiles;
-    plan_scan(rows, box, &items);
-    if (items < 2 * a.sms) {
-      // parts of a 1st to 64th of the longest row of tiles: what the fullest SM has, an item's way in and out as one tile more
-      int most = 0;
-      for (int b = 0; b < p.B; ++b) most = max(most, tiles_of[b]);
-      if (threadIdx.x < 64) {
-        const int len = (most + threadIdx.x) / ((int)threadIdx.x + 1);
-        float work = 0.f, n = 0.f, used = 0.f;
-        if (len > 0) {
-          const float inv = 1.0f / len;
-          for (int b = 0; b < p.B; ++b) {
-            const float rows_b = (float)rows_of[b], s = ceilf(tiles_of[b] * inv);          // (as estimates go)
-            work += rows_b * tiles_of[b];
-            n += rows_b * s;
-            if (s > 1.f) used += rows_b * (s + 1.f);
-          }
-        }
-        const float waves = ceilf(n / a.sms);
-        float c = used > a.slots || (threadIdx.x > 0 && len < 3) ? 1e30f : fmaxf(fminf(waves * (len + 1.f), (work + n) / a.sms + 0.5f * len), len + 1.f);
-        int best = threadIdx.x;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          const float x = __shfl_xor_sync(0xffffffffu, c, o);
-          const int i = __shfl_xor_sync(0xffffffffu, best, o);
-          if (x < c || (x == c && i < best)) {
-            c = x;
-            best = i;
-          }
-        }
-        if ((threadIdx.x & 31) == 0) {
-          cost[threadIdx.x >> 5] = c;
-          cut[threadIdx.x >> 5] = best;
-        }
-      }
-      __syncthreads();
-      const int best = cost[1] < cost[0] ? cut[1] : cut[0];
-      if (threadIdx.x == 0 && best) part = (most + best) / (best + 1);
-    }
-  }
-  __syncthreads();
-  int items = 0, places = 0;
+  long long tiles = 0, total = 0;
   for (int b0 = 0; b0 < p.B; b0 += PLAN_T) {
     const int b = b0 + threadIdx.x;
-    int rows = 0, s = 1;
+    long long rows = 0, n = 0;
     if (b < p.B) {
       const Piece x = paged_piece(p, b);
       if (x.live) {
-        rows = (x.live + PT - 1) / PT * p.H;
-        s = part == 0x7fffffff ? 1 : max(1, (plan_tiles(a, x) + part - 1) / part);
+        rows = (long long)((x.live + PT - 1) / PT) * p.H;
+        n = plan_tiles(a, x) + PIECE_WAY;
       }
     }
-    int all, more;
-    const int at = items + plan_scan(rows * s, box, &all), place = places + plan_scan(s > 1 ? rows * s : 0, box, &more);
+    long long more, all;
+    const long long at = tiles + plan_scan(rows, box, &more), in_front = total + plan_scan(rows * n, box, &all);
     if (b < p.B) {
-      a.prefix[b] = at;
-      a.splits[b] = s;
-      a.places[b] = place;
+      a.tiles[b] = (int)at;
+      a.before[b] = in_front;
     }
-    items += all;
-    places += more;
+    tiles += more;
+    total += all;
   }
-  if (threadIdx.x == 0) a.prefix[p.B] = items;
+  if (threadIdx.x == 0) {
+    *a.next = 0;
+    a.tiles[p.B] = (int)tiles;
+    a.before[p.B] = total;
+    a.before[p.B + 1] = a.slots > 0 && tiles < 2 * a.sms ? max((total + a.sms - 1) / a.sms, (long long)PIECE_WAY + PIECE_LEAST) : 0;
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -163,12 +114,12 @@ __global__ void __launch_bounds__(PLAN_T) paged_plan_kernel(const PiecesArgs a) 
 // rows, the first and last of their keys): three dependent reads that nobody waits for, since it runs one item ahead.  What is of this kernel:
 //  - pages: a box of the tensor map is one page's P tokens of one head; a position without a page is loaded as zeros and masked.
 //  - rows behind a piece's end (a step with a few drafts has 5 of 128) take no exponentials: a softmax warp without a live row passes its tiles on.
-//  - values that a row does not see may be anything (other sequences' leftovers behind the end): in tiles with a mask the drain warps look
-//    through V before its product, put zeros for what is not finite, and add it back to the rows that do see it at the end.
+//  - values that a row does not see may be anything (other sequences' leftovers behind the end): tiles with a mask are looked through before V's
+//    product, by the warp that loaded them, zeros are put for what is not finite, and it is added back to the rows that do see it at the end.
 constexpr int PP_SW = 16, PP_DW = 4;
 constexpr int PP_PV = 2 + PP_SW + PP_DW, PP_VW = PP_PV + 1, PP_IW = PP_VW + 1;
 constexpr int PP_THREADS = 32 * (PP_IW + 1);
-constexpr int PP_RING = 2;                      // items handed round: the one being computed and the next
+constexpr int PP_RING = 2;                      // items handed round: the one being computed and the next (three: the same times)
 constexpr uint32_t PP_BARS = 512;               // barriers, TMEM address, abort flag, items
 
 struct PieceItem {
@@ -209,21 +160,22 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   auto s_free = [&](int s) { return bars + 8u * (20 + s); };
   auto p_full = [&](int s) { return bars + 8u * (23 + s); };
   auto i_full = [&](int s) { return bars + 8u * (26 + s); };
-  auto i_free = [&](int s) { return bars + 8u * (28 + s); };
-  const uint32_t o_full = bars + 8u * 30, o_free = bars + 8u * 31, l_full = bars + 8u * 32, l_free = bars + 8u * 33;
+  auto i_free = [&](int s) { return bars + 8u * (29 + s); };
+  const uint32_t o_full = bars + 8u * 32, o_free = bars + 8u * 33, l_full = bars + 8u * 34, l_free = bars + 8u * 35;
   const uint32_t tmem_slot = bars + 288u;
   volatile uint32_t* tmem_slot_g = reinterpret_cast<volatile uint32_t*>(gen + kBars + 288);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + kBars + 292);
   int* taint = reinterpret_cast<int*>(gen + kBars + 296);                                    // [PP_RING]
+  volatile int* holes = reinterpret_cast<volatile int*>(gen + kBars + 448);                  // [8], by tile: whether a page that it needs is missing
   PieceItem* ring = reinterpret_cast<PieceItem*>(gen + kBars + 320);                         // [PP_RING]
-  static_assert(320 + PP_RING * sizeof(PieceItem) <= PP_BARS && PP_RING == 2, "room");
+  static_assert(PP_RING <= 3 && 320 + PP_RING * sizeof(PieceItem) <= 448 && 448 + 8 * 4 <= PP_BARS, "room");
   float* lsum = reinterpret_cast<float*>(gen + kBars + PP_BARS);                             // [4 column parts][128 rows]
 
   const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int A = p.H * D;
   if (warp == 0) {
-    for (int i = lane; i < 34; i += 32) {
-      const bool by_softmax = (i >= 23 && i < 26) || i == 32, by_drain = (i >= 14 && i < 17) || i == 28 || i == 29 || i == 31 || i == 33;
+    for (int i = lane; i < 36; i += 32) {
+      const bool by_softmax = (i >= 23 && i < 26) || i == 34, by_drain = (i >= 29 && i < 32) || i == 33 || i == 35;
       mbar_init(bars + 8u * (uint32_t)i, by_softmax ? PP_SW : by_drain ? PP_DW : 1);
     }
     if (lane == 0) *abort_flag = 0;
@@ -242,17 +194,18 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   const uint32_t tO = tmem + 384u;
   // the it-th item of this CTA; false behind the last one
   auto take = [&](int it, PieceItem* im) {
-    if (!__all_sync(0xffffffffu, mbar_wait(i_full(it & 1), (uint32_t)((it >> 1) & 1), abort_flag, a.err, ERR_WAIT_AUX))) return false;
-    *im = ring[it & 1];
+    if (!__all_sync(0xffffffffu, mbar_wait(i_full(it % PP_RING), (uint32_t)(it / PP_RING & 1), abort_flag, a.err, ERR_WAIT_AUX))) return false;
+    *im = ring[it % PP_RING];
     return warp_uniform(im->n) > 0;
   };
   // whether some row of the item does not see some key of the tile
   auto masked = [&](const PieceItem& im, int kt) { return kt * PT + PT - 1 > im.pos0 || kt * PT < im.far || im.none; };
   const int per_tile = PT >> p.shift;           // pages of a tile
   // row of the tensor map of lane i's page of tile kt (lanes below per_tile); behind the map, which reads as zeros, where there is none
+  const int none = (int)(((long long)p.pages * p.H) << p.shift);
   auto page_row = [&](const PieceItem& im, int kt) {
     const int i = kt * per_tile + lane;
-    int row = (int)(((long long)p.pages * p.H) << p.shift);
+    int row = none;
     if (lane < per_tile && i < p.M && (i << p.shift) < im.pos0 + im.live) {
       const long long at = paged_at(p, p.table[im.seq * p.ldt + i], im.h);
       if (at >= 0) row = (int)at;
@@ -262,23 +215,45 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   const uint32_t page_bytes = 128u << p.shift;  // of a column half
 
   if (warp == PP_IW) {
-    // The items, in sequence- and head-major order, so that CTAs at work at one time share keys and values through L2.
-    const int total = p.B > 0 ? a.prefix[p.B] : 0;
+    // The items, in sequence- and head-major order, so that CTAs at work at one time share keys and values through L2: drawn, or what a share of all
+    // tiles of keys has of them.
+    const long long share = a.before[p.B + 1], total = share ? a.before[p.B] : a.tiles[p.B];
+    long long at = (long long)blockIdx.x * share;
+    const long long stop = min(at + share, total);
     for (int it = 0;; ++it) {
-      int w = (int)blockIdx.x;
-      if (it > 0) w = (int)gridDim.x + warp_uniform(lane == 0 ? atomicAdd(a.next, 1) : 0);
+      int b = -1, g = 0, from_v = 0, to_v = 0, all_v = 0;           // the sequence, its tile of queries, and which of the tiles of keys that it counts for
+      if (share) {
+        while (at < stop && to_v <= from_v) {
+          b = min(max(paged_owner(a.before, p.B, at), 0), p.B - 1);
+          all_v = plan_tiles(a, paged_piece(p, b));
+          const int per = all_v + PIECE_WAY;
+          const long long in_seq = at - a.before[b];
+          g = (int)(in_seq / per);
+          const int off = (int)(in_seq % per), take = (int)min((long long)(per - off), stop - at);
+          at += take;
+          from_v = max(off - PIECE_WAY, 0);
+          to_v = off + take - PIECE_WAY;
+        }
+        if (to_v <= from_v) b = -1;
+      } else {
+        const int w = it == 0 ? (int)blockIdx.x : (int)gridDim.x + warp_uniform(lane == 0 ? atomicAdd(a.next, 1) : 0);
+        if (w < total) {
+          b = min(max(paged_owner(a.tiles, p.B, w), 0), p.B - 1);
+          g = w - a.tiles[b];
+          to_v = all_v = 1;
+        }
+      }
       PieceItem im = {};
-      if (w < total) {
-        const int b = min(max(paged_owner(a.prefix, p.B, w), 0), p.B - 1);
+      if (b >= 0) {
         const Piece s = paged_piece(p, b);
-        const int splits = a.splits[b], r = w - a.prefix[b], part = r % splits, g = r / splits, rows = (s.live + PT - 1) / PT;
+        const int rows = (s.live + PT - 1) / PT;
         im.seq = b;
         im.h = g / rows;
         const int qt = rows - 1 - (g % rows + im.h) % rows;
         im.row0 = s.row + qt * PT;
         im.live = min(PT, s.live - qt * PT);
         im.pos0 = s.pos + qt * PT;
-        im.place = splits > 1 ? a.places[b] + r : -1;
+        im.place = to_v - from_v < all_v ? 2 * (int)blockIdx.x + (from_v == 0) : -1;
         int lo = 0x7fffffff, hi = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -293,13 +268,13 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         lo = __reduce_min_sync(0xffffffffu, lo);
         im.far = __reduce_max_sync(0xffffffffu, hi);
         const int last = (im.pos0 + im.live - 1) >> 7, first = min(lo >> 7, last), n = last - first + 1;
-        const int from = (int)((long long)part * n / splits), to = (int)((long long)(part + 1) * n / splits);
+        const int from = (int)((long long)from_v * n / all_v), to = (int)((long long)to_v * n / all_v);
         im.none = to <= from;
         im.kt0 = im.none ? last : first + from;
         im.n = im.none ? 1 : to - from;
       }
-      const int slot = it & 1;
-      if (it >= PP_RING && !__all_sync(0xffffffffu, mbar_wait(i_free(slot), (uint32_t)(((it - PP_RING) >> 1) & 1), abort_flag, a.err, ERR_WAIT_EMPTY))) break;
+      const int slot = it % PP_RING;
+      if (it >= PP_RING && !__all_sync(0xffffffffu, mbar_wait(i_free(slot), (uint32_t)((it / PP_RING - 1) & 1), abort_flag, a.err, ERR_WAIT_EMPTY))) break;
       if (lane == 0) {
         ring[slot] = im;
         taint[slot] = 0;
@@ -327,6 +302,9 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         const int ks = g & 1, now = row;
         if (j + 1 < im.n) row = page_row(im, im.kt0 + j + 1);
         if (g >= 2 && !dead) dead = !mbar_wait(k_free(ks), (uint32_t)(((g - 2) >> 1) & 1), abort_flag, a.err, ERR_WAIT_EMPTY);
+        // (at most four tiles are between this one and the oldest whose scores are still read)
+        const uint32_t missing = __ballot_sync(0xffffffffu, lane < per_tile && now == none && ((im.kt0 + j) * per_tile + lane) << p.shift < im.pos0 + im.live);
+        if (lane == 0) holes[g & 7] = (int)missing;
         if (elect_one() && !dead) mbar_arrive_expect_tx(k_full(ks), TILE);
         __syncwarp();
         for (int i = 0; i < per_tile; ++i) {
@@ -339,13 +317,58 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       }
     }
   } else if (warp == PP_VW) {
-    // V loads
+    // V loads; behind each, the tile before it is looked through where some row sees only some of its keys
     PieceItem im;
     int g = 0, vs = 0;
     uint32_t vph = 1;
     bool dead = false;
+    auto look = [&](int stage, uint32_t parity, int it, int kt) {
+      if (!__all_sync(0xffffffffu, mbar_wait(v_full(stage), parity, abort_flag, a.err, ERR_WAIT_FULL))) return false;
+      uint4* tile = reinterpret_cast<uint4*>(gen + TILE * (4 + stage)) + lane;
+      // the largest magnitude of each half: an infinity is larger than the finite, a NaN stays
+      __nv_bfloat162 most[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) most[k] = __float2bfloat162_rn(0.f);
+#pragma unroll 8
+      for (int i = 0; i < (int)(TILE / 512); ++i) {
+        const uint4 u = tile[i * 32];
+        const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&u);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) most[k] = __hmax2_nan(most[k], __habs2(x[k]));
+      }
+#pragma unroll
+      for (int k = 1; k < 4; ++k) most[0] = __hmax2_nan(most[0], most[k]);
+      const uint32_t top = *reinterpret_cast<const uint32_t*>(&most[0]);
+      if (__any_sync(0xffffffffu, (top & 0x7f80u) == 0x7f80u || (top & 0x7f800000u) == 0x7f800000u)) {
+        bool seen = false;
+        for (int i = 0; i < (int)(TILE / 512); ++i) {
+          const uint4 u = tile[i * 32];
+          uint32_t w[4] = {u.x, u.y, u.z, u.w};
+          bool any = false;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t t = ((w[k] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+            if (t) any = true;
+            if (t & 0x8000u) w[k] &= 0xffff0000u;
+            if (t & 0x80000000u) w[k] &= 0xffffu;
+          }
+          if (any) {
+            tile[i * 32] = make_uint4(w[0], w[1], w[2], w[3]);
+            if (kt * PT + (((lane + i * 32) * 16 >> 7) & (PT - 1)) < im.pos0 + im.live) seen = true;        // not a leftover behind the end
+          }
+        }
+        if (__any_sync(0xffffffffu, seen) && lane == 0) atomicOr(&taint[it % PP_RING], 1);
+        fence_proxy_async_smem();
+        __threadfence_block();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(v_fine(stage));
+      return true;
+    };
     for (int it = 0; !dead && take(it, &im); ++it) {
       int row = page_row(im, im.kt0);
+      int last = -1;                                  // the stage of a tile that is still to be looked through, and its parity
+      uint32_t last_parity = 0;
       for (int j = 0; j < im.n; ++j, ++g) {
         const int now = row;
         if (j + 1 < im.n) row = page_row(im, im.kt0 + j + 1);
@@ -359,8 +382,12 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             for (int c = 0; c < D / 64; ++c) tma_load_2d(sV(vs) + c * PATOM + i * page_bytes, &tm_v, v_full(vs), c * 64, at);
           }
         }
+        if (last >= 0 && !look(last, last_parity, it, im.kt0 + j - 1)) dead = true;
+        last = masked(im, im.kt0 + j) ? vs : -1;
+        last_parity = vph ^ 1u;
         if (++vs == 3) { vs = 0; vph ^= 1u; }
       }
+      if (last >= 0 && !look(last, last_parity, it, im.kt0 + im.n - 1)) dead = true;
     }
   } else if (warp == 1) {
     // S = Q K^T of each tile, into the buffer whose O += P V (three tiles before) is done
@@ -401,11 +428,15 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     PieceItem im;
     bool dead = false;
     int ps = 0;                              // P buffer and V stage
-    uint32_t pph = 0;
+    uint32_t pph = 0, fine = 0;              // parity of either; of each stage's looked-through uses
     for (int it = 0; !dead && take(it, &im); ++it) {
       const int n = warp_uniform(im.n);
       for (int j = 0; j < n; ++j) {
-        if (!dead) dead = !mbar_wait(v_fine(ps), pph, abort_flag, a.err, ERR_WAIT_FULL);
+        if (!dead) dead = !mbar_wait(v_full(ps), pph, abort_flag, a.err, ERR_WAIT_FULL);
+        if (masked(im, im.kt0 + j)) {
+          if (!dead) dead = !mbar_wait(v_fine(ps), (fine >> ps) & 1, abort_flag, a.err, ERR_WAIT_AUX);
+          fine ^= 1u << ps;
+        }
         if (j == 0 && it >= 1 && !dead) dead = !mbar_wait(o_free, (uint32_t)((it - 1) & 1), abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
         if (!dead) dead = !mbar_wait(p_full(ps), pph, abort_flag, a.err, ERR_WAIT_AUX);
         tc_fence_after();
@@ -427,7 +458,7 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const int r = q * 32 + lane, c0 = part * 32;
     const uint32_t lane_addr = (uint32_t)(q * 32) << 16;
     PieceItem im;
-    int gs = 0;
+    int gs = 0, g = 0;
     uint32_t sph = 0;
     bool ok = true;
     for (int it = 0; ok && take(it, &im); ++it) {
@@ -439,16 +470,9 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         if (a.doc_start) lo = a.doc_start[im.row0 + r];
         if (a.window_tiles > 0) lo = max(lo, (((im.pos0 + r) >> 7) - (a.window_tiles - 1)) * 128);
       }
-      const int* table = p.table + im.seq * p.ldt;
       float l = 0.f;
-      for (int j = 0; j < im.n; ++j) {
+      for (int j = 0; j < im.n; ++j, ++g) {
         const int k0 = (im.kt0 + j) * PT + c0;
-        bool there_a = true, there_b = true;     // pages of the first and second sixteen keys
-        if (!idle) {
-          const int ia = k0 >> p.shift, ib = (k0 + 16) >> p.shift;
-          there_a = ia < p.M && (uint32_t)table[ia] < (uint32_t)p.pages;
-          there_b = ib < p.M && (uint32_t)table[ib] < (uint32_t)p.pages;
-        }
         const bool got = mbar_wait(s_full(gs), sph, abort_flag, a.err, ERR_WAIT_TMEM_FULL);
         if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
         tc_fence_after();
@@ -463,8 +487,11 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             const float x = fmaf(__uint_as_float(v0[i]), a.c1, -a.c2);
             asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[i]) : "f"(x));
           }
-          if (__any_sync(0xffffffffu, (k0 + 31 > qpos) || (k0 < lo) || !there_a || !there_b)) {
+          const int missing = holes[g & 7];
+          if (__any_sync(0xffffffffu, (k0 + 31 > qpos) || (k0 < lo) || missing)) {
             const int end = qpos - k0, from = lo - k0;
+            // pages of the first and second sixteen keys
+            const bool there_a = !(missing >> (c0 >> p.shift) & 1), there_b = !(missing >> ((c0 + 16) >> p.shift) & 1);
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (i > end || i < from || !(i < 16 ? there_a : there_b)) e[i] = 0.f;
@@ -490,56 +517,11 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       if (lane == 0) mbar_arrive(l_full);
     }
   } else {
-    // Drain: a thread per query row; before, the tiles of V in which some row sees only some keys
+    // Drain: a thread per query row
     const int q = warp & 3, r = q * 32 + lane;
     const uint32_t tOr = tO + ((uint32_t)(q * 32) << 16);
     PieceItem im;
-    int vs = 0;
-    uint32_t vph = 0;
-    bool ok = true;
-    for (int it = 0; ok && take(it, &im); ++it) {
-      const int end = im.pos0 + im.live;
-      for (int j = 0; j < im.n; ++j) {
-        // Every tile is passed on from here, so that no phase of a stage goes by unseen (a wait tells apart two phases, not three)
-        if (!__all_sync(0xffffffffu, mbar_wait(v_full(vs), vph, abort_flag, a.err, ERR_WAIT_FULL))) { ok = false; break; }
-        if (masked(im, im.kt0 + j)) {
-          uint4* tile = reinterpret_cast<uint4*>(gen + TILE * (4 + vs)) + q * (TILE / 64) + lane;        // a quarter; TILE / 16 pieces of 16 bytes
-          uint32_t odd = 0;
-#pragma unroll 8
-          for (int i = 0; i < (int)(TILE / 64 / 32); ++i) {
-            const uint4 u = tile[i * 32];
-            // an exponent of all ones carries into the sign's place
-            odd |= ((u.x & 0x7f807f80u) + 0x00800080u) | ((u.y & 0x7f807f80u) + 0x00800080u) | ((u.z & 0x7f807f80u) + 0x00800080u) | ((u.w & 0x7f807f80u) + 0x00800080u);
-          }
-          if (__any_sync(0xffffffffu, odd & 0x80008000u)) {
-            bool seen = false;
-            for (int i = 0; i < (int)(TILE / 64 / 32); ++i) {
-              uint4 u = tile[i * 32];
-              uint32_t w[4] = {u.x, u.y, u.z, u.w};
-              bool any = false;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const uint32_t t = ((w[k] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-                if (t) any = true;
-                if (t & 0x8000u) w[k] &= 0xffff0000u;
-                if (t & 0x80000000u) w[k] &= 0xffffu;
-              }
-              if (any) {
-                tile[i * 32] = make_uint4(w[0], w[1], w[2], w[3]);
-                const int key = (im.kt0 + j) * PT + (((q * (int)(TILE / 64) + lane + i * 32) * 16 >> 7) & (PT - 1));
-                if (key < end) seen = true;         // not a leftover behind the end
-              }
-            }
-            if (__any_sync(0xffffffffu, seen) && lane == 0) atomicOr(&taint[it & 1], 1);
-            fence_proxy_async_smem();
-            __threadfence_block();
-          }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(v_fine(vs));
-        if (++vs == 3) { vs = 0; vph ^= 1u; }
-      }
-      if (!ok) break;
+    for (int it = 0; take(it, &im); ++it) {
       const bool real = r < im.live;
       bool got = mbar_wait(l_full, (uint32_t)(it & 1), abort_flag, a.err, ERR_WAIT_AUX);
       if (!__all_sync(0xffffffffu, got)) break;
@@ -549,12 +531,12 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       const float inv = l == 0.f ? 0.f : 1.0f / l;        // a row that sees no key has zeros
       const long long col = (long long)im.h * D;
       __nv_bfloat16* y = a.y + (long long)(im.row0 + r) * A + col;
-      float* part = a.parts + ((long long)im.place * PT + r) * D;
+      float* part = a.parts + (long long)im.place * PT * D + r;              // columns of 128 rows: a warp's stores lie side by side
       if (im.place >= 0 && real) a.parts[(long long)a.slots * PT * D + (long long)im.place * PT + r] = l;
       got = mbar_wait(o_full, (uint32_t)(it & 1), abort_flag, a.err, ERR_WAIT_TMEM_FULL);
       if (!__all_sync(0xffffffffu, got)) break;
       tc_fence_after();
-      const bool tainted = warp_uniform(*(volatile int*)&taint[it & 1]) != 0;
+      const bool tainted = warp_uniform(*(volatile int*)&taint[it % PP_RING]) != 0;
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t v[32];
@@ -589,7 +571,7 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         if (im.place >= 0) {
           if (real)
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(part + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            for (int i = 0; i < 32; ++i) part[(c + i) * PT] = __uint_as_float(v[i]);
         } else {
           uint4 u[4];
 #pragma unroll
@@ -606,7 +588,7 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(i_free(it & 1));
+      if (lane == 0) mbar_arrive(i_free(it % PP_RING));
     }
   }
 
@@ -621,45 +603,34 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   }
 }
 
-// Adds the parts of a row and head in their order.  D / 4 threads a row and head.
+// Adds the parts of a tile in their order.  grid: (tiles of queries, D / 8), a thread four columns of a row.
 template <int D>
 __global__ void __launch_bounds__(256) paged_pieces_join_kernel(const PiecesArgs a) {
-  constexpr int T = D / 4, PAIRS = 256 / T;
-  const Paged& p = a.p;
-  const long long item = (long long)blockIdx.x * PAIRS + threadIdx.x / T;
-  const int d = threadIdx.x % T;
-  const bool on = item < (long long)p.N * p.H;
-  const int row = on ? (int)(item / p.H) : -1, h = on ? (int)(item % p.H) : 0;
-  int b = -1;
-#pragma unroll
-  for (int i = 0; i < 32; i += T) {
-    const int x = paged_owner(p.starts, p.B, __shfl_sync(0xffffffffu, row, i));
-    if ((int)(threadIdx.x & 31) >= i) b = x;
-  }
-  Piece s = {};
-  if (on && b >= 0 && b < p.B) s = paged_piece(p, b);
   pdl_wait();
-  const int i = row - s.row;
-  if (!on || !s.live || i < 0 || i >= s.live) return;
-  const int splits = a.splits[b], place0 = a.places[b];
+  const Paged& p = a.p;
+  const long long share = a.before[p.B + 1];
+  if (share == 0) return;
+  const int b = paged_owner(a.tiles, p.B, (int)blockIdx.x);
+  if (b < 0 || b >= p.B) return;
+  const Piece s = paged_piece(p, b);
+  const int g = blockIdx.x - a.tiles[b], n = plan_tiles(a, s);
+  const long long from = a.before[b] + (long long)g * (n + PIECE_WAY) + PIECE_WAY;
+  const int w0 = (int)(from / share), splits = (int)((from + n - 1) / share) - w0 + 1;
   if (splits == 1) return;
-  const int rows = (s.live + PT - 1) / PT, qt = i / PT, g = h * rows + ((rows - 1 - qt - h) % rows + rows) % rows;
-  const long long place = place0 + (long long)g * splits;
-  const float* parts = a.parts + (place * PT + i % PT) * D + 4 * d;
-  const float* sums = a.parts + (long long)a.slots * PT * D + place * PT + i % PT;
-  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
+  const int rows = (s.live + PT - 1) / PT, h = g / rows, qt = rows - 1 - (g % rows + h) % rows, r = threadIdx.x % PT, c = blockIdx.y * 8 + threadIdx.x / PT * 4;
+  if (qt * PT + r >= s.live) return;
+  // the first CTA's second place, the others' first
+  const float* part = a.parts + (2ll * w0 * D + c) * PT + r;
+  const float* sum = a.parts + (long long)a.slots * PT * D + 2ll * w0 * PT + r;
+  float x[4] = {}, l = 0.f;
 #pragma unroll 4
   for (int k = 0; k < splits; ++k) {
-    const float4 z = *reinterpret_cast<const float4*>(parts + (long long)k * PT * D);
-    x.x += z.x;
-    x.y += z.y;
-    x.z += z.z;
-    x.w += z.w;
-    l += sums[(long long)k * PT];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] += part[((2ll * k + (k == 0)) * D + i) * PT];
+    l += sum[(2ll * k + (k == 0)) * PT];
   }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  *reinterpret_cast<uint2*>(a.y + ((long long)row * p.H + h) * D + 4 * d) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+  *reinterpret_cast<uint2*>(a.y + ((long long)(s.row + qt * PT + r) * p.H + h) * D + c) = make_uint2(pack_bf16(x[0] * inv, x[1] * inv), pack_bf16(x[2] * inv, x[3] * inv));
 }
 
 static int tmap_rows_2d(CUtensorMap* out, const void* ptr, long long rows, long long cols, int box_rows) {
@@ -680,8 +651,8 @@ static int launch_pieces(const CUtensorMap& tq, const CUtensorMap& tk, const CUt
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
   // a CTA an SM, fewer where the items cannot be as many
-  const long long most = (p.N / PT + (long long)min(p.B, p.N)) * p.H + a.slots;
-  cfg.gridDim = dim3((unsigned)min(most, (long long)a.sms));
+  const long long tiles = (p.N / PT + (long long)min(p.B, p.N)) * p.H;
+  cfg.gridDim = dim3((unsigned)(a.slots ? a.sms : min(tiles, (long long)a.sms)));
   cfg.blockDim = dim3(PP_THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -689,52 +660,48 @@ static int launch_pieces(const CUtensorMap& tq, const CUtensorMap& tk, const CUt
   cfg.numAttrs = (unsigned)dec_launch_attrs(at, 1, 1);
   BONES_CHECK(cudaLaunchKernelEx(&cfg, paged_pieces_kernel<D>, tq, tk, tv, a));
   if (a.slots == 0) return 0;
-  const long long pairs = (long long)p.N * p.H;
-  cfg.gridDim = dim3((unsigned)((pairs + 1024 / D - 1) / (1024 / D)));
+  cfg.gridDim = dim3((unsigned)tiles, D / 8);
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
   return (int)cudaLaunchKernelEx(&cfg, paged_pieces_join_kernel<D>, a);
 }
 
-}  // namespace bones
+// Places for parts, two a CTA; none where the tiles of queries alone are two an SM, or see a few tiles of keys at most.
+static int pieces_slots(int N, int cap, int H, int window_tiles, int sms) {
+  const long long seen = window_tiles > 0 ? min((long long)cap, window_tiles * 128ll + 128) : cap;
+  return seen > PIECE_LEAST * PT && (long long)(N / PT) * H < 2ll * sms ? 2 * sms : 0;
+}
+static long long pieces_ints(int B) { return (3ll * B + 16 + 7) / 8 * 8; }
 
-extern "C" {
-using namespace bones;
+long long paged_pieces_room(int B, int N, int cap, int H, int D, int window_tiles, int sms) {
+  return 4 * (pieces_ints(B) + (long long)pieces_slots(N, cap, H, window_tiles, sms) * PT * (D + 1));
+}
 
-// As bones_paged_rows.  ints: room for 3 B + 16 ints; parts: room for slots * 128 * (D + 1) floats on 16 bytes, or null with slots 0; both of this
-// call alone until it ends.
-int bones_paged_pieces(const void* q, const void* k, const void* v, int pages, const int* table, long long ldt, const int* starts, const int* pos,
-                       const int* doc_start, void* y, int B, int N, int M, int H, int D, int shift, float scale, int window_tiles, int* ints, float* parts,
-                       int slots, void* stream) {
-  if (paged_refused(B, N, M, H, D, shift, pages, ldt, k, v, starts, pos, table) || !q || !y || (((uintptr_t)q | (uintptr_t)y) & 31) || window_tiles < 0 || !ints ||
-      slots < 0 || (slots && !parts) || misaligned16(parts) || (N / PT + (long long)B) * H > 0x3fffffffll)
-    return -2;
-  if (N == 0) return 0;
+int paged_pieces(const void* q, const void* k, const Paged& p, const int* doc_start, void* y, int D, float scale, int window_tiles, int sms, void* work, void* stream) {
+  if ((p.N / PT + (long long)p.B) * p.H > 0x3fffffffll) return -2;
   const float log2e = 1.4426950408889634f;
   PiecesArgs a = {};
-  a.p = Paged{starts, pos, table, ldt, B, N, M, H, shift, pages, (int)min((long long)M << shift, 0x7fffff00ll), v};
+  a.p = p;
   a.c1 = scale * log2e;
   a.c2 = (scale < 0 ? -scale : scale) * D * log2e;
   a.window_tiles = window_tiles;
   a.doc_start = doc_start;
   a.y = (__nv_bfloat16*)y;
   a.err = error_word();
-  a.next = ints;
-  a.prefix = ints + 4;
-  a.splits = a.prefix + B + 1;
-  a.places = a.splits + B;
-  a.parts = parts;
-  a.slots = slots;
-  a.row_bytes = H * D * 2;
-  int dev = 0;
-  BONES_CHECK(cudaGetDevice(&dev));
-  BONES_CHECK(cudaDeviceGetAttribute(&a.sms, cudaDevAttrMultiProcessorCount, dev));
+  a.next = (int*)work;
+  a.before = (long long*)(a.next + 2);
+  a.tiles = (int*)(a.before + p.B + 2);
+  a.slots = pieces_slots(p.N, p.cap, p.H, window_tiles, sms);
+  a.parts = (float*)work + pieces_ints(p.B);
+  a.row_bytes = p.H * D * 2;
+  a.sms = sms;
   CUtensorMap tq, tk, tv;
-  const long long rows = ((long long)pages * H) << shift;
-  int rc = tmap_rows_2d(&tq, q, N, (long long)H * D, PT);
-  if (!rc) rc = tmap_rows_2d(&tk, k, rows, D, 1 << shift);
-  if (!rc) rc = tmap_rows_2d(&tv, v, rows, D, 1 << shift);
+  const long long rows = ((long long)p.pages * p.H) << p.shift;
+  int rc = tmap_rows_2d(&tq, q, p.N, (long long)p.H * D, PT);
+  if (!rc) rc = tmap_rows_2d(&tk, k, rows, D, 1 << p.shift);
+  if (!rc) rc = tmap_rows_2d(&tv, p.values, rows, D, 1 << p.shift);
   if (rc) return rc;
   return D == 128 ? launch_pieces<128>(tq, tk, tv, a, (cudaStream_t)stream) : launch_pieces<64>(tq, tk, tv, a, (cudaStream_t)stream);
 }
-}  // extern "C"
+
+}  // namespace bones

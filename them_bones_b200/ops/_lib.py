@@ -39,9 +39,8 @@ SIGNATURES = {
     "bones_kv8_read": [_P] * 8 + [_I] * 5 + [_P, _I, _I, _P],
     "bones_kv8_attention": [_P, _L, _P, _P, _I] + [_P] * 6 + [_P, _I, _I, _P, _P] + [_I] * 4 + [_F, _I, _I, _P, _I, _P],
     "bones_paged_append": [_P, _L, _P, _P, _I, _P, _P, _I, _P, _L, _P, _P] + [_I] * 6 + [_P, _P],
-    "bones_paged_rows_ctas": [_I, _I],
-    "bones_paged_rows": [_P] * 3 + [_I, _P, _L] + [_P] * 4 + [_I] * 6 + [_F, _I, _P, _P],
-    "bones_paged_pieces": [_P] * 3 + [_I, _P, _L] + [_P] * 4 + [_I] * 6 + [_F, _I, _P, _P, _I, _P],
+    "bones_paged_room": [_I] * 8,
+    "bones_paged_attention": [_P] * 3 + [_I, _P, _L] + [_P] * 4 + [_I] * 6 + [_F, _I, _I, _P, _L, _P],
     "bones_verify": [_P, _L, _P, _L, _I, _P, _P, _P, _I, _I, _I, ctypes.c_double, _P, _P, _P, _P],
     "bones_logprobs_fwd": [_P, _L, _I, _L, _I, _P, _I] + [_P] * 6,
     "bones_logprobs_bwd": [_P, _L, _I, _L, _I, _I, _P, _I] + [_P] * 6 + [_L, _F, _P],
@@ -59,6 +58,7 @@ def load():
         lib = ctypes.CDLL(_PATH)
         for name, types in SIGNATURES.items():
             getattr(lib, name).argtypes = types
+        lib.bones_paged_room.restype = _L
         _LIB = lib
     return _LIB
 

@@ -21,7 +21,6 @@ PAGES = (16, 32, 64, 128)              # tokens of a page
 SHIFT = 32.0                           # largest |scale| * head_dim: the kernels' soft-max has this fixed shift, and its smallest weights, exp(-2 * 32), stay normal in fp32
 MOST_ROWS = (1 << 31) - 256             # rows of [D] in a cache
 FEW = 16                               # pieces of up to this many tokens go by tiles of 16 rows, longer ones by tiles of 128
-MOST_FEW = 512                         # as do those of more sequences than this
 
 
 class PagedKV(NamedTuple):
@@ -100,24 +99,28 @@ def no_gradient(*xs):
 
 
 # -- native bodies -----------------------------------------------------------------------------------------------------
-def _aligned(x, by):
-    """``x [N, C]`` as the kernels read it: consecutive values, rows that begin on ``by`` bytes."""
-    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) * 2 % by) or x.data_ptr() % by:
+def _rows_on(x, by):
+    """``x [N, C]`` as the kernels read it, and its address: consecutive values, rows that begin on ``by`` bytes."""
+    at = x.data_ptr()
+    if x.stride(1) != 1 or at % by or (x.shape[0] > 1 and x.stride(0) * 2 % by):
         x = x.contiguous() if not x.is_contiguous() else x.clone()
-    return x
+        at = x.data_ptr()
+    return x, at
 
 
 def append(dims, qkv, cos, sin, c, table, starts, pos):
     _bf16(qkv, "qkv")
-    _bf16(c[0], "the cache")
     b, m, h, page, d, dev = dims
-    qkv, cos, sin = _aligned(qkv, 16), _table(cos), _table(sin)
+    k, v = c
+    _bf16(k, "a cache")
+    qkv, at = _rows_on(qkv, 16)
+    cos, sin = _table(cos), _table(sin)
     n = qkv.shape[0]
     q = qkv.new_empty((n, h * d))
     if n:
         with L.device(dev):
-            L.call("bones_paged_append", qkv.data_ptr(), qkv.stride(0), cos.data_ptr(), sin.data_ptr(), cos.shape[0], c[0].data_ptr(), c[1].data_ptr(), c[0].shape[0],
-                   table.data_ptr(), max(table.stride(0), m), starts.data_ptr(), pos.data_ptr(), b, n, m, h, d, page.bit_length() - 1, q.data_ptr(), L.raw_stream())
+            L.call("bones_paged_append", at, qkv.stride(0), cos.data_ptr(), sin.data_ptr(), cos.shape[0], k.data_ptr(), v.data_ptr(), k.shape[0], table.data_ptr(),
+                   table.stride(0) if b > 1 else m, starts.data_ptr(), pos.data_ptr(), b, n, m, h, d, page.bit_length() - 1, q.data_ptr(), L.raw_stream())
         COUNTS["paged_append"] += 1
     return q
 
@@ -125,42 +128,28 @@ def append(dims, qkv, cos, sin, c, table, starts, pos):
 def attention(dims, q, c, table, starts, pos, scale, doc_start, window, longest):
     _bf16(q, "queries")
     b, m, h, page, d, dev = dims
+    k, v = c
     if abs(scale) * d > SHIFT:
         raise ValueError(f"native paged attention does not cover this call: scale {scale} (at most {SHIFT / d} for heads of {d})")
     n = q.shape[0]
     if n > 1 and q.stride(0) != h * d:
         q = q.contiguous()
-    q = _aligned(q, 32)
-    y = torch.empty(n, h * d, dtype=q.dtype, device=q.device)
+    q, at = _rows_on(q, 32)
+    y = torch.empty_like(q)
     if n:
         if longest is None:
             longest = -(-n // b)
         with L.device(dev):
-            common = (q.data_ptr(), c[0].data_ptr(), c[1].data_ptr(), c[0].shape[0], table.data_ptr(), max(table.stride(0), m), starts.data_ptr(), pos.data_ptr(),
-                      0 if doc_start is None else doc_start.data_ptr(), y.data_ptr(), b, n, m, h, d, page.bit_length() - 1, scale, window // 128)
-            if longest > FEW or b > MOST_FEW:
-                slots = part_slots(n, m * page, h, window, dev)
-                ints = torch.empty(3 * b + 16, dtype=torch.int32, device=q.device)
-                parts = torch.empty(slots * 128 * (d + 1), dtype=torch.float32, device=q.device) if slots else None
-                L.call("bones_paged_pieces", *common, ints.data_ptr(), 0 if parts is None else parts.data_ptr(), slots, L.raw_stream(), launches=3 if slots else 2)
-            else:
-                work = torch.empty(rows_work(b, d, dev), dtype=torch.uint8, device=q.device)
-                L.call("bones_paged_rows", *common, work.data_ptr(), L.raw_stream(), launches=2)
+            room = _room(b, n, m * page, h, d, window // 128, longest > FEW, dev)
+            work = torch.empty(room, dtype=torch.uint8, device=q.device)
+            L.call("bones_paged_attention", at, k.data_ptr(), v.data_ptr(), k.shape[0], table.data_ptr(), table.stride(0) if b > 1 else m, starts.data_ptr(),
+                   pos.data_ptr(), 0 if doc_start is None else doc_start.data_ptr(), y.data_ptr(), b, n, m, h, d, page.bit_length() - 1, scale, window // 128,
+                   longest > FEW, work.data_ptr(), room, L.raw_stream(), launches=2)
         COUNTS["paged_attention"] += 1
     return y
 
 
-@functools.lru_cache(maxsize=None)
-def _sms(dev: int) -> int:
-    return torch.cuda.get_device_properties(dev).multi_processor_count
-
-
-def rows_work(b, d, dev):
-    """Bytes that ``bones_paged_rows`` works with."""
-    return L.load().bones_paged_rows_ctas(d, _sms(dev)) * 8 * 16 * (d + 4) * 4 + 12 * b + 16
-
-
-def part_slots(n, capacity, h, window, dev):
-    """Places for parts of a tile of 128 queries: four an SM, none where the tiles alone are two an SM or see a few tiles of keys at most."""
-    seen = min(capacity, window + 128) if window else capacity
-    return 4 * _sms(dev) if seen > 768 and n // 128 * h < 2 * _sms(dev) else 0
+@functools.lru_cache(maxsize=4096)
+def _room(b, n, capacity, h, d, window_tiles, long, dev) -> int:
+    """Bytes that ``bones_paged_attention`` works with."""
+    return L.load().bones_paged_room(b, n, capacity, h, d, window_tiles, long, torch.cuda.get_device_properties(dev).multi_processor_count)
