@@ -84,6 +84,8 @@ __global__ void __launch_bounds__(AT, 3) paged_append_kernel(const __nv_bfloat16
     }
   };
   int item = threadIdx.x / LANES;
+  pdl_wait();
+  pdl_launch();
   load(item);                                // on its way while the rows are looked up
   for (int r = warp; r < rows && row0 + r < p.N; r += AT / 32) {
     const int b = paged_owner(p.starts, p.B, row0 + r);
@@ -267,7 +269,8 @@ __global__ void __launch_bounds__(32 * RW, D == 128 ? 3 : 4) paged_rows_kernel(c
   __shared__ int first_of[RB];
   __shared__ Piece piece_of[RB];
   __shared__ uint4 qs_all[RW][KC * 4 * 32];        // a warp's queries: the A operand's registers, lane by lane
-  pdl_launch();
+  pdl_wait();
+  pdl_launch();                              // (the join reads the pieces ahead of its own wait: they are there behind this one's)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const long long A = (long long)p.p.H * D;
   const int mask = (1 << p.p.shift) - 1;
@@ -502,6 +505,7 @@ __global__ void __launch_bounds__(256) paged_rows_join_kernel(const RowsArgs p) 
   const int i = row - s.row, tile = i / RT;
   const bool live = on && s.live && i >= 0 && i < s.live;
   pdl_wait();
+  pdl_launch();
   bool written = !on;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;
@@ -555,18 +559,19 @@ static int rows_ctas(int D, int sms) { return (D == 128 ? 3 : 4) * sms; }
 template <int D>
 static int launch_rows(RowsArgs& p, int ctas, cudaStream_t s) {
   p.warps = ctas * RW;
-  paged_rows_kernel<D><<<(unsigned)ctas, 32 * RW, 0, s>>>(p);
-  BONES_CHECK(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(32 * RW);
+  cfg.stream = s;
+  cfg.attrs = at;
+  cfg.numAttrs = (unsigned)dec_launch_attrs(at, 1, 1);
+  BONES_CHECK(cudaLaunchKernelEx(&cfg, paged_rows_kernel<D>, (const RowsArgs&)p));
   const long long pairs = (long long)p.p.N * p.p.H;
   const bool few = pairs <= 8 * ctas;
   const int a_cta = 256 / (D / 4 * (few ? 8 : 1));
   cfg.gridDim = dim3((unsigned)((pairs + a_cta - 1) / a_cta));
   cfg.blockDim = dim3(256);
-  cfg.stream = s;
-  cfg.attrs = at;
-  cfg.numAttrs = (unsigned)dec_launch_attrs(at, 1, 1);
   return (int)(few ? cudaLaunchKernelEx(&cfg, paged_rows_join_kernel<D, 8>, p) : cudaLaunchKernelEx(&cfg, paged_rows_join_kernel<D, 1>, p));
 }
 
@@ -592,9 +597,15 @@ int bones_paged_append(const void* qkv, long long ldq, const float* cosT, const 
   const auto* x = (const __nv_bfloat16*)qkv;
   auto *kc = (__nv_bfloat16*)k, *vc = (__nv_bfloat16*)v, *out = (__nv_bfloat16*)q;
   cudaStream_t s = (cudaStream_t)stream;
-  if (D == 128) paged_append_kernel<128><<<grid, AT, 0, s>>>(x, ldq, cosT, sinT, rope_rows, rows, p, kc, vc, out);
-  else paged_append_kernel<64><<<grid, AT, 0, s>>>(x, ldq, cosT, sinT, rope_rows, rows, p, kc, vc, out);
-  return (int)cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[2];
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(AT);
+  cfg.stream = s;
+  cfg.attrs = at;
+  cfg.numAttrs = (unsigned)dec_launch_attrs(at, 1, 1);
+  return (int)(D == 128 ? cudaLaunchKernelEx(&cfg, paged_append_kernel<128>, x, ldq, cosT, sinT, rope_rows, rows, p, kc, vc, out)
+                        : cudaLaunchKernelEx(&cfg, paged_append_kernel<64>, x, ldq, cosT, sinT, rope_rows, rows, p, kc, vc, out));
 }
 
 // q, y: bf16 [N, H * D]; doc_start: int32 [N] or null; window_tiles: of 128 tokens, 0 for all; tall: by tiles of 128 rows (pieces of more than a few tokens),

@@ -32,9 +32,19 @@ struct PiecesArgs {
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int PLAN_T = 256;
 
-__device__ __forceinline__ int plan_tiles(const PiecesArgs& a, const Piece& s) {       // key tiles of the longest row of tiles
-  const int last = (s.pos + s.live - 1) >> 7;
+constexpr int PIECE_WAY = 2;                     // tiles of keys that a tile of queries' way in and out counts for
+constexpr int PIECE_LEAST = 4;                   // tiles of keys that are worth a part
+constexpr int PIECE_JOIN = 6;                    // tiles of keys that the join takes as long as
+
+// Tiles of keys of a piece's tile of queries, documents apart, and of all in front of one, with their ways
+__device__ __forceinline__ int plan_tiles(const PiecesArgs& a, const Piece& s, int qt) {
+  const int last = (s.pos + min(s.live, (qt + 1) * PT) - 1) >> 7;
   return a.window_tiles > 0 ? min(last + 1, a.window_tiles + 1) : last + 1;
+}
+__device__ __forceinline__ long long plan_front(const PiecesArgs& a, const Piece& s, int qt) {
+  long long n = 0;
+  for (int i = 0; i < qt; ++i) n += plan_tiles(a, s, i) + PIECE_WAY;
+  return n;
 }
 // Sums of `v` over the threads in front; the total in *all.
 __device__ __forceinline__ long long plan_scan(long long v, long long* box, long long* all) {
@@ -59,12 +69,11 @@ __device__ __forceinline__ long long plan_scan(long long v, long long* box, long
   return before + up - v;
 }
 
-constexpr int PIECE_WAY = 2;                     // tiles of keys that a tile of queries' way in and out counts for
-constexpr int PIECE_LEAST = 4;                   // tiles of keys that are worth a part
-
 __global__ void __launch_bounds__(PLAN_T) paged_plan_kernel(const PiecesArgs a) {
   __shared__ long long box[PLAN_T / 32];
+  __shared__ int longest;
   const Paged& p = a.p;
+  pdl_wait();
   pdl_launch();
   if (blockIdx.x > 0) {                          // rows without a result: outside all pieces, or left out
     const int lane = threadIdx.x & 31;
@@ -79,18 +88,22 @@ __global__ void __launch_bounds__(PLAN_T) paged_plan_kernel(const PiecesArgs a) 
     return;
   }
   long long tiles = 0, total = 0;
+  if (threadIdx.x == 0) longest = 0;
+  __syncthreads();
   for (int b0 = 0; b0 < p.B; b0 += PLAN_T) {
     const int b = b0 + threadIdx.x;
     long long rows = 0, n = 0;
     if (b < p.B) {
       const Piece x = paged_piece(p, b);
       if (x.live) {
-        rows = (long long)((x.live + PT - 1) / PT) * p.H;
-        n = plan_tiles(a, x) + PIECE_WAY;
+        rows = (x.live + PT - 1) / PT;
+        n = a.slots > 0 ? plan_front(a, x, (int)rows) * p.H : 0;
+        if (a.slots > 0) atomicMax(&longest, plan_tiles(a, x, (int)rows - 1) + PIECE_WAY);
+        rows *= p.H;
       }
     }
     long long more, all;
-    const long long at = tiles + plan_scan(rows, box, &more), in_front = total + plan_scan(rows * n, box, &all);
+    const long long at = tiles + plan_scan(rows, box, &more), in_front = total + plan_scan(n, box, &all);
     if (b < p.B) {
       a.tiles[b] = (int)at;
       a.before[b] = in_front;
@@ -102,7 +115,9 @@ __global__ void __launch_bounds__(PLAN_T) paged_plan_kernel(const PiecesArgs a) 
     *a.next = 0;
     a.tiles[p.B] = (int)tiles;
     a.before[p.B] = total;
-    a.before[p.B + 1] = a.slots > 0 && tiles < 2 * a.sms ? max((total + a.sms - 1) / a.sms, (long long)PIECE_WAY + PIECE_LEAST) : 0;
+    // drawn, the CTAs are done when the longest tile of queries is, or half of one behind the mean
+    const long long mean = (total + a.sms - 1) / a.sms, drawn = max((long long)longest, mean + longest / 2), shared = max(mean, (long long)PIECE_WAY + PIECE_LEAST);
+    a.before[p.B + 1] = a.slots > 0 && tiles < 2 * a.sms && shared + PIECE_JOIN < drawn ? shared : 0;
   }
 }
 
@@ -115,10 +130,11 @@ __global__ void __launch_bounds__(PLAN_T) paged_plan_kernel(const PiecesArgs a) 
 //  - pages: a box of the tensor map is one page's P tokens of one head; a position without a page is loaded as zeros and masked.
 //  - rows behind a piece's end (a step with a few drafts has 5 of 128) take no exponentials: a softmax warp without a live row passes its tiles on.
 //  - values that a row does not see may be anything (other sequences' leftovers behind the end): tiles with a mask are looked through before V's
-//    product, by the warp that loaded them, zeros are put for what is not finite, and it is added back to the rows that do see it at the end.
+//    product by two warps, zeros are put for what is not finite, and it is added back to the rows that do see it at the end.  (By the drain warps they waited for an
+//    item's output, by the loading warp for its loads: 31 us for 26 of the banded case of short pieces.)
 constexpr int PP_SW = 16, PP_DW = 4;
-constexpr int PP_PV = 2 + PP_SW + PP_DW, PP_VW = PP_PV + 1, PP_IW = PP_VW + 1;
-constexpr int PP_THREADS = 32 * (PP_IW + 1);
+constexpr int PP_PV = 2 + PP_SW + PP_DW, PP_VW = PP_PV + 1, PP_IW = PP_VW + 1, PP_LW = PP_IW + 1, PP_LOOK = 2;
+constexpr int PP_THREADS = 32 * (PP_LW + PP_LOOK);
 constexpr int PP_RING = 2;                      // items handed round: the one being computed and the next (three: the same times)
 constexpr uint32_t PP_BARS = 512;               // barriers, TMEM address, abort flag, items
 
@@ -141,6 +157,7 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   extern __shared__ __align__(1024) uint8_t gen[];
   const uint32_t base = smem_u32(gen);
   if (base & 1023u) {                           // the swizzled tiles want it
+    pdl_wait();
     if (threadIdx.x == 0) atomicCAS(a.err, 0, ERR_WAIT_AUX);
     return;
   }
@@ -175,8 +192,8 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   const int A = p.H * D;
   if (warp == 0) {
     for (int i = lane; i < 36; i += 32) {
-      const bool by_softmax = (i >= 23 && i < 26) || i == 34, by_drain = (i >= 29 && i < 32) || i == 33 || i == 35;
-      mbar_init(bars + 8u * (uint32_t)i, by_softmax ? PP_SW : by_drain ? PP_DW : 1);
+      const bool by_softmax = (i >= 23 && i < 26) || i == 34, by_drain = (i >= 29 && i < 32) || i == 33 || i == 35, by_look = i >= 14 && i < 17;
+      mbar_init(bars + 8u * (uint32_t)i, by_softmax ? PP_SW : by_drain ? PP_DW : by_look ? PP_LOOK : 1);
     }
     if (lane == 0) *abort_flag = 0;
     fence_barrier_init();
@@ -188,8 +205,8 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = (uint32_t)warp_uniform((int)*tmem_slot_g);
-  pdl_launch();
   pdl_wait();                                   // the plan
+  pdl_launch();                                 // (the join reads it ahead of its own wait)
   auto tS = [&](int s) { return tmem + (uint32_t)s * 128u; };
   const uint32_t tO = tmem + 384u;
   // the it-th item of this CTA; false behind the last one
@@ -225,12 +242,18 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       if (share) {
         while (at < stop && to_v <= from_v) {
           b = min(max(paged_owner(a.before, p.B, at), 0), p.B - 1);
-          all_v = plan_tiles(a, paged_piece(p, b));
-          const int per = all_v + PIECE_WAY;
-          const long long in_seq = at - a.before[b];
-          g = (int)(in_seq / per);
-          const int off = (int)(in_seq % per), take = (int)min((long long)(per - off), stop - at);
+          const Piece s = paged_piece(p, b);
+          const int rows = (s.live + PT - 1) / PT;
+          const long long head = plan_front(a, s, rows), in_seq = at - a.before[b];
+          int off = (int)(in_seq % head), qt = 0;
+          all_v = plan_tiles(a, s, 0);
+          while (off >= all_v + PIECE_WAY) {
+            off -= all_v + PIECE_WAY;
+            all_v = plan_tiles(a, s, ++qt);
+          }
+          const int take = (int)min((long long)(all_v + PIECE_WAY - off), stop - at);
           at += take;
+          g = (int)(in_seq / head) * rows + qt;
           from_v = max(off - PIECE_WAY, 0);
           to_v = off + take - PIECE_WAY;
         }
@@ -249,7 +272,7 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         const int rows = (s.live + PT - 1) / PT;
         im.seq = b;
         im.h = g / rows;
-        const int qt = rows - 1 - (g % rows + im.h) % rows;
+        const int qt = share ? g % rows : rows - 1 - (g % rows + im.h) % rows;       // drawn: turned from head to head, so that CTAs see a mix of lengths
         im.row0 = s.row + qt * PT;
         im.live = min(PT, s.live - qt * PT);
         im.pos0 = s.pos + qt * PT;
@@ -317,58 +340,13 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       }
     }
   } else if (warp == PP_VW) {
-    // V loads; behind each, the tile before it is looked through where some row sees only some of its keys
+    // V loads
     PieceItem im;
     int g = 0, vs = 0;
     uint32_t vph = 1;
     bool dead = false;
-    auto look = [&](int stage, uint32_t parity, int it, int kt) {
-      if (!__all_sync(0xffffffffu, mbar_wait(v_full(stage), parity, abort_flag, a.err, ERR_WAIT_FULL))) return false;
-      uint4* tile = reinterpret_cast<uint4*>(gen + TILE * (4 + stage)) + lane;
-      // the largest magnitude of each half: an infinity is larger than the finite, a NaN stays
-      __nv_bfloat162 most[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) most[k] = __float2bfloat162_rn(0.f);
-#pragma unroll 8
-      for (int i = 0; i < (int)(TILE / 512); ++i) {
-        const uint4 u = tile[i * 32];
-        const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&u);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) most[k] = __hmax2_nan(most[k], __habs2(x[k]));
-      }
-#pragma unroll
-      for (int k = 1; k < 4; ++k) most[0] = __hmax2_nan(most[0], most[k]);
-      const uint32_t top = *reinterpret_cast<const uint32_t*>(&most[0]);
-      if (__any_sync(0xffffffffu, (top & 0x7f80u) == 0x7f80u || (top & 0x7f800000u) == 0x7f800000u)) {
-        bool seen = false;
-        for (int i = 0; i < (int)(TILE / 512); ++i) {
-          const uint4 u = tile[i * 32];
-          uint32_t w[4] = {u.x, u.y, u.z, u.w};
-          bool any = false;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t t = ((w[k] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-            if (t) any = true;
-            if (t & 0x8000u) w[k] &= 0xffff0000u;
-            if (t & 0x80000000u) w[k] &= 0xffffu;
-          }
-          if (any) {
-            tile[i * 32] = make_uint4(w[0], w[1], w[2], w[3]);
-            if (kt * PT + (((lane + i * 32) * 16 >> 7) & (PT - 1)) < im.pos0 + im.live) seen = true;        // not a leftover behind the end
-          }
-        }
-        if (__any_sync(0xffffffffu, seen) && lane == 0) atomicOr(&taint[it % PP_RING], 1);
-        fence_proxy_async_smem();
-        __threadfence_block();
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(v_fine(stage));
-      return true;
-    };
     for (int it = 0; !dead && take(it, &im); ++it) {
       int row = page_row(im, im.kt0);
-      int last = -1;                                  // the stage of a tile that is still to be looked through, and its parity
-      uint32_t last_parity = 0;
       for (int j = 0; j < im.n; ++j, ++g) {
         const int now = row;
         if (j + 1 < im.n) row = page_row(im, im.kt0 + j + 1);
@@ -382,12 +360,64 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             for (int c = 0; c < D / 64; ++c) tma_load_2d(sV(vs) + c * PATOM + i * page_bytes, &tm_v, v_full(vs), c * 64, at);
           }
         }
-        if (last >= 0 && !look(last, last_parity, it, im.kt0 + j - 1)) dead = true;
-        last = masked(im, im.kt0 + j) ? vs : -1;
-        last_parity = vph ^ 1u;
         if (++vs == 3) { vs = 0; vph ^= 1u; }
       }
-      if (last >= 0 && !look(last, last_parity, it, im.kt0 + im.n - 1)) dead = true;
+    }
+  } else if (warp >= PP_LW) {
+    // Tiles of V in which some row sees only some of the keys are looked through, half by either warp.  Every tile is passed on from here, so that no
+    // phase of a stage goes by unseen (a wait tells apart two phases, not three).
+    const int half = warp - PP_LW;
+    PieceItem im;
+    int vs = 0;
+    uint32_t vph = 0;
+    bool ok = true;
+    for (int it = 0; ok && take(it, &im); ++it) {
+      for (int kt = im.kt0; kt < im.kt0 + im.n; ++kt) {
+        if (!__all_sync(0xffffffffu, mbar_wait(v_full(vs), vph, abort_flag, a.err, ERR_WAIT_FULL))) { ok = false; break; }
+        if (masked(im, kt)) {
+          constexpr int ROUNDS = (int)(TILE / 512 / PP_LOOK);
+          uint4* tile = reinterpret_cast<uint4*>(gen + TILE * (4 + vs)) + half * ROUNDS * 32 + lane;
+          // the largest magnitude of each half: an infinity is larger than the finite, a NaN stays
+          __nv_bfloat162 most[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) most[k] = __float2bfloat162_rn(0.f);
+#pragma unroll 8
+          for (int i = 0; i < ROUNDS; ++i) {
+            const uint4 u = tile[i * 32];
+            const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&u);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) most[k] = __hmax2_nan(most[k], __habs2(x[k]));
+          }
+#pragma unroll
+          for (int k = 1; k < 4; ++k) most[0] = __hmax2_nan(most[0], most[k]);
+          const uint32_t top = *reinterpret_cast<const uint32_t*>(&most[0]);
+          if (__any_sync(0xffffffffu, (top & 0x7f80u) == 0x7f80u || (top & 0x7f800000u) == 0x7f800000u)) {
+            bool seen = false;
+            for (int i = 0; i < ROUNDS; ++i) {
+              const uint4 u = tile[i * 32];
+              uint32_t w[4] = {u.x, u.y, u.z, u.w};
+              bool any = false;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const bool low = (w[k] & 0x7f80u) == 0x7f80u, high = (w[k] & 0x7f800000u) == 0x7f800000u;
+                any = any || low || high;
+                if (low) w[k] &= 0xffff0000u;
+                if (high) w[k] &= 0xffffu;
+              }
+              if (any) {
+                tile[i * 32] = make_uint4(w[0], w[1], w[2], w[3]);
+                if (kt * PT + (((half * ROUNDS * 32 + lane + i * 32) * 16 >> 7) & (PT - 1)) < im.pos0 + im.live) seen = true;        // not a leftover behind the end
+              }
+            }
+            if (__any_sync(0xffffffffu, seen) && lane == 0) atomicOr(&taint[it % PP_RING], 1);
+            fence_proxy_async_smem();
+            __threadfence_block();
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_fine(vs));
+        if (++vs == 3) { vs = 0; vph ^= 1u; }
+      }
     }
   } else if (warp == 1) {
     // S = Q K^T of each tile, into the buffer whose O += P V (three tiles before) is done
@@ -428,15 +458,11 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     PieceItem im;
     bool dead = false;
     int ps = 0;                              // P buffer and V stage
-    uint32_t pph = 0, fine = 0;              // parity of either; of each stage's looked-through uses
+    uint32_t pph = 0;
     for (int it = 0; !dead && take(it, &im); ++it) {
       const int n = warp_uniform(im.n);
       for (int j = 0; j < n; ++j) {
-        if (!dead) dead = !mbar_wait(v_full(ps), pph, abort_flag, a.err, ERR_WAIT_FULL);
-        if (masked(im, im.kt0 + j)) {
-          if (!dead) dead = !mbar_wait(v_fine(ps), (fine >> ps) & 1, abort_flag, a.err, ERR_WAIT_AUX);
-          fine ^= 1u << ps;
-        }
+        if (!dead) dead = !mbar_wait(v_fine(ps), pph, abort_flag, a.err, ERR_WAIT_FULL);
         if (j == 0 && it >= 1 && !dead) dead = !mbar_wait(o_free, (uint32_t)((it - 1) & 1), abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
         if (!dead) dead = !mbar_wait(p_full(ps), pph, abort_flag, a.err, ERR_WAIT_AUX);
         tc_fence_after();
@@ -603,34 +629,46 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   }
 }
 
-// Adds the parts of a tile in their order.  grid: (tiles of queries, D / 8), a thread four columns of a row.
+// Adds the parts of tiles of queries in their order: a CTA the four columns each of 128 rows, then the next that is its own.  (CTAs of 128 threads find room
+// beside the attention's, and have looked up what they need when that ends; where nothing is shared they leave at once.)
 template <int D>
-__global__ void __launch_bounds__(256) paged_pieces_join_kernel(const PiecesArgs a) {
-  pdl_wait();
+__global__ void __launch_bounds__(PT) paged_pieces_join_kernel(const PiecesArgs a) {
   const Paged& p = a.p;
   const long long share = a.before[p.B + 1];
-  if (share == 0) return;
-  const int b = paged_owner(a.tiles, p.B, (int)blockIdx.x);
-  if (b < 0 || b >= p.B) return;
-  const Piece s = paged_piece(p, b);
-  const int g = blockIdx.x - a.tiles[b], n = plan_tiles(a, s);
-  const long long from = a.before[b] + (long long)g * (n + PIECE_WAY) + PIECE_WAY;
-  const int w0 = (int)(from / share), splits = (int)((from + n - 1) / share) - w0 + 1;
-  if (splits == 1) return;
-  const int rows = (s.live + PT - 1) / PT, h = g / rows, qt = rows - 1 - (g % rows + h) % rows, r = threadIdx.x % PT, c = blockIdx.y * 8 + threadIdx.x / PT * 4;
-  if (qt * PT + r >= s.live) return;
-  // the first CTA's second place, the others' first
-  const float* part = a.parts + (2ll * w0 * D + c) * PT + r;
-  const float* sum = a.parts + (long long)a.slots * PT * D + 2ll * w0 * PT + r;
-  float x[4] = {}, l = 0.f;
+  const int items = share ? a.tiles[p.B] * (D / 4) : 0, r = threadIdx.x;
+  bool waited = false;
+  for (int item = blockIdx.x; item < items || !waited; item += gridDim.x) {
+    int splits = 0, w0 = 0, h = 0, row = -1;
+    const int tile = item / (D / 4), c = item % (D / 4) * 4;
+    const int b = item < items ? paged_owner(a.tiles, p.B, tile) : -1;
+    if (b >= 0 && b < p.B) {
+      const Piece s = paged_piece(p, b);
+      const int rows = (s.live + PT - 1) / PT, g = tile - a.tiles[b], qt = g % rows;
+      const long long from = a.before[b] + (g / rows) * plan_front(a, s, rows) + plan_front(a, s, qt) + PIECE_WAY;
+      h = g / rows;
+      w0 = (int)(from / share);
+      splits = (int)((from + plan_tiles(a, s, qt) - 1) / share) - w0 + 1;
+      if (qt * PT + r < s.live) row = s.row + qt * PT + r;
+    }
+    if (!waited) {
+      pdl_wait();                                 // (by every CTA: who comes behind this kernel waits for its end alone)
+      pdl_launch();
+      waited = true;
+    }
+    if (splits < 2 || row < 0) continue;
+    // the first CTA's second place, the others' first
+    const float* part = a.parts + (2ll * w0 * D + c) * PT + r;
+    const float* sum = a.parts + (long long)a.slots * PT * D + 2ll * w0 * PT + r;
+    float x[4] = {}, l = 0.f;
 #pragma unroll 4
-  for (int k = 0; k < splits; ++k) {
+    for (int k = 0; k < splits; ++k) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] += part[((2ll * k + (k == 0)) * D + i) * PT];
-    l += sum[(2ll * k + (k == 0)) * PT];
+      for (int i = 0; i < 4; ++i) x[i] += part[((2ll * k + (k == 0)) * D + i) * PT];
+      l += sum[(2ll * k + (k == 0)) * PT];
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    *reinterpret_cast<uint2*>(a.y + ((long long)row * p.H + h) * D + c) = make_uint2(pack_bf16(x[0] * inv, x[1] * inv), pack_bf16(x[2] * inv, x[3] * inv));
   }
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
-  *reinterpret_cast<uint2*>(a.y + ((long long)(s.row + qt * PT + r) * p.H + h) * D + c) = make_uint2(pack_bf16(x[0] * inv, x[1] * inv), pack_bf16(x[2] * inv, x[3] * inv));
 }
 
 static int tmap_rows_2d(CUtensorMap* out, const void* ptr, long long rows, long long cols, int box_rows) {
@@ -646,22 +684,23 @@ static int launch_pieces(const CUtensorMap& tq, const CUtensorMap& tk, const CUt
   static OncePerDevice limit;
   BONES_ONCE(limit, { BONES_CHECK(cudaFuncSetAttribute(paged_pieces_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); });
   const Paged& p = a.p;
-  paged_plan_kernel<<<1 + (unsigned)min((p.N + 31ll) / 32, (long long)a.sms), PLAN_T, 0, s>>>(a);
-  BONES_CHECK(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
+  cfg.gridDim = dim3(1 + (unsigned)min((p.N + 31ll) / 32, (long long)a.sms));
+  cfg.blockDim = dim3(PLAN_T);
+  cfg.stream = s;
+  cfg.attrs = at;
+  cfg.numAttrs = (unsigned)dec_launch_attrs(at, 1, 1);
+  BONES_CHECK(cudaLaunchKernelEx(&cfg, paged_plan_kernel, a));
   // a CTA an SM, fewer where the items cannot be as many
   const long long tiles = (p.N / PT + (long long)min(p.B, p.N)) * p.H;
   cfg.gridDim = dim3((unsigned)(a.slots ? a.sms : min(tiles, (long long)a.sms)));
   cfg.blockDim = dim3(PP_THREADS);
   cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cfg.attrs = at;
-  cfg.numAttrs = (unsigned)dec_launch_attrs(at, 1, 1);
   BONES_CHECK(cudaLaunchKernelEx(&cfg, paged_pieces_kernel<D>, tq, tk, tv, a));
   if (a.slots == 0) return 0;
-  cfg.gridDim = dim3((unsigned)tiles, D / 8);
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3((unsigned)min(tiles * (D / 4), 12ll * a.sms));
+  cfg.blockDim = dim3(PT);
   cfg.dynamicSmemBytes = 0;
   return (int)cudaLaunchKernelEx(&cfg, paged_pieces_join_kernel<D>, a);
 }

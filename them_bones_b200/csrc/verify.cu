@@ -92,6 +92,7 @@ __device__ __forceinline__ void row_step(RowRun& r, const float* f, int at, floa
 template <typename E, bool GREEDY>
 __global__ void verify_stats_kernel(const VerifyArgs p) {
   const int row = blockIdx.x, model = blockIdx.y;
+  pdl_wait();
   pdl_launch();
   const int seq = paged_owner(p.starts, p.B, row);
   if (seq < 0 || seq >= p.B || (model && row + 1 >= p.starts[seq + 1])) return;      // no sequence's, or nothing was drawn from it
@@ -390,6 +391,7 @@ __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT, 4) verify_draw_
   };
   Draft next = draft_behind(a + lane);
   pdl_wait();
+  pdl_launch();
   __syncthreads();
   if (a == e) {
     if (writer) {
@@ -571,16 +573,18 @@ static int launch_verify(const VerifyArgs& p, cudaStream_t s) {
   const dim3 grid((unsigned)p.N, p.q ? 2 : 1);
   // few rows: many threads for each, so that all of a row is on its way at once
   const unsigned threads = (long long)p.N * grid.y <= 296 ? 1024 : (long long)p.N * grid.y <= 592 ? 512 : 256;
-  if (p.N) {
-    if (p.T == 0.0) verify_stats_kernel<E, true><<<grid, threads, 0, s>>>(p);
-    else verify_stats_kernel<E, false><<<grid, threads, 0, s>>>(p);
-    BONES_CHECK(cudaGetLastError());
-  }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
   cfg.stream = s;
   cfg.attrs = at;
-  cfg.numAttrs = (unsigned)dec_launch_attrs(at, 1, p.N > 0);        // (without a first kernel, what comes before is not the one that it may overlap)
+  cfg.numAttrs = (unsigned)dec_launch_attrs(at, 1, 1);
+  if (p.N) {
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    BONES_CHECK(p.T == 0.0 ? cudaLaunchKernelEx(&cfg, verify_stats_kernel<E, true>, p) : cudaLaunchKernelEx(&cfg, verify_stats_kernel<E, false>, p));
+  } else {
+    cfg.numAttrs = 0;                            // without a first kernel, what comes before is not what the second may begin beside
+  }
   if (p.T == 0.0) {
     cfg.gridDim = dim3((unsigned)((p.B + 3) / 4));
     cfg.blockDim = dim3(128);
