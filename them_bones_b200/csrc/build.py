@@ -1,7 +1,8 @@
 """Builds the native library ``them_bones_b200/lib/libbones_b200.so`` for sm_100a with nvcc.
 
 Each ``.cu`` file is compiled to an object (in parallel, only when it or a header changed) and the objects are linked
-into one shared library that ``ops._lib`` loads with ctypes.  nvcc cross-compiles without a GPU.
+into one shared library that ``ops._lib`` loads with ctypes.  nvcc cross-compiles without a GPU.  Beside it ``lib/bones_calls.so``, a Python module of a few
+calls into that library (``calls.cpp``).
 """
 from __future__ import annotations
 
@@ -20,6 +21,27 @@ FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std
 
 def _newer(a, b):
     return not os.path.exists(b) or os.path.getmtime(a) > os.path.getmtime(b)
+
+
+CALLS = os.path.join(LIB_DIR, "bones_calls.so")       # a Python module: calls of few microseconds without the way through ctypes
+
+
+def build_calls(force: bool = False) -> str:
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension as ext
+    src = os.path.join(HERE, "calls.cpp")
+    if not force and not _newer(src, CALLS):
+        return CALLS
+    inc = [f"-I{d}" for d in (*ext.include_paths(), os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include"), sysconfig.get_paths()["include"])]
+    lib = [f"-L{d}" for d in ext.library_paths()] + [f"-l{n}" for n in ("torch_python", "torch", "torch_cpu", "torch_cuda", "c10", "c10_cuda")]
+    r = subprocess.run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, src,
+                        "-o", CALLS, *lib], capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError("the calls module does not compile")
+    return CALLS
 
 
 LIB_DEBUG = os.path.join(LIB_DIR, "libbones_b200_dbg.so")
@@ -64,6 +86,7 @@ def build(verbose: bool = False, force: bool = False, debug_bounds: bool = False
                 sys.stderr.write(log)
     if failed:
         raise RuntimeError("nvcc failed")
+    build_calls(force)
     objs = [os.path.join(objdir, s[:-3] + ".o") for s in srcs]
     if jobs or not os.path.exists(lib):
         r = subprocess.run([NVCC, "-shared", "-o", lib, *objs, "-lcudart"], capture_output=True, text=True)

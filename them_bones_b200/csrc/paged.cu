@@ -632,8 +632,10 @@ int bones_paged_attention(const void* q, const void* k, const void* v, int pages
   return D == 128 ? launch_rows<128>(a, ctas, (cudaStream_t)stream) : launch_rows<64>(a, ctas, (cudaStream_t)stream);
 }
 
-// Bytes of bones_paged_attention's `work` on a device of `sms` SMs, for caches of `cap` tokens a sequence.
+// Bytes of bones_paged_attention's `work` on a device of `sms` SMs (0: the current one; below 0: an error), for caches of `cap` tokens a sequence.
 long long bones_paged_room(int B, int N, int cap, int H, int D, int window_tiles, int tall, int sms) {
+  int dev = 0;
+  if (sms <= 0 && (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)) return -1;
   if (tall || B > RB) return paged_pieces_room(B, N, cap, H, D, window_tiles, sms);
   return (long long)rows_ctas(D, sms) * RW * 2 * RT * (D + 4) * 4 + 12ll * B + 16;
 }

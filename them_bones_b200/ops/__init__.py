@@ -280,6 +280,10 @@ def paged_append(qkv, cos, sin, cache, table, starts, pos):
     their queries: the tokens of a sequence at a negative position, those past the table or the rotary tables, and rows outside all
     pieces.  A token whose page is not one of the cache's (as -1) is not stored.  No page may be written by two sequences.  No gradient:
     tensors that ask for one, and dual tensors, are refused."""
+    if native(qkv):
+        q = _paged.short_append(qkv, cos, sin, cache, table, starts, pos)
+        if q is not None:
+            return q
     dims = _paged.check_append(qkv, cos, sin, cache, table, starts, pos)
     _paged.no_gradient(qkv)
     if native(qkv):
@@ -294,6 +298,10 @@ def paged_attention(q, cache, table, starts, pos, scale, doc_start=None, window=
     longest piece as far as the host knows (default: the mean); it picks a kernel, not the result.  Tokens that were left out, rows outside all pieces and
     queries that see no key get zeros.  Queries and keys are behind the norm (``|q . k|`` about D at most): natively the soft-max has a
     fixed shift, and ``|scale| * D`` up to 32.  No gradient."""
+    if native(q):
+        y = _paged.short_attention(q, cache, table, starts, pos, scale, doc_start, window, longest)
+        if y is not None:
+            return y
     dims = _paged.check_attention(q, cache, table, starts, pos, scale, doc_start, window, longest)
     _paged.no_gradient(q, *cache)
     if native(q):
@@ -313,6 +321,10 @@ def verify_drafts(logits, ids, starts, uniforms=None, draft_logits=None, tempera
     bits.  A draft outside the vocabulary falls; so does one whose draft row has no number (NaN, +inf or nothing but -inf), and the token is then drawn from p.
     A target row without a number ends a sequence with token -1, as does a sequence without rows.  No gradient."""
     vocab = logits.shape[-1] if vocab is None and logits.dim() else vocab
+    if native(logits):
+        out = _verify.short(logits, ids, starts, uniforms, draft_logits, temperature, vocab)
+        if out is not None:
+            return out
     _verify.check(logits, ids, starts, uniforms, draft_logits, temperature, vocab)
     if native(logits):
         return _verify.native(logits, ids, starts, uniforms, draft_logits, temperature, vocab)

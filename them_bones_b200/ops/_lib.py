@@ -63,6 +63,26 @@ def load():
     return _LIB
 
 
+_CALLS = None
+
+
+def calls():
+    """The module of short calls (``csrc/calls.cpp``), bound to the library's entry points."""
+    global _CALLS
+    if _CALLS is None:
+        import importlib.util
+        path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "lib", "bones_calls.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"native calls missing: {path}; run `python -m them_bones_b200.csrc.build` (or __graft_entry__.build()) first")
+        spec = importlib.util.spec_from_file_location("bones_calls", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        lib = load()
+        mod.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in ("bones_paged_append", "bones_paged_attention", "bones_paged_room", "bones_verify")))
+        _CALLS = mod
+    return _CALLS
+
+
 def available() -> bool:
     try:
         load()

@@ -99,6 +99,23 @@ def no_gradient(*xs):
 
 
 # -- native bodies -----------------------------------------------------------------------------------------------------
+def short_append(*args):
+    """The call by the short way (``csrc/calls.cpp``), or None where its tensors are not as the kernel wants them."""
+    q = L.calls().paged_append(*args)
+    if q is not None:
+        L.LAUNCHES[0] += 1
+        COUNTS["paged_append"] += 1
+    return q
+
+
+def short_attention(q, c, table, starts, pos, scale, doc_start, window, longest):
+    y = L.calls().paged_attention(q, c, table, starts, pos, scale, doc_start, window, longest, FEW, SHIFT)
+    if y is not None:
+        L.LAUNCHES[0] += 2
+        COUNTS["paged_attention"] += 1
+    return y
+
+
 def _rows_on(x, by):
     """``x [N, C]`` as the kernels read it, and its address: consecutive values, rows that begin on ``by`` bytes."""
     at = x.data_ptr()
@@ -152,4 +169,5 @@ def attention(dims, q, c, table, starts, pos, scale, doc_start, window, longest)
 @functools.lru_cache(maxsize=4096)
 def _room(b, n, capacity, h, d, window_tiles, long, dev) -> int:
     """Bytes that ``bones_paged_attention`` works with."""
-    return L.load().bones_paged_room(b, n, capacity, h, d, window_tiles, long, torch.cuda.get_device_properties(dev).multi_processor_count)
+    with L.device(dev):
+        return L.load().bones_paged_room(b, n, capacity, h, d, window_tiles, long, 0)

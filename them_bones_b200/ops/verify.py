@@ -45,6 +45,16 @@ def _rows(x):
     return x if x.stride(1) == 1 and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1]) else x.contiguous()
 
 
+def short(logits, ids, starts, uniforms, draft, temperature, vocab):
+    """The call by the short way (``csrc/calls.cpp``), or None where its tensors are not as the kernels want them."""
+    out = L.calls().verify_drafts(logits, ids, starts, uniforms, draft, temperature, vocab, COLDEST, WARMEST)
+    if out is None:
+        return None
+    L.LAUNCHES[0] += 2
+    COUNTS["verify_drafts"] += 1
+    return Verified(*out)
+
+
 def native(logits, ids, starts, uniforms, draft, temperature, vocab) -> Verified:
     if logits.dtype is not torch.bfloat16 and logits.dtype is not torch.float32:
         raise ValueError(f"native verify_drafts does not cover this call: logits of {logits.dtype} (bf16 and fp32)")
