@@ -117,6 +117,20 @@ def test_ties_go_to_the_lowest_index():
     assert got.accepted.tolist() == [2, 0] and got.token.tolist() == [0, 0]
 
 
+def test_rows_of_the_lowest_value_alone_and_lonely_numbers():
+    from them_bones_b200 import ops
+    for dtype in (torch.float32, torch.bfloat16):
+        low = torch.finfo(dtype).min
+        z = torch.full((4, 70001), float("-inf"), dtype=dtype)
+        z[0] = low
+        z[1, 69999], z[2, 3], z[2, 40000] = -2.0, 1.0, 1.5
+        u = torch.full((4, 2), 0.5)
+        for t in (0.0, 1.0):
+            want = ops.verify_drafts(z, torch.zeros(4, dtype=torch.int64), O.i32([0, 1, 2, 3, 4]), u, temperature=t)
+            got = ops.verify_drafts(z.cuda(), torch.zeros(4, dtype=torch.int64).cuda(), O.i32([0, 1, 2, 3, 4], "cuda"), u.cuda(), temperature=t)
+            assert got.token.tolist() == want.token.tolist() and want.token.tolist()[1:] == [69999, 40000, -1] and (t or want.token[0] == 0)
+
+
 def test_strided_and_unaligned_rows():
     from them_bones_b200 import ops
     z, ids, starts, u, q = _cuda(*problem([5, 4], 1000, 1000, torch.bfloat16, True))

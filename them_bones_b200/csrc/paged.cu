@@ -59,11 +59,12 @@ __device__ __forceinline__ void paged_unpack(const uint4* raw, float* a, float* 
 }
 
 // A CTA takes up to AR rows with all their heads, D / 16 lanes a head: a row's sequence, page and angles are looked up once a CTA, and no lane is left
-// over whatever the number of heads.  What a lane takes stays packed until it is worked on: 96 bytes on their way in 24 registers (unpacked, the kernel had room for
-// half the warps and ran at two thirds of the rate).
-constexpr int AT = 256, AR = 16;
+// over whatever the number of heads.  What a lane takes stays packed until it is worked on: 96 bytes on their way in 24 registers.  Bound by memory: 8 prompts of 2048
+// tokens, 10 heads of 128, 46.6 us (5.6 TB/s, 0.85 of the copy rate); a warp a row with unpacked values 57; this with 256 threads a CTA 48.4, with 8 / 16 rows of 128 / 256 threads
+// 50.4 / 52.2.
+constexpr int AT = 128, AR = 4;
 template <int D>
-__global__ void __launch_bounds__(AT, 3) paged_append_kernel(const __nv_bfloat16* __restrict__ qkv, long long ldq, const float* __restrict__ cosT,
+__global__ void __launch_bounds__(AT, 6) paged_append_kernel(const __nv_bfloat16* __restrict__ qkv, long long ldq, const float* __restrict__ cosT,
                                                              const float* __restrict__ sinT, int rope_rows, int rows, const Paged p, __nv_bfloat16* __restrict__ k,
                                                              __nv_bfloat16* __restrict__ v, __nv_bfloat16* __restrict__ q) {
   constexpr int LANES = D / 16, HALF = D / 2;

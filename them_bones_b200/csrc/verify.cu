@@ -26,7 +26,7 @@ struct VerifyArgs {
   const int* starts;
   const float* u;              // [N, 2]
   int B, N, V;
-  double T;
+  double T, inv, steps, reach;   // 1 / T, K / T, 2^30 T / K
   RowStat* stats;              // [N, 2]
   int* accepted;
   long long* token;
@@ -47,6 +47,12 @@ __device__ __forceinline__ void load_vec(const E* p, float* f) {
     const float4 a = *reinterpret_cast<const float4*>(p);
     f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
   }
+}
+// 16 bytes past the first-level cache, in the order of the program: left to itself the compiler waits for each load to save registers
+__device__ __forceinline__ uint4 load_ahead(const void* p) {
+  uint4 u;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
+  return u;
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -89,16 +95,19 @@ __device__ __forceinline__ void row_step(RowRun& r, const float* f, int at, floa
   }
 }
 
+// A CTA a row.  us of the whole call for 64 sequences, 448 rows of 65536 columns, with 256 / 512 / 1024 threads: 49.7 / 38.5 / 48.8; rows cut into four parts of 256 threads
+// each 41.9; two values an instruction the same.
+constexpr int VST = 512;
 template <typename E, bool GREEDY>
-__global__ void verify_stats_kernel(const VerifyArgs p) {
+__global__ void __launch_bounds__(VST, 4) verify_stats_kernel(const VerifyArgs p) {
   const int row = blockIdx.x, model = blockIdx.y;
   pdl_wait();
   pdl_launch();
   const int seq = paged_owner(p.starts, p.B, row);
   if (seq < 0 || seq >= p.B || (model && row + 1 >= p.starts[seq + 1])) return;      // no sequence's, or nothing was drawn from it
   const E* z = model ? (const E*)p.q + row * p.ldq : (const E*)p.z + row * p.ldz;
-  const float c = GREEDY ? 0.f : (float)(1.4426950408889634 / p.T);
-  RowRun r{-3.402823466e38f, 0.f, -1, false};
+  const float c = GREEDY ? 0.f : (float)(1.4426950408889634 * p.inv);
+  RowRun r{GREEDY ? -__int_as_float(0x7f800000) : -3.402823466e38f, 0.f, -1, false};
   constexpr int W = kVec<E>;
   // single values up to the first 16-byte boundary, vectors, single values
   const int head = min(p.V, (int)((16 - ((uintptr_t)z & 15)) & 15) / (int)sizeof(E)), vecs = (p.V - head) / W, tail = head + vecs * W;
@@ -106,20 +115,20 @@ __global__ void verify_stats_kernel(const VerifyArgs p) {
     const float f = logit(z + threadIdx.x);
     row_step<GREEDY, 1>(r, &f, threadIdx.x, c);
   }
-  constexpr int U = 8;                               // loads of a thread in flight
+  constexpr int U = 4;                               // loads of a thread in flight
   int i = threadIdx.x;
-  for (; i + (U - 1) * (int)blockDim.x < vecs; i += U * blockDim.x) {
+  for (; i + (U - 1) * VST < vecs; i += U * VST) {
     uint4 raw[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) raw[j] = *reinterpret_cast<const uint4*>(z + head + (long long)(i + j * blockDim.x) * W);
+    for (int j = 0; j < U; ++j) raw[j] = load_ahead(z + head + (long long)(i + j * VST) * W);
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       float f[W];
       load_vec(reinterpret_cast<const E*>(&raw[j]), f);
-      row_step<GREEDY, W>(r, f, head + (i + j * blockDim.x) * W, c);
+      row_step<GREEDY, W>(r, f, head + (i + j * VST) * W, c);
     }
   }
-  for (; i < vecs; i += blockDim.x) {
+  for (; i < vecs; i += VST) {
     float f[W];
     load_vec(z + head + (long long)i * W, f);
     row_step<GREEDY, W>(r, f, head + i * W, c);
@@ -132,7 +141,7 @@ __global__ void verify_stats_kernel(const VerifyArgs p) {
   __shared__ float sm[32];
   __shared__ double ss[32];
   __shared__ int si[32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = VST / 32;
   const float wm = warp_max(r.most);
   if (lane == 0) sm[warp] = wm;
   __syncthreads();
@@ -186,11 +195,14 @@ struct Law {
   double scale, offset;                                      // K / T, kMagic - S
   float least;
   const double* powers;                                      // at this lane's column
-  __device__ __forceinline__ Law(float most, double T, const double* powers_) : powers(powers_) {
-    // S stays below 2^49: there the next value of fp32 is 90000 T away from the largest, and any scale does
-    scale = fmin(0x1.71547652b82fep+8 / T, 0x1p49 / fmax(fabs((double)most), 1e-300));
+  // steps: K / T; reach: 2^30 steps
+  __device__ __forceinline__ Law(float most, double steps, double reach, const double* powers_) : scale(steps), powers(powers_) {
+    if (fabs((double)most) * steps > 0x1p49) {               // S stays below: there the next value of fp32 is 90000 T away from the largest, and any scale does
+      scale = 0x1p49 / fabs((double)most);
+      reach = 0x1p30 / scale;
+    }
     offset = kMagic - rint((double)most * scale);
-    least = (float)((double)most - 0x1p30 / scale);          // -inf where that leaves fp32: from there -inf itself, as 2^128, is as near
+    least = (float)((double)most - reach);                   // -inf where that leaves fp32: from there -inf itself, as 2^128, is as near
   }
   // W values side by side: one value's chain would leave the pipe idle
   template <int W>
@@ -418,7 +430,7 @@ __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT, 4) verify_draw_
       else if (next.is) {
         const RowStat sq = p.q ? p.stats[r * 2ll + 1] : RowStat{1.0, 0.f, 0};
         if (sq.sum > 0.0) {
-          const double px = exp(((double)next.p - st.most) / p.T) / st.sum, qx = p.q ? exp(((double)next.q - sq.most) / p.T) / sq.sum : 1.0, need = next.u * qx;
+          const double px = exp(((double)next.p - st.most) * p.inv) / st.sum, qx = p.q ? exp(((double)next.q - sq.most) * p.inv) / sq.sum : 1.0, need = next.u * qx;
           is = fabs(need - px) <= 1e-4 * (need + px) ? CLOSE : need < px ? STANDS : FALLS;
         }
       }
@@ -431,12 +443,12 @@ __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT, 4) verify_draw_
         const int rr = r0 + l;
         const float mp = p.stats[rr * 2ll].most, mq = p.q ? p.stats[rr * 2ll + 1].most : 0.f;
         const long long x = p.ids[rr + 1];
-        const Law lp(mp, p.T, powers), lq(mq, p.T, powers);
+        const Law lp(mp, p.steps, p.reach, powers), lq(mq, p.steps, p.reach, powers);
         const Sums both = share(p.q ? row_sums<E, true>(target(rr), draft(rr), lp, lq, 0.0, -1, cut, p.V, parts)
                                     : row_sums<E, false>(target(rr), nullptr, lp, lq, 0.0, -1, cut, p.V, parts), box);
         const double sum_p = warp_sum64(both.p), sum_q = warp_sum64(both.q);
-        const double px = exp(((double)logit(target(rr) + x) - mp) / p.T) * lp(mp) / sum_p;
-        const double qx = p.q ? exp(((double)logit(draft(rr) + x) - mq) / p.T) * lq(mq) / sum_q : 1.0;
+        const double px = exp(((double)logit(target(rr) + x) - mp) * p.inv) * lp(mp) / sum_p;
+        const double qx = p.q ? exp(((double)logit(draft(rr) + x) - mq) * p.inv) * lq(mq) / sum_q : 1.0;
         if (p.u[2ll * rr] * qx < px) {
           open &= open - 1;
           continue;
@@ -460,7 +472,7 @@ __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT, 4) verify_draw_
   const RowStat st = p.stats[row * 2ll], sq = refused && p.q ? p.stats[row * 2ll + 1] : RowStat{0.0, 0.f, 0};
   const E *z = target(row), *zq = sq.sum > 0.0 ? draft(row) : nullptr;
   const long long without = refused && !p.q ? p.ids[row + 1] : -1;
-  const Law lp(st.most, p.T, powers), lq(sq.most, p.T, powers);
+  const Law lp(st.most, p.steps, p.reach, powers), lq(sq.most, p.steps, p.reach, powers);
   // One pass for both laws' sums and those of the columns where p is above q, with the first kernel's 32-bit sums for the ratio of the scales: where that
   // errs about a column, p and q are the same to seven digits there.  The weights' sums follow with the ratio in 64 bits.
   const E* other = zq;
@@ -571,8 +583,6 @@ __global__ void __launch_bounds__(128) verify_greedy_kernel(const VerifyArgs p) 
 template <typename E>
 static int launch_verify(const VerifyArgs& p, cudaStream_t s) {
   const dim3 grid((unsigned)p.N, p.q ? 2 : 1);
-  // few rows: many threads for each, so that all of a row is on its way at once
-  const unsigned threads = (long long)p.N * grid.y <= 296 ? 1024 : (long long)p.N * grid.y <= 592 ? 512 : 256;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
   cfg.stream = s;
@@ -580,7 +590,7 @@ static int launch_verify(const VerifyArgs& p, cudaStream_t s) {
   cfg.numAttrs = (unsigned)dec_launch_attrs(at, 1, 1);
   if (p.N) {
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
+    cfg.blockDim = dim3(VST);
     BONES_CHECK(p.T == 0.0 ? cudaLaunchKernelEx(&cfg, verify_stats_kernel<E, true>, p) : cudaLaunchKernelEx(&cfg, verify_stats_kernel<E, false>, p));
   } else {
     cfg.numAttrs = 0;                            // without a first kernel, what comes before is not what the second may begin beside
@@ -610,7 +620,8 @@ int bones_verify(const void* z, long long ldz, const void* q, long long ldq, int
                  double T, double* stats, int* accepted, long long* token, void* stream) {
   if (!z || !ids || !starts || (!u && T != 0.0) || B < 1 || B > 65535 || N < 0 || V < 1 || !(T >= 0.0) || !stats || !accepted || !token || misaligned16(stats)) return -2;
   if (N && ((N > 1 && (ldz < V || (q && ldq < V))))) return -2;
-  const VerifyArgs p{z, T == 0.0 ? nullptr : q, ldz, ldq, ids, starts, u, B, N, V, T, (RowStat*)stats, accepted, token};
+  const double inv = T == 0.0 ? 0.0 : 1.0 / T, steps = 0x1.71547652b82fep+8 * inv;
+  const VerifyArgs p{z, T == 0.0 ? nullptr : q, ldz, ldq, ids, starts, u, B, N, V, T, inv, steps, 0x1p30 / steps, (RowStat*)stats, accepted, token};
   return f32 ? launch_verify<float>(p, (cudaStream_t)stream) : launch_verify<__nv_bfloat16>(p, (cudaStream_t)stream);
 }
 }  // extern "C"
