@@ -105,3 +105,24 @@ def test_dual_tensors_are_refused():
         a["qkv"] = fa.make_dual(torch.randn(7, 384), torch.randn(7, 384))
         with pytest.raises(ValueError):
             ops.paged_append(**a)
+
+
+@pytest.mark.parametrize("what", ["cos", "sin", "k", "v"])
+def test_tensors_that_ask_for_a_gradient_are_refused_wherever_they_come(what):
+    a = _ok()
+    if what in a:
+        a[what].requires_grad_()
+    else:
+        getattr(a["cache"], what).requires_grad_()
+    with pytest.raises(ValueError):
+        ops.paged_append(**a)
+    with torch.no_grad():
+        ops.paged_append(**a)
+
+
+def test_a_window_of_any_size():
+    c, table, starts, pos = O.world(2, 1, 64, 16, [3, 40], [200, 300])
+    q = O.queries(43, 1, 64)
+    want = ops.paged_attention(q, c, table, starts, pos, 0.1)
+    for window in (1 << 31, 1 << 45, 128 * ((1 << 32) + 1)):
+        assert torch.equal(ops.paged_attention(q, c, table, starts, pos, 0.1, window=window), want)

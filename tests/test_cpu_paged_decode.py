@@ -93,3 +93,10 @@ def test_generate_offers_it():
     for bad in (dict(kv="paged", logprobs=1), dict(temperature=1.0), dict(drafts=2)):
         with pytest.raises(ValueError):
             w.generate(prompts, 6, **bad)
+
+
+def test_tokens_outside_the_vocabulary_are_refused():
+    from them_bones_b200.utils import paged as P
+    for bad in ([[1, 97]], [[-1, 3]], torch.tensor([[5, 1 << 40]])):
+        with pytest.raises(ValueError):
+            P.paged_decode(_model(), bad, 2)

@@ -346,3 +346,90 @@ def test_a_run_of_pieces_is_the_training_attention():
             p += n
         # both round probabilities and results to bf16: 2^-8 of sums of |v| (up to 4 here at weights' sum 1) and of the result, each
         assert p == t and float((torch.cat(out).float() - want).abs().max()) <= 4 * O.HALF * 4
+
+
+@pytest.mark.parametrize("longest", [1, 4096])
+def test_windows_and_documents_beyond_all_positions(longest):
+    """Windows whose tokens or tiles leave 32 bits hide nothing, and neither does a document that began far in front of its sequence."""
+    from them_bones_b200 import ops
+    c, table, starts, pos = O.world(3, 2, 64, 16, [3, 40, 1], [200, 300, 0], "cuda")
+    q = O.queries(44, 2, 64, "cuda")
+    want = ops.paged_attention(q, c, table, starts, pos, 0.1, longest=longest)
+    for window in (1 << 31, 1 << 32, 128 * ((1 << 25) + 1), 1 << 37, 128 * ((1 << 32) + 1), 1 << 45):
+        assert torch.equal(ops.paged_attention(q, c, table, starts, pos, 0.1, None, window, longest), want), window
+    doc = O.i32([-2 ** 31, -2 ** 31 + 1, -1, 0] * 11, "cuda")
+    assert torch.equal(ops.paged_attention(q, c, table, starts, pos, 0.1, doc, 0, longest), want)
+
+
+@pytest.mark.parametrize("longest", [1, 4096])
+@pytest.mark.parametrize("window", [0, 256])
+def test_positions_next_to_the_last_of_32_bits(window, longest):
+    """A table of 2^31 - 128 positions of which the last three pages are there: as three pages at the start."""
+    from them_bones_b200 import ops
+    m = (1 << 24) - 1
+    c, near, starts, _ = O.world(1, 1, 64, 128, [20], [364], "cuda")
+    table = torch.full((1, m), -1, dtype=torch.int32, device="cuda")
+    table[0, -3:] = near[0, :3]
+    off = (m - 3) * 128
+    q = O.queries(20, 1, 64, "cuda")
+    doc = O.i32([off + 10 * i for i in range(20)], "cuda")
+    for at, ds in ((364, None), (300, doc)):
+        y, tol = O.attend(q, c, near, starts, O.i32([at], "cuda"), 0.1, None if ds is None else ds - off, window)
+        _close(ops.paged_attention(q, c, table, starts, O.i32([off + at], "cuda"), 0.1, ds, window, longest), y, tol)
+
+
+def test_calls_whose_turns_leave_32_bits_go_by_the_larger_tiles():
+    from them_bones_b200.ops import _lib as L
+    room = lambda n, cap, tall: L.load().bones_paged_room(1, n, cap, 1, 64, 0, tall, 148)  # noqa: E731
+    far = (1 << 31) - 128
+    assert room(15, far, 0) == room(15, 4096, 0) != room(15, far, 1)
+    assert room(1000, 1 << 20, 0) == room(1000, 4096, 0) and room(1000, far, 0) == room(1000, far, 1) != room(1000, 4096, 0)
+
+
+def test_the_short_way_and_the_long_one_are_one_operator():
+    """Calls that Python checks and launches give the bits of those that it does not; what the short way does not take it leaves alone."""
+    from them_bones_b200 import ops
+    from them_bones_b200.ops import paged as P
+    for h, d, page, lens, pos in ((2, 64, 16, [5, 0, 33, 1], [10, 3, 100, 127]), (10, 128, 64, [1, 4], [299, 2000])):
+        c, table, starts, at = O.world(len(lens), h, d, page, lens, pos, "cuda")
+        n = int(starts[-1])
+        qkv, (cos, sin) = torch.randn(n, 3 * h * d, device="cuda").bfloat16(), O.angles(4096, d, "cuda")
+        a = (qkv, cos, sin, c, table, starts, at)
+        q = P.short_append(*a)
+        k = c.k.clone()
+        assert q is not None and torch.equal(q, P.append(P.check_append(*a), *a)) and torch.equal(k, c.k)
+        doc = O.i32([3] * n, "cuda")
+        for ds in (None, doc):
+            for window in (0, 128):
+                for longest in (None, 1, 4096):
+                    b = (q, c, table, starts, at, d ** -0.5, ds, window, longest)
+                    y = P.short_attention(*b)
+                    assert y is not None and torch.equal(y, P.attention(P.check_attention(*b), *b))
+        assert torch.equal(ops.paged_attention(q, c, table, starts, at, 0), ops.paged_attention(q, c, table, starts, at, 0.0))          # a whole number
+        before = c.k.clone()
+        for bad in ((qkv.float(), *a[1:]), (qkv[:, 1:], *a[1:]), (qkv, cos.double(), *a[2:]), (*a[:3], ops.PagedKV(c.k, c.v[:-1]), *a[4:]), (*a[:4], table.long(), *a[5:]),
+                    (*a[:5], starts[:-1], at), (*a[:6], at.cpu()), (torch.nn.Parameter(qkv), *a[1:])):
+            assert P.short_append(*bad) is None
+        for i, x in ((0, q.float()), (0, q[:, :-1]), (5, 33.0 / d), (5, float("nan")), (5, 1), (6, doc.long()), (6, doc[:-1]), (7, 100), (7, -128), (7, True), (8, -1),
+                     (8, 1 << 80), (8, 1.0)):
+            b = [q, c, table, starts, at, 0.1, None, 0, None]
+            b[i] = x
+            assert P.short_attention(*b) is None, (i, x)
+        assert torch.equal(before, c.k)
+
+
+def test_the_same_call_on_two_streams_at_once():
+    from them_bones_b200 import ops
+    worlds = [O.world(4, 2, 64, 16, [1, 40, 3, 200], [500, 30 + i, 0, 77], "cuda", seed=i) for i in range(2)]
+    qs = [O.queries(244, 2, 64, "cuda").roll(i, 0) for i in range(2)]
+    run = lambda i, k: ops.paged_attention(qs[i], *worlds[i], 0.1, longest=k)  # noqa: E731
+    for k in (1, 4096):
+        want = [run(i, k) for i in range(2)]
+        torch.cuda.synchronize()
+        streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+        for _ in range(40):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got[i].append(run(i, k))
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])

@@ -194,3 +194,34 @@ def test_native_refusals():
     for bad in (dict(logits=z.half()), dict(logits=z.double()), dict(starts=starts.cpu()), dict(uniforms=u.cpu()), dict(ids=ids.cpu()), dict(draft_logits=z.cpu())):
         with pytest.raises(ValueError):
             ops.verify_drafts(**{**dict(logits=z, ids=ids, starts=starts, uniforms=u), **bad})
+
+
+@pytest.mark.parametrize("t", [0.0, 0.7])
+def test_calls_without_rows(t):
+    from them_bones_b200 import ops
+    for dtype in (torch.float32, torch.bfloat16):
+        z = torch.zeros(0, 10, device="cuda", dtype=dtype)
+        for q in (None, z):
+            got = ops.verify_drafts(z, torch.zeros(0, dtype=torch.int64, device="cuda"), O.i32([0, 0, 0], "cuda"), torch.zeros(0, 2, device="cuda"), q, t)
+            assert got.accepted.tolist() == [0, 0] and got.token.tolist() == [-1, -1]
+
+
+def test_the_short_way_and_the_long_one_are_one_operator():
+    from them_bones_b200 import ops
+    from them_bones_b200.ops import verify as V
+    for dtype, t in ((torch.float32, 0.7), (torch.bfloat16, 1.0), (torch.bfloat16, 0.0)):
+        z, ids, starts, u, q = _cuda(*problem([3, 0, 5, 1], 900, 904, dtype, True))
+        for draft in (q, None):
+            a = (z, ids, starts, u, draft, t, 900)
+            V.check(*a)
+            got, want = V.short(*a), V.native(*a)
+            assert got is not None and torch.equal(got.accepted, want.accepted) and torch.equal(got.token, want.token)
+        one = ops.verify_drafts(z, ids, starts, u, q, 1, 900)                  # a whole number goes the long way
+        assert torch.equal(one.token, ops.verify_drafts(z, ids, starts, u, q, 1.0, 900).token)
+        a = [z, ids, starts, u, q, t, 900]
+        for i, x in ((0, z.half()), (0, z[:, ::2]), (1, ids.int()), (1, ids[:-1]), (2, starts.long()), (2, starts[:1]), (4, q[:-1]), (4, q[:, :899]), (4, q.half()), (5, 1),
+                     (5, float("nan")), (5, -1.0), (5, 1e-9), (6, 0), (6, 905), (6, True)):
+            assert V.short(*a[:i], x, *a[i + 1:]) is None, (i, x)
+        if t:
+            for x in (None, u[:-1], u.double(), u.cpu()):
+                assert V.short(*a[:3], x, *a[4:]) is None

@@ -12,6 +12,7 @@
 #include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <algorithm>
 #include <cmath>
 
 namespace {
@@ -123,8 +124,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const double scale = PyFloat_AS_DOUBLE(a[5]);
   int over = 0;
   const long long window = PyLong_AsLongLongAndOverflow(a[7], &over), longest = a[8] == Py_None || over ? (n + p.b - 1) / p.b : PyLong_AsLongLongAndOverflow(a[8], &over);
-  if (over || window < 0 || window % 128 || window > 1ll << 37 || longest < 0 || !(std::abs(scale) * p.d <= PyFloat_AsDouble(a[10]))) return none();
-  const int tall = longest > PyLong_AsLong(a[9]), tiles = (int)(window / 128);
+  if (over || window < 0 || window % 128 || longest < 0 || !(std::abs(scale) * p.d <= PyFloat_AsDouble(a[10]))) return none();
+  const int tall = longest > PyLong_AsLong(a[9]), tiles = (int)std::min(window / 128, 1ll << 24);
   const long long room = room_fn((int)p.b, (int)n, (int)(p.m * p.page), (int)p.h, (int)p.d, tiles, tall, 0);
   if (room < 1) return none();
   Tensor y = at::empty({n, p.h * p.d}, q->options().requires_grad(false)), work = at::empty({room}, q->options().dtype(at::kByte).requires_grad(false));

@@ -197,7 +197,7 @@ __device__ __forceinline__ int turns_before(int ahead, int live, int t) {
   return n;
 }
 // A warp's turns: from w * share to below (w + 1) * share
-__device__ __forceinline__ int turn_share(long long total, int warps) { return (int)max((total + warps - 1) / warps, 1ll); }
+__device__ __forceinline__ long long turn_share(long long total, int warps) { return max((total + warps - 1) / warps, 1ll); }
 
 // Keys and values are read once a step: past the first-level cache, and first to go from the second.  us with plain loads / past the first / so:
 // 4 sequences of 32768 to 131072 tokens 297 / 253 / 253 (6.6 TB/s), 64 of up to 2048 32.8 / 29.2 / 26.0.
@@ -281,8 +281,9 @@ __global__ void __launch_bounds__(32 * RW, D == 128 ? 3 : 4) paged_rows_kernel(c
       if (b < p.p.B) p.first[b] = first_of[b];
     }
   }
-  const int share = turn_share(total, p.warps), me = blockIdx.x * RW + warp;
-  long long at_turn = (long long)me * share;
+  const int me = blockIdx.x * RW + warp;
+  const long long share = turn_share(total, p.warps);
+  long long at_turn = me * share;
   const long long end_turn = min(at_turn + share, total);
   uint4* qs = qs_all[warp];
   const uint32_t qs_at = smem_u32(qs + lane);
@@ -520,7 +521,8 @@ __global__ void __launch_bounds__(256) paged_rows_join_kernel(const RowsArgs p) 
     const int ahead = s.pos - p.first[b], turns = tile_turns(ahead, s.live, tile);
     if (turns > 0) {
       const long long from = in_front + (long long)h * turns_before(ahead, s.live, (s.live + RT - 1) / RT) + turns_before(ahead, s.live, tile);
-      const int share = turn_share(total, p.warps), w0 = (int)((from + RC) / share), w1 = (int)((from + turns - 1) / share);
+      const long long share = turn_share(total, p.warps);
+      const int w0 = (int)((from + RC) / share), w1 = (int)((from + turns - 1) / share);
       written = w0 == w1;
       if (!written) {
         // the first warp's second place, the others' first
@@ -559,6 +561,9 @@ __global__ void __launch_bounds__(256) paged_rows_join_kernel(const RowsArgs p) 
   *reinterpret_cast<uint2*>(p.y + ((long long)row * p.p.H + h) * D + 4 * d) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
 }
 
+// Whether a call goes by tiles of 16 rows: one of few tokens, whose turns of a head keep to 32 bits whatever lies in the pieces
+static bool by_rows(int B, int N, int cap, int tall) { return !tall && B <= RB && (N / RT + 1ll) * (cap / RT + 1 + RC) < 1ll << 31; }
+
 // CTAs that share a step's turns: what the SMs hold
 static int rows_ctas(int D, int sms) { return (D == 128 ? 3 : 4) * sms; }
 
@@ -592,7 +597,7 @@ long long bones_paged_room(int B, int N, int cap, int H, int D, int window_tiles
 // rows ldt apart; starts: int32 [B + 1]; pos: int32 [B]; q: bf16 [N, H * D].
 int bones_paged_append(const void* qkv, long long ldq, const float* cosT, const float* sinT, int rope_rows, void* k, void* v, int pages, const int* table,
                        long long ldt, const int* starts, const int* pos, int B, int N, int M, int H, int D, int shift, void* q, void* stream) {
-  const Paged p{starts, pos, table, ldt, B, N, M, H, shift, pages, (int)min((long long)M << shift, 0x7fffff00ll), v};
+  const Paged p{starts, pos, table, ldt, B, N, M, H, shift, pages, (int)min((long long)M << shift, 0x7fffff80ll), v};
   if (paged_refused(B, N, M, H, D, shift, pages, ldt, k, v, starts, pos, table) || !qkv || !q || !cosT || !sinT || rope_rows < 0 || misaligned16(qkv, q, cosT, sinT) || (N > 1 && ldq % 8)) return -2;
   if (N == 0) return 0;
   int dev = 0, sms = 0;
@@ -615,7 +620,7 @@ int bones_paged_append(const void* qkv, long long ldq, const float* cosT, const 
 }
 
 // q, y: bf16 [N, H * D]; doc_start: int32 [N] or null; window_tiles: of 128 tokens, 0 for all; tall: by tiles of 128 rows (pieces of more than a few tokens),
-// which calls of more than 512 sequences take in any case; work: of this call alone until it ends, on 32 bytes, as many as bones_paged_room says.
+// which calls of more than 512 sequences take in any case, and those of some thousand tokens or more over the longest caches; work: of this call alone until it ends, on 32 bytes, as many as bones_paged_room says.
 int bones_paged_attention(const void* q, const void* k, const void* v, int pages, const int* table, long long ldt, const int* starts, const int* pos,
                           const int* doc_start, void* y, int B, int N, int M, int H, int D, int shift, float scale, int window_tiles, int tall, void* work,
                           long long room, void* stream) {
@@ -626,9 +631,10 @@ int bones_paged_attention(const void* q, const void* k, const void* v, int pages
   int dev = 0, sms = 0;
   BONES_CHECK(cudaGetDevice(&dev));
   BONES_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  const Paged p{starts, pos, table, ldt, B, N, M, H, shift, pages, (int)min((long long)M << shift, 0x7fffff00ll), v};
+  const Paged p{starts, pos, table, ldt, B, N, M, H, shift, pages, (int)min((long long)M << shift, 0x7fffff80ll), v};
+  window_tiles = min(window_tiles, MOST_WINDOW);
   if (room < bones_paged_room(B, N, p.cap, H, D, window_tiles, tall, sms)) return -2;
-  if (tall || B > RB) return paged_pieces(q, k, p, doc_start, y, D, scale, window_tiles, sms, work, stream);
+  if (!by_rows(B, N, p.cap, tall)) return paged_pieces(q, k, p, doc_start, y, D, scale, window_tiles, sms, work, stream);
   const float log2e = 1.4426950408889634f;
   const int ctas = rows_ctas(D, sms);
   float* parts = (float*)work;
@@ -642,7 +648,7 @@ int bones_paged_attention(const void* q, const void* k, const void* v, int pages
 long long bones_paged_room(int B, int N, int cap, int H, int D, int window_tiles, int tall, int sms) {
   int dev = 0;
   if (sms <= 0 && (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)) return -1;
-  if (tall || B > RB) return paged_pieces_room(B, N, cap, H, D, window_tiles, sms);
+  if (!by_rows(B, N, cap, tall)) return paged_pieces_room(B, N, cap, H, D, min(window_tiles, MOST_WINDOW), sms);
   return (long long)rows_ctas(D, sms) * RW * 2 * RT * (D + 4) * 4 + 12ll * B + 16;
 }
 }  // extern "C"

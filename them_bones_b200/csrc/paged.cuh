@@ -54,6 +54,8 @@ __device__ __forceinline__ long long paged_at(const Paged& p, int id, int h) {
   return id < 0 || id >= p.pages ? -1 : ((long long)id * p.H + h) << p.shift;
 }
 
+constexpr int MOST_WINDOW = 1 << 24;   // tiles of 128 tokens that hide none of any cache's
+
 // Host: attention of longer pieces (paged_pieces.cu) and the bytes that it works with.
 int paged_pieces(const void* q, const void* k, const Paged& p, const int* doc_start, void* y, int D, float scale, int window_tiles, int sms, void* work, void* stream);
 long long paged_pieces_room(int B, int N, int cap, int H, int D, int window_tiles, int sms);
@@ -63,7 +65,7 @@ inline bool paged_refused(int B, int N, int M, int H, int D, int shift, int page
                           const int* table) {
   if (shift < 4 || shift > 7) return true;
   const long long page = 1ll << shift;
-  return (D != 128 && D != 64) || B < 1 || B > 65534 || N < 0 || M < 1 || H < 1 || H > 65535 || pages < 1 || ldt < M || M * page > 0x7fffff00ll ||
+  return (D != 128 && D != 64) || B < 1 || B > 65534 || N < 0 || M < 1 || H < 1 || H > 65535 || pages < 1 || ldt < M || M * page > 0x7fffff80ll ||
          pages * page * H > 0x7fffff00ll || !k || !v || !starts || !pos || !table || (((uintptr_t)k | (uintptr_t)v) & 31);
 }
 

@@ -245,12 +245,14 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           const Piece s = paged_piece(p, b);
           const int rows = (s.live + PT - 1) / PT;
           const long long head = plan_front(a, s, rows), in_seq = at - a.before[b];
-          int off = (int)(in_seq % head), qt = 0;
+          long long off_v = in_seq % head;
+          int qt = 0;
           all_v = plan_tiles(a, s, 0);
-          while (off >= all_v + PIECE_WAY) {
-            off -= all_v + PIECE_WAY;
+          while (off_v >= all_v + PIECE_WAY) {
+            off_v -= all_v + PIECE_WAY;
             all_v = plan_tiles(a, s, ++qt);
           }
+          const int off = (int)off_v;
           const int take = (int)min((long long)(all_v + PIECE_WAY - off), stop - at);
           at += take;
           g = (int)(in_seq / head) * rows + qt;
@@ -493,7 +495,7 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       const int qpos = r >= im.live ? 0x3fffffff : im.none ? -1 : im.pos0 + r;
       int lo = 0;
       if (r < im.live) {
-        if (a.doc_start) lo = a.doc_start[im.row0 + r];
+        if (a.doc_start) lo = max(a.doc_start[im.row0 + r], 0);
         if (a.window_tiles > 0) lo = max(lo, (((im.pos0 + r) >> 7) - (a.window_tiles - 1)) * 128);
       }
       float l = 0.f;
@@ -682,7 +684,9 @@ template <int D>
 static int launch_pieces(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PiecesArgs& a, cudaStream_t s) {
   constexpr size_t smem = (size_t)(D / 64) * PATOM * 7 + PP_BARS + 4 * PT * sizeof(float);
   static OncePerDevice limit;
-  BONES_ONCE(limit, { BONES_CHECK(cudaFuncSetAttribute(paged_pieces_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); });
+  BONES_ONCE(limit, {
+    BONES_CHECK(cudaFuncSetAttribute(paged_pieces_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  });
   const Paged& p = a.p;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];

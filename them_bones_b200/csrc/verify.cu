@@ -602,7 +602,9 @@ static int launch_verify(const VerifyArgs& p, cudaStream_t s) {
   }
   constexpr size_t smem = (EXP_ROWS * EXP_COLS + VT / 32 * VS * 32 * 2) * sizeof(double);
   static OncePerDevice limit;
-  BONES_ONCE(limit, { BONES_CHECK(cudaFuncSetAttribute(verify_draw_kernel<E>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); });
+  BONES_ONCE(limit, {
+    BONES_CHECK(cudaFuncSetAttribute(verify_draw_kernel<E>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  });
   cfg.gridDim = dim3(VC, (unsigned)p.B);
   cfg.blockDim = dim3(VT);
   cfg.dynamicSmemBytes = smem;
@@ -618,7 +620,7 @@ using namespace bones;
 // stats: room for 4 N doubles, of this call alone until it ends; accepted: int32 [B]; token: int64 [B].
 int bones_verify(const void* z, long long ldz, const void* q, long long ldq, int f32, const long long* ids, const int* starts, const float* u, int B, int N, int V,
                  double T, double* stats, int* accepted, long long* token, void* stream) {
-  if (!z || !ids || !starts || (!u && T != 0.0) || B < 1 || B > 65535 || N < 0 || V < 1 || !(T >= 0.0) || !stats || !accepted || !token || misaligned16(stats)) return -2;
+  if ((N && (!z || !ids || (!u && T != 0.0))) || !starts || B < 1 || B > 65535 || N < 0 || V < 1 || !(T >= 0.0) || !stats || !accepted || !token || misaligned16(stats)) return -2;
   if (N && ((N > 1 && (ldz < V || (q && ldq < V))))) return -2;
   const double inv = T == 0.0 ? 0.0 : 1.0 / T, steps = 0x1.71547652b82fep+8 * inv;
   const VerifyArgs p{z, T == 0.0 ? nullptr : q, ldz, ldq, ids, starts, u, B, N, V, T, inv, steps, 0x1p30 / steps, (RowStat*)stats, accepted, token};

@@ -285,7 +285,7 @@ def paged_append(qkv, cos, sin, cache, table, starts, pos):
         if q is not None:
             return q
     dims = _paged.check_append(qkv, cos, sin, cache, table, starts, pos)
-    _paged.no_gradient(qkv)
+    _paged.no_gradient(qkv, cos, sin, *cache)
     if native(qkv):
         return _paged.append(dims, qkv, cos, sin, cache, table, starts, pos)
     return RF.paged_append(qkv, cos, sin, cache, table, starts, pos)

@@ -20,6 +20,7 @@ from .logprobs import has_tangent
 PAGES = (16, 32, 64, 128)              # tokens of a page
 SHIFT = 32.0                           # largest |scale| * head_dim: the kernels' soft-max has this fixed shift, and its smallest weights, exp(-2 * 32), stay normal in fp32
 MOST_ROWS = (1 << 31) - 256             # rows of [D] in a cache
+MOST_WINDOW = 1 << 24                   # tiles of 128 tokens that hide none of any cache's
 FEW = 16                               # pieces of up to this many tokens go by tiles of 16 rows, longer ones by tiles of 128
 
 
@@ -156,11 +157,12 @@ def attention(dims, q, c, table, starts, pos, scale, doc_start, window, longest)
     if n:
         if longest is None:
             longest = -(-n // b)
+        tiles = min(window // 128, MOST_WINDOW)
         with L.device(dev):
-            room = _room(b, n, m * page, h, d, window // 128, longest > FEW, dev)
+            room = _room(b, n, m * page, h, d, tiles, longest > FEW, dev)
             work = torch.empty(room, dtype=torch.uint8, device=q.device)
             L.call("bones_paged_attention", at, k.data_ptr(), v.data_ptr(), k.shape[0], table.data_ptr(), table.stride(0) if b > 1 else m, starts.data_ptr(),
-                   pos.data_ptr(), 0 if doc_start is None else doc_start.data_ptr(), y.data_ptr(), b, n, m, h, d, page.bit_length() - 1, scale, window // 128,
+                   pos.data_ptr(), 0 if doc_start is None else doc_start.data_ptr(), y.data_ptr(), b, n, m, h, d, page.bit_length() - 1, scale, tiles,
                    longest > FEW, work.data_ptr(), room, L.raw_stream(), launches=2)
         COUNTS["paged_attention"] += 1
     return y

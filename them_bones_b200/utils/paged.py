@@ -10,6 +10,8 @@ The reference scores teacher-forced full sequences only (round2/submission/infer
 """
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from .. import ops
@@ -219,6 +221,8 @@ def paged_decode(model, prompts, n_new: int, temperature: float = 0.0, drafts: i
     texts = [[int(x) for x in t] for t in (prompts.tolist() if isinstance(prompts, torch.Tensor) else prompts)]
     if not texts or not all(texts) or n_new < 0 or max(map(len, texts)) + n_new > cfg.sequence_len:
         raise ValueError("prompts of one token or more, which with the new tokens fit the model's sequence length")
+    if any(not 0 <= x < cfg.vocab_size for t in texts for x in t):
+        raise ValueError(f"prompts hold tokens outside the vocabulary of {cfg.vocab_size}")
     if not 0 <= drafts <= 64 or temperature < 0 or (draft is not None and not drafts):
         raise ValueError(f"{drafts} drafts (0 to 64; some, if there is a model for them), temperature {temperature}")
     if draft is not None:
@@ -226,18 +230,19 @@ def paged_decode(model, prompts, n_new: int, temperature: float = 0.0, drafts: i
         if draft.config.vocab_size != cfg.vocab_size or draft.config.sequence_len < cfg.sequence_len or draft.lm_head.weight.device != dev:
             raise ValueError("a draft model has the model's vocabulary, its sequence length and its device")
     goal = [len(t) + n_new for t in texts]
-    b, gen = len(texts), torch.Generator(device=dev).manual_seed(seed)
-    if n_new:
-        cache = PagedCache(model, goal, page)
-        _prefill(model, cache, texts)
-        if drafts:
-            _drafted(model, cache, texts, goal, temperature, drafts, draft, gen)
-        else:
-            for t, new in zip(texts, _plain(model, cache, texts, n_new, temperature, gen)):
-                t.extend(new)
-    if dev.type == "cuda" and not ops.reference_path():
-        from ..ops import _lib as L
-        L.check_error_word()
+    gen = torch.Generator(device=dev).manual_seed(seed)
+    with torch.cuda.device(dev) if dev.type == "cuda" else contextlib.nullcontext():          # streams and graphs are the current device's
+        if n_new:
+            cache = PagedCache(model, goal, page)
+            _prefill(model, cache, texts)
+            if drafts:
+                _drafted(model, cache, texts, goal, temperature, drafts, draft, gen)
+            else:
+                for t, new in zip(texts, _plain(model, cache, texts, n_new, temperature, gen)):
+                    t.extend(new)
+        if dev.type == "cuda" and not ops.reference_path():
+            from ..ops import _lib as L
+            L.check_error_word()
     rows = [torch.tensor(t, dtype=torch.int64, device=dev) for t in texts]
     return torch.stack(rows) if isinstance(prompts, torch.Tensor) else rows
 
