@@ -161,15 +161,14 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     if (threadIdx.x == 0) atomicCAS(a.err, 0, ERR_WAIT_AUX);
     return;
   }
-  auto sQ = [&](int s) { return base + TILE * s; };
-  auto sK = [&](int s) { return base + TILE * (2 + s); };
+  const uint32_t sQ = base;
+  auto sK = [&](int s) { return base + TILE * (1 + s); };
   auto sV = [&](int s) { return base + TILE * (4 + s); };
   constexpr uint32_t kBars = TILE * 7;
   const uint32_t bars = base + kBars;
-  auto q_full = [&](int s) { return bars + 8u * (0 + s); };
-  auto q_free = [&](int s) { return bars + 8u * (2 + s); };
-  auto k_full = [&](int s) { return bars + 8u * (4 + s); };
-  auto k_free = [&](int s) { return bars + 8u * (6 + s); };
+  const uint32_t q_full = bars, q_free = bars + 8u;
+  auto k_full = [&](int s) { return bars + 8u * (2 + s); };
+  auto k_free = [&](int s) { return bars + 8u * (5 + s); };
   auto v_full = [&](int s) { return bars + 8u * (8 + s); };
   auto v_free = [&](int s) { return bars + 8u * (11 + s); };
   auto v_fine = [&](int s) { return bars + 8u * (14 + s); };
@@ -273,8 +272,9 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         const Piece s = paged_piece(p, b);
         const int rows = (s.live + PT - 1) / PT;
         im.seq = b;
-        im.h = g / rows;
-        const int qt = share ? g % rows : rows - 1 - (g % rows + im.h) % rows;       // drawn: turned from head to head, so that CTAs see a mix of lengths
+        // shared: a head's tiles one after another; drawn: the heads' last tiles first, which see the most keys, so that what is drawn last is short
+        im.h = share ? g / rows : g % p.H;
+        const int qt = share ? g % rows : rows - 1 - g / p.H;
         im.row0 = s.row + qt * PT;
         im.live = min(PT, s.live - qt * PT);
         im.pos0 = s.pos + qt * PT;
@@ -311,23 +311,23 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   } else if (warp == 0) {
     // Q and K loads
     PieceItem im;
-    int g = 0;
+    int g = 0, ks = 0;
+    uint32_t kph = 1;
     bool dead = false;
     for (int it = 0; !dead && take(it, &im); ++it) {
-      const int qb = it & 1;
-      if (it >= 2 && !dead) dead = !mbar_wait(q_free(qb), (uint32_t)(((it - 2) >> 1) & 1), abort_flag, a.err, ERR_WAIT_EMPTY);
+      if (it >= 1 && !dead) dead = !mbar_wait(q_free, (uint32_t)((it - 1) & 1), abort_flag, a.err, ERR_WAIT_EMPTY);
       const int h = warp_uniform(im.h), row0 = warp_uniform(im.row0);
       if (elect_one() && !dead) {
-        mbar_arrive_expect_tx(q_full(qb), TILE);
+        mbar_arrive_expect_tx(q_full, TILE);
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) tma_load_2d(sQ(qb) + c * PATOM, &tm_q, q_full(qb), h * D + c * 64, row0);
+        for (int c = 0; c < D / 64; ++c) tma_load_2d(sQ + c * PATOM, &tm_q, q_full, h * D + c * 64, row0);
       }
       int row = page_row(im, im.kt0);
       for (int j = 0; j < im.n; ++j, ++g) {
-        const int ks = g & 1, now = row;
+        const int now = row;
         if (j + 1 < im.n) row = page_row(im, im.kt0 + j + 1);
-        if (g >= 2 && !dead) dead = !mbar_wait(k_free(ks), (uint32_t)(((g - 2) >> 1) & 1), abort_flag, a.err, ERR_WAIT_EMPTY);
-        // (at most four tiles are between this one and the oldest whose scores are still read)
+        if (g >= 3 && !dead) dead = !mbar_wait(k_free(ks), kph, abort_flag, a.err, ERR_WAIT_EMPTY);
+        // (at most six tiles are between this one and the oldest whose scores are still read)
         const uint32_t missing = __ballot_sync(0xffffffffu, lane < per_tile && now == none && ((im.kt0 + j) * per_tile + lane) << p.shift < im.pos0 + im.live);
         if (lane == 0) holes[g & 7] = (int)missing;
         if (elect_one() && !dead) mbar_arrive_expect_tx(k_full(ks), TILE);
@@ -339,6 +339,7 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             for (int c = 0; c < D / 64; ++c) tma_load_2d(sK(ks) + c * PATOM + i * page_bytes, &tm_k, k_full(ks), c * 64, at);
           }
         }
+        if (++ks == 3) { ks = 0; kph ^= 1u; }
       }
     }
   } else if (warp == PP_VW) {
@@ -425,31 +426,34 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     // S = Q K^T of each tile, into the buffer whose O += P V (three tiles before) is done
     constexpr uint32_t kHi = umma_desc_hi(1024, kLayoutSw128);
     const uint32_t idesc_s = umma_idesc_f16(128, 128, 1, 0, 0);   // Q (K-major) x K (K-major)
-    const uint32_t q_lo = (uint32_t)warp_uniform((int)umma_desc_lo(sQ(0), 0)), k_lo = (uint32_t)warp_uniform((int)umma_desc_lo(sK(0), 0));
+    const uint32_t q_lo = (uint32_t)warp_uniform((int)umma_desc_lo(sQ, 0)), k_lo = (uint32_t)warp_uniform((int)umma_desc_lo(sK(0), 0));
     PieceItem im;
     bool dead = false;
-    int g = 0, gs = 0;
-    uint32_t fph = 1;
+    int g = 0, gs = 0;                       // tile; S buffer and K stage
+    uint32_t fph = 1, kph = 0;
     for (int it = 0; !dead && take(it, &im); ++it) {
-      const int n = warp_uniform(im.n), qb = it & 1;
-      if (!dead) dead = !mbar_wait(q_full(qb), (uint32_t)((it >> 1) & 1), abort_flag, a.err, ERR_WAIT_FULL);
+      const int n = warp_uniform(im.n);
+      if (!dead) dead = !mbar_wait(q_full, (uint32_t)(it & 1), abort_flag, a.err, ERR_WAIT_FULL);
       for (int j = 0; j < n; ++j, ++g) {
-        const int kb = g & 1;
-        if (!dead) dead = !mbar_wait(k_full(kb), (uint32_t)((g >> 1) & 1), abort_flag, a.err, ERR_WAIT_FULL);
+        if (!dead) dead = !mbar_wait(k_full(gs), kph, abort_flag, a.err, ERR_WAIT_FULL);
         if (g >= 3 && !dead) dead = !mbar_wait(s_free(gs), fph, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
         tc_fence_after();
-        const uint32_t qd = q_lo + (uint32_t)qb * (TILE >> 4), kd = k_lo + (uint32_t)kb * (TILE >> 4), sd = tS(gs);
+        const uint32_t kd = k_lo + (uint32_t)gs * (TILE >> 4), sd = tS(gs);
         if (elect_one() && !dead) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t off = ((k >> 2) * PATOM + (k & 3) * 32) >> 4;
-            umma_f16_lh(sd, qd + off, kHi, kd + off, kHi, idesc_s, k ? 1u : 0u);
+            umma_f16_lh(sd, q_lo + off, kHi, kd + off, kHi, idesc_s, k ? 1u : 0u);
           }
           tc_commit(s_full(gs));
-          tc_commit(k_free(kb));
-          if (j == n - 1) tc_commit(q_free(qb));
+          tc_commit(k_free(gs));
+          if (j == n - 1) tc_commit(q_free);
         }
-        if (++gs == 3) { gs = 0; fph ^= 1u; }
+        if (++gs == 3) {
+          gs = 0;
+          fph ^= 1u;
+          kph ^= 1u;
+        }
       }
     }
   } else if (warp == PP_PV) {
