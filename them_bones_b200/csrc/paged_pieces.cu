@@ -132,10 +132,20 @@ __global__ void __launch_bounds__(PLAN_T) paged_plan_kernel(const PiecesArgs a) 
 //  - values that a row does not see may be anything (other sequences' leftovers behind the end): tiles with a mask are looked through before V's
 //    product by two warps, zeros are put for what is not finite, and it is added back to the rows that do see it at the end.  (By the drain warps they waited for an
 //    item's output, by the loading warp for its loads: 31 us for 26 of the banded case of short pieces.)
+//  - a stage of Q, three of K and of V: the next item's queries come while the softmax still has two or three tiles of this one's (two stages of Q and of K
+//    99.4 and 50.2 us in the first two cases below).
+// Measured, us of a whole call: 8 prompts of 2048 tokens, 10 heads of 128, 94.8 (88 GFLOP at 0.93 PFLOP/s); 512 tokens behind 15900, 10 heads of 128, 48.5 (0.87); 24 pieces
+// of up to 700 tokens, 4 heads of 64, window 512, documents, 23.5.  A tile takes about 1850 clocks, at the 1.5 GHz that the power cap leaves under this load: 980 of
+// exponentials by sixteen warps (16384 at 16 a clock and SM), some 400 between two tiles' (barriers, TMEM), an item's way in and out 3000 once.  The tensor pipe is
+// active 0.53 of the time, L2 delivers half of what it can (half as many bytes again: 4 % longer).  Slower, us in the first case: two halves of the softmax warps on
+// alternate tiles 101.9, a sixth or a third of the exponentials by a polynomial 108 or 117 (of 104.6 then), two accumulators and two S buffers instead of one and
+// three 108.6.  (The order in which items are drawn and how far ahead: 104.6 with a head's tiles in turn and an item ahead, 94.8 as it is.)
 constexpr int PP_SW = 16, PP_DW = 4;
 constexpr int PP_PV = 2 + PP_SW + PP_DW, PP_VW = PP_PV + 1, PP_IW = PP_VW + 1, PP_LW = PP_IW + 1, PP_LOOK = 2;
 constexpr int PP_THREADS = 32 * (PP_LW + PP_LOOK);
 constexpr int PP_RING = 2;                      // items handed round: the one being computed and the next (three: the same times)
+constexpr int PP_NEAR = 5;                      // tiles of keys from an item's end at which the next is drawn (whole prompts, us: 98.0 / 96.8 / 95.7 / 94.8 / 95.0 / 95.3 / 95.5
+                                                // with 1 / 2 / 3 / 5 / 7 / 9 / 12; 97.5 an item ahead)
 constexpr uint32_t PP_BARS = 512;               // barriers, TMEM address, abort flag, items
 
 struct PieceItem {
@@ -178,10 +188,11 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   auto i_full = [&](int s) { return bars + 8u * (26 + s); };
   auto i_free = [&](int s) { return bars + 8u * (29 + s); };
   const uint32_t o_full = bars + 8u * 32, o_free = bars + 8u * 33, l_full = bars + 8u * 34, l_free = bars + 8u * 35;
-  const uint32_t tmem_slot = bars + 288u;
-  volatile uint32_t* tmem_slot_g = reinterpret_cast<volatile uint32_t*>(gen + kBars + 288);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + kBars + 292);
-  int* taint = reinterpret_cast<int*>(gen + kBars + 296);                                    // [PP_RING]
+  const uint32_t near = bars + 8u * 36;         // an item's end is near
+  const uint32_t tmem_slot = bars + 296u;
+  volatile uint32_t* tmem_slot_g = reinterpret_cast<volatile uint32_t*>(gen + kBars + 296);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + kBars + 300);
+  int* taint = reinterpret_cast<int*>(gen + kBars + 304);                                    // [PP_RING]
   volatile int* holes = reinterpret_cast<volatile int*>(gen + kBars + 448);                  // [8], by tile: whether a page that it needs is missing
   PieceItem* ring = reinterpret_cast<PieceItem*>(gen + kBars + 320);                         // [PP_RING]
   static_assert(PP_RING <= 3 && 320 + PP_RING * sizeof(PieceItem) <= 448 && 448 + 8 * 4 <= PP_BARS, "room");
@@ -190,7 +201,7 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int A = p.H * D;
   if (warp == 0) {
-    for (int i = lane; i < 36; i += 32) {
+    for (int i = lane; i < 37; i += 32) {
       const bool by_softmax = (i >= 23 && i < 26) || i == 34, by_drain = (i >= 29 && i < 32) || i == 33 || i == 35, by_look = i >= 14 && i < 17;
       mbar_init(bars + 8u * (uint32_t)i, by_softmax ? PP_SW : by_drain ? PP_DW : by_look ? PP_LOOK : 1);
     }
@@ -260,6 +271,8 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         }
         if (to_v <= from_v) b = -1;
       } else {
+        // (an item drawn a whole item ahead would be a CTA's own while others have nothing left)
+        if (it >= 1 && !__all_sync(0xffffffffu, mbar_wait(near, (uint32_t)((it - 1) & 1), abort_flag, a.err, ERR_WAIT_AUX))) break;
         const int w = it == 0 ? (int)blockIdx.x : (int)gridDim.x + warp_uniform(lane == 0 ? atomicAdd(a.next, 1) : 0);
         if (w < total) {
           b = min(max(paged_owner(a.tiles, p.B, w), 0), p.B - 1);
@@ -340,6 +353,7 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           }
         }
         if (++ks == 3) { ks = 0; kph ^= 1u; }
+        if (j == max(im.n - PP_NEAR, 0) && lane == 0) mbar_arrive(near);
       }
     }
   } else if (warp == PP_VW) {
