@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(PLAN_T) paged_plan_kernel(const PiecesArgs a) 
 // ---------------------------------------------------------------------------------------------------------------
 // Roles as in the training forward (attention.cu): a warp each for Q and K loads, V loads, S = Q K^T, O += P V; sixteen softmax warps (four per
 // 32-lane TMEM quadrant, 32 keys a thread); four drain warps.  Here a warp of its own draws the items and looks up what they are (the sequence, its
-// rows, the first and last of their keys): three dependent reads that nobody waits for, since it runs one item ahead.  What is of this kernel:
+// rows, the first and last of their keys): three dependent reads that nobody waits for, since it runs ahead.  What is of this kernel:
 //  - pages: a box of the tensor map is one page's P tokens of one head; a position without a page is loaded as zeros and masked.
 //  - rows behind a piece's end (a step with a few drafts has 5 of 128) take no exponentials: a softmax warp without a live row passes its tiles on.
 //  - values that a row does not see may be anything (other sequences' leftovers behind the end): tiles with a mask are looked through before V's
@@ -134,12 +134,13 @@ __global__ void __launch_bounds__(PLAN_T) paged_plan_kernel(const PiecesArgs a) 
 //    item's output, by the loading warp for its loads: 31 us for 26 of the banded case of short pieces.)
 //  - a stage of Q, three of K and of V: the next item's queries come while the softmax still has two or three tiles of this one's (two stages of Q and of K
 //    99.4 and 50.2 us in the first two cases below).
-// Measured, us of a whole call: 8 prompts of 2048 tokens, 10 heads of 128, 94.8 (88 GFLOP at 0.93 PFLOP/s); 512 tokens behind 15900, 10 heads of 128, 48.5 (0.87); 24 pieces
-// of up to 700 tokens, 4 heads of 64, window 512, documents, 23.5.  A tile takes about 1850 clocks, at the 1.5 GHz that the power cap leaves under this load: 980 of
+// Measured, us of a whole call: 8 prompts of 2048 tokens, 10 heads of 128, 92.9 (88 GFLOP at 0.95 PFLOP/s); 512 tokens behind 15900, 10 heads of 128, 48.5 (0.87); 24 pieces
+// of up to 700 tokens, 4 heads of 64, window 512, documents, 21.8.  A tile takes about 1850 clocks, at the 1.5 GHz that the power cap leaves under this load: 980 of
 // exponentials by sixteen warps (16384 at 16 a clock and SM), some 400 between two tiles' (barriers, TMEM), an item's way in and out 3000 once.  The tensor pipe is
 // active 0.53 of the time, L2 delivers half of what it can (half as many bytes again: 4 % longer).  Slower, us in the first case: two halves of the softmax warps on
 // alternate tiles 101.9, a sixth or a third of the exponentials by a polynomial 108 or 117 (of 104.6 then), two accumulators and two S buffers instead of one and
-// three 108.6.  (The order in which items are drawn and how far ahead: 104.6 with a head's tiles in turn and an item ahead, 94.8 as it is.)
+// three 108.6.  (The order in which items are drawn and how far ahead: 104.6 with a head's tiles in turn and an item ahead, 94.8 as it is; the
+// mask as bits, 94.8 -> 92.9, and 24.0 -> 21.8 in the third, where most tiles have one; with the exponentials left out that no row sees 94.9, 50.9 and 21.4.)
 constexpr int PP_SW = 16, PP_DW = 4;
 constexpr int PP_PV = 2 + PP_SW + PP_DW, PP_VW = PP_PV + 1, PP_IW = PP_VW + 1, PP_LW = PP_IW + 1, PP_LOOK = 2;
 constexpr int PP_THREADS = 32 * (PP_LW + PP_LOOK);
@@ -536,11 +537,14 @@ paged_pieces_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           const int missing = holes[g & 7];
           if (__any_sync(0xffffffffu, (k0 + 31 > qpos) || (k0 < lo) || missing)) {
             const int end = qpos - k0, from = lo - k0;
+            // which of its keys the row sees
+            uint32_t seen = end < 0 || from > 31 ? 0u : (0xffffffffu >> (31 - min(end, 31))) & (0xffffffffu << max(from, 0));
             // pages of the first and second sixteen keys
-            const bool there_a = !(missing >> (c0 >> p.shift) & 1), there_b = !(missing >> ((c0 + 16) >> p.shift) & 1);
+            if (missing >> (c0 >> p.shift) & 1) seen &= 0xffff0000u;
+            if (missing >> ((c0 + 16) >> p.shift) & 1) seen &= 0xffffu;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (i > end || i < from || !(i < 16 ? there_a : there_b)) e[i] = 0.f;
+              if (!(seen >> i & 1)) e[i] = 0.f;
           }
           float l4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
