@@ -155,8 +155,8 @@ __global__ void __launch_bounds__(AT, 6) paged_append_kernel(const __nv_bfloat16
 // rows; of the at most two tiles that it shares with others it leaves sums, which a second kernel adds in order.  A tile counts as RC turns more than it
 // has, the way to its first keys: without them a warp got as many tiles of a turn or two as others got turns of one (64 sequences: 33.4 us; with one, two or three 26).
 //
-// Measured, us of a whole call, 10 heads of 128: 4 sequences of 32768 to 131072 tokens 253 (the copy rate); 64 of up to 2048 tokens 26.0 (4.1 TB/s), with up to five new
-// tokens each the same; one of 300 7.6.  In the second the first keys are there 10000 clocks behind the launch (the shares 2800, where in them 1900, tables, and 19 MB that
+// Measured, us of a whole call, 10 heads of 128: 4 sequences of 32768 to 131072 tokens 253 (the copy rate); 64 of up to 2048 tokens 26.0 (4.1 TB/s), 32 of 1500 with up to
+// five new tokens each the same; one of 300 7.6.  In the second the first keys are there 10000 clocks behind the launch (the shares 2800, where in them 1900, tables, and 19 MB that
 // all warps ask for at once), the warps end between 36000 and 41600, and the join takes 2 us.  Stretches drawn from a common counter instead of equal shares: 39 and 301 us.
 constexpr int RW = 4;                       // warps of a CTA
 constexpr int RT = 16;                      // rows of a tile, keys of a turn
