@@ -152,7 +152,7 @@ def verify(logits, ids, starts, uniforms, draft, t, vocab):
                         continue
                 if q is not None:
                     w = [max(pp - qq, 0.0) for pp, qq in zip(p, q)]
-                    w = w if any(w) else p                      # q is p
+                    w = w if math.fsum(w) > 1e-12 else p        # q is p, or as good as
             total, c = math.fsum(w), 0.0
             for i, x in enumerate(w):
                 c += x

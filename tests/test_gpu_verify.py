@@ -225,3 +225,16 @@ def test_the_short_way_and_the_long_one_are_one_operator():
         if t:
             for x in (None, u[:-1], u.double(), u.cpu()):
                 assert V.short(*a[:3], x, *a[4:]) is None
+
+
+def test_next_to_nothing_left_of_p_is_nothing():
+    """p and q alike to 12 digits, and a draft that q would hardly ever give: the token is p's, not that of a rare column whose own weight is well above q's."""
+    z = torch.tensor([[12.351143836975098, -0.10267984122037888, -0.30233708024024963, 4.481926441192627, -3.0466697216033936, 3.10713267326355, 0.4143826365470886]] * 2)
+    q = torch.tensor([[12.44536018371582, -0.10847845673561096, -0.24057084321975708, 4.601906776428223, -2.91764235496521, 3.022629976272583, 0.4767337143421173]] * 2)
+    for k in (0.01, 0.5, 0.77, 0.999):
+        for rows, cols in ((z, 7), (torch.cat([z, z], 1), 14), (torch.nn.functional.pad(z, (0, 3000), value=-40.0), 3007)):
+            if cols == 14 and k == 0.5:
+                continue                                  # half of two equal halves is the border itself: no arithmetic says on which side
+            draft = torch.cat([q, q], 1) if cols == 14 else torch.nn.functional.pad(q, (0, cols - 7), value=-40.0)
+            u = torch.tensor([[0.9918550252914429, k], [0.5, 0.5]])
+            _check(rows, torch.tensor([6, 4]), O.i32([0, 2]), u, draft, 0.3, cols)

@@ -487,10 +487,11 @@ __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT, 4) verify_draw_
   for (int round = 0; round < 2; ++round) {
     const Sums r = share(other ? row_sums<E, true>(z, other, lp, lq, ratio, -1, cut, p.V, parts)
                                : row_sums<E, false>(z, nullptr, lp, lq, 0.0, skip, cut, p.V, parts), box);
-    if (other) ratio = warp_sum64(r.p) / warp_sum64(r.q);
+    const double all_p = warp_sum64(r.p);
+    if (other) ratio = all_p / warp_sum64(r.q);
     const double w = r.p_up - ratio * r.q_up;                 // of warp `lane`
-    const uint32_t some = __ballot_sync(0xffffffffu, weighs(w, r.p_up));
-    if (!some && round == 0) {                                // p and q the same: of p alone
+    const bool some = __any_sync(0xffffffffu, weighs(w, r.p_up)), much = !other || warp_sum64(fmax(w, 0.0)) > 1e-12 * all_p;
+    if (!(some && much) && round == 0) {                      // p and q the same: of p alone.  (What is left of 1e-12 of p hangs on the last bits of its sums.)
       other = nullptr;
       ratio = 0.0;
       skip = -1;

@@ -295,7 +295,7 @@ def paged_attention(q, cache, table, starts, pos, scale, doc_start=None, window=
     """Pieces of new tokens against the cache: ``q [N, H*D]`` as ``paged_append`` returned it, with its ``table``, ``starts`` and ``pos`` -> ``[N, H*D]``.
     Token i of the N sees its sequence's positions from ``doc_start[i]`` (int32 ``[N]``) and the band of ``window`` tokens (as in ``attention``) to its
     own, as far as they have pages.  One token a sequence, drafts, pieces of prompts and whole prompts in one call.  ``longest``: the length of the
-    longest piece as far as the host knows (default: the mean); it picks a kernel, not the result.  Tokens that were left out, rows outside all pieces and
+    longest piece as far as the host knows (default: the mean); it picks a kernel, and the result but for roundings is the same.  Tokens that were left out, rows outside all pieces and
     queries that see no key get zeros.  Queries and keys are behind the norm (``|q . k|`` about D at most): natively the soft-max has a
     fixed shift, and ``|scale| * D`` up to 32.  No gradient."""
     if native(q):
@@ -316,7 +316,7 @@ def verify_drafts(logits, ids, starts, uniforms=None, draft_logits=None, tempera
     which the first is given and the others are drafts.  Row by row, with ``p = softmax(logits / temperature)`` and ``q`` what the drafts were
     drawn from, the soft-max of ``draft_logits [N, C']`` (the row in front of a draft's; a sequence's last row is not read) or, without
     them, certainty: the draft x behind row r stands while ``uniforms[r, 0] * q(x) < p(x)`` (fp32 ``[N, 2]`` in [0, 1)).  At the first that does not the
-    token is drawn from ``max(p - q, 0)`` (from p where that is nothing), behind the last draft from p: the first one whose cumulated weight is above ``uniforms[r, 1]`` of the
+    token is drawn from ``max(p - q, 0)`` (from p where that is nothing: 1e-12 of it at most), behind the last draft from p: the first one whose cumulated weight is above ``uniforms[r, 1]`` of the
     total.  ``temperature=0``: the arg-max (the lowest index of equals) throughout, no ``uniforms``.  -> ``Verified(accepted [B], token [B])``.  Sums in 64
     bits.  A draft outside the vocabulary falls; so does one whose draft row has no number (NaN, +inf or nothing but -inf), and the token is then drawn from p.
     A target row without a number ends a sequence with token -1, as does a sequence without rows.  No gradient."""

@@ -803,7 +803,7 @@ def verify_drafts(logits, ids, starts, uniforms, draft_logits, temperature: floa
                         continue
                 if q is not None:
                     w = (p - q).clamp_min(0.0)
-            w = w if bool((w > 0).any()) else p                    # p and q the same but for rounding
+            w = w if float(w.sum()) > 1e-12 else p                 # p and q the same but for rounding
             c = w.cumsum(0)
             token = min(int((c <= u[1] * float(c[-1])).sum()), int(torch.nonzero(w)[-1]))      # by rounding none: the last one that has weight
             break
