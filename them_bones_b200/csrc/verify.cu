@@ -9,8 +9,8 @@
 // function in 32 would move by more than the gap of a rare token's interval, and the token with it (65536 columns: one draw in some hundred).
 // A draft whose test is closer than the first kernel's 32-bit exponentials can tell is decided on sums in 64 bits too.
 //
-// Measured, us of a whole call: 64 sequences of a token and up to four drafts, 65536 bf16 columns, drafts from a model, 37.6; one sequence of seven looked-up drafts, 8191 fp32
-// columns, 8.5; with arg-max throughout 11.2 and 3.9.  The first kernel takes 15 in the first case, 12.5 of them exponentials at 16 a clock and SM (59 MB at the
+// Measured, us of a whole call: 64 sequences of a token and up to four drafts, 65536 bf16 columns, drafts from a model, 38.2; one sequence of seven looked-up drafts, 8191 fp32
+// columns, 8.8; with arg-max throughout 11.2 and 3.9.  The first kernel takes 15 in the first case, 12.5 of them exponentials at 16 a clock and SM (59 MB at the
 // copy rate: 9); the second 20: 8.4 million exponentials in 64 bits, at most seven operations each with the table's reads between them, by warps
 // that wait for one another's results (the pipe of 64 bits 0.18, the schedulers 0.38 of the time).  Twice the warps with half the columns each: 55 us, and with four values
 // side by side instead of eight 58 to 61.
