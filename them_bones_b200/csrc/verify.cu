@@ -181,6 +181,7 @@ __global__ void __launch_bounds__(VST, 4) verify_stats_kernel(const VerifyArgs p
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int VC = 8, VT = 128, VW = VC * VT / 32;       // CTAs, threads of one, warps of a cluster
 constexpr int VS = 8;                                    // steps of a warp at most
+constexpr int PARTS = VS * 32 + 1;                       // a warp's parts: a lane's of a step, and its nearest column
 static_assert(VW == 32, "a lane has a warp's sums");
 
 // A row's law, exp((z - most) / T), in 64 bits, by a table of powers of two (the method of Tang, "Table-driven implementation of the exponential
@@ -291,21 +292,25 @@ struct Cut {
   __device__ __forceinline__ int column(int step, int lane) const { return (step * 32 + lane) * wide * 8; }
 };
 
-// Four doubles of each warp to all: lane l gets those of warp l of the cluster.
+// The sums of each warp to all: lane l gets those of warp l of the cluster.
 struct Sums {
   double p, q;         // of the law's own terms
   double p_up, q_up;   // of those columns' where p is above q
 };
-__device__ __forceinline__ Sums share(const Sums& s, Sums* box) {
+struct Shared : Sums {
+  int gap;             // the least of |p - ratio q| / p in the warp's columns, as what the high words differ by (with q)
+};
+__device__ __forceinline__ Shared share(const Sums& s, Sums* box, const double2* parts) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (lane == 0) box[warp] = s;
   __syncthreads();
   cluster_barrier();
   const uint32_t at = map_to_rank(smem_u32(box + lane % (VT / 32)), lane / (VT / 32));
-  Sums r;
+  Shared r;
   double* v = &r.p;
 #pragma unroll
   for (int i = 0; i < 4; ++i) asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v[i]) : "r"(at + 8 * i));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(r.gap) : "r"(map_to_rank(smem_u32(parts + (lane % (VT / 32) - warp) * PARTS + VS * 32), lane / (VT / 32))));
   __syncwarp();
   cluster_barrier();
   return r;
@@ -323,6 +328,7 @@ template <typename E, bool BOTH>
 __device__ __noinline__ Sums row_sums(const E* z, const E* q, const Law lp, const Law lq, double ratio, int without, const Cut cut, int V, double2* parts) {
   const int lane = threadIdx.x & 31, n = (cut.to - cut.from) * cut.wide;
   Sums s = {};
+  int gap = 0x7fffffff;
   if (n > 0) {
     int at = cut.column(cut.from, lane), k = 0;
     double up = 0.0, q_up = 0.0;
@@ -347,7 +353,9 @@ __device__ __noinline__ Sums row_sums(const E* z, const E* q, const Law lp, cons
         s.q += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const bool above = __double2hiint(fma(-ratio, y[j], x[j])) > 0;              // by the difference's sign
+          const int d = __double2hiint(fma(-ratio, y[j], x[j]));
+          const bool above = d > 0;                                                     // by the difference's sign
+          gap = min(gap, (d & 0x7fffffff) - __double2hiint(x[j]));
           x[j] = __hiloint2double(above ? __double2hiint(x[j]) : 0, __double2loint(x[j]));        // (what is left without the high word is below 1e-310)
           y[j] = __hiloint2double(above ? __double2hiint(y[j]) : 0, __double2loint(y[j]));
         }
@@ -372,6 +380,10 @@ __device__ __noinline__ Sums row_sums(const E* z, const E* q, const Law lp, cons
   s.q = warp_sum64(s.q);
   s.p_up = warp_sum64(s.p_up);
   s.q_up = warp_sum64(s.q_up);
+  if (BOTH) {
+    gap = __reduce_min_sync(0xffffffffu, gap);
+    if (lane == 0) *reinterpret_cast<int*>(parts + VS * 32) = gap;
+  }
   return s;
 }
 
@@ -382,7 +394,7 @@ template <typename E>
 __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT, 4) verify_draw_kernel(const VerifyArgs p) {
   __shared__ Sums box[VT / 32];
   extern __shared__ __align__(16) double table[];                // the powers, and behind them the warps' parts
-  double2* parts = reinterpret_cast<double2*>(table + EXP_ROWS * EXP_COLS) + (threadIdx.x >> 5) * VS * 32;
+  double2* parts = reinterpret_cast<double2*>(table + EXP_ROWS * EXP_COLS) + (threadIdx.x >> 5) * PARTS;
   const double* powers = table + threadIdx.x % EXP_COLS;
   fill_powers(table);
   // What does not come from the first kernel is read before its end (it began behind all that came before): of the first 32 rows the draft behind each,
@@ -450,8 +462,8 @@ __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT, 4) verify_draw_
         const float mp = p.stats[rr * 2ll].most, mq = p.q ? p.stats[rr * 2ll + 1].most : 0.f;
         const long long x = p.ids[rr + 1];
         const Law lp(mp, p.steps, p.reach, powers), lq(mq, p.steps, p.reach, powers);
-        const Sums both = share(p.q ? row_sums<E, true>(target(rr), draft(rr), lp, lq, 0.0, -1, cut, p.V, parts)
-                                    : row_sums<E, false>(target(rr), nullptr, lp, lq, 0.0, -1, cut, p.V, parts), box);
+        const Shared both = share(p.q ? row_sums<E, true>(target(rr), draft(rr), lp, lq, 0.0, -1, cut, p.V, parts)
+                                    : row_sums<E, false>(target(rr), nullptr, lp, lq, 0.0, -1, cut, p.V, parts), box, parts);
         const double sum_p = warp_sum64(both.p), sum_q = warp_sum64(both.q);
         const double px = exp(((double)logit(target(rr) + x) - mp) * p.inv) * lp(mp) / sum_p;
         const double qx = p.q ? exp(((double)logit(draft(rr) + x) - mq) * p.inv) * lq(mq) / sum_q : 1.0;
@@ -479,19 +491,30 @@ __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT, 4) verify_draw_
   const E *z = target(row), *zq = sq.sum > 0.0 ? draft(row) : nullptr;
   const long long without = refused && !p.q ? p.ids[row + 1] : -1;
   const Law lp(st.most, p.steps, p.reach, powers), lq(sq.most, p.steps, p.reach, powers);
-  // One pass for both laws' sums and those of the columns where p is above q, with the first kernel's 32-bit sums for the ratio of the scales: where that
-  // errs about a column, p and q are the same to seven digits there.  The weights' sums follow with the ratio in 64 bits.
+  // One pass for both laws' sums and those of the columns where p is above q, with the first kernel's 32-bit sums for the ratio of the scales.  The ratio in
+  // 64 bits follows, some 1e-7 of itself away.  Where p and q of some column are as near to each other as that, the first may have put it on the wrong side, and
+  // the pass is made again; the weights' sums are with the ratio in 64 bits either way.
   const E* other = zq;
   double ratio = zq ? st.sum * lp(st.most) / (sq.sum * lq(sq.most)) : 0.0;
   int skip = without >= 0 && without < p.V ? (int)without : -1;
-  for (int round = 0; round < 2; ++round) {
-    const Sums r = share(other ? row_sums<E, true>(z, other, lp, lq, ratio, -1, cut, p.V, parts)
-                               : row_sums<E, false>(z, nullptr, lp, lq, 0.0, skip, cut, p.V, parts), box);
+  bool alone = !other && skip < 0;
+  for (int round = 0; round < 3; ++round) {
+    const Shared r = share(other ? row_sums<E, true>(z, other, lp, lq, ratio, -1, cut, p.V, parts)
+                               : row_sums<E, false>(z, nullptr, lp, lq, 0.0, skip, cut, p.V, parts), box, parts);
     const double all_p = warp_sum64(r.p);
-    if (other) ratio = all_p / warp_sum64(r.q);
+    if (other) {
+      const double first = ratio;
+      ratio = all_p / warp_sum64(r.q);
+      // A column changes sides only where |p - first q| <= off q, so where |p - first q| / p is below twice off / first (off is 1e-8 of it, and with
+      // 2^30 columns not half of it); another factor of two covers that high words tell either quotient to 6.2 %.  In 425 rows drawn as in the first case
+      // above off was 4e-8 at most and no row went through twice.
+      const double off = fabs(ratio - first);
+      if (round == 0 && off > 0.0 && __reduce_min_sync(0xffffffffu, r.gap) <= __double2hiint(4.0 * off) - __double2hiint(first)) continue;
+    }
     const double w = r.p_up - ratio * r.q_up;                 // of warp `lane`
     const bool some = __any_sync(0xffffffffu, weighs(w, r.p_up)), much = !other || warp_sum64(fmax(w, 0.0)) > 1e-12 * all_p;
-    if (!(some && much) && round == 0) {                      // p and q the same: of p alone.  (What is left of 1e-12 of p hangs on the last bits of its sums.)
+    if (!(some && much) && !alone) {                          // p and q the same: of p alone.  (What is left of 1e-12 of p hangs on the last bits of its sums.)
+      alone = true;
       other = nullptr;
       ratio = 0.0;
       skip = -1;
@@ -607,7 +630,7 @@ static int launch_verify(const VerifyArgs& p, cudaStream_t s) {
     cfg.blockDim = dim3(128);
     return (int)cudaLaunchKernelEx(&cfg, verify_greedy_kernel, p);
   }
-  constexpr size_t smem = (EXP_ROWS * EXP_COLS + VT / 32 * VS * 32 * 2) * sizeof(double);
+  constexpr size_t smem = (EXP_ROWS * EXP_COLS + VT / 32 * PARTS * 2) * sizeof(double);
   static OncePerDevice limit;
   BONES_ONCE(limit, {
     BONES_CHECK(cudaFuncSetAttribute(verify_draw_kernel<E>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
