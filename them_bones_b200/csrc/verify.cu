@@ -486,17 +486,17 @@ __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT, 4) verify_draw_
     return;
   }
   // the row that decides: w = p, max(p - q, 0) or p without the draft
-  const bool refused = row + 1 < e;
+  const long long drafted = row + 1 < e ? p.ids[row + 1] : -1;
+  const bool refused = drafted >= 0 && drafted < p.V;         // a draft outside the vocabulary was not drawn from q: what falls with it leaves all of p
   const RowStat st = p.stats[row * 2ll], sq = refused && p.q ? p.stats[row * 2ll + 1] : RowStat{0.0, 0.f, 0};
   const E *z = target(row), *zq = sq.sum > 0.0 ? draft(row) : nullptr;
-  const long long without = refused && !p.q ? p.ids[row + 1] : -1;
   const Law lp(st.most, p.steps, p.reach, powers), lq(sq.most, p.steps, p.reach, powers);
   // One pass for both laws' sums and those of the columns where p is above q, with the first kernel's 32-bit sums for the ratio of the scales.  The ratio in
   // 64 bits follows, some 1e-7 of itself away.  Where p and q of some column are as near to each other as that, the first may have put it on the wrong side, and
   // the pass is made again; the weights' sums are with the ratio in 64 bits either way.
   const E* other = zq;
   double ratio = zq ? st.sum * lp(st.most) / (sq.sum * lq(sq.most)) : 0.0;
-  int skip = without >= 0 && without < p.V ? (int)without : -1;
+  int skip = refused && !p.q ? (int)drafted : -1;
   bool alone = !other && skip < 0;
   for (int round = 0; round < 3; ++round) {
     const Shared r = share(other ? row_sums<E, true>(z, other, lp, lq, ratio, -1, cut, p.V, parts)

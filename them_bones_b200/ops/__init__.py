@@ -319,7 +319,8 @@ def verify_drafts(logits, ids, starts, uniforms=None, draft_logits=None, tempera
     token is drawn from ``max(p - q, 0)`` (from p where that is nothing: 1e-12 of it at most), behind the last draft from p: the first one whose cumulated weight is above ``uniforms[r, 1]`` of the
     total.  ``temperature=0``: the arg-max (the lowest index of equals) throughout, no ``uniforms``.  -> ``Verified(accepted [B], token [B])``.  Sums in 64
     bits, natively of weights that are off by 1.6e-13 of themselves at most: where p and q agree but for a part W of the whole, the borders between tokens are where the definition has
-    them but for 6.4e-13 / W.  A draft outside the vocabulary falls; so does one whose draft row has no number (NaN, +inf or nothing but -inf), and the token is then drawn from p.
+    them but for 6.4e-13 / W.  A draft outside the vocabulary (-1, say, where a fixed width is filled up) falls, and so does one whose draft row has no number (NaN, +inf or nothing but -inf); in
+    either case the token is drawn from p, with and without draft logits.
     A target row without a number ends a sequence with token -1, as does a sequence without rows.  No gradient."""
     vocab = logits.shape[-1] if vocab is None and logits.dim() else vocab
     if native(logits):

@@ -801,8 +801,7 @@ def verify_drafts(logits, ids, starts, uniforms, draft_logits, temperature: floa
                     if u[0] * float(q[x]) < float(p[x]):
                         i += 1
                         continue
-                if q is not None:
-                    w = (p - q).clamp_min(0.0)
+                    w = (p - q).clamp_min(0.0)             # a draft that nobody could draw leaves all of p
             w = w if float(w.sum()) > 1e-12 else p                 # p and q the same but for rounding
             c = w.cumsum(0)
             token = min(int((c <= u[1] * float(c[-1])).sum()), int(torch.nonzero(w)[-1]))      # by rounding none: the last one that has weight
