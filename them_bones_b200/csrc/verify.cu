@@ -7,7 +7,7 @@
 // Two kernels.  The first reads every row once and leaves its maximum and its sum of exponentials.  The second, a cluster a sequence, goes
 // through the sequence's drafts and draws the token from the one row that decides.  Its sums are in 64 bits: a border of the distribution
 // function in 32 would move by more than the gap of a rare token's interval, and the token with it (65536 columns: one draw in some hundred).
-// A draft whose test is closer than the first kernel's 32-bit exponentials can tell is decided on sums in 64 bits too.
+// A draft whose test is closer than the first kernel's 32-bit exponentials and sums can tell is decided on sums in 64 bits too.
 //
 // Measured, us of a whole call: 64 sequences of a token and up to four drafts, 65536 bf16 columns, drafts from a model, 38.2; one sequence of seven looked-up drafts, 8191 fp32
 // columns, 8.8; with arg-max throughout 11.2 and 3.9.  The first kernel takes 15 in the first case, 12.5 of them exponentials at 16 a clock and SM (59 MB at the
@@ -32,11 +32,13 @@ struct VerifyArgs {
   const int* starts;
   const float* u;              // [N, 2]
   int B, N, V;
+  float close;                   // how near to its border, of both sides' sum, a draft is not decided on the first kernel's sums
   double T, inv, steps, reach;   // 1 / T, K / T, 2^30 T / K
   RowStat* stats;              // [N, 2]
   int* accepted;
   long long* token;
 };
+static_assert(sizeof(VerifyArgs) == 128, "eight bytes more cost 1.5 us in the first case and 0.4 in the second");
 
 template <typename E>
 __device__ __forceinline__ float logit(const E* p) {
@@ -449,7 +451,7 @@ __global__ void __cluster_dims__(VC, 1, 1) __launch_bounds__(VT, 4) verify_draw_
         const RowStat sq = p.q ? p.stats[r * 2ll + 1] : RowStat{1.0, 0.f, 0};
         if (sq.sum > 0.0) {
           const double px = exp(((double)next.p - st.most) * p.inv) / st.sum, qx = p.q ? exp(((double)next.q - sq.most) * p.inv) / sq.sum : 1.0, need = next.u * qx;
-          is = fabs(need - px) <= 1e-4 * (need + px) ? CLOSE : need < px ? STANDS : FALLS;
+          is = fabs(need - px) <= p.close * (need + px) ? CLOSE : need < px ? STANDS : FALLS;
         }
       }
     }
@@ -610,8 +612,17 @@ __global__ void __launch_bounds__(128) verify_greedy_kernel(const VerifyArgs p) 
   }
 }
 
+// What the first kernel's sums may be off by.  A thread adds V / (512 W) times; each time the sum is rounded, and where a larger value came by scaled by an exponential
+// (2^-22 of itself) and rounded: 6 * 2^-24 in all, of the target's and of the draft's sum, each over twice what it is compared with.  What does not grow with
+// the columns (the exponentials of the values themselves, the threads' together) is some 1e-5, and 1e-4 covers it.  65536 bf16 columns: 1.07e-4; 2^27 of fp32: 0.026.
 template <typename E>
-static int launch_verify(const VerifyArgs& p, cudaStream_t s) {
+static float too_close(int V) {
+  return 1e-4f + (V / (VST * kVec<E>) + 2) * (6.0f * 0x1p-24f);
+}
+
+template <typename E>
+static int launch_verify(VerifyArgs p, cudaStream_t s) {
+  p.close = too_close<E>(p.V);
   const dim3 grid((unsigned)p.N, p.q ? 2 : 1);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
@@ -653,7 +664,7 @@ int bones_verify(const void* z, long long ldz, const void* q, long long ldq, int
   if ((N && (!z || !ids || (!u && T != 0.0))) || !starts || B < 1 || B > 65535 || N < 0 || V < 1 || !(T >= 0.0) || !stats || !accepted || !token || misaligned16(stats)) return -2;
   if (N && ((N > 1 && (ldz < V || (q && ldq < V))))) return -2;
   const double inv = T == 0.0 ? 0.0 : 1.0 / T, steps = 0x1.71547652b82fep+8 * inv;
-  const VerifyArgs p{z, T == 0.0 ? nullptr : q, ldz, ldq, ids, starts, u, B, N, V, T, inv, steps, 0x1p30 / steps, (RowStat*)stats, accepted, token};
+  const VerifyArgs p{z, T == 0.0 ? nullptr : q, ldz, ldq, ids, starts, u, B, N, V, 0.f, T, inv, steps, 0x1p30 / steps, (RowStat*)stats, accepted, token};
   return f32 ? launch_verify<float>(p, (cudaStream_t)stream) : launch_verify<__nv_bfloat16>(p, (cudaStream_t)stream);
 }
 }  // extern "C"
