@@ -184,6 +184,7 @@ class _ModelDrafts:
         b, w = len(texts), model.lm_head.weight
         self.logits = torch.zeros(b * (drafts + 1), model.config.vocab_size, dtype=torch.float32, device=w.device)
         self.held = [len(t) - 1 for t in texts]
+        self.docs = None                                       # [drafts, B]: start of the document behind each pass, of one draft more each
         self.first, self.next = _Step(model, self.cache, 2, temperature), _Step(model, self.cache, 1, temperature)
 
     def draw(self, texts, done, gen):
@@ -194,19 +195,24 @@ class _ModelDrafts:
         step.starts.copy_(_starts(lens, dev))
         packed = [x for t, n in zip(texts, lens) for x in (t[len(t) - n:] if n else ())]
         step.ids.copy_(torch.tensor(packed + [0] * (2 * b - len(packed)), dtype=torch.int64))
-        out = []
+        out, docs = [], []
         for i in range(self.k):
             step(gen)
             out.append(step.out.token.clamp(min=0))
             self.logits[i::self.k + 1].copy_(step.logits)
             step.advance(step.starts[1:] - step.starts[:-1])
+            docs.append(self.cache.doc_start.clone())
             step = self.next
             step.ids.copy_(out[-1])
         self.held = [h if d else len(t) + self.k - 1 for h, t, d in zip(self.held, texts, done)]
+        self.docs = torch.stack(docs)
         return torch.stack(out, 1)
 
     def forget(self, texts, accepted):
-        """Of the drafts only ``accepted`` stand: what the cache holds of the others is written over by what comes there."""
+        """Of the drafts only ``accepted`` stand: what the cache holds of the others is written over by what comes there, and a document that began among
+        them did not."""
+        last = torch.tensor([min(a, self.k - 1) for a in accepted], device=self.docs.device)
+        self.cache.doc_start.copy_(self.docs.gather(0, last[None])[0])
         self.held = [min(h, n + a) for h, n, a in zip(self.held, texts, accepted)]
 
 
