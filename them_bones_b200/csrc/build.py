@@ -26,21 +26,31 @@ def _newer(a, b):
 CALLS = os.path.join(LIB_DIR, "bones_calls.so")       # a Python module: calls of few microseconds without the way through ctypes
 
 
+def calls_for() -> str:
+    """What the module of short calls is built for: its binary form is that of one PyTorch and one Python."""
+    import torch
+    return f"PyTorch {torch.__version__}, Python {'.'.join(map(str, sys.version_info[:3]))}, C++11 strings {int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
+
+
 def build_calls(force: bool = False) -> str:
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension as ext
-    src = os.path.join(HERE, "calls.cpp")
-    if not force and not _newer(src, CALLS):
+    src, note, want = os.path.join(HERE, "calls.cpp"), os.path.join(LIB_DIR, "obj", "calls.txt"), calls_for()
+    if not force and not _newer(src, CALLS) and os.path.exists(note) and open(note).read() == want:
         return CALLS
+    os.makedirs(os.path.dirname(note), exist_ok=True)
     inc = [f"-I{d}" for d in (*ext.include_paths(), os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include"), sysconfig.get_paths()["include"])]
     lib = [f"-L{d}" for d in ext.library_paths()] + [f"-l{n}" for n in ("torch_python", "torch", "torch_cpu", "torch_cuda", "c10", "c10_cuda")]
-    r = subprocess.run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, src,
+    r = subprocess.run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                        f'-DBONES_BUILT_WITH="{want}"', *inc, src,
                         "-o", CALLS, *lib], capture_output=True, text=True)
     if r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)
         raise RuntimeError("the calls module does not compile")
+    with open(note, "w") as fh:
+        fh.write(want)
     return CALLS
 
 

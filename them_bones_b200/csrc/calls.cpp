@@ -188,9 +188,13 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   Py_RETURN_NONE;
 }
 
+// What the module was compiled for (calls_for in build.py)
+PyObject* built_with(PyObject*, PyObject*) { return PyUnicode_FromString(BONES_BUILT_WITH); }
+
 PyMethodDef methods[] = {{"paged_append", (PyCFunction)(void (*)(void))paged_append, METH_FASTCALL, nullptr},
                          {"paged_attention", (PyCFunction)(void (*)(void))paged_attention, METH_FASTCALL, nullptr},
                          {"verify_drafts", (PyCFunction)(void (*)(void))verify_drafts, METH_FASTCALL, nullptr},
+                         {"built_with", built_with, METH_NOARGS, nullptr},
                          {"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "bones_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

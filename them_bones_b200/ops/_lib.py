@@ -77,6 +77,9 @@ def calls():
         spec = importlib.util.spec_from_file_location("bones_calls", path)
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
+        from ..csrc.build import calls_for
+        if mod.built_with() != calls_for():
+            raise RuntimeError(f"native calls were built for {mod.built_with()}, not for {calls_for()}; run `python -m them_bones_b200.csrc.build` (or __graft_entry__.build())")
         lib = load()
         mod.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in ("bones_paged_append", "bones_paged_attention", "bones_paged_room", "bones_verify")))
         _CALLS = mod
