@@ -160,7 +160,8 @@ __global__ void __launch_bounds__(AT, 6) paged_append_kernel(const __nv_bfloat16
 // all warps ask for at once), the warps end between 36000 and 41600, and the join takes 2 us.  Stretches drawn from a common counter instead of equal shares: 39 and 301 us.
 constexpr int RW = 4;                       // warps of a CTA
 constexpr int RT = 16;                      // rows of a tile, keys of a turn
-constexpr int RB = 512;                     // sequences of a call
+constexpr int RB = 512;                     // sequences of a call: what is known of each lies in shared memory.  More go by tiles of 128 rows: one token each of 512 / 513 / 1024
+                                            // sequences of up to 256, 10 heads of 128, 68 / 139 / 270 us
 constexpr int RC = 1;                       // turns that getting to a tile counts for
 
 __device__ __forceinline__ void mma_bf16_16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {

@@ -134,12 +134,12 @@ __global__ void __launch_bounds__(PLAN_T) paged_plan_kernel(const PiecesArgs a) 
 //    item's output, by the loading warp for its loads: 31 us for 26 of the banded case of short pieces.)
 //  - a stage of Q, three of K and of V: the next item's queries come while the softmax still has two or three tiles of this one's (two stages of Q and of K
 //    99.4 and 50.2 us in the first two cases below).
-// Measured, us of a whole call: 8 prompts of 2048 tokens, 10 heads of 128, 91.7 (88 GFLOP at 0.96 PFLOP/s); 512 tokens behind 15900, 10 heads of 128, 48.5 (0.87); 24 pieces
-// of up to 700 tokens, 4 heads of 64, window 512, documents, 21.8.  A tile takes about 1850 clocks, at about 1.7 GHz: 980 of
+// Measured, us of a whole call: 8 prompts of 2048 tokens, 10 heads of 128, 91.7 (86 GFLOP at 0.94 PFLOP/s); 512 tokens behind 15900, 10 heads of 128, 48.5 (0.87); 24 pieces
+// of up to 700 tokens, 4 heads of 64, window 512, documents, 21.8.  A tile takes about 1850 clocks, at about 1.7 GHz: 1024 of
 // exponentials by sixteen warps (16384 at 16 a clock and SM), some 400 between two tiles' (barriers, TMEM), an item's way in and out 3000 once.  The tensor pipe is
 // active 0.56 of the time; shared memory moves 160 KB a tile (Q and K read for S, V for O, both written by TMA), 1280 clocks at 128 bytes each; L2 delivers half of what
 // it can (half as many bytes again: 4 % longer).  CTA pairs with half of each tile of K and V apiece would take 96 KB.  Calls without a pause between them settle at a lower
-// clock: 110, 56 and 22 us.  Slower, us in the first case: two halves of the softmax warps on
+// clock: 110 (0.78 PFLOP/s), 56 and 22 us.  Slower, us in the first case: two halves of the softmax warps on
 // alternate tiles 93.8 (for 91.7), a sixth or a third of the exponentials by a polynomial 108 or 117 (of 104.6 then), two accumulators and two S buffers instead of one and
 // three 108.6.  (The order in which items are drawn and how far ahead: 104.6 with a head's tiles in turn and an item ahead, 94.8 as it is; the
 // mask as bits, 94.8 -> 92.9, and 24.0 -> 21.8 in the third, where most tiles have one; with the exponentials left out that no row sees 94.9, 50.9 and 21.4.)

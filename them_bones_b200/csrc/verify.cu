@@ -9,11 +9,13 @@
 // function in 32 would move by more than the gap of a rare token's interval, and the token with it (65536 columns: one draw in some hundred).
 // A draft whose test is closer than the first kernel's 32-bit exponentials and sums can tell is decided on sums in 64 bits too.
 //
-// Measured, us of a whole call: 64 sequences of a token and up to four drafts, 65536 bf16 columns, drafts from a model, 38.2; one sequence of seven looked-up drafts, 8191 fp32
-// columns, 8.8; with arg-max throughout 11.2 and 3.9.  The first kernel takes 15 in the first case, 12.5 of them exponentials at 16 a clock and SM (59 MB at the
-// copy rate: 9); the second 20: 8.4 million exponentials in 64 bits, at most seven operations each with the table's reads between them, by warps
-// that wait for one another's results (the pipe of 64 bits 0.18, the schedulers 0.38 of the time).  Twice the warps with half the columns each: 55 us, and with four values
-// side by side instead of eight 58 to 61.
+// Measured, us of a whole call: 64 sequences of a token and three drafts each, 65536 bf16 columns, drafts from a model, 39.6; one sequence of seven looked-up drafts, 8191 fp32
+// columns, 8.9; with arg-max throughout 11.2 and 4.2.  By itself the first kernel takes 17.5 in the first case (59 MB at the copy rate: 9.0), the second 30, part of it beside the
+// first's end.  The first is held up by neither memory (0.5 of that rate) nor its 29.4 million exponentials alone (12400 of 23500 clocks at 16 a clock and SM): 448
+// rows are three an SM and four on some, the exponentials' pipe is active 0.62 of the time on the mean and 0.81 on the fullest SM, and a thread asks for its next four loads when
+// it is done with the last.  The second: 8.4 million exponentials in 64 bits, at most seven operations each with the table's reads between them, by warps
+// that wait for one another's results (the pipe of 64 bits 0.17, the schedulers 0.37 of the time).  Twice the warps with half the columns each: 55 us, and with four values
+// side by side instead of eight 58 to 61 (of 38.2 then; the nearest column, tracked beside the sums, is 1.3 of the 39.6).
 #include "decode_common.cuh"
 #include "paged.cuh"
 

@@ -295,7 +295,9 @@ def paged_attention(q, cache, table, starts, pos, scale, doc_start=None, window=
     """Pieces of new tokens against the cache: ``q [N, H*D]`` as ``paged_append`` returned it, with its ``table``, ``starts`` and ``pos`` -> ``[N, H*D]``.
     Token i of the N sees its sequence's positions from ``doc_start[i]`` (int32 ``[N]``) and the band of ``window`` tokens (as in ``attention``) to its
     own, as far as they have pages.  One token a sequence, drafts, pieces of prompts and whole prompts in one call.  ``longest``: the length of the
-    longest piece as far as the host knows (default: the mean); it picks a kernel, and the result but for roundings is the same.  Tokens that were left out, rows outside all pieces and
+    longest piece as far as the host knows (default: the mean); it picks a kernel, and the result but for roundings is the same.  Say it where lengths differ: with one piece of 900 tokens
+    beside 63 single ones the default takes 90 us for 67 (in documents 80 for 38).  Calls of more than 512 sequences take the kernel for longer pieces whatever it is, which for
+    single tokens is twice the time a sequence.  Tokens that were left out, rows outside all pieces and
     queries that see no key get zeros.  Queries and keys are behind the norm (``|q . k|`` about D at most): natively the soft-max has a
     fixed shift, and ``|scale| * D`` up to 32.  No gradient."""
     if native(q):

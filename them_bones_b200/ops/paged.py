@@ -21,7 +21,10 @@ PAGES = (16, 32, 64, 128)              # tokens of a page
 SHIFT = 32.0                           # largest |scale| * head_dim: the kernels' soft-max has this fixed shift, and its smallest weights, exp(-2 * 32), stay normal in fp32
 MOST_ROWS = (1 << 31) - 256             # rows of [D] in a cache
 MOST_WINDOW = 1 << 24                   # tiles of 128 tokens that hide none of any cache's
-FEW = 16                               # pieces of up to this many tokens go by tiles of 16 rows, longer ones by tiles of 128
+# Pieces of up to this many tokens go by tiles of 16 rows, longer ones by tiles of 128: a second tile of 16 reads the keys again.  us by tiles of 16 / of 128, 10 heads of 128, sequences
+# of n tokens each: 8 behind up to 1500, n = 8 18.1 / 20.8, 16 21.2 / 21.2, 17 23.2 / 21.2, 64 35.5 / 22.6; 32 behind up to 1500, n = 1 30.0 / 35.8, 16 37.2 / 37.2, 17 48.8 / 36.9,
+# 64 97 / 40; 4 behind up to 32768, n = 1 71.7 / 77.5, 16 76.5 / 77.5, 17 134 / 78; one behind 1500, n = 1 11.3 / 15.4, 16 16.4 / 15.4, 64 19.5 / 16.4.
+FEW = 16
 
 
 class PagedKV(NamedTuple):
